@@ -1,0 +1,458 @@
+// Attention of decoded tokens (rows with one query) over the 8-bit cache (q8.cuh): bfloat16 queries, heads of 64 and 128, up to 16 query heads to a kv head.
+//     s_j = scale * k_scale * (q . k_code_j);   out = sum_j exp(s_j) v_scale v_code_j / (sum_j exp(s_j) + exp(sink)),   kv_len - window <= j < kv_len
+// A token reads every visible code once, so the kernel is built to stream codes at the rate of DRAM.
+//
+// Work: all rows' and heads' keys in blocks of 64 are one line that a resident grid shares out evenly, whatever the rows' lengths; a CTA's piece of a
+// (row, kv head) is summed on its own, and where a pair was cut the CTA that finishes its last piece joins the pieces in the order of keys (a counter per
+// pair, which it leaves at zero).  Inside a piece warp w of four takes tiles w, w + 4, ... of 16 keys; each warp has a ring of its own that cp.async fills,
+// so nothing in the loop waits for another warp.
+//
+// Arithmetic: codes are exact in float16 (cvt), so both products run as mma.sync with float16 operands and float32 sums, keys as rows: S^T = K Q^T and
+// O^T = V^T P^T, eight queries to an instruction (padding of G query heads to 8 and not to 16).  q is exact in float16 once a power of two has brought
+// its largest number to [2^14, 2^15); numbers 2^-38 times that are lost.  P times the key's v_scale is rounded to float16 below 2^14 (a power of two that
+// follows the largest v_scale so far is taken out): 11 bits, where bfloat16 would keep 8.  Maxima, sums and scores are float32.
+// The order of the elements of a head among the k indices of S^T, and among the rows of O^T, is free as long as both operands agree: lane (g, c) owns
+// numbers c * HD / 4 ... of a key and g * HD / 8 ... of the values, so a lane's codes are whole 16-byte reads (8 bytes for the values of heads of 64).
+// Rows lie in shared memory with their 16-byte parts in an order turned by the key, which keeps those reads free of bank conflicts.
+#include "mma_utils.cuh"
+#include "q8.cuh"
+using namespace arle;
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 16;                 // keys of a warp's tile
+constexpr int kBlock = kWarps * kTile;    // keys of a block of work
+
+struct DecodeArgs {
+  const __nv_bfloat16* q;
+  int q_row_stride;
+  __nv_bfloat16* out;
+  const uint8_t *k_cache, *v_cache;
+  const float *k_scale, *v_scale;
+  const int *q_indptr, *kv_lens, *block_table;
+  int bt_stride;
+  float *part_o, *part_ml;
+  int* counters;
+  int nq, nkv, page_size, ps_shift, window, rows;
+  float scale_log2;
+  const float* sinks;
+};
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t v) {      // an 8 x 8 matrix of 16-bit numbers, transposed across the warp
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Blocks of 64 keys that a row's query sees, counted on the grid of absolute positions; a row that sees no key has one (which writes its zeros).
+__device__ __forceinline__ int row_blocks(const DecodeArgs& a, int r) {
+  if (a.q_indptr[r + 1] - a.q_indptr[r] != 1) return 0;
+  const int kv = a.kv_lens[r];
+  if (kv <= 0) return 1;
+  return (kv + kBlock - 1) / kBlock - first_visible_key(kv - 1, a.window, 0) / kBlock;
+}
+
+template <int HD> struct Shape {
+  static constexpr int kStages = HD == 128 ? 4 : 6;
+  static constexpr int kStageBytes = 2 * kTile * HD;
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kScales = kWarps * kStages * 32 * 4;
+  static constexpr int kSmem = kRing + kScales;
+  static constexpr int kPitch = HD + 8;      // of the partial results
+};
+
+// NT: query heads of a kv head in eights.  P16: pages of a multiple of 16 tokens, so that a tile lies in one page.
+template <int HD, int NT, bool P16>
+__global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
+  pdl_launch_dependents();
+  pdl_wait();
+  using S = Shape<HD>;
+  constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
+  constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int sum_s[kWarps + 1], start_s[3], last_s;
+  __shared__ float ml_s[kWarps][NT * 8][2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int G = a.nq / a.nkv, nkv = a.nkv;
+  unsigned char* ring = smem + warp * NS * S::kStageBytes;
+  float* scales = reinterpret_cast<float*>(smem + S::kRing) + warp * NS * 32;
+
+  // this CTA's share of the line, and the row where it begins
+  const int each = (a.rows + kThreads - 1) / kThreads, r0 = min(tid * each, a.rows), r1 = min(r0 + each, a.rows);
+  int mine = 0;
+  for (int r = r0; r < r1; ++r) mine += row_blocks(a, r);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) sum_s[warp] = upto;
+  __syncthreads();
+  int total = 0, front = upto - mine;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) front += sum_s[w];
+    total += sum_s[w];
+  }
+  total *= nkv;
+  const int share = (total + gridDim.x - 1) / gridDim.x;
+  const int begin = blockIdx.x * share, end = min(begin + share, total);
+  if (begin >= end) return;
+  if (begin >= front * nkv && begin < (front + mine) * nkv) {
+    int r = r0, at = front * nkv;
+    for (;; ++r) {
+      const int n = row_blocks(a, r) * nkv;
+      if (begin < at + n) break;
+      at += n;
+    }
+    start_s[0] = r;
+    start_s[1] = at;
+  }
+  __syncthreads();
+  int row = start_s[0], row_at = start_s[1];      // the row and where its blocks begin on the line
+
+  for (int pos = begin; pos < end;) {
+    int nb = row_blocks(a, row);
+    while (pos >= row_at + nb * nkv) {
+      row_at += nb * nkv;
+      nb = row_blocks(a, ++row);
+    }
+    const int h = (pos - row_at) / nb, pair_at = row_at + h * nb;
+    const int blk0 = pos - pair_at, blk1 = min(nb, end - pair_at);
+    const int t = a.q_indptr[row], kv = a.kv_lens[row];
+    const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0;
+    const int base_key = lo / kBlock * kBlock;
+    const int tile0 = (base_key + blk0 * kBlock) / kTile + warp, tile_end = min((base_key + blk1 * kBlock) / kTile, (kv + kTile - 1) / kTile);
+    const int* bt = a.block_table + (size_t)row * a.bt_stride;
+
+    auto page_of = [&](int tile) -> int {      // of key (lane & 15) of the tile; -1: a key that is not seen
+      const int key = tile * kTile + (lane & 15);
+      if (tile >= tile_end || key < lo || key >= kv) return -1;
+      const int p = a.ps_shift >= 0 ? key >> a.ps_shift : key / a.page_size;
+      return bt[p];
+    };
+    auto load_tile = [&](int tile, int stage, int page) {
+      unsigned char* dst = ring + stage * S::kStageBytes;
+#pragma unroll
+      for (int i = 0; i < CH / 2; ++i) {
+        const int part = i * 32 + lane, key = part / CH, col = part % CH;
+        const int pg = __shfl_sync(0xffffffffu, page, key), abs_key = tile * kTile + key;
+        const int slot = a.ps_shift >= 0 ? abs_key & (a.page_size - 1) : abs_key % a.page_size;
+        const size_t off = pg >= 0 ? (((size_t)pg * nkv + h) * a.page_size + slot) * HD + col * 16 : 0;
+        const int turn = HD == 128 ? (key & 7) : ((key >> 1) & 3);
+        const uint32_t to = smem_u32(dst + key * HD + ((col ^ turn) * 16));
+        cp_async16(to, a.k_cache + off, pg >= 0 ? 16 : 0);
+        cp_async16(to + kTile * HD, a.v_cache + off, pg >= 0 ? 16 : 0);
+      }
+      const float* from = lane < 16 ? a.k_scale : a.v_scale;
+      cp_async4(smem_u32(scales + stage * 32 + lane), from + (page >= 0 ? (size_t)page * nkv + h : 0), page >= 0 ? 4 : 0);
+    };
+
+    int page_next;
+    {
+      int pg[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) pg[i] = page_of(tile0 + i * kWarps);
+#pragma unroll
+      for (int i = 0; i < NS - 1; ++i) {
+        if (tile0 + i * kWarps < tile_end) load_tile(tile0 + i * kWarps, i, pg[i]);
+        cp_commit();
+      }
+      page_next = pg[NS - 1];
+    }
+
+    // q: lane (g, c) holds numbers c * HD / 4 ... of query g
+    uint32_t qb[NT][KS][2];
+    float qf[NT][2];                       // scale, log2 e and q's power of two for queries 2c and 2c + 1
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      uint4 raw[HD / 32];
+      const bool have = nt * 8 + g < G;
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + (size_t)t * a.q_row_stride + (size_t)(h * G + nt * 8 + g) * HD + c * (HD / 4));
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) raw[i] = have ? src[i] : make_uint4(0, 0, 0, 0);
+      auto number = [&](int e) {           // number e of the lane's
+        const uint32_t w = reinterpret_cast<const uint32_t*>(raw)[e >> 1];
+        return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+      };
+#pragma unroll
+      for (int e = 0; e < HD / 4; ++e) most = fmaxf(most, fabsf(number(e)));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int x = min(max((int)(__float_as_uint(most) >> 23) - 127, -100), 127);
+      const float up = exp2_int(14 - x);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        qb[nt][s][0] = pack_f16(number(4 * s) * up, number(4 * s + 1) * up);
+        qb[nt][s][1] = pack_f16(number(4 * s + 2) * up, number(4 * s + 3) * up);
+      }
+      const float down = ldexpf(a.scale_log2, x - 14);
+      qf[nt][0] = __shfl_sync(0xffffffffu, down, 8 * c);
+      qf[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
+    }
+
+    float o[NT][MT][4], m[NT][2], l[NT][2], vtop = 0.f, vnorm = 0.f;      // o times vnorm; vtop: the largest v_scale so far, as a power of two
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+    }
+
+    int stage = 0;
+    for (int tile = tile0; tile < tile_end; tile += kWarps) {
+      const int ahead = tile + (NS - 1) * kWarps;
+      if (ahead < tile_end) load_tile(ahead, stage == 0 ? NS - 1 : stage - 1, page_next);
+      cp_commit();
+      page_next = page_of(ahead + kWarps);
+      cp_wait<NS - 1>();
+      __syncwarp();
+      const unsigned char* kt = ring + stage * S::kStageBytes;
+      const unsigned char* vt = kt + kTile * HD;
+      const float ks0 = scales[stage * 32 + g], ks1 = scales[stage * 32 + g + 8];
+      const float vs0 = scales[stage * 32 + 16 + g], vs1 = scales[stage * 32 + 24 + g];
+
+      float s[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 64; ++i) {
+        const int part = HD == 128 ? ((2 * c + i) ^ g) : (c ^ ((g >> 1) & 3));
+        const uint4 w0 = *reinterpret_cast<const uint4*>(kt + g * HD + part * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(kt + (g + 8) * HD + part * 16);
+        const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a0 = q8_half2(x0[e]), a2 = q8_half2(x0[e] >> 16), a1 = q8_half2(x1[e]), a3 = q8_half2(x1[e] >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][4 * i + e][0], qb[nt][4 * i + e][1]);
+        }
+      }
+
+      const int key0 = tile * kTile + g;
+      const bool in0 = key0 >= lo && key0 < kv, in1 = key0 + 8 >= lo && key0 + 8 < kv;
+      float top = fmaxf(in0 ? vs0 : 0.f, in1 ? vs1 : 0.f);
+      bool grew = top > vtop;
+      float mn[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          s[nt][e] = in0 ? s[nt][e] * qf[nt][e] * ks0 : -INFINITY;
+          s[nt][2 + e] = in1 ? s[nt][2 + e] * qf[nt][e] * ks1 : -INFINITY;
+          float x = fmaxf(s[nt][e], s[nt][2 + e]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          mn[nt][e] = fmaxf(m[nt][e], x);
+          grew |= mn[nt][e] > m[nt][e];
+        }
+      }
+      if (__any_sync(0xffffffffu, grew)) {      // sums so far follow a larger maximum, or a larger v_scale
+        top = fmaxf(vtop, warp_max(top));
+        const uint32_t tb = __float_as_uint(top);
+        const int te = min(max((int)(tb >> 23) - 127 + ((tb & 0x7fffffu) != 0), -100), 127);
+        const float was = vnorm;
+        vtop = top > 0.f ? exp2_int(te) : 0.f;
+        vnorm = top > 0.f ? exp2_int(14 - te) : 0.f;
+        const float by = was > 0.f ? vnorm / was : 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            f[e] = mn[nt][e] == -INFINITY ? 1.f : exp2f(m[nt][e] - mn[nt][e]);
+            l[nt][e] *= f[e];
+            m[nt][e] = mn[nt][e];
+            f[e] *= by;
+          }
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            o[nt][j][0] *= f[0];
+            o[nt][j][1] *= f[1];
+            o[nt][j][2] *= f[0];
+            o[nt][j][3] *= f[1];
+          }
+        }
+      }
+      const float w0 = vs0 * vnorm, w1 = vs1 * vnorm;
+      uint32_t pb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float top_s = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+          p[e] = exp2f(s[nt][e] - top_s);
+          p[2 + e] = exp2f(s[nt][2 + e] - top_s);
+          l[nt][e] += p[e] + p[2 + e];
+        }
+        pb[nt][0] = turned(pack_f16(in0 ? p[0] * w0 : 0.f, in0 ? p[1] * w0 : 0.f));
+        pb[nt][1] = turned(pack_f16(in1 ? p[2] * w1 : 0.f, in1 ? p[3] * w1 : 0.f));
+      }
+
+      // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
+      constexpr int VW = HD / 32;      // words of 4 codes
+      uint32_t v[4][VW];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int key = 2 * c + (y & 1) + (y >> 1) * 8;
+        if constexpr (HD == 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(vt + key * HD + ((g ^ (key & 7)) * 16));
+          v[y][0] = w.x, v[y][1] = w.y, v[y][2] = w.z, v[y][3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(vt + key * HD + (((g >> 1) ^ ((key >> 1) & 3)) * 16) + (g & 1) * 8);
+          v[y][0] = w.x, v[y][1] = w.y;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t x = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+          const uint32_t a0 = q8_half2(x), a1 = q8_half2(x >> 16), a2 = q8_half2(y), a3 = q8_half2(y >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+      }
+      __syncwarp();
+      stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    cp_wait<0>();
+
+    // the four warps' sums: o[nt][j] holds numbers g * HD / 8 + 2j (rows g) and + 1 (rows g + 8) of queries 2c, 2c + 1
+    __syncthreads();                                   // the rings are free
+    float* mo = reinterpret_cast<float*>(smem);        // [4][NT * 8][kPitch]
+    const float out_by = vnorm > 0.f ? 1.0f / vnorm : 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[nt][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        const int query = nt * 8 + 2 * c + e;
+        if (g == 0) {
+          ml_s[warp][query][0] = m[nt][e];
+          ml_s[warp][query][1] = x;
+        }
+        if (query < G) {
+          float* dst = mo + (warp * NT * 8 + query) * S::kPitch + g * (HD / 8);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[nt][j][e] * out_by, o[nt][j][2 + e] * out_by);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = blk0 == 0 && blk1 == nb;
+    const size_t slot = (size_t)blockIdx.x * 2 + (pos == begin ? 0 : 1);
+    for (int i = tid; i < G * HD; i += kThreads) {
+      const int query = i / HD, d = i % HD;
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[w][query][0]);
+      const float top_s = M == -INFINITY ? 0.f : M;
+      float L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = exp2f(ml_s[w][query][0] - top_s);
+        L += ml_s[w][query][1] * f;
+        O += mo[(w * NT * 8 + query) * S::kPitch + d] * f;
+      }
+      if (whole) {
+        const float sink = a.sinks ? exp2f(a.sinks[h * G + query] * 1.4426950408889634f - top_s) : 0.f;
+        a.out[((size_t)t * a.nq + h * G + query) * HD + d] = __float2bfloat16_rn(kv > 0 ? O / (L + sink) : 0.f);
+      } else {
+        a.part_o[(slot * 16 + query) * HD + d] = O;
+        if (d == 0) {
+          a.part_ml[(slot * 16 + query) * 2] = M;
+          a.part_ml[(slot * 16 + query) * 2 + 1] = L;
+        }
+      }
+    }
+    if (!whole) {
+      // the pieces of this pair: of CTA first_cta (its last piece, unless the pair begins with its share) up to last_cta (their first pieces)
+      const int first_cta = pair_at / share, last_cta = (pair_at + nb - 1) / share, pieces = last_cta - first_cta + 1;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        int* counter = a.counters + row * nkv + h;
+        last_s = atomicAdd(counter, 1) == pieces - 1;
+        if (last_s) *counter = 0;
+      }
+      __syncthreads();
+      if (last_s) {
+        __threadfence();
+        const size_t slot0 = (size_t)first_cta * 2 + (pair_at == first_cta * share ? 0 : 1);
+        for (int i = tid; i < G * HD; i += kThreads) {
+          const int query = i / HD, d = i % HD;
+          auto piece = [&](int k) { return (k == 0 ? slot0 : (size_t)(first_cta + k) * 2) * 16 + query; };
+          float M = -INFINITY;
+#pragma unroll 8
+          for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(a.part_ml + piece(k) * 2));
+          const float top_s = M == -INFINITY ? 0.f : M;
+          float L = a.sinks ? exp2f(a.sinks[h * G + query] * 1.4426950408889634f - top_s) : 0.f, O = 0.f;
+#pragma unroll 8
+          for (int k = 0; k < pieces; ++k) {
+            const float f = exp2f(__ldcg(a.part_ml + piece(k) * 2) - top_s);
+            L += __ldcg(a.part_ml + piece(k) * 2 + 1) * f;
+            O += __ldcg(a.part_o + piece(k) * HD + d) * f;
+          }
+          a.out[((size_t)t * a.nq + h * G + query) * HD + d] = __float2bfloat16_rn(O / L);
+        }
+      }
+    }
+    __syncthreads();
+    pos += blk1 - blk0;
+  }
+}
+
+template <int HD, int NT, bool P16>
+int launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
+  using S = Shape<HD>;
+  constexpr size_t merge = (size_t)kWarps * NT * 8 * S::kPitch * 4;
+  constexpr size_t smem = S::kSmem > merge ? S::kSmem : merge;
+  static SharedLimit limit;
+  const cudaError_t raised = limit.raise((const void*)q8_decode_kernel<HD, NT, P16>, smem);
+  if (raised != cudaSuccess) return (int)raised;
+  launch_kernel(q8_decode_kernel<HD, NT, P16>, dim3(ctas), dim3(kThreads), smem, s, 1, a);
+  return launch_status();
+}
+
+template <int HD>
+int launch_by(const DecodeArgs& a, int ctas, cudaStream_t s) {
+  const bool p16 = a.page_size % 16 == 0;
+  if (a.nq / a.nkv <= 8) return p16 ? launch<HD, 1, true>(a, ctas, s) : launch<HD, 1, false>(a, ctas, s);
+  return p16 ? launch<HD, 2, true>(a, ctas, s) : launch<HD, 2, false>(a, ctas, s);
+}
+
+}  // namespace
+
+// Rows with one query; others are left alone.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 2], counters int32
+// [rows * nkv], zero before the first launch (the kernel leaves them zero).
+ARLE_API int arle_attention_q8_decode(const void* q, int q_row_stride, void* out, const void* k_cache, const void* v_cache, const float* k_scale,
+                                      const float* v_scale, const int* q_indptr, const int* kv_lens, const int* block_table, int bt_stride, float* part_o,
+                                      float* part_ml, int* counters, int nq, int nkv, int hd, int page_size, float scale, int window, const float* sinks, int rows,
+                                      int ctas, cudaStream_t s) {
+  if (rows <= 0) return 0;
+  if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > 16 || page_size <= 0 || ctas <= 0 || (hd != 64 && hd != 128) || q_row_stride % 8) return ARLE_E_UNSUPPORTED;
+  int shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (shift = 0; (1 << shift) < page_size; ++shift) {}
+  const DecodeArgs a{(const __nv_bfloat16*)q, q_row_stride, (__nv_bfloat16*)out, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, q_indptr,
+                     kv_lens, block_table, bt_stride, part_o, part_ml, counters, nq, nkv, page_size, shift, window, rows, scale * 1.4426950408889634f, sinks};
+  return hd == 128 ? launch_by<128>(a, ctas, s) : launch_by<64>(a, ctas, s);
+}

@@ -128,6 +128,11 @@ _SIGNATURES = {
     "arle_token_shift": [_P, _I, _I, _P, _I, _P, ctypes.c_long, _P, _P, _P, _P, ctypes.c_long, _I, _I, _I, _I, _P],
     "arle_gate_mul": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
     "arle_square_relu": [_P, _I, _P, _I, _I, _I, _I, _P],
+    "arle_store_q8": [_P, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, ctypes.c_long, _I, _I, _I, _I, _P],
+    "arle_expand_q8": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P],
+    "arle_attention_q8": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P],
+    "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _P],
+    "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
 
@@ -2282,3 +2287,147 @@ def token_shift(h, mu, state, q_indptr, row_of_token, state_slots, out, max_q_le
                                       _ptr(state_slots), _ptr(out), T * C, T, R, C, single, _stream()), "token_shift")
     if not single:
         add_launches(1)
+
+
+# ------------------------------------------------------------------ the 8-bit cache
+_E4M3 = torch.float8_e4m3fn
+
+
+def _q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, vd: int, page_size: int) -> None:
+    if k_cache.dtype != _E4M3 or v_cache.dtype != _E4M3:
+        raise KernelError(f"{what}: the caches hold float8_e4m3fn codes, got {k_cache.dtype} and {v_cache.dtype}")
+    pages = k_cache.shape[0]
+    if (tuple(k_cache.shape) != (pages, nkv, page_size, hd) or tuple(v_cache.shape) != (pages, nkv, page_size, vd) or not k_cache.is_contiguous()
+            or not v_cache.is_contiguous()):
+        raise KernelError(f"{what}: cache shapes {tuple(k_cache.shape)}, {tuple(v_cache.shape)} are not contiguous [pages, {nkv}, {page_size}, {hd}] and "
+                          f"[pages, {nkv}, {page_size}, {vd}]")
+    for s in (k_scale, v_scale):
+        if s.dtype != torch.float32 or tuple(s.shape) != (pages, nkv) or not s.is_contiguous():
+            raise KernelError(f"{what}: scales must be contiguous float32 [pages, {nkv}]")
+
+
+def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
+    """The store of a step's keys and values into a cache of 8 bits: e4m3 codes with one float32 scale for each page and head.
+
+    k [T, nkv*hd] and v [T, nkv*vd] (``vd`` None: hd), float32 or bfloat16, rows of any stride (columns of a packed projection); slot_mapping int32 [T]:
+    page * page_size + place in the page, negative (or behind the cache): not stored.  Caches float8_e4m3fn [pages, nkv, page_size, hd | vd], scales float32
+    [pages, nkv]; a number is code * scale.
+
+    A scale is a power of two, the least with max |x| <= 448 * scale (at least 2^-100; at most 2^119, beyond which numbers end at 448 * 2^119).  Tokens
+    that go to a page from its first place on give it a new scale.  Tokens that go behind others, which are taken to fill every place in front, keep the
+    larger of the page's scale and their own; where that grows, the older codes are rounded once more to it.  Infinities become the largest number of their page's
+    scale, NaN stays NaN; neither counts for the scale.  A step's tokens of one page stand in consecutive rows, in the order of their places, as an engine's do."""
+    vd = hd if vd is None else int(vd)
+    T = slot_mapping.numel()
+    if k.shape != (T, nkv * hd) or v.shape != (T, nkv * vd) or k.dtype != v.dtype or (T and (k.stride(1) != 1 or v.stride(1) != 1)):
+        raise KernelError("store_q8: k must be [T, nkv*hd] and v [T, nkv*vd] of one type, with unit inner stride")
+    _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
+    if not slot_mapping.is_contiguous():
+        raise KernelError("store_q8: slot_mapping must be contiguous")
+    _i32(slot_mapping, "slot_mapping")
+    if T == 0:
+        return
+    _check(library().arle_store_q8(_ptr(k), k.stride(0), _ptr(v), v.stride(0), _dt(k), _ptr(slot_mapping), T, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+                                   _ptr(v_scale), k_cache.shape[0], nkv, hd, vd, page_size, _stream()), "store_q8")
+
+
+# Bytes of bfloat16 keys and values that prompt portions are expanded into at a time; rows that see more go by themselves.
+Q8_EXPAND_BYTES = 1 << 30
+
+
+def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table, nq: int, nkv: int, hd: int, page_size: int, scale: float,
+                       window, batch=None, vd: int = None, sink=None) -> None:
+    """Causal attention of this step's queries over a paged cache of 8 bits (``store_q8``): ``paged_attention`` with e4m3 codes and their scales
+    in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros.
+
+    ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
+    bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens read the codes as they are; the keys and values that
+    portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels."""
+    T = q.shape[0]
+    vd = hd if vd is None else int(vd)
+    if q.stride(1) != 1 or q.shape[1] != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
+        raise KernelError("paged_attention_q8: q must be [T, nq*hd] with unit inner stride and out contiguous [T, nq*vd]")
+    if out.dtype != q.dtype:
+        raise KernelError("paged_attention_q8: q and out must share a type")
+    if hd > 256 or vd > 256 or nq % nkv:
+        raise KernelError(f"paged_attention_q8: head_dim {hd} / value width {vd} / heads {nq}:{nkv} not supported")
+    _q8_cache("paged_attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
+    _i32(positions, "positions"), _i32(row_of_token, "row_of_token"), _i32(block_table, "block_table")
+    if block_table.stride(1) != 1:
+        raise KernelError("paged_attention_q8: block table rows must be contiguous")
+    if T == 0:
+        return
+    sinks, w = _sinks(sink, nq, q.device), int(window) if window else 0
+    if (batch is not None and _KERNEL_SET == "fast" and vd == hd and fast_attention_supported(q, nq, nkv, hd)
+            and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0):
+        R = batch.num_rows
+        if batch.max_q_len > 1:
+            _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
+        if batch.num_single > 0:
+            ctas = 3 * sm_count(q.device)
+            part_o = batch.ws.get("attn_q8_part_o", (ctas * 2 * 16 * hd,), torch.float32)
+            part_ml = batch.ws.get("attn_q8_part_ml", (ctas * 2 * 16 * 2,), torch.float32)
+            counters = batch.ws.get_zeroed("attn_q8_counters", (R * nkv,), torch.int32)
+            _check(library().arle_attention_q8_decode(
+                _ptr(q), q.stride(0), _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(batch.q_indptr), _ptr(batch.kv_lens),
+                _ptr(block_table), block_table.stride(0), _ptr(part_o), _ptr(part_ml), _ptr(counters), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks), R, ctas,
+                _stream()), "attention_q8_decode")
+        return
+    _check(library().arle_attention_q8(
+        _ptr(q), q.stride(0), _ptr(out), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(positions), _ptr(row_of_token),
+        _ptr(block_table), block_table.stride(0), nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
+
+
+def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks) -> None:
+    """The rows with several queries: their keys and values in bfloat16, then the prompt kernels, for as many rows at a time as ``Q8_EXPAND_BYTES`` hold."""
+    page = 64
+    prefill = paged_attention_prefill_tc if tc_attention_supported(q, hd, page) else paged_attention_prefill
+    pages = [0 if n < 2 else -(-kv // page) - (max(0, kv - n - window + 1) if window else 0) // page for n, kv in zip(batch.q_lens, batch.kv_lens_host)]
+    width = max(1, -(-max(batch.kv_lens_host) // page))
+    most = max(1, Q8_EXPAND_BYTES // (4 * nkv * page * hd))
+    r0, R = 0, batch.num_rows
+    while r0 < R:
+        r1, total = r0, 0
+        while r1 < R and (total == 0 or total + pages[r1] <= most):
+            total += pages[r1]
+            r1 += 1
+        if total:
+            kx = batch.ws.get("attn_q8_keys", (total, nkv, page, hd), torch.bfloat16)
+            vx = batch.ws.get("attn_q8_values", (total, nkv, page, hd), torch.bfloat16)
+            table = batch.ws.get("attn_q8_table", (r1 - r0, width), torch.int32)
+            indptr, lens = batch.q_indptr[r0: r1 + 1], batch.kv_lens[r0: r1]
+            bt = block_table[r0: r1]
+            _check(library().arle_expand_q8(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(indptr), _ptr(lens), _ptr(bt), bt.stride(0),
+                                            page_size, nkv, hd, window, r1 - r0, 2, _ptr(kx), _ptr(vx), total, _ptr(table), width, _stream()), "expand_q8")
+            prefill(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, max(batch.q_lens[r0: r1]),
+                    skip_single=min(batch.q_lens[r0: r1]) < 2, sink=sinks)
+        r0 = r1
+
+
+# ------------------------------------------------------------------ a step's tables
+def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, page_size: int, q_indptr, kv_lens, positions, row_of_token, slot_of_token,
+                slot_mapping, block_table, status) -> None:
+    """A step's tables from the lengths of its requests, on the device (everything int32).
+
+    In: slots [R], the requests' slots, each once; starts [R], the tokens that they hold; q_lens [R], the tokens that they bring (0 is fine);
+    new_pages [N], pages for what does not fit the pages that they have, taken in the order of the rows (more than needed is fine);
+    page_table [slots, pages a request may have], contiguous: the pages of every request, to which the new ones are added; num_pages: pages of the cache.
+
+    Out: q_indptr [R + 1], kv_lens [R], positions, row_of_token, slot_of_token and slot_mapping [T] (what lies behind the step's last token is left as it
+    was), block_table [R, width], contiguous: a row's pages, -1 behind them, and status [1]: 0, or the sum of what is wrong with the step: 1 more tokens
+    than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
+    cache.  Such a step leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
+    R, T = slots.numel(), positions.numel()
+    for t, name in ((slots, "slots"), (starts, "starts"), (q_lens, "q_lens"), (new_pages, "new_pages"), (page_table, "page_table"), (q_indptr, "q_indptr"),
+                    (kv_lens, "kv_lens"), (positions, "positions"), (row_of_token, "row_of_token"), (slot_of_token, "slot_of_token"),
+                    (slot_mapping, "slot_mapping"), (block_table, "block_table"), (status, "status")):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise KernelError(f"step_tables: {name} must be contiguous int32")
+    if (starts.numel() != R or q_lens.numel() != R or q_indptr.numel() != R + 1 or kv_lens.numel() != R or row_of_token.numel() != T or slot_of_token.numel() != T
+            or slot_mapping.numel() != T or status.numel() != 1 or block_table.dim() != 2 or block_table.shape[0] != R or page_table.dim() != 2):
+        raise KernelError("step_tables: slots, starts, q_lens and kv_lens are [R], q_indptr [R + 1], the tokens' tables [T], block_table [R, width], "
+                          "page_table [slots, pages], status [1]")
+    _check(library().arle_step_tables(
+        _ptr(slots), _ptr(starts), _ptr(q_lens), R, _ptr(new_pages), new_pages.numel(), _ptr(page_table), page_table.shape[0], page_table.shape[1], int(num_pages),
+        int(page_size), _ptr(q_indptr), _ptr(kv_lens), _ptr(positions), _ptr(row_of_token), _ptr(slot_of_token), _ptr(slot_mapping), T, _ptr(block_table),
+        block_table.shape[1], _ptr(status), _stream()), "step_tables")
