@@ -9,8 +9,10 @@
 //
 // Arithmetic: codes are exact in float16 (cvt), so both products run as mma.sync with float16 operands and float32 sums, keys as rows: S^T = K Q^T and
 // O^T = V^T P^T, eight queries to an instruction (padding of G query heads to 8 and not to 16).  q is exact in float16 once a power of two has brought
-// its largest number to [2^14, 2^15); numbers 2^-38 times that are lost.  P times the key's v_scale is rounded to float16 below 2^14 (a power of two that
-// follows the largest v_scale so far is taken out): 11 bits, where bfloat16 would keep 8.  Maxima, sums and scores are float32.
+// its largest number to [2^14, 2^15); numbers 2^-38 times that are lost.  Scores, sums and the maximum that the exponentials are taken against are float32.
+// That maximum is followed only where a score passes it by more than kSlack (in log2): the weights stay below 2^kSlack, most tiles need no reduction across
+// lanes and no correction of the sums.  A weight times its key's v_scale, over the largest v_scale so far, times 2^kUp is rounded to float16: 11 bits
+// (bfloat16 would keep 8) at most 2^(kSlack + kUp) = 2^15, in whole down to 2^(-14 - kUp) of the largest.
 // The order of the elements of a head among the k indices of S^T, and among the rows of O^T, is free as long as both operands agree: lane (g, c) owns
 // numbers c * HD / 4 ... of a key and g * HD / 8 ... of the values, so a lane's codes are whole 16-byte reads (8 bytes for the values of heads of 64).
 // Rows lie in shared memory with their 16-byte parts in an order turned by the key, which keeps those reads free of bank conflicts.
@@ -23,6 +25,8 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;                 // keys of a warp's tile
 constexpr int kBlock = kWarps * kTile;    // keys of a block of work
+constexpr int kUp = 9;
+constexpr float kSlack = 6.0f;
 
 struct DecodeArgs {
   const __nv_bfloat16* q;
@@ -49,6 +53,11 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {      // an 8 x 8 matrix
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
+__device__ __forceinline__ float exp2_fast(float x) {      // what is below 2^-126 is zero
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -56,8 +65,8 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 
 // Blocks of 64 keys that a row's query sees, counted on the grid of absolute positions; a row that sees no key has one (which writes its zeros).
 __device__ __forceinline__ int row_blocks(const DecodeArgs& a, int r) {
-  if (a.q_indptr[r + 1] - a.q_indptr[r] != 1) return 0;
-  const int kv = a.kv_lens[r];
+  const int t0 = a.q_indptr[r], t1 = a.q_indptr[r + 1], kv = a.kv_lens[r];
+  if (t1 - t0 != 1) return 0;
   if (kv <= 0) return 1;
   return (kv + kBlock - 1) / kBlock - first_visible_key(kv - 1, a.window, 0) / kBlock;
 }
@@ -86,6 +95,14 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
   const int G = a.nq / a.nkv, nkv = a.nkv;
   unsigned char* ring = smem + warp * NS * S::kStageBytes;
   float* scales = reinterpret_cast<float*>(smem + S::kRing) + warp * NS * 32;
+  const uint32_t ring_u32 = smem_u32(ring), scales_u32 = smem_u32(scales);
+  // where the lane's 16-byte parts of a tile go, beside i * 512: part i * 32 + lane is part lane % CH of key (i * 32 + lane) / CH
+  uint32_t turned_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int key = (i * 32 + lane) / CH, turn = HD == 128 ? (key & 7) : ((key >> 1) & 3);
+    turned_at[i] = key * HD + (((lane % CH) ^ turn) * 16) - i * 512;
+  }
 
   // this CTA's share of the line, and the row where it begins
   const int each = (a.rows + kThreads - 1) / kThreads, r0 = min(tid * each, a.rows), r1 = min(r0 + each, a.rows);
@@ -135,27 +152,50 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
     const int tile0 = (base_key + blk0 * kBlock) / kTile + warp, tile_end = min((base_key + blk1 * kBlock) / kTile, (kv + kTile - 1) / kTile);
     const int* bt = a.block_table + (size_t)row * a.bt_stride;
 
-    auto page_of = [&](int tile) -> int {      // of key (lane & 15) of the tile; -1: a key that is not seen
-      const int key = tile * kTile + (lane & 15);
-      if (tile >= tile_end || key < lo || key >= kv) return -1;
-      const int p = a.ps_shift >= 0 ? key >> a.ps_shift : key / a.page_size;
-      return bt[p];
+    // Page of the tile (P16) or of its key lane & 15; -1: nothing of it is seen.
+    auto page_of = [&](int tile) -> int {
+      const int key = tile * kTile + (P16 ? 0 : lane & 15);
+      if (tile >= tile_end || (!P16 && (key < lo || key >= kv))) return -1;
+      return bt[a.ps_shift >= 0 ? key >> a.ps_shift : key / a.page_size];
     };
     auto load_tile = [&](int tile, int stage, int page) {
-      unsigned char* dst = ring + stage * S::kStageBytes;
+      const uint32_t dst = ring_u32 + stage * S::kStageBytes;
+      const int first = tile * kTile;
+      if constexpr (P16) {
+        const int slot = a.ps_shift >= 0 ? first & (a.page_size - 1) : first % a.page_size;
+        const long unit = (long)page * nkv + h;
+        const bool whole = first >= lo && first + kTile <= kv && page >= 0;
+        const long off = page >= 0 ? (unit * a.page_size + slot) * HD + lane * 16 : 0;
+        const uint8_t *kp = a.k_cache + off, *vp = a.v_cache + off;
+        if (whole) {
 #pragma unroll
-      for (int i = 0; i < CH / 2; ++i) {
-        const int part = i * 32 + lane, key = part / CH, col = part % CH;
-        const int pg = __shfl_sync(0xffffffffu, page, key), abs_key = tile * kTile + key;
-        const int slot = a.ps_shift >= 0 ? abs_key & (a.page_size - 1) : abs_key % a.page_size;
-        const size_t off = pg >= 0 ? (((size_t)pg * nkv + h) * a.page_size + slot) * HD + col * 16 : 0;
-        const int turn = HD == 128 ? (key & 7) : ((key >> 1) & 3);
-        const uint32_t to = smem_u32(dst + key * HD + ((col ^ turn) * 16));
-        cp_async16(to, a.k_cache + off, pg >= 0 ? 16 : 0);
-        cp_async16(to + kTile * HD, a.v_cache + off, pg >= 0 ? 16 : 0);
+          for (int i = 0; i < CH / 2; ++i) {
+            cp_async16(dst + i * 512 + turned_at[i & 1], kp + i * 512, 16);
+            cp_async16(dst + kTile * HD + i * 512 + turned_at[i & 1], vp + i * 512, 16);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH / 2; ++i) {
+            const int key = first + (i * 32 + lane) / CH;
+            const int bytes = key >= lo && key < kv && page >= 0 ? 16 : 0;
+            cp_async16(dst + i * 512 + turned_at[i & 1], bytes ? kp + i * 512 : a.k_cache, bytes);
+            cp_async16(dst + kTile * HD + i * 512 + turned_at[i & 1], bytes ? vp + i * 512 : a.v_cache, bytes);
+          }
+        }
+        if (lane < 2) cp_async4(scales_u32 + (stage * 32 + lane) * 4, (lane ? a.v_scale : a.k_scale) + (page >= 0 ? unit : 0), page >= 0 ? 4 : 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+          const int part = i * 32 + lane, key = part / CH, abs_key = first + key;
+          const int pg = __shfl_sync(0xffffffffu, page, key);
+          const int slot = a.ps_shift >= 0 ? abs_key & (a.page_size - 1) : abs_key % a.page_size;
+          const size_t off = pg >= 0 ? (((size_t)pg * nkv + h) * a.page_size + slot) * HD + (part % CH) * 16 : 0;
+          cp_async16(dst + i * 512 + turned_at[i & 1], a.k_cache + off, pg >= 0 ? 16 : 0);
+          cp_async16(dst + kTile * HD + i * 512 + turned_at[i & 1], a.v_cache + off, pg >= 0 ? 16 : 0);
+        }
+        const float* from = lane < 16 ? a.k_scale : a.v_scale;
+        cp_async4(scales_u32 + (stage * 32 + lane) * 4, from + (page >= 0 ? (size_t)page * nkv + h : 0), page >= 0 ? 4 : 0);
       }
-      const float* from = lane < 16 ? a.k_scale : a.v_scale;
-      cp_async4(smem_u32(scales + stage * 32 + lane), from + (page >= 0 ? (size_t)page * nkv + h : 0), page >= 0 ? 4 : 0);
     };
 
     int page_next;
@@ -221,8 +261,14 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
       __syncwarp();
       const unsigned char* kt = ring + stage * S::kStageBytes;
       const unsigned char* vt = kt + kTile * HD;
-      const float ks0 = scales[stage * 32 + g], ks1 = scales[stage * 32 + g + 8];
-      const float vs0 = scales[stage * 32 + 16 + g], vs1 = scales[stage * 32 + 24 + g];
+      float ks0, ks1, vs0, vs1;
+      if constexpr (P16) {
+        const float2 sc = *reinterpret_cast<const float2*>(scales + stage * 32);
+        ks0 = ks1 = sc.x;
+        vs0 = vs1 = sc.y;
+      } else {
+        ks0 = scales[stage * 32 + g], ks1 = scales[stage * 32 + g + 8], vs0 = scales[stage * 32 + 16 + g], vs1 = scales[stage * 32 + 24 + g];
+      }
 
       float s[NT][4];
 #pragma unroll
@@ -235,7 +281,9 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
         const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t a0 = q8_half2(x0[e]), a2 = q8_half2(x0[e] >> 16), a1 = q8_half2(x1[e]), a3 = q8_half2(x1[e] >> 16);
+          uint32_t a0, a1, a2, a3;
+          q8_half4(x0[e], a0, a2);
+          q8_half4(x1[e], a1, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][4 * i + e][0], qb[nt][4 * i + e][1]);
         }
@@ -243,39 +291,36 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
 
       const int key0 = tile * kTile + g;
       const bool in0 = key0 >= lo && key0 < kv, in1 = key0 + 8 >= lo && key0 + 8 < kv;
-      float top = fmaxf(in0 ? vs0 : 0.f, in1 ? vs1 : 0.f);
-      bool grew = top > vtop;
-      float mn[NT][2];
+      bool grew = (in0 && vs0 > vtop) || (in1 && vs1 > vtop);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          s[nt][e] = in0 ? s[nt][e] * qf[nt][e] * ks0 : -INFINITY;
-          s[nt][2 + e] = in1 ? s[nt][2 + e] * qf[nt][e] * ks1 : -INFINITY;
-          float x = fmaxf(s[nt][e], s[nt][2 + e]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          mn[nt][e] = fmaxf(m[nt][e], x);
-          grew |= mn[nt][e] > m[nt][e];
+          s[nt][e] = in0 ? s[nt][e] * (qf[nt][e] * ks0) : -INFINITY;
+          s[nt][2 + e] = in1 ? s[nt][2 + e] * (qf[nt][e] * ks1) : -INFINITY;
+          grew |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kSlack;
         }
-      }
-      if (__any_sync(0xffffffffu, grew)) {      // sums so far follow a larger maximum, or a larger v_scale
-        top = fmaxf(vtop, warp_max(top));
+      if (__any_sync(0xffffffffu, grew)) {      // the sums so far follow a larger maximum, or a larger v_scale
+        const float top = fmaxf(vtop, warp_max(fmaxf(in0 ? vs0 : 0.f, in1 ? vs1 : 0.f)));
         const uint32_t tb = __float_as_uint(top);
         const int te = min(max((int)(tb >> 23) - 127 + ((tb & 0x7fffffu) != 0), -100), 127);
         const float was = vnorm;
         vtop = top > 0.f ? exp2_int(te) : 0.f;
-        vnorm = top > 0.f ? exp2_int(14 - te) : 0.f;
+        vnorm = top > 0.f ? exp2_int(kUp - te) : 0.f;
         const float by = was > 0.f ? vnorm / was : 0.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            f[e] = mn[nt][e] == -INFINITY ? 1.f : exp2f(m[nt][e] - mn[nt][e]);
+            float x = fmaxf(s[nt][e], s[nt][2 + e]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float mn = fmaxf(m[nt][e], x);
+            f[e] = mn == -INFINITY ? 1.f : exp2_fast(m[nt][e] - mn);
             l[nt][e] *= f[e];
-            m[nt][e] = mn[nt][e];
+            m[nt][e] = mn;
             f[e] *= by;
           }
 #pragma unroll
@@ -287,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
           }
         }
       }
-      const float w0 = vs0 * vnorm, w1 = vs1 * vnorm;
+      const float w0 = in0 ? vs0 * vnorm : 0.f, w1 = in1 ? vs1 * vnorm : 0.f;
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -295,12 +340,12 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const float top_s = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-          p[e] = exp2f(s[nt][e] - top_s);
-          p[2 + e] = exp2f(s[nt][2 + e] - top_s);
+          p[e] = exp2_fast(s[nt][e] - top_s);
+          p[2 + e] = exp2_fast(s[nt][2 + e] - top_s);
           l[nt][e] += p[e] + p[2 + e];
         }
-        pb[nt][0] = turned(pack_f16(in0 ? p[0] * w0 : 0.f, in0 ? p[1] * w0 : 0.f));
-        pb[nt][1] = turned(pack_f16(in1 ? p[2] * w1 : 0.f, in1 ? p[3] * w1 : 0.f));
+        pb[nt][0] = turned(pack_f16(p[0] * w0, p[1] * w0));
+        pb[nt][1] = turned(pack_f16(p[2] * w1, p[3] * w1));
       }
 
       // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
@@ -322,7 +367,9 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const uint32_t x = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
-          const uint32_t a0 = q8_half2(x), a1 = q8_half2(x >> 16), a2 = q8_half2(y), a3 = q8_half2(y >> 16);
+          uint32_t a0, a1, a2, a3;
+          q8_half4(x, a0, a1);
+          q8_half4(y, a2, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
         }

@@ -12,8 +12,6 @@ using namespace arle;
 
 namespace {
 
-constexpr int kRegVecs = 16;      // four numbers each: 64 numbers a lane
-
 struct StoreSide {
   const void* x;
   int row_stride, width;
@@ -21,24 +19,39 @@ struct StoreSide {
   float* scale;
 };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, bool wide, float (&v)[4]) {
-  if (wide) load_vec<T, 4>(p, v);
-  else
-    for (int i = 0; i < 4; ++i) v[i] = to_f32(p[i]);
-}
-
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
   return a <= 3.4028234663852886e38f ? a : 0.f;      // neither infinities nor NaN
 }
 
-// Threads of a group: `warps` warps.  `chunk`: tokens among which a group looks for the starts of runs (at most 32).
-template <typename T>
-__global__ void store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restrict__ slot_mapping, int tokens, int chunk, int nkv, int page_size, long places,
-                                int warps, long groups) {
+template <typename T, int VEC>
+__device__ __forceinline__ float most_of(const Pack<T, VEC>& p, float most) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) most = fmaxf(most, finite_abs(to_f32(p.e[j])));
+  return most;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void put(uint8_t* dst, const Pack<T, VEC>& p, float inv) {
+  if constexpr (VEC == 1) {
+    *dst = (uint8_t)q8_codes2(to_f32(p.e[0]) * inv, 0.f);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int j = 0; j < VEC / 4; ++j)
+      w[j] = q8_codes4(to_f32(p.e[4 * j]) * inv, to_f32(p.e[4 * j + 1]) * inv, to_f32(p.e[4 * j + 2]) * inv, to_f32(p.e[4 * j + 3]) * inv);
+    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+  }
+}
+
+// A group has `warps` warps.  `chunk`: tokens among which a group looks for the starts of runs (at most 32).  VEC: numbers of a load, 16 bytes or one.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restrict__ slot_mapping, int tokens, int chunk, int nkv, int page_size,
+                                                       long places, int warps, long groups) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int kKept = VEC == 1 ? 1 : 64 / VEC;      // loads a lane keeps: 64 numbers
   __shared__ float most_s[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lane_g = warps == 1 ? lane : threadIdx.x, size_g = warps * 32;
@@ -57,8 +70,9 @@ __global__ void store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restric
   const bool first = held && (s % page_size == 0 || before != s - 1 || t0 + lane == 0);
   const unsigned goes_on = __ballot_sync(0xffffffffu, held && !first);
   unsigned starts = __ballot_sync(0xffffffffu, first && lane < chunk);
-  const bool quads = (hd & 3) == 0;
-  const bool wide = quads && vec_aligned<4>(side.x, sizeof(T)) && side.row_stride % 4 == 0;
+  const int per_row = hd / VEC;                       // loads of a row
+  const bool even = size_g % per_row == 0;            // a lane keeps its column
+  const int row0 = lane_g / per_row, col0 = lane_g - row0 * per_row, row_step = size_g / per_row;
 
   while (starts) {
     const int at = __ffs(starts) - 1;
@@ -77,81 +91,77 @@ __global__ void store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restric
     uint8_t* codes = side.cache + ((long)page * nkv + head) * page_size * hd;
     float* scale = side.scale + (long)page * nkv + head;
     const float older = off ? *scale : 0.f;
+    const int loads = n * per_row;
+    auto load = [&](int i) {
+      const int e = i * size_g + lane_g;
+      const int row = even ? row0 + i * row_step : e / per_row, col = even ? col0 : e - row * per_row;
+      return *reinterpret_cast<const Pack<T, VEC>*>(rows + (long)row * side.row_stride + col * VEC);
+    };
+    auto to = [&](int i) { return codes + (long)off * hd + (long)(i * size_g + lane_g) * VEC; };
 
-    if (quads) {
-      const int per_row = hd >> 2, vecs = n * per_row;
-      float v[kRegVecs][4];
-      float most = 0.f;
-      const bool kept = vecs <= kRegVecs * size_g;
-      if (kept) {
+    Pack<T, VEC> kept[kKept];
+    float most = 0.f;
+    const bool once = loads <= kKept * size_g;
+    if (once) {
 #pragma unroll
-        for (int i = 0; i < kRegVecs; ++i) {
-          const int e = i * size_g + lane_g;
-          if (e < vecs) load4(rows + (long)(e / per_row) * side.row_stride + (e % per_row) * 4, wide, v[i]);
-        }
+      for (int i = 0; i < kKept; ++i)
+        if (i * size_g + lane_g < loads) kept[i] = load(i);
 #pragma unroll
-        for (int i = 0; i < kRegVecs; ++i)
-          if (i * size_g + lane_g < vecs) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) most = fmaxf(most, finite_abs(v[i][j]));
-          }
-      } else {
-        for (int e = lane_g; e < vecs; e += size_g) {
-          float w[4];
-          load4(rows + (long)(e / per_row) * side.row_stride + (e % per_row) * 4, wide, w);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) most = fmaxf(most, finite_abs(w[j]));
-        }
-      }
-      most = warp_max(most);
-      if (warps > 1) {
-        __syncthreads();
-        if (lane == 0) most_s[warp] = most;
-        __syncthreads();
-        for (int i = 0; i < warps; ++i) most = fmaxf(most, most_s[i]);
-      }
-      const float now = fmaxf(older, q8_scale(most)), inv = 1.0f / now;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(codes + (long)off * hd);
-      if (kept) {
-#pragma unroll
-        for (int i = 0; i < kRegVecs; ++i) {
-          const int e = i * size_g + lane_g;
-          if (e < vecs) dst[e] = q8_codes4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-        }
-      } else {
-        for (int e = lane_g; e < vecs; e += size_g) {
-          float w[4];
-          load4(rows + (long)(e / per_row) * side.row_stride + (e % per_row) * 4, wide, w);
-          dst[e] = q8_codes4(w[0] * inv, w[1] * inv, w[2] * inv, w[3] * inv);
-        }
-      }
-      if (off && now != older) {
-        uint32_t* old = reinterpret_cast<uint32_t*>(codes);
-        const float by = older * inv;
-        for (int e = lane_g; e < off * per_row; e += size_g) {
-          const float2 a = q8_float2(old[e] & 0xffffu), b = q8_float2(old[e] >> 16);
-          old[e] = q8_codes4(a.x * by, a.y * by, b.x * by, b.y * by);
-        }
-      }
-      if (lane_g == 0 && !(off && now == older)) *scale = now;
-    } else {      // sizes that are no multiple of four: number by number
-      float most = 0.f;
-      for (int e = lane_g; e < n * hd; e += size_g) most = fmaxf(most, finite_abs(to_f32(rows[(long)(e / hd) * side.row_stride + e % hd])));
-      most = warp_max(most);
-      if (warps > 1) {
-        __syncthreads();
-        if (lane == 0) most_s[warp] = most;
-        __syncthreads();
-        for (int i = 0; i < warps; ++i) most = fmaxf(most, most_s[i]);
-      }
-      const float now = fmaxf(older, q8_scale(most)), inv = 1.0f / now;
-      for (int e = lane_g; e < n * hd; e += size_g)
-        codes[(long)off * hd + e] = (uint8_t)(q8_codes2(to_f32(rows[(long)(e / hd) * side.row_stride + e % hd]) * inv, 0.f) & 0xffu);
-      if (off && now != older)
-        for (int e = lane_g; e < off * hd; e += size_g) codes[e] = (uint8_t)(q8_codes2(q8_float(codes[e]) * (older * inv), 0.f) & 0xffu);
-      if (lane_g == 0 && !(off && now == older)) *scale = now;
+      for (int i = 0; i < kKept; ++i)
+        if (i * size_g + lane_g < loads) most = most_of(kept[i], most);
+    } else {
+#pragma unroll 4
+      for (int i = 0; i * size_g + lane_g < loads; ++i) most = most_of(load(i), most);
     }
+    most = warp_max(most);
+    if (warps > 1) {
+      __syncthreads();
+      if (lane == 0) most_s[warp] = most;
+      __syncthreads();
+      for (int i = 0; i < warps; ++i) most = fmaxf(most, most_s[i]);
+    }
+    const float now = fmaxf(older, q8_scale(most)), inv = 1.0f / now;
+    if (once) {
+#pragma unroll
+      for (int i = 0; i < kKept; ++i)
+        if (i * size_g + lane_g < loads) put(to(i), kept[i], inv);
+    } else {
+#pragma unroll 4
+      for (int i = 0; i * size_g + lane_g < loads; ++i) put(to(i), load(i), inv);
+    }
+    if (off && now == older) continue;
+    if (off) {                                        // the page's older codes follow its scale
+      const float by = older * inv;
+      for (int e = lane_g; e < off * hd; e += size_g) {
+        if constexpr (VEC == 1) {
+          codes[e] = (uint8_t)q8_codes2(q8_float(codes[e]) * by, 0.f);
+        } else {
+          if (e * 4 >= off * hd) break;
+          uint32_t* w = reinterpret_cast<uint32_t*>(codes) + e;
+          const float2 a = q8_float2(*w & 0xffffu), b = q8_float2(*w >> 16);
+          *w = q8_codes4(a.x * by, a.y * by, b.x * by, b.y * by);
+        }
+      }
+    }
+    if (lane_g == 0) *scale = now;
   }
+}
+
+template <typename T>
+int launch_store(const StoreSide& k, const StoreSide& v, const int* slot_mapping, int tokens, int nkv, int page_size, long places, cudaStream_t s) {
+  constexpr int VEC = 16 / sizeof(T);
+  bool wide = true;
+  for (const StoreSide* x : {&k, &v}) wide = wide && x->width % VEC == 0 && x->row_stride % VEC == 0 && (uintptr_t)x->x % 16 == 0 && (uintptr_t)x->cache % 8 == 0;
+  const int chunk = tokens <= 512 ? 1 : 16;
+  int warps = 1;
+  while (warps < 8 && (long)warps * 2048 < (long)page_size * (k.width > v.width ? k.width : v.width)) warps *= 2;
+  const long groups = (long)((tokens + chunk - 1) / chunk) * nkv * 2;
+  const int threads = warps == 1 ? 128 : warps * 32;
+  const long blocks = warps == 1 ? (groups + 3) / 4 : groups;
+  if (blocks > 0x7fffffffL) return ARLE_E_UNSUPPORTED;
+  launch_kernel(wide ? store_q8_kernel<T, VEC> : store_q8_kernel<T, 1>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, k, v, slot_mapping, tokens, chunk, nkv,
+                page_size, places, warps, groups);
+  return launch_status();
 }
 
 // expand: the keys and values that rows with at least `least` queries see, as bfloat16 pages of 64 tokens [pages, nkv, 64, width] with a block table of
@@ -264,22 +274,9 @@ ARLE_API int arle_store_q8(const void* k, int k_stride, const void* v, int v_str
   if (nkv <= 0 || hd <= 0 || vd <= 0 || page_size <= 0 || hd > 256 || vd > 256) return ARLE_E_UNSUPPORTED;
   if (pages * page_size > 0x7fffffffL) return ARLE_E_UNSUPPORTED;      // places are 32-bit
   const StoreSide ks{k, k_stride, hd, (uint8_t*)k_cache, k_scale}, vs{v, v_stride, vd, (uint8_t*)v_cache, v_scale};
-  const int chunk = tokens <= 512 ? 1 : 4;
-  int warps = 1;
-  while (warps < 8 && (long)warps * 2048 < (long)page_size * (hd > vd ? hd : vd)) warps *= 2;
-  const long groups = (long)((tokens + chunk - 1) / chunk) * nkv * 2;
-  const int threads = warps == 1 ? 128 : warps * 32;
-  const long blocks = warps == 1 ? (groups + 3) / 4 : groups;
-  if (blocks > 0x7fffffffL) return ARLE_E_UNSUPPORTED;
-  if (dtype == 0)
-    launch_kernel(store_q8_kernel<float>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, ks, vs, slot_mapping, tokens, chunk, nkv, page_size, pages * page_size,
-                  warps, groups);
-  else if (dtype == 1)
-    launch_kernel(store_q8_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, ks, vs, slot_mapping, tokens, chunk, nkv, page_size,
-                  pages * page_size, warps, groups);
-  else
-    return ARLE_E_BADARG;
-  return launch_status();
+  if (dtype == 0) return launch_store<float>(ks, vs, slot_mapping, tokens, nkv, page_size, pages * page_size, s);
+  if (dtype == 1) return launch_store<__nv_bfloat16>(ks, vs, slot_mapping, tokens, nkv, page_size, pages * page_size, s);
+  return ARLE_E_BADARG;
 }
 
 // pages: the sum over the rows of the pages of 64 that they see (fewer blocks run than asked for if it is less).  Outputs as above; table_out

@@ -25,10 +25,13 @@ __device__ __forceinline__ uint32_t q8_codes2(float lo, float hi) { return __nv_
 
 __device__ __forceinline__ uint32_t q8_codes4(float a, float b, float c, float d) { return q8_codes2(a, b) | (q8_codes2(c, d) << 16); }
 
-// Two codes (the low 16 bits) as float16 numbers, exactly.
-__device__ __forceinline__ uint32_t q8_half2(uint32_t codes) {
+// Four codes as float16 numbers, exactly: the first two and the last two.
+__device__ __forceinline__ void q8_half4(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;}\n" : "=r"(lo), "=r"(hi) : "r"(codes));
+}
+__device__ __forceinline__ uint32_t q8_half2(uint32_t codes) {      // the low 16 bits
   uint32_t r;
-  asm("{.reg .b16 lo;\n cvt.u16.u32 lo, %1;\n cvt.rn.f16x2.e4m3x2 %0, lo;}\n" : "=r"(r) : "r"(codes));
+  asm("{.reg .b16 a, b;\n mov.b32 {a, b}, %1;\n cvt.rn.f16x2.e4m3x2 %0, a;}\n" : "=r"(r) : "r"(codes));
   return r;
 }
 

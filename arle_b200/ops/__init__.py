@@ -2293,17 +2293,23 @@ def token_shift(h, mu, state, q_indptr, row_of_token, state_slots, out, max_q_le
 _E4M3 = torch.float8_e4m3fn
 
 
-def _q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, vd: int, page_size: int) -> None:
-    if k_cache.dtype != _E4M3 or v_cache.dtype != _E4M3:
-        raise KernelError(f"{what}: the caches hold float8_e4m3fn codes, got {k_cache.dtype} and {v_cache.dtype}")
-    pages = k_cache.shape[0]
-    if (tuple(k_cache.shape) != (pages, nkv, page_size, hd) or tuple(v_cache.shape) != (pages, nkv, page_size, vd) or not k_cache.is_contiguous()
-            or not v_cache.is_contiguous()):
-        raise KernelError(f"{what}: cache shapes {tuple(k_cache.shape)}, {tuple(v_cache.shape)} are not contiguous [pages, {nkv}, {page_size}, {hd}] and "
-                          f"[pages, {nkv}, {page_size}, {vd}]")
-    for s in (k_scale, v_scale):
-        if s.dtype != torch.float32 or tuple(s.shape) != (pages, nkv) or not s.is_contiguous():
-            raise KernelError(f"{what}: scales must be contiguous float32 [pages, {nkv}]")
+def _q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, vd: int, page_size: int) -> int:
+    # these run before every launch of a step: one comparison for what is in order, the reason only where something is not
+    k_shape, f32 = k_cache.shape, torch.float32
+    pages = k_shape[0]
+    if (k_cache.dtype is _E4M3 and v_cache.dtype is _E4M3 and k_scale.dtype is f32 and v_scale.dtype is f32 and k_shape == (pages, nkv, page_size, hd)
+            and (v_cache.shape == k_shape if vd == hd else v_cache.shape == (pages, nkv, page_size, vd)) and k_scale.shape == (pages, nkv)
+            and v_scale.shape == (pages, nkv) and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        return pages
+    raise KernelError(f"{what}: caches must be contiguous float8_e4m3fn [pages, {nkv}, {page_size}, {hd}] and [pages, {nkv}, {page_size}, {vd}] and scales contiguous "
+                      f"float32 [pages, {nkv}]; got {k_cache.dtype} {tuple(k_cache.shape)}, {v_cache.dtype} {tuple(v_cache.shape)}, {k_scale.dtype} "
+                      f"{tuple(k_scale.shape)}, {v_scale.dtype} {tuple(v_scale.shape)}")
+
+
+def _on_cuda(what: str, *tensors) -> None:
+    for t in tensors:
+        if not t.is_cuda:
+            raise KernelError(f"{what}: a tensor is on {t.device}: arle_b200 kernels run on CUDA devices only (there is no CPU path)")
 
 
 def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
@@ -2319,16 +2325,19 @@ def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, h
     scale, NaN stays NaN; neither counts for the scale.  A step's tokens of one page stand in consecutive rows, in the order of their places, as an engine's do."""
     vd = hd if vd is None else int(vd)
     T = slot_mapping.numel()
-    if k.shape != (T, nkv * hd) or v.shape != (T, nkv * vd) or k.dtype != v.dtype or (T and (k.stride(1) != 1 or v.stride(1) != 1)):
-        raise KernelError("store_q8: k must be [T, nkv*hd] and v [T, nkv*vd] of one type, with unit inner stride")
-    _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
-    if not slot_mapping.is_contiguous():
-        raise KernelError("store_q8: slot_mapping must be contiguous")
-    _i32(slot_mapping, "slot_mapping")
+    if k.shape != (T, nkv * hd) or v.shape != (T, nkv * vd) or k.dtype is not v.dtype:
+        raise KernelError("store_q8: k must be [T, nkv*hd] and v [T, nkv*vd] of one type")
+    (k_stride, k_unit), (v_stride, v_unit) = k.stride(), v.stride()
+    if T and (k_unit != 1 or v_unit != 1):
+        raise KernelError("store_q8: rows of k and v must have unit inner stride")
+    pages = _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
+    if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
+        raise KernelError("store_q8: slot_mapping must be contiguous int32")
+    _on_cuda("store_q8", k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale)
     if T == 0:
         return
-    _check(library().arle_store_q8(_ptr(k), k.stride(0), _ptr(v), v.stride(0), _dt(k), _ptr(slot_mapping), T, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
-                                   _ptr(v_scale), k_cache.shape[0], nkv, hd, vd, page_size, _stream()), "store_q8")
+    _check(library().arle_store_q8(k.data_ptr(), k_stride, v.data_ptr(), v_stride, _dt(k), slot_mapping.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
+                                   k_scale.data_ptr(), v_scale.data_ptr(), pages, nkv, hd, vd, page_size, _stream()), "store_q8")
 
 
 # Bytes of bfloat16 keys and values that prompt portions are expanded into at a time; rows that see more go by themselves.
@@ -2343,39 +2352,41 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
     bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens read the codes as they are; the keys and values that
     portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels."""
-    T = q.shape[0]
-    vd = hd if vd is None else int(vd)
-    if q.stride(1) != 1 or q.shape[1] != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
+    (T, width), (q_stride, q_unit), vd = q.shape, q.stride(), hd if vd is None else int(vd)
+    if q_unit != 1 or width != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
         raise KernelError("paged_attention_q8: q must be [T, nq*hd] with unit inner stride and out contiguous [T, nq*vd]")
-    if out.dtype != q.dtype:
+    if out.dtype is not q.dtype:
         raise KernelError("paged_attention_q8: q and out must share a type")
     if hd > 256 or vd > 256 or nq % nkv:
         raise KernelError(f"paged_attention_q8: head_dim {hd} / value width {vd} / heads {nq}:{nkv} not supported")
     _q8_cache("paged_attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
-    _i32(positions, "positions"), _i32(row_of_token, "row_of_token"), _i32(block_table, "block_table")
-    if block_table.stride(1) != 1:
-        raise KernelError("paged_attention_q8: block table rows must be contiguous")
+    i32, (bt_stride, bt_unit) = torch.int32, block_table.stride()
+    if positions.dtype is not i32 or row_of_token.dtype is not i32 or block_table.dtype is not i32 or bt_unit != 1:
+        raise KernelError("paged_attention_q8: positions, row_of_token and block_table must be int32, rows of the block table contiguous")
+    sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, int(window) if window else 0
+    _on_cuda("paged_attention_q8", q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table)
     if T == 0:
         return
-    sinks, w = _sinks(sink, nq, q.device), int(window) if window else 0
-    if (batch is not None and _KERNEL_SET == "fast" and vd == hd and fast_attention_supported(q, nq, nkv, hd)
-            and k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0):
-        R = batch.num_rows
+    qp, kp, vp, op, lib = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), library()
+    # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
+    if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
+            and not (qp | kp | vp | op) % 16):
         if batch.max_q_len > 1:
             _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0:
-            ctas = 3 * sm_count(q.device)
-            part_o = batch.ws.get("attn_q8_part_o", (ctas * 2 * 16 * hd,), torch.float32)
-            part_ml = batch.ws.get("attn_q8_part_ml", (ctas * 2 * 16 * 2,), torch.float32)
-            counters = batch.ws.get_zeroed("attn_q8_counters", (R * nkv,), torch.int32)
-            _check(library().arle_attention_q8_decode(
-                _ptr(q), q.stride(0), _ptr(out), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(batch.q_indptr), _ptr(batch.kv_lens),
-                _ptr(block_table), block_table.stride(0), _ptr(part_o), _ptr(part_ml), _ptr(counters), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks), R, ctas,
-                _stream()), "attention_q8_decode")
+            # scratch: two pieces of a (row, kv head) for each CTA, their sums and then their maxima and totals
+            ctas = 3 * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
+            parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
+            counters = batch.ws.get_zeroed("attn_q8_counters", (batch.num_rows * nkv,), torch.int32)
+            at = parts.data_ptr()
+            _check(lib.arle_attention_q8_decode(
+                qp, q_stride, op, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(),
+                block_table.data_ptr(), bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
+                batch.num_rows, ctas, _stream()), "attention_q8_decode")
         return
-    _check(library().arle_attention_q8(
-        _ptr(q), q.stride(0), _ptr(out), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(positions), _ptr(row_of_token),
-        _ptr(block_table), block_table.stride(0), nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
+    _check(lib.arle_attention_q8(
+        qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
+        block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
 def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks) -> None:
@@ -2418,16 +2429,18 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
     cache.  Such a step leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
     R, T = slots.numel(), positions.numel()
-    for t, name in ((slots, "slots"), (starts, "starts"), (q_lens, "q_lens"), (new_pages, "new_pages"), (page_table, "page_table"), (q_indptr, "q_indptr"),
-                    (kv_lens, "kv_lens"), (positions, "positions"), (row_of_token, "row_of_token"), (slot_of_token, "slot_of_token"),
-                    (slot_mapping, "slot_mapping"), (block_table, "block_table"), (status, "status")):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise KernelError(f"step_tables: {name} must be contiguous int32")
+    every = (slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table, status)
+    i32 = torch.int32
+    for t in every:
+        if t.dtype is not i32 or not t.is_contiguous() or not t.is_cuda:
+            _on_cuda("step_tables", *every)
+            raise KernelError(f"step_tables: every tensor must be contiguous int32, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
     if (starts.numel() != R or q_lens.numel() != R or q_indptr.numel() != R + 1 or kv_lens.numel() != R or row_of_token.numel() != T or slot_of_token.numel() != T
             or slot_mapping.numel() != T or status.numel() != 1 or block_table.dim() != 2 or block_table.shape[0] != R or page_table.dim() != 2):
         raise KernelError("step_tables: slots, starts, q_lens and kv_lens are [R], q_indptr [R + 1], the tokens' tables [T], block_table [R, width], "
                           "page_table [slots, pages], status [1]")
+    max_slots, table_width = page_table.shape
     _check(library().arle_step_tables(
-        _ptr(slots), _ptr(starts), _ptr(q_lens), R, _ptr(new_pages), new_pages.numel(), _ptr(page_table), page_table.shape[0], page_table.shape[1], int(num_pages),
-        int(page_size), _ptr(q_indptr), _ptr(kv_lens), _ptr(positions), _ptr(row_of_token), _ptr(slot_of_token), _ptr(slot_mapping), T, _ptr(block_table),
-        block_table.shape[1], _ptr(status), _stream()), "step_tables")
+        slots.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), R, new_pages.data_ptr(), new_pages.numel(), page_table.data_ptr(), max_slots, table_width, int(num_pages),
+        int(page_size), q_indptr.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(), slot_of_token.data_ptr(), slot_mapping.data_ptr(), T,
+        block_table.data_ptr(), block_table.shape[1], status.data_ptr(), _stream()), "step_tables")
