@@ -71,8 +71,9 @@ __device__ __forceinline__ int row_blocks(const DecodeArgs& a, int r) {
   return (kv + kBlock - 1) / kBlock - first_visible_key(kv - 1, a.window, 0) / kBlock;
 }
 
-template <int HD> struct Shape {
-  static constexpr int kStages = HD == 128 ? 4 : 6;
+template <int HD, int NT> struct Shape {
+  static constexpr int kResident = NT == 1 ? 4 : 3;      // CTAs of an SM: 128 and 168 registers a thread
+  static constexpr int kStages = HD == 128 ? (NT == 1 ? 3 : 4) : (NT == 1 ? 5 : 6);
   static constexpr int kStageBytes = 2 * kTile * HD;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kScales = kWarps * kStages * 32 * 4;
@@ -82,10 +83,10 @@ template <int HD> struct Shape {
 
 // NT: query heads of a kv head in eights.  P16: pages of a multiple of 16 tokens, so that a tile lies in one page.
 template <int HD, int NT, bool P16>
-__global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_kernel(DecodeArgs a) {
   pdl_launch_dependents();
   pdl_wait();
-  using S = Shape<HD>;
+  using S = Shape<HD, NT>;
   constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
   extern __shared__ __align__(128) unsigned char smem[];
@@ -433,31 +434,46 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
     if (!whole) {
       // the pieces of this pair: of CTA first_cta (its last piece, unless the pair begins with its share) up to last_cta (their first pieces)
       const int first_cta = pair_at / share, last_cta = (pair_at + nb - 1) / share, pieces = last_cta - first_cta + 1;
-      __threadfence();
       __syncthreads();
       if (tid == 0) {
+        __threadfence();
         int* counter = a.counters + row * nkv + h;
         last_s = atomicAdd(counter, 1) == pieces - 1;
-        if (last_s) *counter = 0;
+        if (last_s) {
+          *counter = 0;
+          __threadfence();
+        }
       }
       __syncthreads();
       if (last_s) {
-        __threadfence();
         const size_t slot0 = (size_t)first_cta * 2 + (pair_at == first_cta * share ? 0 : 1);
         for (int i = tid; i < G * HD; i += kThreads) {
           const int query = i / HD, d = i % HD;
-          auto piece = [&](int k) { return (k == 0 ? slot0 : (size_t)(first_cta + k) * 2) * 16 + query; };
-          float M = -INFINITY;
-#pragma unroll 8
-          for (int k = 0; k < pieces; ++k) M = fmaxf(M, __ldcg(a.part_ml + piece(k) * 2));
-          const float top_s = M == -INFINITY ? 0.f : M;
-          float L = a.sinks ? exp2f(a.sinks[h * G + query] * 1.4426950408889634f - top_s) : 0.f, O = 0.f;
-#pragma unroll 8
-          for (int k = 0; k < pieces; ++k) {
-            const float f = exp2f(__ldcg(a.part_ml + piece(k) * 2) - top_s);
-            L += __ldcg(a.part_ml + piece(k) * 2 + 1) * f;
-            O += __ldcg(a.part_o + piece(k) * HD + d) * f;
+          float M = -INFINITY, L = 0.f, O = 0.f;
+          for (int k0 = 0; k0 < pieces; k0 += 8) {      // eight pieces' numbers under way at once
+            float2 ml[8];
+            float po[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const size_t at = (k0 + k == 0 ? slot0 : (size_t)(first_cta + k0 + k) * 2) * 16 + query;
+              ml[k] = k0 + k < pieces ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at) : make_float2(-INFINITY, 0.f);
+              po[k] = k0 + k < pieces ? __ldcg(a.part_o + at * HD + d) : 0.f;
+            }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+            const float top_s = top == -INFINITY ? 0.f : top, was = exp2_fast(M - top_s);
+            L *= was;
+            O *= was;
+            M = top;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float f = exp2_fast(ml[k].x - top_s);
+              L += ml[k].y * f;
+              O += po[k] * f;
+            }
           }
+          if (a.sinks) L += exp2f(a.sinks[h * G + query] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
           a.out[((size_t)t * a.nq + h * G + query) * HD + d] = __float2bfloat16_rn(O / L);
         }
       }
@@ -469,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 3) q8_decode_kernel(DecodeArgs a) {
 
 template <int HD, int NT, bool P16>
 int launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
-  using S = Shape<HD>;
+  using S = Shape<HD, NT>;
   constexpr size_t merge = (size_t)kWarps * NT * 8 * S::kPitch * 4;
   constexpr size_t smem = S::kSmem > merge ? S::kSmem : merge;
   static SharedLimit limit;

@@ -2374,8 +2374,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         if batch.max_q_len > 1:
             _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0:
-            # scratch: two pieces of a (row, kv head) for each CTA, their sums and then their maxima and totals
-            ctas = 3 * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
+            # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
+            ctas = (4 if nq <= 8 * nkv else 3) * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
             parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
             counters = batch.ws.get_zeroed("attn_q8_counters", (batch.num_rows * nkv,), torch.int32)
             at = parts.data_ptr()
