@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
   constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int sum_s[kWarps + 1], start_s[3], last_s;
+  __shared__ int sum_s[kWarps], start_s[2], cut_s[2], last_s;
   __shared__ float ml_s[kWarps][NT * 8][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = a.nq / a.nkv, nkv = a.nkv;
@@ -123,21 +123,40 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
     total += sum_s[w];
   }
   total *= nkv;
-  const int share = (total + gridDim.x - 1) / gridDim.x;
-  const int begin = blockIdx.x * share, end = min(begin + share, total);
-  if (begin >= end) return;
-  if (begin >= front * nkv && begin < (front + mine) * nkv) {
-    int r = r0, at = front * nkv;
-    for (;; ++r) {
-      const int n = row_blocks(a, r) * nkv;
-      if (begin < at + n) break;
-      at += n;
+  // Cuts of the line: every `share` blocks, moved to the end, or else to the start, of the pair that they fall into where that is at most `slack` blocks
+  // away: a piece costs as much as about two blocks beside its keys (its first tiles' latency and the joining), and pairs shorter than a share stay whole.
+  const int share = (total + gridDim.x - 1) / gridDim.x, slack = min(3, (share + 1) / 2);
+  if ((int)blockIdx.x * share >= total) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int at = ((int)blockIdx.x + i) * share;
+    if (at >= total) {
+      if (tid == 0) cut_s[i] = total;
+    } else if (at >= front * nkv && at < (front + mine) * nkv) {
+      int r = r0, row_at = front * nkv, nb = row_blocks(a, r);
+      while (at >= row_at + nb * nkv) {
+        row_at += nb * nkv;
+        nb = row_blocks(a, ++r);
+      }
+      const int from = (at - row_at) % nb, left = nb - from;
+      cut_s[i] = from == 0 ? at : left <= slack ? at + left : from <= slack ? at - from : at;
+      if (i == 0) {
+        start_s[0] = r;
+        start_s[1] = row_at;
+      }
     }
-    start_s[0] = r;
-    start_s[1] = at;
   }
   __syncthreads();
+  const int begin = cut_s[0], end = cut_s[1];
+  if (begin >= end) return;
   int row = start_s[0], row_at = start_s[1];      // the row and where its blocks begin on the line
+
+  auto finish = [&](int t, int head, int d, float M, float L, const float4& O) {
+    if (a.sinks) L += exp2f(a.sinks[head] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(O.x / L, O.y / L), hi = __floats2bfloat162_rn(O.z / L, O.w / L);
+    *reinterpret_cast<uint2*>(a.out + ((size_t)t * a.nq + head) * HD + d) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  };
 
   for (int pos = begin; pos < end;) {
     int nb = row_blocks(a, row);
@@ -406,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
     }
     __syncthreads();
     const bool whole = blk0 == 0 && blk1 == nb;
-    const size_t slot = (size_t)blockIdx.x * 2 + (pos == begin ? 0 : 1);
+    const size_t slot = (size_t)blockIdx.x * 2 + (blk0 == 0);      // a CTA has one cut pair's start and one cut pair's further part at most
     for (int i = tid; i < G * HD; i += kThreads) {
       const int query = i / HD, d = i % HD;
       float M = -INFINITY;
@@ -432,8 +451,8 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
       }
     }
     if (!whole) {
-      // the pieces of this pair: of CTA first_cta (its last piece, unless the pair begins with its share) up to last_cta (their first pieces)
-      const int first_cta = pair_at / share, last_cta = (pair_at + nb - 1) / share, pieces = last_cta - first_cta + 1;
+      // the cuts inside this pair are those farther than `slack` from both of its ends; the piece in front of cut k belongs to CTA k - 1
+      const int cut0 = (pair_at + slack) / share + 1, cut1 = (pair_at + nb - slack - 1) / share, pieces = cut1 - cut0 + 2, first_cta = cut0 - 1;
       __syncthreads();
       if (tid == 0) {
         __threadfence();
@@ -446,35 +465,59 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
       }
       __syncthreads();
       if (last_s) {
-        const size_t slot0 = (size_t)first_cta * 2 + (pair_at == first_cta * share ? 0 : 1);
-        for (int i = tid; i < G * HD; i += kThreads) {
-          const int query = i / HD, d = i % HD;
-          float M = -INFINITY, L = 0.f, O = 0.f;
-          for (int k0 = 0; k0 < pieces; k0 += 8) {      // eight pieces' numbers under way at once
+        // four numbers a thread; where there are fewer such quads than threads, `sets` of threads take every sets-th piece of a quad and add up their sums
+        const int quads = G * (HD / 4), sets = max(1, min(8, kThreads / quads)), set = tid / quads;
+        float4* so = reinterpret_cast<float4*>(smem);
+        float2* sml = reinterpret_cast<float2*>(smem + kThreads * 16);
+        for (int i = sets > 1 ? tid - set * quads : tid; i < quads; i += kThreads) {
+          const int query = i / (HD / 4), d = i % (HD / 4) * 4;
+          float M = -INFINITY, L = 0.f;
+          float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k0 = sets > 1 ? set : 0; k0 < (set < sets || sets == 1 ? pieces : 0); k0 += 8 * sets) {      // eight pieces' numbers under way at once
             float2 ml[8];
-            float po[8];
+            float4 po[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const size_t at = (k0 + k == 0 ? slot0 : (size_t)(first_cta + k0 + k) * 2) * 16 + query;
-              ml[k] = k0 + k < pieces ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at) : make_float2(-INFINITY, 0.f);
-              po[k] = k0 + k < pieces ? __ldcg(a.part_o + at * HD + d) : 0.f;
+              const int piece = k0 + k * sets;
+              const size_t at = ((size_t)(first_cta + piece) * 2 + (piece == 0)) * 16 + query;
+              ml[k] = piece < pieces ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at) : make_float2(-INFINITY, 0.f);
+              po[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float top = M;
 #pragma unroll
             for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
             const float top_s = top == -INFINITY ? 0.f : top, was = exp2_fast(M - top_s);
             L *= was;
-            O *= was;
+            O = make_float4(O.x * was, O.y * was, O.z * was, O.w * was);
             M = top;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float f = exp2_fast(ml[k].x - top_s);
               L += ml[k].y * f;
-              O += po[k] * f;
+              O = make_float4(O.x + po[k].x * f, O.y + po[k].y * f, O.z + po[k].z * f, O.w + po[k].w * f);
             }
           }
-          if (a.sinks) L += exp2f(a.sinks[h * G + query] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
-          a.out[((size_t)t * a.nq + h * G + query) * HD + d] = __float2bfloat16_rn(O / L);
+          if (sets > 1) {
+            so[tid] = O;
+            sml[tid] = make_float2(M, L);
+            continue;
+          }
+          finish(t, h * G + query, d, M, L, O);
+        }
+        if (sets > 1) {
+          __syncthreads();
+          for (int i = tid; i < quads; i += kThreads) {
+            float M = -INFINITY, L = 0.f;
+            float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int k = 0; k < sets; ++k) M = fmaxf(M, sml[k * quads + i].x);
+            for (int k = 0; k < sets; ++k) {
+              const float f = exp2_fast(sml[k * quads + i].x - (M == -INFINITY ? 0.f : M));
+              const float4 x = so[k * quads + i];
+              L += sml[k * quads + i].y * f;
+              O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
+            }
+            finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, O);
+          }
         }
       }
     }
