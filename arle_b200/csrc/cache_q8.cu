@@ -6,7 +6,8 @@
 //     s' = s(a) for a run from offset 0, else max(s, s(a));   codes in front of the run: rne(code * s / s');   new codes: rne(x / s')
 // One group of `warps` warps owns a run of one head of the keys or the values, so the page's scale and older codes are read and written by one owner.
 // A page of up to 2,048 numbers a warp stays in registers between the maximum and the rounding (one read of x); what is larger is read again (from L2).
-// The kernel is bound by the latency of its three dependent reads (place, numbers, stores) for decoded tokens and by DRAM for prompts.
+// Decoded tokens are bound by the latency of three dependent accesses (place, numbers, codes): 2.2 us for one token, 2.3 us for 64.  Prompts come near
+// DRAM's rate: 15,000 tokens of 8 heads of 128 in 20.7 us, 4.7 TB/s; what is left is instructions (five for two numbers in the rounding alone).
 #include "q8.cuh"
 using namespace arle;
 
@@ -15,6 +16,7 @@ namespace {
 struct StoreSide {
   const void* x;
   int row_stride, width;
+  int per_row, row_step;      // loads of a row; rows between a lane's loads, 0 where it does not keep its column
   uint8_t* cache;
   float* scale;
 };
@@ -24,8 +26,35 @@ __device__ __forceinline__ float finite_abs(float v) {
   return a <= 3.4028234663852886e38f ? a : 0.f;      // neither infinities nor NaN
 }
 
+__device__ __forceinline__ float reciprocal(float s) {      // exactly, of a power of two
+  const uint32_t b = __float_as_uint(s);
+  return (b & 0x7fffffu) == 0 && b >= (1u << 23) && b < (254u << 23) ? __uint_as_float((254u << 23) - b) : 1.0f / s;
+}
+
+// The largest |x| of the loads taken in, of the finite ones.  Bits of numbers without their signs are in the order of the numbers, so the maximum is taken
+// over whole words (two bfloat16 at a time); where it comes out as an infinity or a NaN the loads are gone through once more.
 template <typename T, int VEC>
-__device__ __forceinline__ float most_of(const Pack<T, VEC>& p, float most) {
+struct Most {
+  uint32_t bits = 0;
+  __device__ __forceinline__ void take(const Pack<T, VEC>& p) {
+    if constexpr (VEC == 1) {
+      bits = max(bits, __float_as_uint(finite_abs(to_f32(p.e[0]))));
+    } else {
+      const uint4 w = *reinterpret_cast<const uint4*>(&p);
+      if constexpr (sizeof(T) == 2)
+        bits = __vmaxu2(__vmaxu2(bits, __vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu)), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+      else
+        bits = max(max(bits, max(w.x & 0x7fffffffu, w.y & 0x7fffffffu)), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
+    }
+  }
+  __device__ __forceinline__ float value() const {
+    if constexpr (VEC > 1 && sizeof(T) == 2) return __uint_as_float(max(bits & 0xffffu, bits >> 16) << 16);
+    else return __uint_as_float(bits);
+  }
+};
+template <typename T, int VEC>
+__device__ __forceinline__ float finite_of(const Pack<T, VEC>& p) {
+  float most = 0.f;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) most = fmaxf(most, finite_abs(to_f32(p.e[j])));
   return most;
@@ -45,22 +74,23 @@ __device__ __forceinline__ void put(uint8_t* dst, const Pack<T, VEC>& p, float i
   }
 }
 
-// A group has `warps` warps.  `chunk`: tokens among which a group looks for the starts of runs (at most 32).  VEC: numbers of a load, 16 bytes or one.
+// A group has `warps` warps; where it has one, a block's warps take neighbouring heads (of the keys, then of the values).  `chunk`: tokens among which a
+// group looks for the starts of runs (at most 31).  VEC: numbers of a load, 16 bytes or one.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restrict__ slot_mapping, int tokens, int chunk, int nkv, int page_size,
-                                                       long places, int warps, long groups) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restrict__ slot_mapping, int tokens, int chunk,
+                                                                               int nkv, int page_size, int places, int warps) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int kKept = VEC == 1 ? 1 : 64 / VEC;      // loads a lane keeps: 64 numbers
   __shared__ float most_s[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lane_g = warps == 1 ? lane : threadIdx.x, size_g = warps * 32;
-  const long group = warps == 1 ? (long)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
-  if (group >= groups) return;
-  const StoreSide& side = (group & 1) ? vs : ks;
-  const int head = (int)((group >> 1) % nkv), t0 = (int)((group >> 1) / nkv) * chunk;
+  const int unit = warps == 1 ? blockIdx.y * (blockDim.x >> 5) + warp : blockIdx.y;
+  if (unit >= 2 * nkv) return;
+  const StoreSide& side = unit < nkv ? ks : vs;
+  const int head = unit < nkv ? unit : unit - nkv, t0 = blockIdx.x * chunk;
   const int hd = side.width;
-  const T* x = reinterpret_cast<const T*>(side.x) + (long)head * hd;
+  const T* x = reinterpret_cast<const T*>(side.x) + head * hd;
 
   // places of the chunk's tokens and of those behind it, one a lane
   const int s = t0 + lane < tokens ? slot_mapping[t0 + lane] : -1;
@@ -70,9 +100,64 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) store_q8_kernel(S
   const bool first = held && (s % page_size == 0 || before != s - 1 || t0 + lane == 0);
   const unsigned goes_on = __ballot_sync(0xffffffffu, held && !first);
   unsigned starts = __ballot_sync(0xffffffffu, first && lane < chunk);
-  const int per_row = hd / VEC;                       // loads of a row
-  const bool even = size_g % per_row == 0;            // a lane keeps its column
-  const int row0 = lane_g / per_row, col0 = lane_g - row0 * per_row, row_step = size_g / per_row;
+  const int per_row = side.per_row, row_step = side.row_step;
+
+  auto rescale = [&](uint8_t* codes, int numbers, float by, int at, int step) {      // a page's older codes follow its scale
+    if constexpr (VEC == 1) {
+      for (int e = at; e < numbers; e += step) codes[e] = (uint8_t)q8_codes2(q8_float(codes[e]) * by, 0.f);
+    } else {
+      for (int e = at * 4; e < numbers; e += step * 4) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(codes + e);
+        const float2 a = q8_float2(*w & 0xffffu), b = q8_float2(*w >> 16);
+        *w = q8_codes4(a.x * by, a.y * by, b.x * by, b.y * by);
+      }
+    }
+  };
+
+  // runs of one token: eight lanes each
+  const unsigned single = starts & ~(goes_on >> 1) & 0x7fffffffu;      // (what follows token 31 is not known here)
+  starts &= ~single;
+  for (int i0 = 0; single && i0 < chunk; i0 += size_g / 8) {
+    const int i = i0 + lane_g / 8, sub = lane_g % 8;
+    const bool mine = i < chunk && ((single >> i) & 1u);
+    if (!__any_sync(0xffffffffu, mine)) continue;
+    const int place = __shfl_sync(0xffffffffu, s, min(i, 31));
+    const int page = mine ? place / page_size : 0, off = mine ? place - page * page_size : 0;
+    const T* row = x + (long)(t0 + (mine ? i : 0)) * side.row_stride;
+    uint8_t* codes = side.cache + ((long)page * nkv + head) * page_size * hd;
+    float* scale = side.scale + (long)page * nkv + head;
+    const float older = mine && off ? *scale : 0.f;
+    constexpr int kRow = VEC == 1 ? 1 : 16 / VEC;       // loads of a lane that are kept: 128 numbers of a row
+    Pack<T, VEC> kept[kRow];
+    float most = 0.f;
+    if (mine) {
+      Most<T, VEC> all;
+#pragma unroll
+      for (int j = 0; j < kRow; ++j)
+        if (j * 8 + sub < per_row) kept[j] = *reinterpret_cast<const Pack<T, VEC>*>(row + (j * 8 + sub) * VEC);
+#pragma unroll
+      for (int j = 0; j < kRow; ++j)
+        if (j * 8 + sub < per_row) all.take(kept[j]);
+      for (int e = kRow * 8 + sub; e < per_row; e += 8) all.take(*reinterpret_cast<const Pack<T, VEC>*>(row + e * VEC));
+      most = all.value();
+      if (!isfinite(most)) {
+        most = 0.f;
+        for (int e = sub; e < per_row; e += 8) most = fmaxf(most, finite_of(*reinterpret_cast<const Pack<T, VEC>*>(row + e * VEC)));
+      }
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (!mine) continue;
+    const float now = fmaxf(older, q8_scale(most)), inv = reciprocal(now);
+    uint8_t* dst = codes + (long)off * hd;
+#pragma unroll
+    for (int j = 0; j < kRow; ++j)
+      if (j * 8 + sub < per_row) put(dst + (j * 8 + sub) * VEC, kept[j], inv);
+    for (int e = kRow * 8 + sub; e < per_row; e += 8) put(dst + e * VEC, *reinterpret_cast<const Pack<T, VEC>*>(row + e * VEC), inv);
+    if (off && now == older) continue;
+    if (off) rescale(codes, off * hd, older * inv, sub, 8);
+    if (sub == 0) *scale = now;
+  }
 
   while (starts) {
     const int at = __ffs(starts) - 1;
@@ -92,26 +177,37 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) store_q8_kernel(S
     float* scale = side.scale + (long)page * nkv + head;
     const float older = off ? *scale : 0.f;
     const int loads = n * per_row;
-    auto load = [&](int i) {
-      const int e = i * size_g + lane_g;
-      const int row = even ? row0 + i * row_step : e / per_row, col = even ? col0 : e - row * per_row;
-      return *reinterpret_cast<const Pack<T, VEC>*>(rows + (long)row * side.row_stride + col * VEC);
-    };
-    auto to = [&](int i) { return codes + (long)off * hd + (long)(i * size_g + lane_g) * VEC; };
-
+    uint8_t* dst = codes + (long)off * hd + lane_g * VEC;
     Pack<T, VEC> kept[kKept];
-    float most = 0.f;
-    const bool once = loads <= kKept * size_g;
+    Most<T, VEC> all;
+    auto at_load = [&](int e) { return *reinterpret_cast<const Pack<T, VEC>*>(rows + (long)(e / per_row) * side.row_stride + (e % per_row) * VEC); };
+    const bool once = row_step && loads <= kKept * size_g, full = row_step && loads == kKept * size_g;      // a whole page of 2,048 numbers a warp: no conditions
     if (once) {
+      const int row0 = lane_g / per_row, col0 = lane_g - row0 * per_row;
+      const T* src = rows + (long)row0 * side.row_stride + col0 * VEC;
+      const long step = (long)row_step * side.row_stride;
+      if (full) {
 #pragma unroll
-      for (int i = 0; i < kKept; ++i)
-        if (i * size_g + lane_g < loads) kept[i] = load(i);
+        for (int i = 0; i < kKept; ++i) kept[i] = *reinterpret_cast<const Pack<T, VEC>*>(src + i * step);
 #pragma unroll
-      for (int i = 0; i < kKept; ++i)
-        if (i * size_g + lane_g < loads) most = most_of(kept[i], most);
+        for (int i = 0; i < kKept; ++i) all.take(kept[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) {
+          kept[i] = Pack<T, VEC>{};
+          if (i * size_g + lane_g < loads) kept[i] = *reinterpret_cast<const Pack<T, VEC>*>(src + i * step);
+        }
+#pragma unroll
+        for (int i = 0; i < kKept; ++i) all.take(kept[i]);
+      }
     } else {
-#pragma unroll 4
-      for (int i = 0; i * size_g + lane_g < loads; ++i) most = most_of(load(i), most);
+#pragma unroll 2
+      for (int e = lane_g; e < loads; e += size_g) all.take(at_load(e));
+    }
+    float most = all.value();
+    if (!isfinite(most)) {
+      most = 0.f;
+      for (int e = lane_g; e < loads; e += size_g) most = fmaxf(most, finite_of(at_load(e)));
     }
     most = warp_max(most);
     if (warps > 1) {
@@ -120,47 +216,42 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) store_q8_kernel(S
       __syncthreads();
       for (int i = 0; i < warps; ++i) most = fmaxf(most, most_s[i]);
     }
-    const float now = fmaxf(older, q8_scale(most)), inv = 1.0f / now;
-    if (once) {
+    const float now = fmaxf(older, q8_scale(most)), inv = reciprocal(now);
+    if (full) {
+#pragma unroll
+      for (int i = 0; i < kKept; ++i) put(dst + i * size_g * VEC, kept[i], inv);
+    } else if (once) {
 #pragma unroll
       for (int i = 0; i < kKept; ++i)
-        if (i * size_g + lane_g < loads) put(to(i), kept[i], inv);
+        if (i * size_g + lane_g < loads) put(dst + i * size_g * VEC, kept[i], inv);
     } else {
-#pragma unroll 4
-      for (int i = 0; i * size_g + lane_g < loads; ++i) put(to(i), load(i), inv);
+#pragma unroll 2
+      for (int e = lane_g; e < loads; e += size_g) put(dst + (e - lane_g) * VEC, at_load(e), inv);
     }
     if (off && now == older) continue;
-    if (off) {                                        // the page's older codes follow its scale
-      const float by = older * inv;
-      for (int e = lane_g; e < off * hd; e += size_g) {
-        if constexpr (VEC == 1) {
-          codes[e] = (uint8_t)q8_codes2(q8_float(codes[e]) * by, 0.f);
-        } else {
-          if (e * 4 >= off * hd) break;
-          uint32_t* w = reinterpret_cast<uint32_t*>(codes) + e;
-          const float2 a = q8_float2(*w & 0xffffu), b = q8_float2(*w >> 16);
-          *w = q8_codes4(a.x * by, a.y * by, b.x * by, b.y * by);
-        }
-      }
-    }
+    if (off) rescale(codes, off * hd, older * inv, lane_g, size_g);
     if (lane_g == 0) *scale = now;
   }
 }
 
 template <typename T>
-int launch_store(const StoreSide& k, const StoreSide& v, const int* slot_mapping, int tokens, int nkv, int page_size, long places, cudaStream_t s) {
-  constexpr int VEC = 16 / sizeof(T);
+int launch_store(StoreSide k, StoreSide v, const int* slot_mapping, int tokens, int nkv, int page_size, int places, cudaStream_t s) {
   bool wide = true;
-  for (const StoreSide* x : {&k, &v}) wide = wide && x->width % VEC == 0 && x->row_stride % VEC == 0 && (uintptr_t)x->x % 16 == 0 && (uintptr_t)x->cache % 8 == 0;
-  const int chunk = tokens <= 512 ? 1 : 16;
+  for (const StoreSide* x : {&k, &v})
+    wide = wide && x->width % (16 / sizeof(T)) == 0 && x->row_stride % (16 / sizeof(T)) == 0 && (uintptr_t)x->x % 16 == 0 && (uintptr_t)x->cache % 8 == 0;
+  // Few tokens are likely to be decoded ones, a run each: four to a warp, eight lanes each.  Many are mostly prompts', whose runs are pages: with 16 to a warp
+  // a page of 16 has a warp and none looks on (15,000 tokens: 20.7 us); 16 decoded ones among them are four passes of a warp.
+  const int chunk = tokens <= 512 ? 4 : 16;
   int warps = 1;
   while (warps < 8 && (long)warps * 2048 < (long)page_size * (k.width > v.width ? k.width : v.width)) warps *= 2;
-  const long groups = (long)((tokens + chunk - 1) / chunk) * nkv * 2;
+  for (StoreSide* x : {&k, &v}) {
+    x->per_row = wide ? x->width / (int)(16 / sizeof(T)) : x->width;
+    x->row_step = warps * 32 % x->per_row ? 0 : warps * 32 / x->per_row;
+  }
   const int threads = warps == 1 ? 128 : warps * 32;
-  const long blocks = warps == 1 ? (groups + 3) / 4 : groups;
-  if (blocks > 0x7fffffffL) return ARLE_E_UNSUPPORTED;
-  launch_kernel(wide ? store_q8_kernel<T, VEC> : store_q8_kernel<T, 1>, dim3((unsigned)blocks), dim3(threads), 0, s, 1, k, v, slot_mapping, tokens, chunk, nkv,
-                page_size, places, warps, groups);
+  const dim3 grid((tokens + chunk - 1) / chunk, warps == 1 ? (2 * nkv + 3) / 4 : 2 * nkv);
+  launch_kernel(wide ? store_q8_kernel<T, 16 / sizeof(T)> : store_q8_kernel<T, 1>, grid, dim3(threads), 0, s, 1, k, v, slot_mapping, tokens, chunk, nkv, page_size,
+                places, warps);
   return launch_status();
 }
 
@@ -271,11 +362,11 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(ExpandArgs a) {
 ARLE_API int arle_store_q8(const void* k, int k_stride, const void* v, int v_stride, int dtype, const int* slot_mapping, int tokens, void* k_cache, void* v_cache,
                            float* k_scale, float* v_scale, long pages, int nkv, int hd, int vd, int page_size, cudaStream_t s) {
   if (tokens <= 0) return 0;
-  if (nkv <= 0 || hd <= 0 || vd <= 0 || page_size <= 0 || hd > 256 || vd > 256) return ARLE_E_UNSUPPORTED;
+  if (nkv <= 0 || hd <= 0 || vd <= 0 || page_size <= 0 || hd > 256 || vd > 256 || nkv > 16384) return ARLE_E_UNSUPPORTED;
   if (pages * page_size > 0x7fffffffL) return ARLE_E_UNSUPPORTED;      // places are 32-bit
-  const StoreSide ks{k, k_stride, hd, (uint8_t*)k_cache, k_scale}, vs{v, v_stride, vd, (uint8_t*)v_cache, v_scale};
-  if (dtype == 0) return launch_store<float>(ks, vs, slot_mapping, tokens, nkv, page_size, pages * page_size, s);
-  if (dtype == 1) return launch_store<__nv_bfloat16>(ks, vs, slot_mapping, tokens, nkv, page_size, pages * page_size, s);
+  const StoreSide ks{k, k_stride, hd, 0, 0, (uint8_t*)k_cache, k_scale}, vs{v, v_stride, vd, 0, 0, (uint8_t*)v_cache, v_scale};
+  if (dtype == 0) return launch_store<float>(ks, vs, slot_mapping, tokens, nkv, page_size, (int)(pages * page_size), s);
+  if (dtype == 1) return launch_store<__nv_bfloat16>(ks, vs, slot_mapping, tokens, nkv, page_size, (int)(pages * page_size), s);
   return ARLE_E_BADARG;
 }
 
