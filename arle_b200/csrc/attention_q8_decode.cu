@@ -41,6 +41,7 @@ struct DecodeArgs {
   int nq, nkv, page_size, ps_shift, window, rows;
   float scale_log2;
   const float* sinks;
+  int beside;
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -83,9 +84,7 @@ template <int HD, int NT> struct Shape {
 
 // NT: query heads of a kv head in eights.  P16: pages of a multiple of 16 tokens, so that a tile lies in one page.
 template <int HD, int NT, bool P16>
-__global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_kernel(DecodeArgs a) {
-  pdl_launch_dependents();
-  pdl_wait();
+__device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   using S = Shape<HD, NT>;
   constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
@@ -527,6 +526,14 @@ __global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_
 }
 
 template <int HD, int NT, bool P16>
+__global__ void __launch_bounds__(kThreads, Shape<HD, NT>::kResident) q8_decode_kernel(DecodeArgs a) {
+  pdl_launch_dependents();
+  if (!a.beside) pdl_wait();
+  q8_decode<HD, NT, P16>(a);
+  if (a.beside) pdl_wait();      // what comes behind this kernel may rely on the one in front of it too
+}
+
+template <int HD, int NT, bool P16>
 int launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
   using S = Shape<HD, NT>;
   constexpr size_t merge = (size_t)kWarps * NT * 8 * S::kPitch * 4;
@@ -534,7 +541,7 @@ int launch(const DecodeArgs& a, int ctas, cudaStream_t s) {
   static SharedLimit limit;
   const cudaError_t raised = limit.raise((const void*)q8_decode_kernel<HD, NT, P16>, smem);
   if (raised != cudaSuccess) return (int)raised;
-  launch_kernel(q8_decode_kernel<HD, NT, P16>, dim3(ctas), dim3(kThreads), smem, s, 1, a);
+  launch_kernel_as(a.beside || (pdl_enabled() & 1), q8_decode_kernel<HD, NT, P16>, dim3(ctas), dim3(kThreads), smem, s, 1, a);
   return launch_status();
 }
 
@@ -549,16 +556,19 @@ int launch_by(const DecodeArgs& a, int ctas, cudaStream_t s) {
 
 // Rows with one query; others are left alone.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 2], counters int32
 // [rows * nkv], zero before the first launch (the kernel leaves them zero).
+// beside: the kernel in front of it on the stream is a prompt kernel launched in stream order that writes none of what this one reads; then this one starts
+// as soon as that one's last block has started, on the SMs that it leaves free.  (It starts when all in front of that kernel is done.)
 ARLE_API int arle_attention_q8_decode(const void* q, int q_row_stride, void* out, const void* k_cache, const void* v_cache, const float* k_scale,
                                       const float* v_scale, const int* q_indptr, const int* kv_lens, const int* block_table, int bt_stride, float* part_o,
                                       float* part_ml, int* counters, int nq, int nkv, int hd, int page_size, float scale, int window, const float* sinks, int rows,
-                                      int ctas, cudaStream_t s) {
+                                      int ctas, int beside, cudaStream_t s) {
   if (rows <= 0) return 0;
   if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > 16 || page_size <= 0 || ctas <= 0 || (hd != 64 && hd != 128) || q_row_stride % 8) return ARLE_E_UNSUPPORTED;
   int shift = -1;
   if ((page_size & (page_size - 1)) == 0)
     for (shift = 0; (1 << shift) < page_size; ++shift) {}
   const DecodeArgs a{(const __nv_bfloat16*)q, q_row_stride, (__nv_bfloat16*)out, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, q_indptr,
-                     kv_lens, block_table, bt_stride, part_o, part_ml, counters, nq, nkv, page_size, shift, window, rows, scale * 1.4426950408889634f, sinks};
+                     kv_lens, block_table, bt_stride, part_o, part_ml, counters, nq, nkv, page_size, shift, window, rows, scale * 1.4426950408889634f, sinks,
+                     beside && !(pdl_enabled() & 1)};
   return hd == 128 ? launch_by<128>(a, ctas, s) : launch_by<64>(a, ctas, s);
 }

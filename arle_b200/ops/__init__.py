@@ -131,7 +131,7 @@ _SIGNATURES = {
     "arle_store_q8": [_P, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, ctypes.c_long, _I, _I, _I, _I, _P],
     "arle_expand_q8": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P],
     "arle_attention_q8": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P],
-    "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _P],
+    "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
@@ -2371,8 +2371,9 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
     if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
             and not (qp | kp | vp | op) % 16):
-        if batch.max_q_len > 1:
-            _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
+        beside = batch.max_q_len > 1
+        if beside:
+            beside = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0:
             # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
             ctas = (4 if nq <= 8 * nkv else 3) * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
@@ -2382,21 +2383,22 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
             _check(lib.arle_attention_q8_decode(
                 qp, q_stride, op, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(),
                 block_table.data_ptr(), bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
-                batch.num_rows, ctas, _stream()), "attention_q8_decode")
+                batch.num_rows, ctas, int(beside), _stream()), "attention_q8_decode")
         return
     _check(lib.arle_attention_q8(
         qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
         block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
-def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks) -> None:
-    """The rows with several queries: their keys and values in bfloat16, then the prompt kernels, for as many rows at a time as ``Q8_EXPAND_BYTES`` hold."""
+def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks) -> bool:
+    """The rows with several queries: their keys and values in bfloat16, then the prompt kernels, for as many rows at a time as ``Q8_EXPAND_BYTES`` hold.
+    Whether a prompt kernel was launched (last, then)."""
     page = 64
     prefill = paged_attention_prefill_tc if tc_attention_supported(q, hd, page) else paged_attention_prefill
     pages = [0 if n < 2 else -(-kv // page) - (max(0, kv - n - window + 1) if window else 0) // page for n, kv in zip(batch.q_lens, batch.kv_lens_host)]
     width = max(1, -(-max(batch.kv_lens_host) // page))
     most = max(1, Q8_EXPAND_BYTES // (4 * nkv * page * hd))
-    r0, R = 0, batch.num_rows
+    r0, R, launched = 0, batch.num_rows, False
     while r0 < R:
         r1, total = r0, 0
         while r1 < R and (total == 0 or total + pages[r1] <= most):
@@ -2412,7 +2414,9 @@ def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nk
                                             page_size, nkv, hd, window, r1 - r0, 2, _ptr(kx), _ptr(vx), total, _ptr(table), width, _stream()), "expand_q8")
             prefill(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, max(batch.q_lens[r0: r1]),
                     skip_single=min(batch.q_lens[r0: r1]) < 2, sink=sinks)
+            launched = True
         r0 = r1
+    return launched
 
 
 # ------------------------------------------------------------------ a step's tables
