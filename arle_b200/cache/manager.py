@@ -22,6 +22,14 @@ same.
 Growth is atomic over a whole step: ``append`` first counts the pages every
 group needs for every request of the step and raises ``OutOfPages`` with nothing
 changed if any group falls short.
+
+A cache of 8 bits (``cache_dtype`` float8_e4m3fn) has one more array per stream, float32
+``[layer, page, head]``: the scale of a page's codes (``ops.store_q8``).
+
+With ``device_tables`` the pages of every request are also listed on the device, one row per
+slot, and a step's tables are made there from its requests' lengths (``ops.step_tables``);
+the host's tables say what is allocated, as ever.  Groups that give pages back while a request lives
+(windows, chunks) do without.
 """
 from __future__ import annotations
 
@@ -48,6 +56,7 @@ class LayerCacheView:
     block_table: torch.Tensor       # int32 [rows of the step, max pages]; -1 where a window has passed
     slot_mapping: torch.Tensor      # int32 [tokens of the step]: page * page_size + slot_in_page
     writable: bool = True
+    scales: Optional[List[torch.Tensor]] = None      # 8-bit caches: float32 [pages, heads] per stream
 
     @property
     def k(self) -> torch.Tensor:    # attention's names for its two streams
@@ -67,6 +76,10 @@ class CacheGroup:
         self.pool = PagePool(num_pages)
         self.arrays = [torch.zeros((len(layers), num_pages, heads, page_size, width), dtype=dtype, device=device)
                        for heads, width in need.arrays()]
+        self.scales = None
+        if dtype == torch.float8_e4m3fn:
+            self.scales = [torch.zeros((len(layers), num_pages, heads), dtype=torch.float32, device=device) for heads, _ in need.arrays()]
+        self.device_table: Optional[torch.Tensor] = None          # int32, ``table`` as the device has it (see ``device_tables``)
         # host block tables, one row per slot; logical page -> physical page, -1 = not held
         self.table = np.full((max_slots, max_pages_per_request), -1, dtype=np.int32)
         self.first_held = np.zeros(max_slots, dtype=np.int64)     # first logical page still held (past the kept first pages)
@@ -78,14 +91,24 @@ class CacheGroup:
         return max(0, -(-new_tokens // self.page_size) - int(self.num_logical[slot]))
 
     def bytes_per_page(self) -> int:
-        return len(self.layers) * self.need.elements_per_token() * self.page_size * self.arrays[0].element_size()
+        n = len(self.layers) * self.need.elements_per_token() * self.page_size * self.arrays[0].element_size()
+        return n + (len(self.layers) * 4 * sum(heads for heads, _ in self.need.arrays()) if self.scales is not None else 0)
 
 
 class CacheManager:
     def __init__(self, cache_needs: Sequence[CacheNeed], state_needs: Sequence[StateNeed], page_size: int,
-                 num_pages: int, max_slots: int, max_tokens_per_request: int, dtype: torch.dtype, device="cuda"):
+                 num_pages: int, max_slots: int, max_tokens_per_request: int, dtype: torch.dtype, device="cuda",
+                 cache_dtype: Optional[torch.dtype] = None, device_tables: bool = False):
         if page_size <= 0:
             raise ValueError("page_size must be positive")
+        if cache_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise ValueError(f"a cache holds the model's type ({dtype}) or float8_e4m3fn, not {cache_dtype}")
+        dtype = cache_dtype or dtype
+        self.device_tables = bool(device_tables)
+        if device_tables and any(n.window is not None or n.chunk is not None for n in cache_needs):
+            raise ValueError("tables on the device are for caches that keep all keys: a layer of this model has a window or chunks")
+        if device_tables and max_slots > 4096:
+            raise ValueError(f"tables on the device are for up to 4,096 requests at a time, not {max_slots}")
         self.page_size = page_size
         self.max_slots = max_slots
         self.max_tokens_per_request = max_tokens_per_request
@@ -101,6 +124,8 @@ class CacheManager:
             g = CacheGroup(cache_needs[layers[0]], layers, page_size, num_pages, max_slots, max_pages, dtype, self.device)
             for j, layer in enumerate(layers):
                 self.layer_to_group[layer] = (len(self.groups), j)
+            if self.device_tables:
+                g.device_table = torch.full((max_slots, max_pages), -1, dtype=torch.int32, device=self.device)
             self.groups.append(g)
         self.states = [torch.zeros((max_slots, *n.shape), dtype=n.dtype, device=self.device) for n in state_needs]
         self._free_slots = list(range(max_slots - 1, -1, -1))
@@ -255,7 +280,8 @@ class CacheManager:
                    writable: bool) -> LayerCacheView:
         gi, j = self.layer_to_group[cache_layer]
         g = self.groups[gi]
-        return LayerCacheView([a[j] for a in g.arrays], g.page_size, block_table, slot_mapping, writable)
+        scales = [a[j] for a in g.scales] if g.scales is not None else None
+        return LayerCacheView([a[j] for a in g.arrays], g.page_size, block_table, slot_mapping, writable, scales)
 
     def group_of_layer(self, cache_layer: int) -> int:
         return self.layer_to_group[cache_layer][0]

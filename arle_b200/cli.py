@@ -52,6 +52,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--num-pages", type=int, default=None)
     ap.add_argument("--kernel-set", default="fast", choices=["fast", "plain"],
                     help="plain: run the general kernels only (to bisect a discrepancy)")
+    ap.add_argument("--cache-dtype", default="auto", choices=["auto", "float8_e4m3"], help="float8_e4m3: keys and values as 8-bit codes")
+    ap.add_argument("--device-tables", action="store_true", help="make a step's tables on the device from its requests' lengths")
     sub = ap.add_subparsers(dest="command")
     run = sub.add_parser("run", help="run prompts and exit")
     g = run.add_mutually_exclusive_group(required=True)
@@ -92,7 +94,7 @@ def main(argv=None) -> int:
         max_num_batched_tokens=args.max_num_batched_tokens, chunked_prefill_size=args.chunked_prefill_size,
         max_prefill_tokens=args.max_prefill_tokens, prefill_max_requests=args.prefill_max_requests,
         scheduler_mixed_policy=args.scheduler_mixed_policy, max_tokens=args.max_tokens, seed=args.seed,
-        cuda_graph=not args.no_cuda_graph, kernel_set=args.kernel_set))
+        cuda_graph=not args.no_cuda_graph, kernel_set=args.kernel_set, cache_dtype=args.cache_dtype, device_tables=args.device_tables))
     sp = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p, min_p=args.min_p,
                         ignore_eos=args.ignore_eos, max_new_tokens=args.max_tokens)
     outs = eng.generate(prompts, sp)

@@ -6,6 +6,8 @@ with one token.  All integer tables of the step are packed into ONE pinned host
 array and copied to the device in one transfer, the way cklxx/arle uploads
 positions / indptr / page indices per step (crates/cuda-kernels/src/tilelang.rs:424-612,
 :703-818), but without separate code paths for decode, prefill and mixed batches.
+With the cache manager's ``device_tables`` only tokens, slots, lengths and newly given pages
+are copied, and a kernel (``ops.step_tables``) makes the tables from them.
 """
 from __future__ import annotations
 
@@ -136,6 +138,7 @@ class StepContext:
         self.memo: dict = {}                                 # what parts derive from a step once for all layers (cleared per step)
         self._pinned: Optional[torch.Tensor] = None
         self._dev: Optional[torch.Tensor] = None
+        self._made: Optional[torch.Tensor] = None            # tables made on the device
         self._copied = torch.cuda.Event() if self.device.type == "cuda" else None
 
     # ------------------------------------------------------------------ build
@@ -166,6 +169,8 @@ class StepContext:
                 raise ValueError(f"a request needs {need} pages, the fixed table width is {table_width}")
             widths.append(table_width if table_width is not None else need)
         self.table_width = max(widths) if widths else 0
+        if cm.device_tables and n_groups:
+            return self._build_on_device(entries, starts, widths)
         # layout of the packed int32 array
         sizes = [T, T, T, R + 1, R, R, max(W, 1), T, max(W, 1)]
         for gi in range(n_groups):
@@ -248,6 +253,64 @@ class StepContext:
         for gi in range(n_groups):
             bt = d[offs[9 + 2 * gi]:offs[9 + 2 * gi] + R * widths[gi]].view(R, widths[gi])
             sm = d[offs[10 + 2 * gi]:offs[10 + 2 * gi] + T]
+            self.groups.append(GroupTables(bt, sm))
+        return self
+
+    def _build_on_device(self, entries, starts, widths) -> "StepContext":
+        from .. import ops
+
+        cm, T, R, W = self.cache, self.num_tokens, self.num_rows, self.num_wanted
+        starts_np, lens = np.asarray(starts, dtype=np.int64), np.asarray(self.q_lens, dtype=np.int64)
+        slots = np.fromiter((cm.slot(e.request) for e in entries), dtype=np.int64, count=R)
+        # room for the pages that a step of these lengths may gain: what follows lies where it lay in a step of the same shape
+        room = [int((-(-lens // g.page_size) + 1).sum()) for g in cm.groups]
+        sizes = [T, max(W, 1), max(W, 1), R, R, R] + room
+        offs = np.concatenate([[0], np.cumsum([(s + 3) // 4 * 4 for s in sizes])])
+        host = self._host_buffer(int(offs[-1]))
+        h = host.numpy()
+        h[offs[0]:offs[0] + T] = np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in entries])
+        firsts = np.cumsum(lens) - lens
+        for e, n in zip(entries, self.q_lens):
+            for w in e.want:
+                if not 0 <= w < n:
+                    raise ValueError(f"request {e.request!r}: wanted place {w} is not among its {n} tokens")
+        counts = [len(e.want) for e in entries]
+        if W:
+            h[offs[1]:offs[1] + W] = np.repeat(firsts, counts) + np.concatenate([np.asarray(e.want, dtype=np.int64) for e in entries if len(e.want)])
+            h[offs[2]:offs[2] + W] = np.repeat(slots, counts)
+        h[offs[3]:offs[3] + R] = slots
+        h[offs[4]:offs[4] + R] = starts_np
+        h[offs[5]:offs[5] + R] = lens
+        gained = []
+        for gi, g in enumerate(cm.groups):
+            ps = g.page_size
+            held, pages = -(-starts_np // ps), -(-(starts_np + lens) // ps)
+            more = np.nonzero(pages > held)[0]
+            new = np.concatenate([g.table[slots[r], held[r]:pages[r]] for r in more]) if more.size else np.zeros(0, dtype=np.int32)
+            if (new < 0).any():
+                raise RuntimeError(f"a token of this step has no page in cache group {gi}")
+            h[offs[6 + gi]:offs[6 + gi] + new.size] = new
+            gained.append(int(new.size))
+        last = len(cm.groups) - 1
+        total = int(offs[6 + last]) + gained[last]
+        dev = self._device_buffer(int(offs[-1]))
+        dev[:total].copy_(host[:total], non_blocking=True)
+        if self._copied is not None:
+            self._copied.record()
+        self.h2d_bytes = total * 4
+        cut = lambda k, n: dev[offs[k]:offs[k] + n]      # noqa: E731
+        self.token_ids, self.want_rows, self.want_slots, self.state_slots = cut(0, T), cut(1, W), cut(2, W), cut(3, R)
+        made = [T, T, T, R + 1, R, 1] + [x for w in widths for x in (R * w, T)]
+        at = np.concatenate([[0], np.cumsum([(s + 3) // 4 * 4 for s in made])])
+        if self._made is None or self._made.numel() < at[-1]:
+            self._made = torch.zeros(max(int(at[-1]), 4096), dtype=torch.int32, device=self.device)
+        piece = lambda k: self._made[at[k]:at[k] + made[k]]      # noqa: E731
+        self.positions, self.row_of_token, self.slot_of_token, self.q_indptr, self.kv_lens = (piece(k) for k in range(5))
+        self.groups = []
+        for gi, g in enumerate(cm.groups):
+            bt, sm = piece(6 + 2 * gi).view(R, widths[gi]), piece(7 + 2 * gi)
+            ops.step_tables(self.state_slots, cut(4, R), cut(5, R), cut(6 + gi, gained[gi]), g.device_table, g.pool.num_pages, g.page_size, self.q_indptr, self.kv_lens,
+                            self.positions, self.row_of_token, self.slot_of_token, sm, bt, piece(5))
             self.groups.append(GroupTables(bt, sm))
         return self
 

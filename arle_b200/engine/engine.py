@@ -40,6 +40,8 @@ class EngineOptions:
     seed: int = 42
     cuda_graph: bool = True
     kernel_set: str = "fast"                   # "plain": the general kernels only, whatever the shapes
+    cache_dtype: str = "auto"                  # "auto": keys and values as the model computes them; "float8_e4m3": 8-bit codes, a scale per page and head
+    device_tables: bool = False                # a step's tables are made on the device from its requests' lengths, instead of copied there
 
 
 @dataclass
@@ -64,10 +66,14 @@ class Engine:
             raise ValueError(f"the given model was loaded as {model.dtype}, the options ask for {dtype}")
         self.model = model
         max_seq = o.max_seq_len or model.spec.max_position
-        per_page = self._bytes_per_page(model, o.page_size, dtype)
+        if o.cache_dtype not in ("auto", "float8_e4m3"):
+            raise ValueError(f"cache_dtype must be 'auto' or 'float8_e4m3', got {o.cache_dtype!r}")
+        q8 = o.cache_dtype == "float8_e4m3"
+        per_page = self._bytes_per_page_q8(model, o.page_size) if q8 else self._bytes_per_page(model, o.page_size, dtype)
         pages = o.num_pages if o.num_pages is not None else self._pages_from_memory(
-            per_page, o, max_seq, self._bytes_beside_the_cache(model, o))
-        self.runner = ModelRunner(model, o.page_size, pages, o.num_slots, max_seq, o.device, kernel_set=o.kernel_set)
+            per_page, o, max_seq, self._bytes_beside_the_cache(model, o) + (self._bytes_expanded(model, max_seq) if q8 else 0))
+        self.runner = ModelRunner(model, o.page_size, pages, o.num_slots, max_seq, o.device, kernel_set=o.kernel_set,
+                                  cache_dtype=torch.float8_e4m3fn if q8 else None, device_tables=o.device_tables)
         if o.cuda_graph and torch.device(o.device).type == "cuda":
             self.runner.enable_graphs()
         self.scheduler = Scheduler(self.runner.cache, SchedulerConfig(
@@ -82,6 +88,18 @@ class Engine:
     def _bytes_per_page(model, page_size: int, dtype) -> int:
         width = 2 if dtype == torch.bfloat16 else 4
         return sum(n.elements_per_token() * page_size * width for n in model.cache_needs)
+
+    @staticmethod
+    def _bytes_per_page_q8(model, page_size: int) -> int:
+        return sum(n.elements_per_token() * page_size + 4 * sum(heads for heads, _ in n.arrays()) for n in model.cache_needs)
+
+    @staticmethod
+    def _bytes_expanded(model, max_seq: int) -> int:
+        """The bfloat16 pages that a step's prompt portions are read from when the cache has 8 bits (one layer's at a time)."""
+        from .. import ops
+
+        longest = -(-max_seq // 64) * 64 * 2 * max((n.elements_per_token() for n in model.cache_needs), default=0)
+        return max(ops.Q8_EXPAND_BYTES, longest)
 
     @staticmethod
     def _bytes_beside_the_cache(model, o: EngineOptions) -> int:

@@ -27,14 +27,20 @@ from .batch import StepContext, StepEntry, Workspace
 
 class ModelRunner:
     def __init__(self, model: DecoderModel, page_size: int, num_pages: int, max_slots: int,
-                 max_tokens_per_request: Optional[int] = None, device="cuda", kernel_set: str = "fast"):
+                 max_tokens_per_request: Optional[int] = None, device="cuda", kernel_set: str = "fast",
+                 cache_dtype: Optional[torch.dtype] = None, device_tables: bool = False):
         if kernel_set not in ("fast", "plain"):
             raise ValueError(f"kernel_set must be 'fast' or 'plain', got {kernel_set!r}")
+        if cache_dtype == torch.float8_e4m3fn:
+            for m in (getattr(b, "mixer", None) for b in model.blocks):
+                if m is not None and m.cache_need() is not None and not m.takes_q8_cache():
+                    raise ValueError(f"a cache of 8 bits is not for this model: its {type(m).__name__} layers read keys and values as they are")
         self.model = model
         self.kernel_set = kernel_set
         self.device = torch.device(device)
         self.cache = CacheManager(model.cache_needs, model.state_needs, page_size, num_pages, max_slots,
-                                  max_tokens_per_request or model.spec.max_position, model.dtype, self.device)
+                                  max_tokens_per_request or model.spec.max_position, model.dtype, self.device,
+                                  cache_dtype, device_tables)
         self.ws = Workspace(self.device)
         self.ctx = StepContext(self.cache, self.ws)
         # the token each request sampled last, written by the sampling kernels; a step entry

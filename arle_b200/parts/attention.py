@@ -350,6 +350,35 @@ class Attention(Mixer):
             ops.bias_add(out, self.b_o)
         return out
 
+    # ------------------------------------------------- the plain form on a cache of 8 bits
+    def takes_q8_cache(self):
+        return self.plain_form and not self.general_form and not self.post_form
+
+    def _forward_q8(self, x, ctx, cache, sink):
+        """Norm and rotation in place on the projection's columns, then the codes of the new keys and values, then attention over codes: a step's own
+        keys are read as they were rounded, however the prompt is cut."""
+        s = self.spec
+        T, nq, nkv, hd = x.shape[0], s.num_heads, s.num_kv_heads, s.head_dim
+        rot = self.position.rotary() if self.position is not None else None
+        inv_freq, rdim = rot if rot is not None else (None, 0)
+        eps = s.qk_norm_eps if s.qk_norm_eps is not None else 0.0
+        name, columns = ("qkv", (nq + 2 * nkv) * hd) if cache.writable else ("q_only", nq * hd)
+        proj = ctx.ws.get(name, (T, columns), x.dtype)
+        ops.gemm(x, self.w_qkv if cache.writable else self.w_qkv[:columns], proj)
+        q = ctx.ws.cut(name, proj, 0, nq * hd)
+        angles = self._angles(proj, ctx, inv_freq, rdim)
+        ops.attention_prep(q, ctx.positions, None, self.q_norm, None, eps, inv_freq, rdim, None, None, nq, 0, hd, cache.page_size, angles=angles)
+        if cache.writable:
+            k = ctx.ws.cut(name, proj, nq * hd, (nq + nkv) * hd)
+            ops.attention_prep(k, ctx.positions, None, self.k_norm, None, eps, inv_freq, rdim, None, None, nkv, 0, hd, cache.page_size, angles=angles)
+            ops.store_q8(k, ctx.ws.cut(name, proj, (nq + nkv) * hd, (nq + 2 * nkv) * hd), cache.slot_mapping, cache.k, cache.v, *cache.scales, nkv, hd,
+                         cache.page_size)
+        attn = ctx.ws.get("attn_out", (T, nq * hd), x.dtype)
+        ops.paged_attention_q8(q, attn, cache.k, cache.v, *cache.scales, ctx.positions, ctx.row_of_token, cache.block_table, nq, nkv, hd, cache.page_size,
+                               s.scale, s.window, batch=ctx)
+        out = ctx.ws.get("mixer_out", (T, s.hidden_size), x.dtype)
+        return None if ops.gemm(attn, self.w_o, out, sink=sink) else out
+
     # ------------------------------------------------- the general form, up to the output projection
     def pre_output_width(self):
         return None if self.general_form or self.spec.out_gate else self.spec.num_heads * self.vd
@@ -408,6 +437,8 @@ class Attention(Mixer):
                 ops.gate_mul(attn, proj[:, self.gate_at: self.gate_at + s.num_heads * self.vd], attn)
             out = ctx.ws.get("mixer_out", (T, s.hidden_size), x.dtype)
             return None if ops.gemm(attn, self.w_o, out, sink=sink) else out
+        if cache.scales is not None:
+            return self._forward_q8(x, ctx, cache, sink)
         nq, nkv, hd = s.num_heads, s.num_kv_heads, s.head_dim
         rot = self.position.rotary() if self.position is not None else None
         inv_freq, rdim = rot if rot is not None else (None, 0)

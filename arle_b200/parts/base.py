@@ -166,6 +166,10 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    def takes_q8_cache(self) -> bool:
+        """Whether this mixer runs on a cache of 8 bits (``cache.scales`` beside its streams)."""
+        return False
+
     def forward(self, x: torch.Tensor, ctx, cache, state) -> torch.Tensor:
         """x: [T, hidden] normalised input of this step's tokens.  ``cache`` is a
         ``LayerCacheView`` (or None; ``cache.writable`` is False when this run reads
