@@ -46,6 +46,8 @@
 // A third form has sigmoid weights, sigmoid(score + pb[head]), in the softmax's place, and chunks (a query sees only the keys
 // of its own chunk of positions, counted from 0) or a window: no maximum, no sum and no rescaling; two scores share one
 // reciprocal, since the special-function unit is what bounds the softmax warps.
+// A fourth form, for launches of fewer blocks than SMs, cuts a block's key tiles into `splits` parts, each a block of its own that leaves float32 sums,
+// maxima and totals in scratch; paged_prefill_join_kernel adds them up.
 // Scores, maxima, sums and the accumulators are float32.  Every mbarrier wait is bounded; when one runs
 // out the kernel raises the error flag, stops, draws the remaining tickets so that the counter ends at
 // zero, frees its TMEM and returns.
@@ -183,6 +185,23 @@ struct Block {
     p_last = rows_x[1] > 0 ? pl_x[1] : pl_x[0];        // last key any row of the block sees
     return true;
   }
+  // This block's part `split` of `splits` equal ones of its key tiles (without kept first keys); false: it has none.
+  __device__ bool cut(int split, int splits) {
+    const int each = (ntiles + splits - 1) / splits, j0 = split * each, j1 = min(ntiles, j0 + each);
+    if (j0 >= j1) return false;
+    ntiles = 0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      jlo_x[x] = max(jlo_x[x] - j0, 0);
+      jhi_x[x] = min(jhi_x[x], j1) - j0;
+      if (jhi_x[x] <= jlo_x[x]) jlo_x[x] = jhi_x[x] = 0;      // no key of this part is one that the query tile sees
+      ntiles = max(ntiles, jhi_x[x]);
+    }
+    kb += j0 * BKV;
+    lo = max(lo, kb);
+    p_last = min(p_last, kb + ntiles * BKV - 1);
+    return ntiles > 0;
+  }
   // E: the form with kept first keys (the usual form compiles to what it was without them: nk is zero there)
   template <bool E> __device__ bool in_range(int x, int j) const {
     return E ? (j >= jlo_x[x] || j < nk) && j < jhi_x[x] : j >= jlo_x[x] && j < jhi_x[x];
@@ -192,7 +211,7 @@ struct Block {
 
 constexpr int kWorkReaders = 11;             // who reads a drawn ticket: the two loader warps, the MMA thread, eight softmax warps
 
-// FORM 0: the usual one; 1: with kept first keys and a score cap; 2: sigmoid weights, with chunks or a window.
+// FORM 0: the usual one; 1: with kept first keys and a score cap; 2: sigmoid weights, with chunks or a window; 3: a block's key tiles in parts.
 template <int FORM>
 __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -200,10 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
     const int* __restrict__ kv_lens, const int* __restrict__ block_table, int bt_stride, int bt_width, int nq, int nkv,
     int page_size, float scale_log2, HeadTail<__nv_bfloat16> tail, int window, int skip_single, int nyb, int nblocks, int ticket_slot, int* __restrict__ err,
     int keep_arg, float cap_arg, float scale_over_cap, int chunk_arg, const float* __restrict__ pb, const __nv_bfloat16* __restrict__ v_cache,
-    int row_behind) {
+    int row_behind, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr bool EXT = FORM == 1, SIG = FORM == 2;
+  constexpr bool EXT = FORM == 1, SIG = FORM == 2, PARTS = FORM == 3;
   const int chunk = SIG ? chunk_arg : 0;
   const int keep_first = EXT ? keep_arg : 0;
   const float cap_log2 = EXT ? cap_arg : 0.f;
@@ -222,9 +241,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the CTA's first block is the one of its own index: its shape is worked out while the rest is set up
+  auto shape_of = [&](Block& blk, int b) {
+    if (!PARTS) return blk.init(b, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, keep_first, chunk);
+    return blk.init(b / splits, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, keep_first, chunk) && blk.cut(b % splits, splits);
+  };
   bool first_has_queries = false;
-  if (warp == kKeyWarp && lane == 0)
-    first_has_queries = work_blk[0].init((int)blockIdx.x, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, keep_first, chunk);
+  if (warp == kKeyWarp && lane == 0) first_has_queries = shape_of(work_blk[0], (int)blockIdx.x);
   if (threadIdx.x == 0) {
     mbar_init(smem_addr(&q_full), 1);
     mbar_init(smem_addr(&q_empty), 1);
@@ -288,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
             if (!*aborted) {
               const unsigned int tk = draw_ticket(nblocks, ticket_slot);
               if (tk < (unsigned int)nblocks) b = (int)tk; else ended = true;
-              if (b >= 0 && !work_blk[it & 1].init(b, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, keep_first, chunk)) b = -2;
+              if (b >= 0 && !shape_of(work_blk[it & 1], b)) b = -2;
             }
           } else {
             abort_flag = 1;
@@ -658,6 +680,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
       }
       // asked for before the wait for the last product: a sink's score (log2 units; -inf: none), the head's gate
       const float sink_log2 = SIG ? 0.f : tail.sink_log2(blk.h);
+      if constexpr (PARTS) {
+        if (row < rows_here) part_ml[(size_t)b * BQ2 + x * BQ + row] = n > 0 ? make_float2(m_used, l) : make_float2(-INFINITY, 0.f);
+      }
       const float gate = row < rows_here ? tail.gate_of(blk.t0 + blk.mbeg + x * BQ + row, blk.h) : 1.0f;
       if (ok && n > 0) {
         const bool ready = mbar_wait_bounded(smem_addr(&o_full[x]), (uint32_t)(o_all & 1), aborted);
@@ -679,7 +704,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_addr(&o_empty[x]));
           }
-          if (row < rows_here) {
+          if (PARTS) {
+            if (row < rows_here) {
+              float4* prow = reinterpret_cast<float4*>(part_o + ((size_t)b * BQ2 + x * BQ + row) * HD + c * 32);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                prow[i] = make_float4(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1]), __uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3]));
+            }
+          } else if (row < rows_here) {
             uint32_t p[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -704,17 +736,52 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
   if (threadIdx.x == 0 && abort_flag && err) atomicExch(err, 3);
 }
 
+// The parts of a block: out = sum_s o_s 2^(m_s - M) / (sum_s l_s 2^(m_s - M) + 2^(sink - M)).  A warp a row, four numbers a lane.
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out,
+                                                                 const int* __restrict__ q_indptr, const int* __restrict__ kv_lens, int nq, int nkv, int nyb,
+                                                                 int window, int skip_single, int splits, HeadTail<__nv_bfloat16> tail) {
+  pdl_launch_dependents();
+  pdl_wait();
+  Block blk;
+  if (!blk.init((int)blockIdx.x, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, 0, 0)) return;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= blk.rows_x[0] + blk.rows_x[1]) return;
+  const int each = (blk.ntiles + splits - 1) / splits, parts = (blk.ntiles + each - 1) / each;
+  const size_t first = (size_t)blockIdx.x * splits * BQ2 + row;
+  const float sink = tail.sink_log2(blk.h);
+  float M = sink;
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, part_ml[first + (size_t)s * BQ2].x);
+  const float top = M == -INFINITY ? 0.f : M;
+  float L = exp2f(sink - top);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = part_ml[first + (size_t)s * BQ2];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;      // a part without keys that this row sees may have no sums
+    const float4 x = *reinterpret_cast<const float4*>(part_o + (first + (size_t)s * BQ2) * HD + lane * 4);
+    const float f = exp2f(ml.x - top);
+    L += ml.y * f;
+    o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+  }
+  const int t = blk.t0 + blk.mbeg + row;
+  const float inv = tail.gate_of(t, blk.h) / L;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(out + ((size_t)t * nq + blk.h) * HD + lane * 4) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
 }  // namespace
 
 // q: the packed projection output [T, q_row_stride] whose first nq * 128 columns are the queries.
 // k_cache / v_cache: [pages, nkv, page_size, 128].  Needs page_size % 16 == 0, head size 128,
 // q_row_stride % 8 == 0, 16-byte aligned q, and out rows of nq * 128 elements.
-ARLE_API int arle_paged_attention_prefill_tc(const void* q, int q_row_stride, int num_tokens, void* out, const void* k_cache,
+static int launch_prefill_tc(const void* q, int q_row_stride, int num_tokens, void* out, const void* k_cache,
                                              const void* v_cache, long long cache_pages, const int* q_indptr,
                                              const int* kv_lens, const int* block_table, int bt_stride, int bt_width, int nq, int nkv,
                                              int hd, int page_size, float scale, const float* sinks, const void* gate,
                                              int gate_stride, int window, int rows, int max_q_len,
-                                             int skip_single, int* err, int keep_first, float softcap, int chunk, const float* pb, cudaStream_t s) {
+                                             int skip_single, int* err, int keep_first, float softcap, int chunk, const float* pb, int splits, float* part_o, float* part_ml,
+                                             cudaStream_t s) {
   if (rows <= 0 || max_q_len <= 0) return 0;
   if (bt_width < 1) return ARLE_E_BADARG;
   if (hd != HD || page_size % 16 != 0 || nq <= 0 || nkv <= 0 || nq % nkv != 0 || rows > 65535 || (max_q_len + BQ2 - 1) / BQ2 > 65535)
@@ -732,14 +799,14 @@ ARLE_API int arle_paged_attention_prefill_tc(const void* q, int q_row_stride, in
   const size_t smem = (2 + 2 * kStages) * (size_t)TILE + 1024;
   if (keep_first < 0 || softcap < 0.f || chunk < 0 || (chunk > 0 && window > 0)) return ARLE_E_BADARG;
   if (pb ? (keep_first > 0 || softcap > 0.f) : chunk > 0) return ARLE_E_UNSUPPORTED;      // the sigmoid form has neither; only it has chunks
-  const int form = pb ? 2 : ((window > 0 && keep_first > 0) || softcap > 0.f) ? 1 : 0;
-  auto kernel = form == 2 ? paged_prefill_tc_kernel<2> : form == 1 ? paged_prefill_tc_kernel<1> : paged_prefill_tc_kernel<0>;
-  static SharedLimit limits[3];
+  const int form = splits > 1 ? 3 : pb ? 2 : ((window > 0 && keep_first > 0) || softcap > 0.f) ? 1 : 0;
+  auto kernel = form == 3 ? paged_prefill_tc_kernel<3> : form == 2 ? paged_prefill_tc_kernel<2> : form == 1 ? paged_prefill_tc_kernel<1> : paged_prefill_tc_kernel<0>;
+  static SharedLimit limits[4];
   const cudaError_t raised = limits[form].raise((const void*)kernel, smem);
   if (raised != cudaSuccess) return (int)raised;
   // CTAs stay resident and draw blocks (a query head, 256 queries of a request) from a counter, the heaviest first
   const int nyb = (max_q_len + BQ2 - 1) / BQ2;
-  const long long nblocks = (long long)nq * nyb * rows;
+  const long long nblocks = (long long)nq * nyb * rows * splits;
   if (nblocks > 0x3fffffffLL) return ARLE_E_UNSUPPORTED;
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
@@ -751,7 +818,40 @@ ARLE_API int arle_paged_attention_prefill_tc(const void* q, int q_row_stride, in
                                 q_indptr, kv_lens, block_table, bt_stride, bt_width, nq, nkv, page_size,
                                 scale * 1.4426950408889634f, HeadTail<__nv_bfloat16>{sinks, (const __nv_bfloat16*)gate, gate_stride}, window, skip_single, nyb, (int)nblocks, ticket_slot, err,
                                 window > 0 ? keep_first : 0, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f,
-                                softcap > 0.f ? scale / softcap : 0.f, chunk, pb, (const __nv_bfloat16*)v_cache, (int)(cache_rows < 0x7fffffff ? cache_rows : 0x7fffffff));
+                                softcap > 0.f ? scale / softcap : 0.f, chunk, pb, (const __nv_bfloat16*)v_cache, (int)(cache_rows < 0x7fffffff ? cache_rows : 0x7fffffff), splits, part_o, (float2*)part_ml);
   if (e != cudaSuccess) return (int)e;
+  return launch_status();
+}
+
+ARLE_API int arle_paged_attention_prefill_tc(const void* q, int q_row_stride, int num_tokens, void* out, const void* k_cache,
+                                             const void* v_cache, long long cache_pages, const int* q_indptr,
+                                             const int* kv_lens, const int* block_table, int bt_stride, int bt_width, int nq, int nkv,
+                                             int hd, int page_size, float scale, const float* sinks, const void* gate,
+                                             int gate_stride, int window, int rows, int max_q_len,
+                                             int skip_single, int* err, int keep_first, float softcap, int chunk, const float* pb, cudaStream_t s) {
+  return launch_prefill_tc(q, q_row_stride, num_tokens, out, k_cache, v_cache, cache_pages, q_indptr, kv_lens, block_table, bt_stride, bt_width, nq, nkv, hd, page_size,
+                           scale, sinks, gate, gate_stride, window, rows, max_q_len, skip_single, err, keep_first, softcap, chunk, pb, 1, nullptr, nullptr, s);
+}
+
+// The usual form with every block's key tiles in `splits` parts (2 or more), whose sums go to part_o, float32 [blocks * splits * 256 * 128], and part_ml,
+// float32 [blocks * splits * 256 * 2], blocks = nq * ceil(max_q_len / 256) * rows; arle_paged_prefill_join then writes out (and needs the same arguments).
+ARLE_API int arle_paged_attention_prefill_tc_parts(const void* q, int q_row_stride, int num_tokens, void* out, const void* k_cache, const void* v_cache,
+                                                   long long cache_pages, const int* q_indptr, const int* kv_lens, const int* block_table, int bt_stride,
+                                                   int bt_width, int nq, int nkv, int hd, int page_size, float scale, int window, int rows, int max_q_len,
+                                                   int skip_single, int* err, int splits, float* part_o, float* part_ml, cudaStream_t s) {
+  if (splits < 2 || !part_o || !part_ml) return ARLE_E_BADARG;
+  return launch_prefill_tc(q, q_row_stride, num_tokens, out, k_cache, v_cache, cache_pages, q_indptr, kv_lens, block_table, bt_stride, bt_width, nq, nkv, hd, page_size,
+                           scale, nullptr, nullptr, 0, window, rows, max_q_len, skip_single, err, 0, 0.f, 0, nullptr, splits, part_o, part_ml, s);
+}
+
+ARLE_API int arle_paged_prefill_join(const float* part_o, const float* part_ml, void* out, const int* q_indptr, const int* kv_lens, int nq, int nkv, int hd,
+                                     const float* sinks, int window, int rows, int max_q_len, int skip_single, int splits, cudaStream_t s) {
+  if (rows <= 0 || max_q_len <= 0) return 0;
+  if (hd != HD || splits < 2) return ARLE_E_UNSUPPORTED;
+  const int nyb = (max_q_len + BQ2 - 1) / BQ2;
+  const long long blocks = (long long)nq * nyb * rows;
+  if (blocks > 0x3fffffffLL) return ARLE_E_UNSUPPORTED;
+  launch_kernel(paged_prefill_join_kernel, dim3((unsigned)blocks, BQ2 / 8), dim3(256), 0, s, 1, part_o, (const float2*)part_ml, (__nv_bfloat16*)out, q_indptr, kv_lens, nq,
+                nkv, nyb, window, skip_single, splits, HeadTail<__nv_bfloat16>{sinks, nullptr, 0});
   return launch_status();
 }

@@ -82,6 +82,8 @@ _SIGNATURES = {
     "arle_paged_attention_prefill": [_P, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P],
     "arle_paged_attention_prefill_tc": [_P, _I, _I, _P, _P, _P, ctypes.c_longlong, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _I, _I,
                                         _I, _I, _I, _P, _I, _F, _I, _P, _P],
+    "arle_paged_attention_prefill_tc_parts": [_P, _I, _I, _P, _P, _P, ctypes.c_longlong, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P, _I, _P, _P, _P],
+    "arle_paged_prefill_join": [_P, _P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _I, _I, _I, _P],
     "arle_gemm_f32": [_P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _P],
     "arle_gemm_f32_tc": [_P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P],
     "arle_gemm_plain_bf16": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
@@ -2371,9 +2373,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
     if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
             and not (qp | kp | vp | op) % 16):
-        beside = batch.max_q_len > 1
-        if beside:
-            beside = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
+        beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks) if (
+            batch.max_q_len > 1) else (False, None)
         if batch.num_single > 0:
             # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
             ctas = (4 if nq <= 8 * nkv else 3) * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
@@ -2384,39 +2385,80 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
                 qp, q_stride, op, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(),
                 block_table.data_ptr(), bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
                 batch.num_rows, ctas, int(beside), _stream()), "attention_q8_decode")
+        if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
+            join()
         return
     _check(lib.arle_attention_q8(
         qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
         block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
-def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks) -> bool:
+def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks):
     """The rows with several queries: their keys and values in bfloat16, then the prompt kernels, for as many rows at a time as ``Q8_EXPAND_BYTES`` hold.
-    Whether a prompt kernel was launched (last, then)."""
-    page = 64
-    prefill = paged_attention_prefill_tc if tc_attention_supported(q, hd, page) else paged_attention_prefill
-    pages = [0 if n < 2 else -(-kv // page) - (max(0, kv - n - window + 1) if window else 0) // page for n, kv in zip(batch.q_lens, batch.kv_lens_host)]
+    Returns whether a prompt kernel was launched (last, then), and what the caller has to call at the end, if anything."""
+    page, R, q_lens = 64, batch.num_rows, batch.q_lens
+    pages = [0 if n < 2 else -(-kv // page) - (max(0, kv - n - window + 1) if window else 0) // page for n, kv in zip(q_lens, batch.kv_lens_host)]
     width = max(1, -(-max(batch.kv_lens_host) // page))
     most = max(1, Q8_EXPAND_BYTES // (4 * nkv * page * hd))
-    r0, R, launched = 0, batch.num_rows, False
-    while r0 < R:
-        r1, total = r0, 0
+    join, launched, r0 = None, False, 0
+    while True:
+        while r0 < R and not pages[r0]:
+            r0 += 1
+        if r0 == R:
+            return launched, join
+        if join is not None:
+            join()
+        r1, total, end = r0, 0, r0
         while r1 < R and (total == 0 or total + pages[r1] <= most):
             total += pages[r1]
             r1 += 1
-        if total:
-            kx = batch.ws.get("attn_q8_keys", (total, nkv, page, hd), torch.bfloat16)
-            vx = batch.ws.get("attn_q8_values", (total, nkv, page, hd), torch.bfloat16)
-            table = batch.ws.get("attn_q8_table", (r1 - r0, width), torch.int32)
-            indptr, lens = batch.q_indptr[r0: r1 + 1], batch.kv_lens[r0: r1]
-            bt = block_table[r0: r1]
-            _check(library().arle_expand_q8(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(indptr), _ptr(lens), _ptr(bt), bt.stride(0),
-                                            page_size, nkv, hd, window, r1 - r0, 2, _ptr(kx), _ptr(vx), total, _ptr(table), width, _stream()), "expand_q8")
-            prefill(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, max(batch.q_lens[r0: r1]),
-                    skip_single=min(batch.q_lens[r0: r1]) < 2, sink=sinks)
-            launched = True
-        r0 = r1
-    return launched
+            if pages[r1 - 1]:
+                end = r1                   # rows behind the last one with a portion are left out
+        after, r1 = r1, end
+        kx = batch.ws.get("attn_q8_keys", (total, nkv, page, hd), torch.bfloat16)
+        vx = batch.ws.get("attn_q8_values", (total, nkv, page, hd), torch.bfloat16)
+        table = batch.ws.get("attn_q8_table", (r1 - r0, width), torch.int32)
+        indptr, lens, bt = batch.q_indptr[r0: r1 + 1], batch.kv_lens[r0: r1], block_table[r0: r1]
+        longest, single = max(q_lens[r0: r1]), min(q_lens[r0: r1]) < 2
+        _check(library().arle_expand_q8(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(indptr), _ptr(lens), _ptr(bt), bt.stride(0),
+                                        page_size, nkv, hd, window, r1 - r0, 2, _ptr(kx), _ptr(vx), total, _ptr(table), width, _stream()), "expand_q8")
+        if hd == 128:
+            splits = prompt_splits_q8(nq, q_lens[r0: r1], max(pages[r0: r1]), q.device)
+            if splits == 1:
+                paged_attention_prefill_tc(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, longest, skip_single=single, sink=sinks)
+                join = None
+            else:
+                join = _prefill_tc_parts(q, out, kx, vx, indptr, lens, table, nq, nkv, page, scale, window, longest, single, sinks, splits, batch.ws)
+        else:
+            paged_attention_prefill(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, longest, skip_single=single, sink=sinks)
+        launched, r0 = True, after
+
+
+def prompt_splits_q8(nq: int, q_lens, pages: int, device) -> int:
+    """Parts that the prompt kernel's blocks (a query head, 256 queries) cut their keys into: as many as bring the blocks to the number of SMs, none of
+    fewer than two tiles of 128 keys.  A block takes some 6 us and 2.3 us for each tile, the parts' sums and the joining 3 us: 32 heads with 509 queries
+    behind 1,600 keys, 64 blocks, take PARTS_FIGURE.  Scratch is for the blocks that the launch counts, rows without a portion among them."""
+    sms = _SM_COUNT.get(device.index) or sm_count(device)
+    tall = -(-max(q_lens) // 256)
+    blocks, counted = nq * sum(-(-n // 256) for n in q_lens if n > 1), nq * tall * len(q_lens)
+    return max(1, min(sms // max(blocks, 1), pages // 4, 4 * sms // counted))
+
+
+def _prefill_tc_parts(q, out, k_cache, v_cache, q_indptr, kv_lens, block_table, nq, nkv, page_size, scale, window: int, longest: int, single: bool, sinks, splits: int, ws):
+    """The tcgen05 prompt kernel with its blocks' keys in parts; returns the call that joins them and writes ``out``."""
+    blocks, rows = nq * -(-longest // 256) * kv_lens.numel() * splits, kv_lens.numel()
+    parts = ws.get("attn_q8_prompt_parts", (blocks * 256 * 130,), torch.float32)
+    part_o, part_ml = _ptr(parts), parts.data_ptr() + blocks * 256 * 128 * 4
+    _check(library().arle_paged_attention_prefill_tc_parts(
+        _ptr(q), q.stride(0), q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], _ptr(q_indptr), _ptr(kv_lens), _ptr(block_table),
+        block_table.stride(0), block_table.shape[1], nq, nkv, 128, page_size, float(scale), window, rows, longest, int(single), _ptr(error_flag(q.device)), splits,
+        part_o, part_ml, _stream()), "paged_attention_prefill_tc_parts")
+
+    def join():
+        _check(library().arle_paged_prefill_join(part_o, part_ml, _ptr(out), _ptr(q_indptr), _ptr(kv_lens), nq, nkv, 128, _ptr(sinks), window, rows, longest, int(single),
+                                                 splits, _stream()), "paged_prefill_join")
+
+    return join
 
 
 # ------------------------------------------------------------------ a step's tables

@@ -167,8 +167,22 @@ def test_portions(rows, hd, ps, window, sink, monkeypatch):
     out = _run(s, window, sinks)
     _near(out, want, hd, 2.0 ** -8, max(s.kvs))
     _near(_run(s, window, sinks, batch=False), want, hd, 0.0, max(s.kvs))
-    monkeypatch.setattr(ops, "Q8_EXPAND_BYTES", 1)             # every row by itself
     assert torch.equal(_run(s, window, sinks), out)
+    monkeypatch.setattr(ops, "Q8_EXPAND_BYTES", 1)             # every row by itself: in how many parts its keys are summed goes by the rows that run together
+    _near(_run(s, window, sinks), want, hd, 2.0 ** -8, max(s.kvs))
+    ops.check_errors(DEV)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 5, 16, 18])
+@pytest.mark.parametrize("rows,window", [([(300, 2100)], None), ([(300, 2100)], 200), ([(257, 257), (1, 900), (2, 700), (600, 1290)], None), ([(2, 2), (130, 130)], 40)])
+def test_portions_in_parts(splits, rows, window, monkeypatch):
+    """The prompt kernel's key tiles in any number of parts, more than there are tiles among them."""
+    s = _case(rows, 8, 2, 128, 16, seed=9)
+    monkeypatch.setattr(ops, "prompt_splits_q8", lambda *a: splits)
+    for sinks in (None, torch.randn(8, generator=torch.Generator().manual_seed(5)).to(DEV)):
+        out = _run(s, window, sinks)
+        _near(out, _want(s, window, sinks), 128, 2.0 ** -8, max(s.kvs))
+        assert torch.equal(_run(s, window, sinks), out)
     ops.check_errors(DEV)
 
 
