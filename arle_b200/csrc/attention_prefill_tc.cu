@@ -736,38 +736,60 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
   if (threadIdx.x == 0 && abort_flag && err) atomicExch(err, 3);
 }
 
-// The parts of a block: out = sum_s o_s 2^(m_s - M) / (sum_s l_s 2^(m_s - M) + 2^(sink - M)).  A warp a row, four numbers a lane.
-__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, __nv_bfloat16* __restrict__ out,
-                                                                 const int* __restrict__ q_indptr, const int* __restrict__ kv_lens, int nq, int nkv, int nyb,
-                                                                 int window, int skip_single, int splits, HeadTail<__nv_bfloat16> tail) {
+// The parts of a block: out = sum_s o_s 2^(m_s - M) / (sum_s l_s 2^(m_s - M) + 2^(sink - M)).  A warp has two rows, whose reads are under way together,
+// and a lane four numbers of each; bound by the latency of two dependent reads and by L2.
+constexpr int kJoinRows = 2;
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const float* part_o, const float2* part_ml, __nv_bfloat16* out, const int* q_indptr,
+                                                                 const int* kv_lens, int nq, int nkv, int nyb,
+                                                                 int window, int skip_single, int splits, HeadTail<__nv_bfloat16> tail, int early) {
   pdl_launch_dependents();
-  pdl_wait();
+  // It starts beside the kernel in front of it (the prompt kernel, or the decoded tokens' beside that one), which itself started when all in front of the
+  // prompt kernel was done: the lengths, which neither writes, may be read before that one's end.
+  if (!early) pdl_wait();
   Block blk;
-  if (!blk.init((int)blockIdx.x, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, 0, 0)) return;
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= blk.rows_x[0] + blk.rows_x[1]) return;
+  const bool mine = blk.init((int)blockIdx.x, nq, nkv, nyb, q_indptr, kv_lens, window, skip_single, 0, 0);
+  if (early) pdl_wait();
+  if (!mine) return;
+  const int row0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * kJoinRows, lane = threadIdx.x & 31, rows = min(kJoinRows, blk.rows_x[0] + blk.rows_x[1] - row0);
+  if (rows <= 0) return;
   const int each = (blk.ntiles + splits - 1) / splits, parts = (blk.ntiles + each - 1) / each;
-  const size_t first = (size_t)blockIdx.x * splits * BQ2 + row;
+  const size_t first = (size_t)blockIdx.x * splits * BQ2 + row0;
   const float sink = tail.sink_log2(blk.h);
-  float M = sink;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, part_ml[first + (size_t)s * BQ2].x);
-  const float top = M == -INFINITY ? 0.f : M;
-  float L = exp2f(sink - top);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = part_ml[first + (size_t)s * BQ2];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;      // a part without keys that this row sees may have no sums
-    const float4 x = *reinterpret_cast<const float4*>(part_o + (first + (size_t)s * BQ2) * HD + lane * 4);
-    const float f = exp2f(ml.x - top);
-    L += ml.y * f;
-    o = make_float4(o.x + x.x * f, o.y + x.y * f, o.z + x.z * f, o.w + x.w * f);
+  float M[kJoinRows], L[kJoinRows];
+  float4 o[kJoinRows];
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) {
+    M[i] = sink;
+    L[i] = sink == -INFINITY ? 0.f : 1.f;
+    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  const int t = blk.t0 + blk.mbeg + row;
-  const float inv = tail.gate_of(t, blk.h) / L;
-  const __nv_bfloat162 lo = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi = __floats2bfloat162_rn(o.z * inv, o.w * inv);
-  *reinterpret_cast<uint2*>(out + ((size_t)t * nq + blk.h) * HD + lane * 4) =
-      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  for (int s = 0; s < parts; ++s) {
+    float2 ml[kJoinRows];
+    float4 x[kJoinRows];
+#pragma unroll
+    for (int i = 0; i < kJoinRows; ++i) {
+      const size_t at = first + (size_t)s * BQ2 + min(i, rows - 1);
+      ml[i] = part_ml[at];
+      x[i] = *reinterpret_cast<const float4*>(part_o + at * HD + lane * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < kJoinRows; ++i) {
+      if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;      // a part without keys that this row sees may have no sums
+      const float top = fmaxf(M[i], ml[i].x), base = top == -INFINITY ? 0.f : top, was = exp2f(M[i] - base), f = exp2f(ml[i].x - base);
+      M[i] = top;
+      L[i] = L[i] * was + ml[i].y * f;
+      o[i] = make_float4(o[i].x * was + x[i].x * f, o[i].y * was + x[i].y * f, o[i].z * was + x[i].z * f, o[i].w * was + x[i].w * f);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kJoinRows; ++i) {
+    if (i >= rows) break;
+    const int t = blk.t0 + blk.mbeg + row0 + i;
+    const float inv = tail.gate_of(t, blk.h) / L[i];
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(o[i].x * inv, o[i].y * inv), hi = __floats2bfloat162_rn(o[i].z * inv, o[i].w * inv);
+    *reinterpret_cast<uint2*>(out + ((size_t)t * nq + blk.h) * HD + lane * 4) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
 }
 
 }  // namespace
@@ -851,7 +873,7 @@ ARLE_API int arle_paged_prefill_join(const float* part_o, const float* part_ml, 
   const int nyb = (max_q_len + BQ2 - 1) / BQ2;
   const long long blocks = (long long)nq * nyb * rows;
   if (blocks > 0x3fffffffLL) return ARLE_E_UNSUPPORTED;
-  launch_kernel(paged_prefill_join_kernel, dim3((unsigned)blocks, BQ2 / 8), dim3(256), 0, s, 1, part_o, (const float2*)part_ml, (__nv_bfloat16*)out, q_indptr, kv_lens, nq,
-                nkv, nyb, window, skip_single, splits, HeadTail<__nv_bfloat16>{sinks, nullptr, 0});
+  launch_early(paged_prefill_join_kernel, dim3((unsigned)blocks, BQ2 / (8 * kJoinRows)), dim3(256), 0, s, 1, part_o, (const float2*)part_ml, (__nv_bfloat16*)out, q_indptr, kv_lens, nq,
+                nkv, nyb, window, skip_single, splits, HeadTail<__nv_bfloat16>{sinks, nullptr, 0}, (pdl_enabled() & 1) == 0);
   return launch_status();
 }

@@ -2396,11 +2396,13 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
 def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks):
     """The rows with several queries: their keys and values in bfloat16, then the prompt kernels, for as many rows at a time as ``Q8_EXPAND_BYTES`` hold.
     Returns whether a prompt kernel was launched (last, then), and what the caller has to call at the end, if anything."""
-    page, R, q_lens = 64, batch.num_rows, batch.q_lens
-    pages = [0 if n < 2 else -(-kv // page) - (max(0, kv - n - window + 1) if window else 0) // page for n, kv in zip(q_lens, batch.kv_lens_host)]
-    width = max(1, -(-max(batch.kv_lens_host) // page))
+    page, R, q_lens, kvs = 64, batch.num_rows, batch.q_lens, batch.kv_lens_host
+    pages = [0 if n < 2 else -(-kv // 64) - (max(0, kv - n - window + 1) // 64 if window else 0) for n, kv in zip(q_lens, kvs)]
+    width = max(1, -(-max(kvs) // 64))
     most = max(1, Q8_EXPAND_BYTES // (4 * nkv * page * hd))
-    join, launched, r0 = None, False, 0
+    lib, stream, ws, join, launched, r0 = library(), _stream(), batch.ws, None, False, 0
+    T, q_stride, qp, op, bt_stride = q.shape[0], q.stride(0), q.data_ptr(), out.data_ptr(), block_table.stride(0)
+    indptr0, lens0, bt0, sink_p, err = batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), block_table.data_ptr(), _ptr(sinks), error_flag(q.device).data_ptr()
     while True:
         while r0 < R and not pages[r0]:
             r0 += 1
@@ -2414,51 +2416,49 @@ def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nk
             r1 += 1
             if pages[r1 - 1]:
                 end = r1                   # rows behind the last one with a portion are left out
-        after, r1 = r1, end
-        kx = batch.ws.get("attn_q8_keys", (total, nkv, page, hd), torch.bfloat16)
-        vx = batch.ws.get("attn_q8_values", (total, nkv, page, hd), torch.bfloat16)
-        table = batch.ws.get("attn_q8_table", (r1 - r0, width), torch.int32)
-        indptr, lens, bt = batch.q_indptr[r0: r1 + 1], batch.kv_lens[r0: r1], block_table[r0: r1]
-        longest, single = max(q_lens[r0: r1]), min(q_lens[r0: r1]) < 2
-        _check(library().arle_expand_q8(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(indptr), _ptr(lens), _ptr(bt), bt.stride(0),
-                                        page_size, nkv, hd, window, r1 - r0, 2, _ptr(kx), _ptr(vx), total, _ptr(table), width, _stream()), "expand_q8")
-        if hd == 128:
-            splits = prompt_splits_q8(nq, q_lens[r0: r1], max(pages[r0: r1]), q.device)
-            if splits == 1:
-                paged_attention_prefill_tc(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, longest, skip_single=single, sink=sinks)
-                join = None
-            else:
-                join = _prefill_tc_parts(q, out, kx, vx, indptr, lens, table, nq, nkv, page, scale, window, longest, single, sinks, splits, batch.ws)
+        rows, mine = end - r0, q_lens[r0: end]
+        longest, single = max(mine), int(min(mine) < 2)
+        kx = ws.get("attn_q8_keys", (total * nkv * page * hd,), torch.bfloat16).data_ptr()
+        vx = ws.get("attn_q8_values", (total * nkv * page * hd,), torch.bfloat16).data_ptr()
+        table = ws.get("attn_q8_table", (rows * width,), torch.int32).data_ptr()
+        indptr, lens = indptr0 + 4 * r0, lens0 + 4 * r0
+        _check(lib.arle_expand_q8(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), indptr, lens, bt0 + 4 * r0 * bt_stride, bt_stride,
+                                  page_size, nkv, hd, window, rows, 2, kx, vx, total, table, width, stream), "expand_q8")
+        join = None
+        if hd != 128:
+            _check(lib.arle_paged_attention_prefill(qp, q_stride, op, kx, vx, indptr, lens, table, width, nq, nkv, hd, page, float(scale), sink_p, None, 0, window, rows,
+                                                    longest, single, 0, 0.0, 0, None, stream), "paged_attention_prefill")
         else:
-            paged_attention_prefill(q, out, kx, vx, indptr, lens, table, nq, nkv, hd, page, scale, window, longest, skip_single=single, sink=sinks)
-        launched, r0 = True, after
+            splits = prompt_splits_q8(nq, mine, max(pages[r0: end]), q.device)
+            if splits == 1:
+                _check(lib.arle_paged_attention_prefill_tc(qp, q_stride, T, op, kx, vx, total, indptr, lens, table, width, width, nq, nkv, hd, page, float(scale), sink_p,
+                                                           None, 0, window, rows, longest, single, err, 0, 0.0, 0, None, stream), "paged_attention_prefill_tc")
+            else:
+                blocks = nq * -(-longest // 256) * rows * splits
+                part_o = ws.get("attn_q8_prompt_parts", (blocks * 256 * 130,), torch.float32).data_ptr()
+                part_ml = part_o + blocks * 256 * 128 * 4
+                _check(lib.arle_paged_attention_prefill_tc_parts(qp, q_stride, T, op, kx, vx, total, indptr, lens, table, width, width, nq, nkv, hd, page, float(scale),
+                                                                 window, rows, longest, single, err, splits, part_o, part_ml, stream), "paged_attention_prefill_tc_parts")
+
+                def join(args=(part_o, part_ml, op, indptr, lens, nq, nkv, hd, sink_p, window, rows, longest, single, splits, stream)):
+                    _check(lib.arle_paged_prefill_join(*args), "paged_prefill_join")
+        launched, r0 = True, r1
 
 
 def prompt_splits_q8(nq: int, q_lens, pages: int, device) -> int:
     """Parts that the prompt kernel's blocks (a query head, 256 queries) cut their keys into: as many as bring the blocks to the number of SMs, none of
-    fewer than two tiles of 128 keys.  A block takes some 6 us and 2.3 us for each tile, the parts' sums and the joining 3 us: 32 heads with 509 queries
-    behind 1,600 keys, 64 blocks, take PARTS_FIGURE.  Scratch is for the blocks that the launch counts, rows without a portion among them."""
+    fewer than two tiles of 128 keys.  A block takes some 6 us and 2.3 us for each tile, the parts' sums and the joining about 5 us: with the expanding,
+    32 heads with 509 queries and 2,100 keys, 64 blocks, take 53.5 us whole, 44.8 in two parts and 57 in three; 16 heads with 200 queries and 1,500 keys 41
+    us whole and 26 in six to eight.  Scratch is for the blocks that the launch counts, rows without a portion among them."""
     sms = _SM_COUNT.get(device.index) or sm_count(device)
-    tall = -(-max(q_lens) // 256)
-    blocks, counted = nq * sum(-(-n // 256) for n in q_lens if n > 1), nq * tall * len(q_lens)
-    return max(1, min(sms // max(blocks, 1), pages // 4, 4 * sms // counted))
-
-
-def _prefill_tc_parts(q, out, k_cache, v_cache, q_indptr, kv_lens, block_table, nq, nkv, page_size, scale, window: int, longest: int, single: bool, sinks, splits: int, ws):
-    """The tcgen05 prompt kernel with its blocks' keys in parts; returns the call that joins them and writes ``out``."""
-    blocks, rows = nq * -(-longest // 256) * kv_lens.numel() * splits, kv_lens.numel()
-    parts = ws.get("attn_q8_prompt_parts", (blocks * 256 * 130,), torch.float32)
-    part_o, part_ml = _ptr(parts), parts.data_ptr() + blocks * 256 * 128 * 4
-    _check(library().arle_paged_attention_prefill_tc_parts(
-        _ptr(q), q.stride(0), q.shape[0], _ptr(out), _ptr(k_cache), _ptr(v_cache), k_cache.shape[0], _ptr(q_indptr), _ptr(kv_lens), _ptr(block_table),
-        block_table.stride(0), block_table.shape[1], nq, nkv, 128, page_size, float(scale), window, rows, longest, int(single), _ptr(error_flag(q.device)), splits,
-        part_o, part_ml, _stream()), "paged_attention_prefill_tc_parts")
-
-    def join():
-        _check(library().arle_paged_prefill_join(part_o, part_ml, _ptr(out), _ptr(q_indptr), _ptr(kv_lens), nq, nkv, 128, _ptr(sinks), window, rows, longest, int(single),
-                                                 splits, _stream()), "paged_prefill_join")
-
-    return join
+    blocks, tall = 0, 0
+    for n in q_lens:
+        if n > 1:
+            b = (n + 255) // 256
+            blocks += b
+            if b > tall:
+                tall = b
+    return max(1, min(sms // (nq * blocks), pages // 4, 4 * sms // (nq * tall * len(q_lens))))
 
 
 # ------------------------------------------------------------------ a step's tables
