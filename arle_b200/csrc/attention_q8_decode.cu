@@ -64,13 +64,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Blocks of 64 keys that a row's query sees, counted on the grid of absolute positions; a row that sees no key has one (which writes its zeros).
-__device__ __forceinline__ int row_blocks(const DecodeArgs& a, int r) {
+// A row: its token, its keys, the block of 64 keys (on the grid of absolute positions) that its first visible key lies in, and how many blocks its query
+// sees: none if the row has not exactly one query, one (which writes its zeros) if it has no keys.
+struct Row {
+  int t, kv, first, nb;
+};
+__device__ __forceinline__ Row row_of(const DecodeArgs& a, int r) {
   const int t0 = a.q_indptr[r], t1 = a.q_indptr[r + 1], kv = a.kv_lens[r];
-  if (t1 - t0 != 1) return 0;
-  if (kv <= 0) return 1;
-  return (kv + kBlock - 1) / kBlock - first_visible_key(kv - 1, a.window, 0) / kBlock;
+  const int first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock : 0;
+  return Row{t0, kv, first, t1 - t0 != 1 ? 0 : kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first};
 }
+
+template <int HD> constexpr int kPause = HD == 128 ? 6 : 12;      // see where the line is cut
 
 template <int HD, int NT> struct Shape {
   static constexpr int kResident = NT == 1 ? 4 : 3;      // CTAs of an SM: 128 and 168 registers a thread
@@ -89,7 +94,9 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int sum_s[kWarps], start_s[2], cut_s[2], last_s;
+  __shared__ int2 sum_s[kWarps];
+  __shared__ int start_s[2], cut_s[2], last_s;
+  __shared__ Row start_row;
   __shared__ float ml_s[kWarps][NT * 8][2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = a.nq / a.nkv, nkv = a.nkv;
@@ -106,24 +113,36 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
 
   // this CTA's share of the line, and the row where it begins
   const int each = (a.rows + kThreads - 1) / kThreads, r0 = min(tid * each, a.rows), r1 = min(r0 + each, a.rows);
-  int mine = 0;
-  for (int r = r0; r < r1; ++r) mine += row_blocks(a, r);
-  int upto = mine;
+  int mine = 0, mine_rows = 0;
+  Row own{};                                       // the thread's first row
+  for (int r = r1 - 1; r >= r0; --r) {
+    own = row_of(a, r);
+    mine += own.nb;
+    mine_rows += own.nb > 0;
+  }
+  int upto = mine, upto_rows = mine_rows;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += x;
+    const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_rows, o);
+    if (lane >= o) upto += x, upto_rows += y;
   }
-  if (lane == 31) sum_s[warp] = upto;
+  if (lane == 31) sum_s[warp] = make_int2(upto, upto_rows);
   __syncthreads();
-  int total = 0, front = upto - mine;
+  int total = 0, total_rows = 0, front = upto - mine, front_rows = upto_rows - mine_rows;
   for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) front += sum_s[w];
-    total += sum_s[w];
+    const int2 x = sum_s[w];
+    if (w < warp) front += x.x, front_rows += x.y;
+    total += x.x, total_rows += x.y;
   }
-  total *= nkv;
+  // A CTA that goes on to another pair waits for that one's first tiles behind everybody's loads, about as long as `pause` blocks take it (6 us; 64 rows of
+  // ragged lengths, CTAs of one, two and three pieces with the same keys: done after 51, 58 and 63 us).  So where shares are long a pair counts that
+  // much more on the line, at its start; short shares are one piece each, mostly.
+  const int pause = (total * nkv + (int)gridDim.x - 1) / (int)gridDim.x >= 4 * kPause<HD> ? kPause<HD> : 0;
+  total = (total + pause * total_rows) * nkv;
+  front = (front + pause * front_rows) * nkv;
+  mine = (mine + pause * mine_rows) * nkv;
   // Cuts of the line: every `share` blocks, moved to the end, or else to the start, of the pair that they fall into where that is at most `slack` blocks
-  // away: a piece costs as much as about two blocks beside its keys (its first tiles' latency and the joining), and pairs shorter than a share stay whole.
+  // away: a piece costs its first tiles' latency and the joining beside its keys, and pairs shorter than a share stay whole.
   const int share = (total + gridDim.x - 1) / gridDim.x, slack = min(3, (share + 1) / 2);
   if ((int)blockIdx.x * share >= total) return;
 #pragma unroll
@@ -131,17 +150,21 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     const int at = ((int)blockIdx.x + i) * share;
     if (at >= total) {
       if (tid == 0) cut_s[i] = total;
-    } else if (at >= front * nkv && at < (front + mine) * nkv) {
-      int r = r0, row_at = front * nkv, nb = row_blocks(a, r);
-      while (at >= row_at + nb * nkv) {
-        row_at += nb * nkv;
-        nb = row_blocks(a, ++r);
+    } else if (at >= front && at < front + mine) {
+      int r = r0, row_at = front;
+      Row x = own;
+      for (;;) {
+        const int n = x.nb > 0 ? (x.nb + pause) * nkv : 0;
+        if (at < row_at + n) break;
+        row_at += n;
+        x = row_of(a, ++r);
       }
-      const int from = (at - row_at) % nb, left = nb - from;
-      cut_s[i] = from == 0 ? at : left <= slack ? at + left : from <= slack ? at - from : at;
+      const int from = (at - row_at) % (x.nb + pause), blk = max(0, from - pause), left = x.nb - blk;
+      cut_s[i] = from == 0 ? at : left <= slack ? at - from + x.nb + pause : blk <= slack ? at - from : at;
       if (i == 0) {
         start_s[0] = r;
         start_s[1] = row_at;
+        start_row = x;
       }
     }
   }
@@ -149,6 +172,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   const int begin = cut_s[0], end = cut_s[1];
   if (begin >= end) return;
   int row = start_s[0], row_at = start_s[1];      // the row and where its blocks begin on the line
+  Row at_row = start_row;
 
   auto finish = [&](int t, int head, int d, float M, float L, const float4& O) {
     if (a.sinks) L += exp2f(a.sinks[head] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
@@ -158,16 +182,16 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   };
 
   for (int pos = begin; pos < end;) {
-    int nb = row_blocks(a, row);
-    while (pos >= row_at + nb * nkv) {
-      row_at += nb * nkv;
-      nb = row_blocks(a, ++row);
+    for (;;) {
+      const int n = at_row.nb > 0 ? (at_row.nb + pause) * nkv : 0;
+      if (pos < row_at + n) break;
+      row_at += n;
+      at_row = row_of(a, ++row);
     }
-    const int h = (pos - row_at) / nb, pair_at = row_at + h * nb;
-    const int blk0 = pos - pair_at, blk1 = min(nb, end - pair_at);
-    const int t = a.q_indptr[row], kv = a.kv_lens[row];
-    const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0;
-    const int base_key = lo / kBlock * kBlock;
+    const int nb = at_row.nb, t = at_row.t, kv = at_row.kv;
+    const int h = (pos - row_at) / (nb + pause), pair_at = row_at + h * (nb + pause), keys_at = pair_at + pause;
+    const int blk0 = max(0, pos - keys_at), blk1 = min(nb, end - keys_at);
+    const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0, base_key = at_row.first * kBlock;
     const int tile0 = (base_key + blk0 * kBlock) / kTile + warp, tile_end = min((base_key + blk1 * kBlock) / kTile, (kv + kTile - 1) / kTile);
     const int* bt = a.block_table + (size_t)row * a.bt_stride;
 
@@ -451,7 +475,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     }
     if (!whole) {
       // the cuts inside this pair are those farther than `slack` from both of its ends; the piece in front of cut k belongs to CTA k - 1
-      const int cut0 = (pair_at + slack) / share + 1, cut1 = (pair_at + nb - slack - 1) / share, pieces = cut1 - cut0 + 2, first_cta = cut0 - 1;
+      const int cut0 = (keys_at + slack) / share + 1, cut1 = (keys_at + nb - slack - 1) / share, pieces = cut1 - cut0 + 2, first_cta = cut0 - 1;
       __syncthreads();
       if (tid == 0) {
         __threadfence();
@@ -521,7 +545,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
       }
     }
     __syncthreads();
-    pos += blk1 - blk0;
+    pos = blk1 == nb ? keys_at + nb : end;
   }
 }
 
