@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(256) expand_q8_kernel(ExpandArgs a) {
   const int logical = span.x + page - at_s, kv = a.kv_lens[r], first = logical * kExpanded;
   if (head == 0) {
     int* t = a.table_out + (long)r * a.table_width;
-    if (tid == 0) t[logical] = page;
+    if (tid == 0 && logical < a.table_width) t[logical] = page;
     if (logical == span.x)
       for (int j = tid; j < a.table_width; j += 256)
         if (j < span.x || j >= span.y) t[j] = -1;

@@ -2353,7 +2353,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
 
     ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
     bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens read the codes as they are; the keys and values that
-    portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels."""
+    portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels.  A captured call of decoded tokens goes by the
+    lengths on the device when it is replayed; one with portions keeps room for the lengths that the host's copies had, and those have to stay."""
     (T, width), (q_stride, q_unit), vd = q.shape, q.stride(), hd if vd is None else int(vd)
     if q_unit != 1 or width != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
         raise KernelError("paged_attention_q8: q must be [T, nq*hd] with unit inner stride and out contiguous [T, nq*vd]")
@@ -2365,7 +2366,7 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     i32, (bt_stride, bt_unit) = torch.int32, block_table.stride()
     if positions.dtype is not i32 or row_of_token.dtype is not i32 or block_table.dtype is not i32 or bt_unit != 1:
         raise KernelError("paged_attention_q8: positions, row_of_token and block_table must be int32, rows of the block table contiguous")
-    sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, int(window) if window else 0
+    sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, max(0, int(window)) if window else 0
     _on_cuda("paged_attention_q8", q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table)
     if T == 0:
         return

@@ -207,6 +207,40 @@ def test_the_plain_kernel_set_and_columns_of_a_wider_row():
     _near(_run(s), want, 128, 0.0, 400)
 
 
+@pytest.mark.parametrize("rows", [[(1, 70), (1, 300)], [(40, 70), (1, 300)]])
+def test_no_window(rows):
+    s = _case(rows, 8, 2, 128, 16)
+    for batch in (True, False):
+        all_keys = _run(s, None, batch=batch)
+        for window in (0, -5, 10 ** 6):
+            assert torch.equal(_run(s, window, batch=batch), all_keys)
+
+
+def test_a_captured_step_with_portions():
+    """The queries and codes change between replays, the lengths stay; decoded tokens run beside the prompt kernel, its parts are joined behind them."""
+    s = _case([(70, 800), (1, 700), (300, 301), (1, 1)], 8, 2, 128, 16, seed=3)
+    out = torch.empty(s.T, s.nq * s.hd, dtype=BF, device=DEV)
+
+    def call():
+        ops.paged_attention_q8(s.q, out, s.k, s.v, s.ks, s.vs, s.positions, s.row_of, s.bt, s.nq, s.nkv, s.hd, s.ps, s.scale, None, batch=s.batch)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for step in range(3):
+        s.q.copy_(torch.randn(s.q.shape, generator=torch.Generator().manual_seed(step)))
+        s.ks *= 2
+        graph.replay()
+        _near(out, _want(s), 128, 2.0 ** -8, 800)
+    ops.check_errors(DEV)
+
+
 def test_captured_steps_that_share_their_scratch():
     """Two graphs over one workspace, replayed in turn while lengths, queries and codes change."""
     a, b = _case([(1, 700), (1, 90)], 16, 2, 128, 16, seed=1), _case([(1, 200)] * 9, 16, 2, 128, 16, seed=2)
