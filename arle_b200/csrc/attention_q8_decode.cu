@@ -42,6 +42,7 @@ struct DecodeArgs {
   float scale_log2;
   const float* sinks;
   int beside;
+  const int *positions, *row_of_token;      // null: rows are the step's rows; else its tokens, each by itself
 };
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -65,14 +66,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 
 // A row: its token, its keys, the block of 64 keys (on the grid of absolute positions) that its first visible key lies in, and how many blocks its query
-// sees: none if the row has not exactly one query, one (which writes its zeros) if it has no keys.
+// sees: none if the row has not exactly one query, one (which writes its zeros) if it has no keys.  By tokens a token is a row of the keys up to its own.
 struct Row {
-  int t, kv, first, nb;
+  int t, kv, first, nb, table;
 };
 __device__ __forceinline__ Row row_of(const DecodeArgs& a, int r) {
+  if (a.positions) {
+    const int kv = a.positions[r] + 1, first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock : 0;
+    return Row{r, kv, first, kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first, a.row_of_token[r]};
+  }
   const int t0 = a.q_indptr[r], t1 = a.q_indptr[r + 1], kv = a.kv_lens[r];
   const int first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock : 0;
-  return Row{t0, kv, first, t1 - t0 != 1 ? 0 : kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first};
+  return Row{t0, kv, first, t1 - t0 != 1 ? 0 : kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first, r};
 }
 
 template <int HD> constexpr int kPause = HD == 128 ? 6 : 12;      // see where the line is cut
@@ -193,7 +198,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     const int blk0 = max(0, pos - keys_at), blk1 = min(nb, end - keys_at);
     const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0, base_key = at_row.first * kBlock;
     const int tile0 = (base_key + blk0 * kBlock) / kTile + warp, tile_end = min((base_key + blk1 * kBlock) / kTile, (kv + kTile - 1) / kTile);
-    const int* bt = a.block_table + (size_t)row * a.bt_stride;
+    const int* bt = a.block_table + (size_t)at_row.table * a.bt_stride;
 
     // Page of the tile (P16) or of its key lane & 15; -1: nothing of it is seen.
     auto page_of = [&](int tile) -> int {
@@ -578,14 +583,14 @@ int launch_by(const DecodeArgs& a, int ctas, cudaStream_t s) {
 
 }  // namespace
 
-// Rows with one query; others are left alone.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 2], counters int32
+// Rows with one query; others are left alone.  With positions and row_of_token (int32 [rows]) the rows are the step's tokens, all of them.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 2], counters int32
 // [rows * nkv], zero before the first launch (the kernel leaves them zero).
 // beside: the kernel in front of it on the stream is a prompt kernel launched in stream order that writes none of what this one reads; then this one starts
 // as soon as that one's last block has started, on the SMs that it leaves free.  (It starts when all in front of that kernel is done.)
 ARLE_API int arle_attention_q8_decode(const void* q, int q_row_stride, void* out, const void* k_cache, const void* v_cache, const float* k_scale,
                                       const float* v_scale, const int* q_indptr, const int* kv_lens, const int* block_table, int bt_stride, float* part_o,
                                       float* part_ml, int* counters, int nq, int nkv, int hd, int page_size, float scale, int window, const float* sinks, int rows,
-                                      int ctas, int beside, cudaStream_t s) {
+                                      int ctas, int beside, const int* positions, const int* row_of_token, cudaStream_t s) {
   if (rows <= 0) return 0;
   if (nkv <= 0 || nq <= 0 || nq % nkv || nq / nkv > 16 || page_size <= 0 || ctas <= 0 || (hd != 64 && hd != 128) || q_row_stride % 8) return ARLE_E_UNSUPPORTED;
   int shift = -1;
@@ -593,6 +598,6 @@ ARLE_API int arle_attention_q8_decode(const void* q, int q_row_stride, void* out
     for (shift = 0; (1 << shift) < page_size; ++shift) {}
   const DecodeArgs a{(const __nv_bfloat16*)q, q_row_stride, (__nv_bfloat16*)out, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, q_indptr,
                      kv_lens, block_table, bt_stride, part_o, part_ml, counters, nq, nkv, page_size, shift, window, rows, scale * 1.4426950408889634f, sinks,
-                     beside && !(pdl_enabled() & 1)};
+                     beside && !(pdl_enabled() & 1), positions, row_of_token};
   return hd == 128 ? launch_by<128>(a, ctas, s) : launch_by<64>(a, ctas, s);
 }

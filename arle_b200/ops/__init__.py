@@ -133,7 +133,7 @@ _SIGNATURES = {
     "arle_store_q8": [_P, _I, _P, _I, _I, _P, _I, _P, _P, _P, _P, ctypes.c_long, _I, _I, _I, _I, _P],
     "arle_expand_q8": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P],
     "arle_attention_q8": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P],
-    "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _P],
+    "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _P, _P, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
@@ -2374,24 +2374,41 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
     if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
             and not (qp | kp | vp | op) % 16):
-        beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks) if (
-            batch.max_q_len > 1) else (False, None)
-        if batch.num_single > 0:
+        rows, beside, join, pos_p, row_p = batch.num_rows, False, None, None, None
+        if batch.max_q_len > 1:
+            if _by_tokens_q8(batch, nkv, hd, w):
+                rows, pos_p, row_p = T, positions.data_ptr(), row_of_token.data_ptr()
+            else:
+                beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
+        if batch.num_single > 0 or pos_p is not None:
             # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
             ctas = (4 if nq <= 8 * nkv else 3) * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
             parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
-            counters = batch.ws.get_zeroed("attn_q8_counters", (batch.num_rows * nkv,), torch.int32)
+            counters = batch.ws.get_zeroed("attn_q8_counters", (rows * nkv,), torch.int32)
             at = parts.data_ptr()
             _check(lib.arle_attention_q8_decode(
                 qp, q_stride, op, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(),
                 block_table.data_ptr(), bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
-                batch.num_rows, ctas, int(beside), _stream()), "attention_q8_decode")
+                rows, ctas, int(beside), pos_p, row_p, _stream()), "attention_q8_decode")
         if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
             join()
         return
     _check(lib.arle_attention_q8(
         qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
         block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
+
+
+# Bytes of codes up to which a step's short portions are read token by token.
+Q8_TOKENS_BYTES = 64 << 20
+
+
+def _by_tokens_q8(batch, nkv: int, hd: int, window: int) -> bool:
+    """Whether a step with portions runs token by token, each token a row of the keys up to its own."""
+    keys = 0
+    for n, kv in zip(batch.q_lens, batch.kv_lens_host):
+        if n > 1:
+            keys += n * (min(kv, window) if window else kv)
+    return keys * nkv * hd * 2 <= Q8_TOKENS_BYTES
 
 
 def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks):
