@@ -99,7 +99,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int2 sum_s[kWarps];
+  __shared__ int4 sum_s[kWarps];
   __shared__ int start_s[2], cut_s[2], last_s;
   __shared__ Row start_row;
   __shared__ float ml_s[kWarps][NT * 8][2];
@@ -118,12 +118,13 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
 
   // this CTA's share of the line, and the row where it begins
   const int each = (a.rows + kThreads - 1) / kThreads, r0 = min(tid * each, a.rows), r1 = min(r0 + each, a.rows);
-  int mine = 0, mine_rows = 0;
+  int mine = 0, mine_rows = 0, longest = 0;
   Row own{};                                       // the thread's first row
   for (int r = r1 - 1; r >= r0; --r) {
     own = row_of(a, r);
     mine += own.nb;
     mine_rows += own.nb > 0;
+    longest = max(longest, own.nb);
   }
   int upto = mine, upto_rows = mine_rows;
 #pragma unroll
@@ -131,13 +132,15 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     const int x = __shfl_up_sync(0xffffffffu, upto, o), y = __shfl_up_sync(0xffffffffu, upto_rows, o);
     if (lane >= o) upto += x, upto_rows += y;
   }
-  if (lane == 31) sum_s[warp] = make_int2(upto, upto_rows);
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) sum_s[warp] = make_int4(upto, upto_rows, longest, 0);
   __syncthreads();
   int total = 0, total_rows = 0, front = upto - mine, front_rows = upto_rows - mine_rows;
   for (int w = 0; w < kWarps; ++w) {
-    const int2 x = sum_s[w];
+    const int4 x = sum_s[w];
     if (w < warp) front += x.x, front_rows += x.y;
     total += x.x, total_rows += x.y;
+    longest = max(longest, x.z);
   }
   // A CTA that goes on to another pair waits for that one's first tiles behind everybody's loads, about as long as `pause` blocks take it (6 us; 64 rows of
   // ragged lengths, CTAs of one, two and three pieces with the same keys: done after 51, 58 and 63 us).  So where shares are long a pair counts that
@@ -148,7 +151,10 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   mine = (mine + pause * mine_rows) * nkv;
   // Cuts of the line: every `share` blocks, moved to the end, or else to the start, of the pair that they fall into where that is at most `slack` blocks
   // away: a piece costs its first tiles' latency and the joining beside its keys, and pairs shorter than a share stay whole.
-  const int share = (total + gridDim.x - 1) / gridDim.x, slack = min(3, (share + 1) / 2);
+  // The longest pair is in no more pieces than pay: a block takes a CTA alone some 0.5 us, and the CTA that joins reads G * HD numbers of every piece, one
+  // after the other; share * 0.5 us + longest / share * G * 25 ns is least at 0.22 sqrt(longest * G).  (One row of 4,096 with 64 heads on 8: 21.3 us with
+  // pieces of one block, 14.4 with four.)
+  const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (int)(0.22f * sqrtf((float)longest * G) + 0.5f)), slack = min(3, (share + 1) / 2);
   if ((int)blockIdx.x * share >= total) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
