@@ -220,10 +220,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
     int page_size, float scale_log2, HeadTail<__nv_bfloat16> tail, int window, int skip_single, int nyb, int nblocks, int ticket_slot, int* __restrict__ err,
     int keep_arg, float cap_arg, float scale_over_cap, int chunk_arg, const float* __restrict__ pb, const __nv_bfloat16* __restrict__ v_cache,
     int row_behind, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
-  constexpr bool EXT = FORM == 1, SIG = FORM == 2, PARTS = FORM == 3;
   pdl_launch_dependents();
-  // The form in parts is launched beside the kernel that writes its keys, values and tables, and sets itself up meanwhile; the lengths are older.
-  if (!PARTS) pdl_wait();
+  pdl_wait();
+  constexpr bool EXT = FORM == 1, SIG = FORM == 2, PARTS = FORM == 3;
   const int chunk = SIG ? chunk_arg : 0;
   const int keep_first = EXT ? keep_arg : 0;
   const float cap_log2 = EXT ? cap_arg : 0.f;
@@ -276,7 +275,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
-  if (PARTS) pdl_wait();
   // columns: S of tile A, S of tile B, O of tile A, O of tile B (128 each).  P of a tile is written over
   // the first 64 columns of its S (two bfloat16 a column) once the row of S is in registers.
   const volatile int* aborted = &abort_flag;
@@ -344,12 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
           }
         }
         const int* bt = block_table + (size_t)blk.r * bt_stride;
-        auto table_at = [](const int* p) { return PARTS ? __ldcg(p) : __ldg(p); };      // no non-coherent reads of what the kernel in front may still write
         // Page ids come 32 at a time, one per lane, with the next 32 already in flight, so that no
         // tile waits for a read of the block table; a lane picks its page with a shuffle.
         int p0 = blk.template tile_key<EXT>(0) / page_size;
-        int cur = table_at(bt + min(p0 + lane, bt_width - 1));
-        int nxt = table_at(bt + min(p0 + 32 + lane, bt_width - 1));
+        int cur = __ldg(bt + min(p0 + lane, bt_width - 1));
+        int nxt = __ldg(bt + min(p0 + 32 + lane, bt_width - 1));
         bool stop = false;
         for (int j = 0; j < blk.ntiles; ++j) {
           const int st = issued % kStages;
@@ -357,13 +354,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
           const int key0 = blk.template tile_key<EXT>(j) + c * 16;
           if (EXT && blk.template tile_key<EXT>(j) / page_size - p0 >= 64) {          // from the kept tiles on to the window's: start again there
             p0 = blk.template tile_key<EXT>(j) / page_size;
-            cur = table_at(bt + min(p0 + lane, bt_width - 1));
-            nxt = table_at(bt + min(p0 + 32 + lane, bt_width - 1));
+            cur = __ldg(bt + min(p0 + lane, bt_width - 1));
+            nxt = __ldg(bt + min(p0 + 32 + lane, bt_width - 1));
           }
           while (blk.template tile_key<EXT>(j) / page_size - p0 >= 32) {
             cur = nxt;
             p0 += 32;
-            nxt = table_at(bt + min(p0 + 32 + lane, bt_width - 1));
+            nxt = __ldg(bt + min(p0 + 32 + lane, bt_width - 1));
           }
           const int pi = key0 / page_size;
           const int rel = pi - p0;                                // 0 .. 63: a tile spans at most 8 pages
@@ -406,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_prefill_tc_kernel(
             for (int i = lane; i < 16 * 16; i += 32) {                          // 16 rows of 16 pieces of 16 bytes, swizzled as TMA does
               const int r = i >> 4, piece = i & 15;
               *reinterpret_cast<uint4*>(tile_s + st * TILE + (piece >> 3) * SUB + (cut_box * 16 + r) * 128 + (((piece & 7) ^ (r & 7)) << 4)) =
-                  r < cut ? (PARTS ? __ldcg(src + i) : src[i]) : make_uint4(0, 0, 0, 0);
+                  r < cut ? src[i] : make_uint4(0, 0, 0, 0);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
@@ -839,7 +836,7 @@ static int launch_prefill_tc(const void* q, int q_row_stride, int num_tokens, vo
   const int ctas = (int)(nblocks < sms ? nblocks : sms);
   static unsigned int launches = 0;
   const int ticket_slot = (int)(launches++ % kTicketSlots);
-  cudaError_t e = launch_kernel_as(form == 3 || (pdl_enabled() & 1), kernel, dim3(ctas), dim3(kThreads), smem, s, 1, mq, mk, mv, (__nv_bfloat16*)out,
+  cudaError_t e = launch_kernel(kernel, dim3(ctas), dim3(kThreads), smem, s, 1, mq, mk, mv, (__nv_bfloat16*)out,
                                 q_indptr, kv_lens, block_table, bt_stride, bt_width, nq, nkv, page_size,
                                 scale * 1.4426950408889634f, HeadTail<__nv_bfloat16>{sinks, (const __nv_bfloat16*)gate, gate_stride}, window, skip_single, nyb, (int)nblocks, ticket_slot, err,
                                 window > 0 ? keep_first : 0, softcap > 0.f ? softcap * 1.4426950408889634f : 0.f,
@@ -860,7 +857,6 @@ ARLE_API int arle_paged_attention_prefill_tc(const void* q, int q_row_stride, in
 
 // The usual form with every block's key tiles in `splits` parts (2 or more), whose sums go to part_o, float32 [blocks * splits * 256 * 128], and part_ml,
 // float32 [blocks * splits * 256 * 2], blocks = nq * ceil(max_q_len / 256) * rows; arle_paged_prefill_join then writes out (and needs the same arguments).
-// It starts beside the kernel in front of it on the stream, which has to be one launched in stream order that does not write q_indptr and kv_lens.
 ARLE_API int arle_paged_attention_prefill_tc_parts(const void* q, int q_row_stride, int num_tokens, void* out, const void* k_cache, const void* v_cache,
                                                    long long cache_pages, const int* q_indptr, const int* kv_lens, const int* block_table, int bt_stride,
                                                    int bt_width, int nq, int nkv, int hd, int page_size, float scale, int window, int rows, int max_q_len,
