@@ -77,7 +77,7 @@ __device__ __forceinline__ void put(uint8_t* dst, const Pack<T, VEC>& p, float i
 // A group has `warps` warps; where it has one, a block's warps take neighbouring heads (of the keys, then of the values).  `chunk`: tokens among which a
 // group looks for the starts of runs (at most 31).  VEC: numbers of a load, 16 bytes or one.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_q8_kernel(StoreSide ks, StoreSide vs, const int* __restrict__ slot_mapping, int tokens, int chunk,
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) store_q8_kernel(StoreSide ks, StoreSide vs, const int* slot_mapping, int tokens, int chunk,
                                                                                int nkv, int page_size, int places, int warps) {
   pdl_launch_dependents();
   pdl_wait();
@@ -250,7 +250,8 @@ int launch_store(StoreSide k, StoreSide v, const int* slot_mapping, int tokens, 
   }
   const int threads = warps == 1 ? 128 : warps * 32;
   const dim3 grid((tokens + chunk - 1) / chunk, warps == 1 ? (2 * nkv + 3) / 4 : 2 * nkv);
-  launch_kernel(wide ? store_q8_kernel<T, 16 / sizeof(T)> : store_q8_kernel<T, 1>, grid, dim3(threads), 0, s, 1, k, v, slot_mapping, tokens, chunk, nkv, page_size,
+  // early: 15,000 tokens behind one another 22.6 -> 20.8 us, one token 7.4 -> 6.9 (launched one by one)
+  launch_early(wide ? store_q8_kernel<T, 16 / sizeof(T)> : store_q8_kernel<T, 1>, grid, dim3(threads), 0, s, 1, k, v, slot_mapping, tokens, chunk, nkv, page_size,
                 places, warps);
   return launch_status();
 }
