@@ -2308,10 +2308,14 @@ def _q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, 
                       f"{tuple(k_scale.shape)}, {v_scale.dtype} {tuple(v_scale.shape)}")
 
 
-def _on_cuda(what: str, *tensors) -> None:
+def _on_device(what: str, *tensors) -> None:
+    """Every tensor on the current device, whose stream the launch goes to."""
+    d = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise KernelError(f"{what}: a tensor is on {t.device}: arle_b200 kernels run on CUDA devices only (there is no CPU path)")
+        if t.get_device() != d or d < 0:
+            raise KernelError(f"{what}: a tensor is on {t.device}, another on {tensors[0].device}: arle_b200 kernels run on one CUDA device (there is no CPU path)")
+    if d != torch._C._cuda_getDevice():
+        raise KernelError(f"{what}: the tensors are on cuda:{d}, which is not the current device")
 
 
 def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
@@ -2335,7 +2339,7 @@ def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, h
     pages = _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
     if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
         raise KernelError("store_q8: slot_mapping must be contiguous int32")
-    _on_cuda("store_q8", k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale)
+    _on_device("store_q8", k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale)
     if T == 0:
         return
     _check(library().arle_store_q8(k.data_ptr(), k_stride, v.data_ptr(), v_stride, _dt(k), slot_mapping.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
@@ -2349,7 +2353,8 @@ Q8_EXPAND_BYTES = 1 << 30
 def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table, nq: int, nkv: int, hd: int, page_size: int, scale: float,
                        window, batch=None, vd: int = None, sink=None) -> None:
     """Causal attention of this step's queries over a paged cache of 8 bits (``store_q8``): ``paged_attention`` with e4m3 codes and their scales
-    in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros.
+    in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros; with a
+    ``batch``, rows of q and out behind its last token are left alone.
 
     ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
     bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens read the codes as they are; the keys and values that
@@ -2367,7 +2372,7 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     if positions.dtype is not i32 or row_of_token.dtype is not i32 or block_table.dtype is not i32 or bt_unit != 1:
         raise KernelError("paged_attention_q8: positions, row_of_token and block_table must be int32, rows of the block table contiguous")
     sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, max(0, int(window)) if window else 0
-    _on_cuda("paged_attention_q8", q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table)
+    _on_device("paged_attention_q8", q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table)
     if T == 0:
         return
     qp, kp, vp, op, lib = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), library()
@@ -2377,7 +2382,7 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         rows, beside, join, pos_p, row_p = batch.num_rows, False, None, None, None
         if batch.max_q_len > 1:
             if _by_tokens_q8(batch, nkv, hd, w):
-                rows, pos_p, row_p = T, positions.data_ptr(), row_of_token.data_ptr()
+                rows, pos_p, row_p = min(T, sum(batch.q_lens)), positions.data_ptr(), row_of_token.data_ptr()
             else:
                 beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0 or pos_p is not None:
@@ -2393,6 +2398,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
             join()
         return
+    if batch is not None:
+        T = min(T, sum(batch.q_lens))
     _check(lib.arle_attention_q8(
         qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
         block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
@@ -2493,16 +2500,17 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
     cache.  Such a step leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
     R, T = slots.numel(), positions.numel()
-    every = (slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table, status)
-    i32 = torch.int32
+    every = (status, slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table)
+    i32, d = torch.int32, status.get_device()
     for t in every:
-        if t.dtype is not i32 or not t.is_contiguous() or not t.is_cuda:
-            _on_cuda("step_tables", *every)
-            raise KernelError(f"step_tables: every tensor must be contiguous int32, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+        if t.dtype is not i32 or not t.is_contiguous() or t.get_device() != d:
+            raise KernelError(f"step_tables: every tensor must be contiguous int32 on status's device ({status.device}), got {t.dtype} {tuple(t.shape)} with strides "
+                              f"{t.stride()} on {t.device}")
     if (starts.numel() != R or q_lens.numel() != R or q_indptr.numel() != R + 1 or kv_lens.numel() != R or row_of_token.numel() != T or slot_of_token.numel() != T
             or slot_mapping.numel() != T or status.numel() != 1 or block_table.dim() != 2 or block_table.shape[0] != R or page_table.dim() != 2):
         raise KernelError("step_tables: slots, starts, q_lens and kv_lens are [R], q_indptr [R + 1], the tokens' tables [T], block_table [R, width], "
                           "page_table [slots, pages], status [1]")
+    _on_device("step_tables", status)
     max_slots, table_width = page_table.shape
     _check(library().arle_step_tables(
         slots.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), R, new_pages.data_ptr(), new_pages.numel(), page_table.data_ptr(), max_slots, table_width, int(num_pages),

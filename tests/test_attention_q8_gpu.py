@@ -216,6 +216,26 @@ def test_no_window(rows):
             assert torch.equal(_run(s, window, batch=batch), all_keys)
 
 
+@pytest.mark.parametrize("rows", [[(1, 70), (1, 300)], [(3, 70), (1, 300)], [(200, 1500), (1, 300)]], ids=["decoded", "by tokens", "portions"])
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+def test_rows_behind_the_last_token_are_left_alone(rows, dtype):
+    """A padded batch: queries without a request, whose positions and rows are not numbers that anything may be read by."""
+    s = _case(rows, 8, 8, 128, 16, dtype=dtype)
+    want, pad = _want(s), torch.full((5,), 2 ** 30, dtype=torch.int32, device=DEV)
+    s.q, s.positions, s.row_of = torch.cat([s.q, s.q[:1].expand(5, -1)]), torch.cat([s.positions, pad]), torch.cat([s.row_of, pad])
+    real, s.T = s.T, s.T + 5
+    out = _run(s)
+    assert (out[real:] == 7.0).all()
+    _near(out[:real], want, 128, 2.0 ** -8, 1500)
+
+
+def test_tensors_of_another_device():
+    s = _case([(1, 70)], 8, 2, 128, 16)
+    s.ks = s.ks.cpu()
+    with pytest.raises(ops.KernelError, match="cpu"):
+        _run(s)
+
+
 def test_a_captured_step_with_portions():
     """The queries and codes change between replays, the lengths stay; decoded tokens run beside the prompt kernel, its parts are joined behind them."""
     s = _case([(70, 800), (1, 700), (300, 301), (1, 1)], 8, 2, 128, 16, seed=3)
