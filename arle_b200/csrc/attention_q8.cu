@@ -43,11 +43,12 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
   for (int i = 0; i < kQuads; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   for (int i0 = w * 32; i0 < nvis; i0 += kWarps * 32) {
     const int j = lo + i0 + lane;
-    const bool seen = i0 + lane < nvis;
+    const int page = i0 + lane < nvis ? bt[j / page_size] : -1;
+    const bool seen = page >= 0;                     // an empty step's tables have no pages
     float sc = -INFINITY, vs = 0.f;
     long row = 0;
     if (seen) {
-      const long unit = (long)bt[j / page_size] * nkv + kvh;
+      const long unit = (long)page * nkv + kvh;
       row = unit * page_size + j % page_size;
       const float ks = k_scale[unit];
       vs = v_scale[unit];

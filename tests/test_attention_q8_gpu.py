@@ -156,7 +156,9 @@ PORTIONS = [[(70, 70)], [(300, 700)], [(5, 90), (1, 400), (129, 129), (1, 1), (2
 @pytest.mark.parametrize("rows", PORTIONS, ids=["70", "300", "mixed", "three"])
 @pytest.mark.parametrize("hd,ps", [(128, 16), (64, 64), (128, 12)])
 @pytest.mark.parametrize("window,sink", [(None, False), (40, False), (256, True)])
-def test_portions(rows, hd, ps, window, sink, monkeypatch):
+@pytest.mark.parametrize("by_tokens", [True, False], ids=["by tokens", "expanded"])
+def test_portions(rows, hd, ps, window, sink, by_tokens, monkeypatch):
+    monkeypatch.setattr(ops, "Q8_TOKENS_BYTES", 1 << 40 if by_tokens else 0)
     s = _case(rows, 8, 2, hd, ps, seed=7)
     if window:
         for r, (n, kv) in enumerate(rows):
@@ -165,7 +167,7 @@ def test_portions(rows, hd, ps, window, sink, monkeypatch):
     sinks = torch.randn(8, generator=torch.Generator().manual_seed(5)).to(DEV) if sink else None
     want = _want(s, window, sinks)
     out = _run(s, window, sinks)
-    _near(out, want, hd, 2.0 ** -8, max(s.kvs))
+    _near(out, want, hd, 2.0 ** -11 if by_tokens else 2.0 ** -8, max(s.kvs))
     _near(_run(s, window, sinks, batch=False), want, hd, 0.0, max(s.kvs))
     assert torch.equal(_run(s, window, sinks), out)
     monkeypatch.setattr(ops, "Q8_EXPAND_BYTES", 1)             # every row by itself: in how many parts its keys are summed goes by the rows that run together
@@ -179,6 +181,7 @@ def test_portions_in_parts(splits, rows, window, monkeypatch):
     """The prompt kernel's key tiles in any number of parts, more than there are tiles among them."""
     s = _case(rows, 8, 2, 128, 16, seed=9)
     monkeypatch.setattr(ops, "prompt_splits_q8", lambda *a: splits)
+    monkeypatch.setattr(ops, "Q8_TOKENS_BYTES", 0)
     for sinks in (None, torch.randn(8, generator=torch.Generator().manual_seed(5)).to(DEV)):
         out = _run(s, window, sinks)
         _near(out, _want(s, window, sinks), 128, 2.0 ** -8, max(s.kvs))
@@ -227,6 +230,48 @@ def test_rows_behind_the_last_token_are_left_alone(rows, dtype):
     out = _run(s)
     assert (out[real:] == 7.0).all()
     _near(out[:real], want, 128, 2.0 ** -8, 1500)
+
+
+def test_an_empty_step():
+    """What step_tables leaves of a step that is not in order: no row has queries or keys, no page is there; nothing is read, in whatever form."""
+    for dtype, bytes_ in ((BF, 1 << 40), (BF, 0), (torch.float32, 0)):
+        s = _case([(30, 300), (1, 70)], 8, 2, 128, 16, dtype=dtype)
+        for x in (s.batch.q_indptr, s.batch.kv_lens, s.positions, s.row_of):
+            x.zero_()
+        s.bt.fill_(-1)
+        before, ops.Q8_TOKENS_BYTES = ops.Q8_TOKENS_BYTES, bytes_
+        try:
+            _run(s)
+        finally:
+            ops.Q8_TOKENS_BYTES = before
+        torch.cuda.synchronize()
+
+
+def test_offsets_beyond_32_bits():
+    """Caches of more than 2^32 codes: the pages of a request at their end, for the store, the decoded tokens, portions, and the general kernel."""
+    nkv, hd, ps, rows = 8, 128, 16, [(1, 700), (200, 1100), (1, 33)]
+    small = _case(rows, 16, nkv, hd, ps)
+    pages = 2 ** 32 // (nkv * hd * ps) + 200
+    shift = pages - small.k.shape[0]
+    s = _case(rows, 16, nkv, hd, ps)
+    big = {}
+    for n in ("k", "v"):
+        big[n] = torch.empty((pages, nkv, ps, hd), dtype=torch.uint8, device=DEV)
+        big[n][shift:] = getattr(small, n).view(torch.uint8)
+        setattr(s, n, big[n].view(E4M3))
+    for n in ("ks", "vs"):
+        x = torch.full((pages, nkv), math.nan, device=DEV)
+        x[shift:] = getattr(small, n)
+        setattr(s, n, x)
+    s.bt = torch.where(s.bt >= 0, s.bt + shift, s.bt)
+    for batch in (True, False):
+        assert torch.equal(_run(s, batch=batch), _run(small, batch=batch))
+    x = [torch.randn(40, nkv * hd, generator=torch.Generator().manual_seed(i)).to(DEV) for i in range(2)]
+    for c, to in ((small, 0), (s, shift)):
+        m = torch.arange(40, dtype=torch.int32, device=DEV) + (to + 2) * ps + 5
+        ops.store_q8(*x, m, c.k, c.v, c.ks, c.vs, nkv, hd, ps)
+    assert torch.equal(big["k"][shift:], small.k.view(torch.uint8)) and torch.equal(big["v"][shift:], small.v.view(torch.uint8))
+    assert torch.equal(s.ks[shift:].nan_to_num(), small.ks.nan_to_num())
 
 
 def test_tensors_of_another_device():
