@@ -185,11 +185,14 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   int row = start_s[0], row_at = start_s[1];      // the row and where its blocks begin on the line
   Row at_row = start_row;
 
-  auto finish = [&](int t, int head, int d, float M, float L, const float4& O) {
+  // Sums lie in the order in which lanes have them, which keeps their way through shared memory free of bank conflicts: place p = 16 j + 2 g + b is
+  // number g * HD / 8 + 2 j + b.  Four places' results (p a multiple of 4) of a head; none: the row has no keys.
+  auto finish = [&](int t, int head, int p, float M, float L, const float4& O, bool none) {
     if (a.sinks) L += exp2f(a.sinks[head] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(O.x / L, O.y / L), hi = __floats2bfloat162_rn(O.z / L, O.w / L);
-    *reinterpret_cast<uint2*>(a.out + ((size_t)t * a.nq + head) * HD + d) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    const float inv = none ? 0.f : 1.0f / L;
+    __nv_bfloat16* to = a.out + ((size_t)t * a.nq + head) * HD + (p % 16 / 2) * (HD / 8) + p / 16 * 2;
+    *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(O.x * inv, O.y * inv);
+    *reinterpret_cast<__nv_bfloat162*>(to + HD / 8) = __floats2bfloat162_rn(O.z * inv, O.w * inv);
   };
 
   for (int pos = begin; pos < end;) {
@@ -451,37 +454,35 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           ml_s[warp][query][1] = x;
         }
         if (query < G) {
-          float* dst = mo + (warp * NT * 8 + query) * S::kPitch + g * (HD / 8);
+          float* dst = mo + (warp * NT * 8 + query) * S::kPitch + 2 * g;
 #pragma unroll
-          for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[nt][j][e] * out_by, o[nt][j][2 + e] * out_by);
+          for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(dst + 16 * j) = make_float2(o[nt][j][e] * out_by, o[nt][j][2 + e] * out_by);
         }
       }
     }
     __syncthreads();
     const bool whole = blk0 == 0 && blk1 == nb;
     const size_t slot = (size_t)blockIdx.x * 2 + (blk0 == 0);      // a CTA has one cut pair's start and one cut pair's further part at most
-    for (int i = tid; i < G * HD; i += kThreads) {
-      const int query = i / HD, d = i % HD;
+    for (int i = tid; i < G * (HD / 4); i += kThreads) {
+      const int query = i / (HD / 4), p = i % (HD / 4) * 4;
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[w][query][0]);
       const float top_s = M == -INFINITY ? 0.f : M;
-      float L = 0.f, O = 0.f;
+      float L = 0.f;
+      float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2f(ml_s[w][query][0] - top_s);
+        const float f = exp2_fast(ml_s[w][query][0] - top_s);
+        const float4 x = *reinterpret_cast<const float4*>(mo + (w * NT * 8 + query) * S::kPitch + p);
         L += ml_s[w][query][1] * f;
-        O += mo[(w * NT * 8 + query) * S::kPitch + d] * f;
+        O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
       }
       if (whole) {
-        const float sink = a.sinks ? exp2f(a.sinks[h * G + query] * 1.4426950408889634f - top_s) : 0.f;
-        a.out[((size_t)t * a.nq + h * G + query) * HD + d] = __float2bfloat16_rn(kv > 0 ? O / (L + sink) : 0.f);
+        finish(t, h * G + query, p, M, L, O, kv <= 0);
       } else {
-        a.part_o[(slot * 16 + query) * HD + d] = O;
-        if (d == 0) {
-          a.part_ml[(slot * 16 + query) * 2] = M;
-          a.part_ml[(slot * 16 + query) * 2 + 1] = L;
-        }
+        *reinterpret_cast<float4*>(a.part_o + (slot * 16 + query) * HD + p) = O;
+        if (p == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * 16 + query) * 2) = make_float2(M, L);
       }
     }
     if (!whole) {
@@ -536,7 +537,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
             sml[tid] = make_float2(M, L);
             continue;
           }
-          finish(t, h * G + query, d, M, L, O);
+          finish(t, h * G + query, d, M, L, O, false);
         }
         if (sets > 1) {
           __syncthreads();
@@ -550,7 +551,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
               L += sml[k * quads + i].y * f;
               O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
             }
-            finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, O);
+            finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, O, false);
           }
         }
       }
