@@ -11,8 +11,9 @@
 // O^T = V^T P^T, eight queries to an instruction (padding of G query heads to 8 and not to 16).  q is exact in float16 once a power of two has brought
 // its largest number to [2^14, 2^15); numbers 2^-38 times that are lost.  Scores, sums and the maximum that the exponentials are taken against are float32.
 // That maximum is followed only where a score passes it by more than kSlack (in log2): the weights stay below 2^kSlack, most tiles need no reduction across
-// lanes and no correction of the sums.  A weight times its key's v_scale, over the largest v_scale so far, times 2^kUp is rounded to float16: 11 bits
-// (bfloat16 would keep 8) at most 2^(kSlack + kUp) = 2^15, in whole down to 2^(-14 - kUp) of the largest.
+// lanes and no correction of the sums.  A weight times its key's v_scale is rounded to float16, 11 bits (bfloat16 would keep 8), relative to a second
+// maximum, of weight times scale, that is followed in the same way: at most 2^(kSlack + kUp) = 2^15, in whole down to 2^(-14 - kUp) of the largest.  So
+// keys that carry a query's result keep their bits however much larger the values of other pages are.
 // The order of the elements of a head among the k indices of S^T, and among the rows of O^T, is free as long as both operands agree: lane (g, c) owns
 // numbers c * HD / 4 ... of a key and g * HD / 8 ... of the values, so a lane's codes are whole 16-byte reads (8 bytes for the values of heads of 64).
 // Rows lie in shared memory with their 16-byte parts in an order turned by the key, which keeps those reads free of bank conflicts.
@@ -58,6 +59,11 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {      // an 8 x 8 matrix
 __device__ __forceinline__ float exp2_fast(float x) {      // what is below 2^-126 is zero
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float log2_fast(float x) {      // of zero minus infinity
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
   return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -299,11 +305,13 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
       qf[nt][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
     }
 
-    float o[NT][MT][4], m[NT][2], l[NT][2], vtop = 0.f, vnorm = 0.f;      // o times vnorm; vtop: the largest v_scale so far, as a power of two
+    float o[NT][MT][4], m[NT][2], l[NT][2];
+    float mw[NT][2], up[NT][2];            // the second maximum, in log2; 2^(m - mw + kUp), which o is multiplied by
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+      l[nt][0] = l[nt][1] = up[nt][0] = up[nt][1] = 0.f;
+      mw[nt][0] = mw[nt][1] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
@@ -348,37 +356,35 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
 
       const int key0 = tile * kTile + g;
       const bool in0 = key0 >= lo && key0 < kv, in1 = key0 + 8 >= lo && key0 + 8 < kv;
-      bool grew = (in0 && vs0 > vtop) || (in1 && vs1 > vtop);
+      const float lv0 = log2_fast(vs0), lv1 = P16 ? lv0 : log2_fast(vs1);
+      bool grew = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           s[nt][e] = in0 ? s[nt][e] * (qf[nt][e] * ks0) : -INFINITY;
           s[nt][2 + e] = in1 ? s[nt][2 + e] * (qf[nt][e] * ks1) : -INFINITY;
-          grew |= fmaxf(s[nt][e], s[nt][2 + e]) > m[nt][e] + kSlack;
+          const float x = fmaxf(s[nt][e], s[nt][2 + e]), w = P16 ? x + lv0 : fmaxf(s[nt][e] + lv0, s[nt][2 + e] + lv1);
+          grew |= x > m[nt][e] + kSlack || w > mw[nt][e] + kSlack;
         }
-      if (__any_sync(0xffffffffu, grew)) {      // the sums so far follow a larger maximum, or a larger v_scale
-        const float top = fmaxf(vtop, warp_max(fmaxf(in0 ? vs0 : 0.f, in1 ? vs1 : 0.f)));
-        const uint32_t tb = __float_as_uint(top);
-        const int te = min(max((int)(tb >> 23) - 127 + ((tb & 0x7fffffu) != 0), -100), 127);
-        const float was = vnorm;
-        vtop = top > 0.f ? exp2_int(te) : 0.f;
-        vnorm = top > 0.f ? exp2_int(kUp - te) : 0.f;
-        const float by = was > 0.f ? vnorm / was : 0.f;
+      if (__any_sync(0xffffffffu, grew)) {      // the sums so far follow the maxima
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[nt][e], s[nt][2 + e]);
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            const float mn = fmaxf(m[nt][e], x);
-            f[e] = mn == -INFINITY ? 1.f : exp2_fast(m[nt][e] - mn);
-            l[nt][e] *= f[e];
+            float x = fmaxf(s[nt][e], s[nt][2 + e]), w = fmaxf(s[nt][e] + lv0, s[nt][2 + e] + lv1);
+#pragma unroll
+            for (int d = 4; d <= 16; d *= 2) {
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
+            }
+            const float mn = fmaxf(m[nt][e], x), wn = fmaxf(mw[nt][e], w);
+            l[nt][e] *= mn == -INFINITY ? 1.f : exp2_fast(m[nt][e] - mn);
+            f[e] = wn == -INFINITY ? 1.f : exp2_fast(mw[nt][e] - wn);
             m[nt][e] = mn;
-            f[e] *= by;
+            mw[nt][e] = wn;
+            up[nt][e] = wn == -INFINITY ? 0.f : exp2_fast(mn - wn + kUp);
           }
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
@@ -389,7 +395,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           }
         }
       }
-      const float w0 = in0 ? vs0 * vnorm : 0.f, w1 = in1 ? vs1 * vnorm : 0.f;
+      const float w0 = in0 ? vs0 : 0.f, w1 = in1 ? vs1 : 0.f;
       uint32_t pb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -401,8 +407,8 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           p[2 + e] = exp2_fast(s[nt][2 + e] - top_s);
           l[nt][e] += p[e] + p[2 + e];
         }
-        pb[nt][0] = turned(pack_f16(p[0] * w0, p[1] * w0));
-        pb[nt][1] = turned(pack_f16(p[2] * w1, p[3] * w1));
+        pb[nt][0] = turned(pack_f16(p[0] * (w0 * up[nt][0]), p[1] * (w0 * up[nt][1])));
+        pb[nt][1] = turned(pack_f16(p[2] * (w1 * up[nt][0]), p[3] * (w1 * up[nt][1])));
       }
 
       // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
@@ -439,7 +445,6 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     // the four warps' sums: o[nt][j] holds numbers g * HD / 8 + 2j (rows g) and + 1 (rows g + 8) of queries 2c, 2c + 1
     __syncthreads();                                   // the rings are free
     float* mo = reinterpret_cast<float*>(smem);        // [4][NT * 8][kPitch]
-    const float out_by = vnorm > 0.f ? 1.0f / vnorm : 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -449,6 +454,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         const int query = nt * 8 + 2 * c + e;
+        const float out_by = up[nt][e] > 0.f ? 1.0f / up[nt][e] : 0.f;
         if (g == 0) {
           ml_s[warp][query][0] = m[nt][e];
           ml_s[warp][query][1] = x;

@@ -133,6 +133,27 @@ def test_scales_and_queries_of_all_sizes(hd):
     _near(_run(s), _want(s), hd, 2.0 ** -11, 900)
 
 
+@pytest.mark.parametrize("hd,ps", [(64, 16), (128, 16), (128, 12)])
+@pytest.mark.parametrize("big", [13, 60])
+def test_small_values_that_carry_the_result(hd, ps, big):
+    """The keys with all the weight lie in a page whose values are 2^-27 and less, other pages' values are 2^13 or 2^60 times larger; in front and behind."""
+    for at in (0, 7, 24):
+        s = _case([(1, 400)], 8, 2, hd, ps, seed=11)
+        s.vs.fill_(2.0 ** (big - 27))
+        page = int(s.table[0, at])
+        s.vs[page] = 2.0 ** -27
+        # keys of that page along the first query of each kv head, and the queries of a group alike: scores some 300 above the others'
+        kq = s.q.view(2, 4, hd)[:, :1].expand(2, 4, hd).contiguous()
+        s.q.copy_(kq.reshape(1, -1))
+        s.ks.fill_(2.0 ** -9)
+        s.ks[page] = 2.0 ** -1
+        s.k.view(torch.uint8)[page] = (kq[:, 0].float() * 50).clamp(-448, 448).to(E4M3).view(torch.uint8)[:, None, :].expand(2, ps, hd)
+        want = _want(s)
+        assert float(want[0].abs().max()) < 2.0 ** -10
+        _near(_run(s), want, hd, 2.0 ** -11, 400)
+        _near(_run(s, batch=False), want, hd, 0.0, 400)
+
+
 @pytest.mark.parametrize("where", ["key", "value", "query"])
 def test_nan_and_infinity_stay_with_those_who_see_them(where):
     s = _case([(1, 200), (1, 300), (1, 100)], 8, 2, 128, 16)
