@@ -2328,8 +2328,8 @@ def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, h
     A scale is a power of two, the least with max |x| <= 448 * scale (at least 2^-100; at most 2^119, beyond which numbers end at 448 * 2^119).  Tokens
     that go to a page from its first place on give it a new scale.  Tokens that go behind others, which are taken to fill every place in front, keep the
     larger of the page's scale and their own; where that grows, the older codes are rounded once more to it.  Infinities become the largest number of their page's
-    scale, NaN stays NaN; neither counts for the scale.  A step's tokens of one page stand in consecutive rows, in the order of their places, each place once, as
-    an engine's do (else which of them the page keeps is left open)."""
+    scale, NaN stays NaN; neither counts for the scale.  What a call stores in one page is one run: consecutive rows, consecutive places, each once, as an engine's tokens
+    are (two runs of one call in one page would each set the page's scale, and which one stays is left open)."""
     vd = hd if vd is None else int(vd)
     T = slot_mapping.numel()
     if k.shape != (T, nkv * hd) or v.shape != (T, nkv * vd) or k.dtype is not v.dtype:
