@@ -18,6 +18,7 @@ cuBLAS through ``torch.mm``, as cklxx/arle calls cuBLASLt for all its projection
 from __future__ import annotations
 
 import ctypes
+import operator
 import threading
 from ctypes import c_float, c_int, c_void_p
 
@@ -2308,14 +2309,19 @@ def _q8_cache(what: str, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, 
                       f"{tuple(k_scale.shape)}, {v_scale.dtype} {tuple(v_scale.shape)}")
 
 
-def _on_device(what: str, *tensors) -> None:
-    """Every tensor on the current device, whose stream the launch goes to."""
-    d = tensors[0].get_device()
-    for t in tensors:
-        if t.get_device() != d or d < 0:
-            raise KernelError(f"{what}: a tensor is on {t.device}, another on {tensors[0].device}: arle_b200 kernels run on one CUDA device (there is no CPU path)")
-    if d != torch._C._cuda_getDevice():
-        raise KernelError(f"{what}: the tensors are on cuda:{d}, which is not the current device")
+# a step's launches are as fast as their checks: methods mapped over the tensors, not called one by one
+_DTYPE, _NUMEL, _DEVICE, _POINTER, _CONTIGUOUS = (operator.attrgetter("dtype"), torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.data_ptr,
+                                                  torch.Tensor.is_contiguous)
+
+
+def _pointers(what: str, tensors):
+    """The tensors' addresses; all of them are on the current device, whose stream the launch goes to."""
+    on = set(map(_DEVICE, tensors))
+    if len(on) != 1 or -1 in on:
+        raise KernelError(f"{what}: tensors on {sorted({str(t.device) for t in tensors})}: arle_b200 kernels run on one CUDA device (there is no CPU path)")
+    if torch._C._cuda_getDevice() not in on:
+        raise KernelError(f"{what}: the tensors are on {tensors[0].device}, which is not the current device")
+    return map(_POINTER, tensors)
 
 
 def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
@@ -2340,11 +2346,10 @@ def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, h
     pages = _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
     if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
         raise KernelError("store_q8: slot_mapping must be contiguous int32")
-    _on_device("store_q8", k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale)
+    kp, vp, sp, kcp, vcp, ksp, vsp = _pointers("store_q8", (k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale))
     if T == 0:
         return
-    _check(library().arle_store_q8(k.data_ptr(), k_stride, v.data_ptr(), v_stride, _dt(k), slot_mapping.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(),
-                                   k_scale.data_ptr(), v_scale.data_ptr(), pages, nkv, hd, vd, page_size, _stream()), "store_q8")
+    _check(library().arle_store_q8(kp, k_stride, vp, v_stride, _dt(k), sp, T, kcp, vcp, ksp, vsp, pages, nkv, hd, vd, page_size, _stream()), "store_q8")
 
 
 # Bytes of bfloat16 keys and values that prompt portions are expanded into at a time; rows that see more go by themselves.
@@ -2373,17 +2378,17 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     if positions.dtype is not i32 or row_of_token.dtype is not i32 or block_table.dtype is not i32 or bt_unit != 1:
         raise KernelError("paged_attention_q8: positions, row_of_token and block_table must be int32, rows of the block table contiguous")
     sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, max(0, int(window)) if window else 0
-    _on_device("paged_attention_q8", q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table)
+    qp, op, kp, vp, ksp, vsp, pp, rp, tp = _pointers("paged_attention_q8", (q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table))
     if T == 0:
         return
-    qp, kp, vp, op, lib = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), library()
+    lib = library()
     # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
     if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
             and not (qp | kp | vp | op) % 16):
         rows, beside, join, pos_p, row_p = batch.num_rows, False, None, None, None
         if batch.max_q_len > 1:
             if _by_tokens_q8(batch, nkv, hd, w):
-                rows, pos_p, row_p = min(T, sum(batch.q_lens)), positions.data_ptr(), row_of_token.data_ptr()
+                rows, pos_p, row_p = min(T, sum(batch.q_lens)), pp, rp
             else:
                 beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0 or pos_p is not None:
@@ -2393,8 +2398,7 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
             counters = batch.ws.get_zeroed("attn_q8_counters", (rows * nkv,), torch.int32)
             at = parts.data_ptr()
             _check(lib.arle_attention_q8_decode(
-                qp, q_stride, op, kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(),
-                block_table.data_ptr(), bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
+                qp, q_stride, op, kp, vp, ksp, vsp, batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), tp, bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
                 rows, ctas, int(beside), pos_p, row_p, _stream()), "attention_q8_decode")
         if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
             join()
@@ -2402,8 +2406,7 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     if batch is not None:
         T = min(T, sum(batch.q_lens))
     _check(lib.arle_attention_q8(
-        qp, q_stride, op, _dt(q), kp, vp, k_scale.data_ptr(), v_scale.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(),
-        block_table.data_ptr(), bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
+        qp, q_stride, op, _dt(q), kp, vp, ksp, vsp, pp, rp, tp, bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
 # Bytes of codes up to which a step's short portions are read token by token.
@@ -2500,20 +2503,15 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     was), block_table [R, width], contiguous: a row's pages, -1 behind them, and status [1]: 0, or the sum of what is wrong with the step: 1 more tokens
     than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
     cache.  Such a step leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
-    R, T = slots.numel(), positions.numel()
-    every = (status, slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table)
-    i32, d = torch.int32, status.get_device()
-    for t in every:
-        if t.dtype is not i32 or not t.is_contiguous() or t.get_device() != d:
-            raise KernelError(f"step_tables: every tensor must be contiguous int32 on status's device ({status.device}), got {t.dtype} {tuple(t.shape)} with strides "
-                              f"{t.stride()} on {t.device}")
-    if (starts.numel() != R or q_lens.numel() != R or q_indptr.numel() != R + 1 or kv_lens.numel() != R or row_of_token.numel() != T or slot_of_token.numel() != T
-            or slot_mapping.numel() != T or status.numel() != 1 or block_table.dim() != 2 or block_table.shape[0] != R or page_table.dim() != 2):
+    every = (slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table, status)
+    if set(map(_DTYPE, every)) != {torch.int32} or not all(map(_CONTIGUOUS, every)):
+        raise KernelError(f"step_tables: every tensor must be contiguous int32, got {[(str(t.dtype), tuple(t.shape), t.stride()) for t in every]}")
+    R, rs, rq, news, _, r1, rk, T, tr, ts, tm, _, one = map(_NUMEL, every)
+    if not (rs == rq == rk == R and r1 == R + 1 and tr == ts == tm == T and one == 1 and page_table.dim() == 2 and block_table.dim() == 2 and block_table.shape[0] == R):
         raise KernelError("step_tables: slots, starts, q_lens and kv_lens are [R], q_indptr [R + 1], the tokens' tables [T], block_table [R, width], "
                           "page_table [slots, pages], status [1]")
-    _on_device("step_tables", status)
+    slots, starts, q_lens, new_pages, table, *outs = _pointers("step_tables", every)
     max_slots, table_width = page_table.shape
-    _check(library().arle_step_tables(
-        slots.data_ptr(), starts.data_ptr(), q_lens.data_ptr(), R, new_pages.data_ptr(), new_pages.numel(), page_table.data_ptr(), max_slots, table_width, int(num_pages),
-        int(page_size), q_indptr.data_ptr(), kv_lens.data_ptr(), positions.data_ptr(), row_of_token.data_ptr(), slot_of_token.data_ptr(), slot_mapping.data_ptr(), T,
-        block_table.data_ptr(), block_table.shape[1], status.data_ptr(), _stream()), "step_tables")
+    q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, blocks, status = outs
+    _check(library().arle_step_tables(slots, starts, q_lens, R, new_pages, news, table, max_slots, table_width, int(num_pages), int(page_size), q_indptr, kv_lens, positions,
+                                      row_of_token, slot_of_token, slot_mapping, T, blocks, block_table.shape[1], status, _stream()), "step_tables")
