@@ -1,6 +1,8 @@
 // Attention of decoded tokens (rows with one query) over the 8-bit cache (q8.cuh): bfloat16 queries, heads of 64 and 128, up to 16 query heads to a kv head.
 //     s_j = scale * k_scale * (q . k_code_j);   out = sum_j exp(s_j) v_scale v_code_j / (sum_j exp(s_j) + exp(sink)),   kv_len - window <= j < kv_len
-// A token reads every visible code once, so the kernel is built to stream codes at the rate of DRAM.
+// A token reads every visible code once, so the kernel is built to stream codes at the rate of DRAM: 64 rows of up to 4,096 keys with 8 kv heads of 128 (374
+// MB) take 66 us, 8 rows of up to 131,072 (1.3 GB) 207 us, 6.2 TB/s.  Some 12 us are latency whatever the keys: reading the rows' lengths, page ids and
+// first tiles 3 to 6 us, joining sums 3; one row of 1,000 keys takes 8 us.
 //
 // Work: all rows' and heads' keys in blocks of 64 are one line that a resident grid shares out evenly, whatever the rows' lengths; a CTA's piece of a
 // (row, kv head) is summed on its own, and where a pair was cut the CTA that finishes its last piece joins the pieces in the order of keys (a counter per

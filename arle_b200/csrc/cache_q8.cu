@@ -6,7 +6,7 @@
 //     s' = s(a) for a run from offset 0, else max(s, s(a));   codes in front of the run: rne(code * s / s');   new codes: rne(x / s')
 // One group of `warps` warps owns a run of one head of the keys or the values, so the page's scale and older codes are read and written by one owner.
 // A page of up to 2,048 numbers a warp stays in registers between the maximum and the rounding (one read of x); what is larger is read again (from L2).
-// Decoded tokens are bound by the latency of three dependent accesses (place, numbers, codes): 2.2 us for one token, 2.3 us for 64.  Prompts come near
+// Decoded tokens are bound by the latency of three dependent accesses (place, numbers, codes): 2.0 us for one token, 2.2 us for 64.  Prompts come near
 // DRAM's rate: 15,000 tokens of 8 heads of 128 in 20.7 us, 4.7 TB/s; what is left is instructions (five for two numbers in the rounding alone).
 #include "q8.cuh"
 using namespace arle;
@@ -259,7 +259,7 @@ int launch_store(StoreSide k, StoreSide v, const int* slot_mapping, int tokens, 
 // expand: the keys and values that rows with at least `least` queries see, as bfloat16 pages of 64 tokens [pages, nkv, 64, width] with a block table of
 // their own, for the prompt kernels: a code is exact in bfloat16, and so is its product with a power of two.  Row r's pages follow those of the rows in
 // front of it; its table names them at their logical places (page j holds tokens 64 j ...), -1 elsewhere.  Places behind the row's last token are zeros.
-// A block per page and head, bound by DRAM (one byte in, two out).
+// A block per page and head, bound by DRAM (one byte in, two out: 16,384 keys of 8 heads of 128 in 24 us, 4.2 TB/s) or by latency (2,100 keys: 5 us).
 constexpr int kExpanded = 64;
 
 struct ExpandArgs {
