@@ -2385,6 +2385,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
     if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
             and not (qp | kp | vp | op) % 16):
+        if batch.q_indptr.dtype is not i32 or batch.kv_lens.dtype is not i32:
+            raise KernelError("paged_attention_q8: the batch's q_indptr and kv_lens must be int32")
         rows, beside, join, pos_p, row_p = batch.num_rows, False, None, None, None
         if batch.max_q_len > 1:
             if _by_tokens_q8(batch, nkv, hd, w):

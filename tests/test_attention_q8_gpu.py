@@ -295,6 +295,13 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(s.ks[shift:].nan_to_num(), small.ks.nan_to_num())
 
 
+def test_a_batch_of_other_types():
+    s = _case([(1, 70)], 8, 2, 128, 16)
+    s.batch.kv_lens = s.batch.kv_lens.long()
+    with pytest.raises(ops.KernelError, match="int32"):
+        _run(s)
+
+
 def test_tensors_of_another_device():
     s = _case([(1, 70)], 8, 2, 128, 16)
     s.ks = s.ks.cpu()
