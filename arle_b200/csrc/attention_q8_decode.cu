@@ -4,10 +4,10 @@
 // MB) take 66 us, 8 rows of up to 131,072 (1.3 GB) 207 us, 6.2 TB/s.  Some 12 us are latency whatever the keys: reading the rows' lengths, page ids and
 // first tiles 3 to 6 us, joining sums 3; one row of 1,000 keys takes 8 us.
 //
-// Work: all rows' and heads' keys in blocks of 64 are one line that a resident grid shares out evenly, whatever the rows' lengths; a CTA's piece of a
+// Work: all rows' and heads' keys in blocks of 64 (128) are one line that a resident grid shares out evenly, whatever the rows' lengths; a CTA's piece of a
 // (row, kv head) is summed on its own, and where a pair was cut the CTA that finishes its last piece joins the pieces in the order of keys (a counter per
-// pair, which it leaves at zero).  Inside a piece warp w of four takes tiles w, w + 4, ... of 16 keys; each warp has a ring of its own that cp.async fills,
-// so nothing in the loop waits for another warp.
+// pair, which it leaves at zero).  Inside a piece warp w of four takes tiles w, w + 4, ... of 16 keys (32 of heads of 64); each warp has a ring of its own that
+// cp.async fills, so nothing in the loop waits for another warp.
 //
 // Arithmetic: codes are exact in float16 (cvt), so both products run as mma.sync with float16 operands and float32 sums, keys as rows: S^T = K Q^T and
 // O^T = V^T P^T, eight queries to an instruction (padding of G query heads to 8 and not to 16).  q is exact in float16 once a power of two has brought
@@ -26,8 +26,11 @@ using namespace arle;
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kTile = 16;                 // keys of a warp's tile
-constexpr int kBlock = kWarps * kTile;    // keys of a block of work
+constexpr int kTile = 16;                 // keys of a product
+// Products that a warp has in hand at a time (its tile): two where heads are small, so that a tile has as many bytes and its bookkeeping as much to do.
+template <int HD> constexpr int kSub = HD == 64 ? 2 : 1;
+template <int HD> constexpr int kKeys = kTile * kSub<HD>;           // keys of a warp's tile
+template <int HD> constexpr int kBlock = kWarps * kKeys<HD>;        // keys of a block of work: 16 KB of codes
 constexpr int kUp = 9;
 constexpr float kSlack = 6.0f;
 
@@ -73,29 +76,30 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// A row: its token, its keys, the block of 64 keys (on the grid of absolute positions) that its first visible key lies in, and how many blocks its query
+// A row: its token, its keys, the block (on the grid of absolute positions) that its first visible key lies in, and how many blocks its query
 // sees: none if the row has not exactly one query, one (which writes its zeros) if it has no keys.  By tokens a token is a row of the keys up to its own.
 struct Row {
   int t, kv, first, nb, table;
 };
+template <int HD>
 __device__ __forceinline__ Row row_of(const DecodeArgs& a, int r) {
   if (a.positions) {
-    const int kv = a.positions[r] + 1, first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock : 0;
-    return Row{r, kv, first, kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first, a.row_of_token[r]};
+    const int kv = a.positions[r] + 1, first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock<HD> : 0;
+    return Row{r, kv, first, kv <= 0 ? 1 : (kv + kBlock<HD> - 1) / kBlock<HD> - first, a.row_of_token[r]};
   }
   const int t0 = a.q_indptr[r], t1 = a.q_indptr[r + 1], kv = a.kv_lens[r];
-  const int first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock : 0;
-  return Row{t0, kv, first, t1 - t0 != 1 ? 0 : kv <= 0 ? 1 : (kv + kBlock - 1) / kBlock - first, r};
+  const int first = kv > 0 ? first_visible_key(kv - 1, a.window, 0) / kBlock<HD> : 0;
+  return Row{t0, kv, first, t1 - t0 != 1 ? 0 : kv <= 0 ? 1 : (kv + kBlock<HD> - 1) / kBlock<HD> - first, r};
 }
 
-template <int HD> constexpr int kPause = HD == 128 ? 6 : 12;      // see where the line is cut
+constexpr int kPause = 6;      // blocks; see where the line is cut
 
 template <int HD, int NT> struct Shape {
   static constexpr int kResident = NT == 1 ? 4 : 3;      // CTAs of an SM: 128 and 168 registers a thread
-  static constexpr int kStages = HD == 128 ? (NT == 1 ? 3 : 4) : (NT == 1 ? 5 : 6);
-  static constexpr int kStageBytes = 2 * kTile * HD;
+  static constexpr int kStages = NT == 1 ? 3 : 4;
+  static constexpr int kStageBytes = 2 * kKeys<HD> * HD;
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kScales = kWarps * kStages * 32 * 4;
+  static constexpr int kScales = kWarps * kStages * kSub<HD> * 32 * 4;
   static constexpr int kSmem = kRing + kScales;
   static constexpr int kPitch = HD + 8;      // of the partial results
 };
@@ -104,7 +108,7 @@ template <int HD, int NT> struct Shape {
 template <int HD, int NT, bool P16>
 __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   using S = Shape<HD, NT>;
-  constexpr int NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
+  constexpr int SUB = kSub<HD>, NS = S::kStages, CH = HD / 16;      // 16-byte parts of a row
   constexpr int KS = HD / 16, MT = HD / 16;         // steps of 16 numbers of a head in S^T, tiles of 16 numbers in O^T
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int4 sum_s[kWarps];
@@ -114,7 +118,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = a.nq / a.nkv, nkv = a.nkv;
   unsigned char* ring = smem + warp * NS * S::kStageBytes;
-  float* scales = reinterpret_cast<float*>(smem + S::kRing) + warp * NS * 32;
+  float* scales = reinterpret_cast<float*>(smem + S::kRing) + warp * NS * SUB * 32;
   const uint32_t ring_u32 = smem_u32(ring), scales_u32 = smem_u32(scales);
   // where the lane's 16-byte parts of a tile go, beside i * 512: part i * 32 + lane is part lane % CH of key (i * 32 + lane) / CH
   uint32_t turned_at[2];
@@ -129,7 +133,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   int mine = 0, mine_rows = 0, longest = 0;
   Row own{};                                       // the thread's first row
   for (int r = r1 - 1; r >= r0; --r) {
-    own = row_of(a, r);
+    own = row_of<HD>(a, r);
     mine += own.nb;
     mine_rows += own.nb > 0;
     longest = max(longest, own.nb);
@@ -153,7 +157,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   // A CTA that goes on to another pair waits for that one's first tiles behind everybody's loads, about as long as `pause` blocks take it (6 us; 64 rows of
   // ragged lengths, CTAs of one, two and three pieces with the same keys: done after 51, 58 and 63 us).  So where shares are long a pair counts that
   // much more on the line, at its start; short shares are one piece each, mostly.
-  const int pause = (total * nkv + (int)gridDim.x - 1) / (int)gridDim.x >= 4 * kPause<HD> ? kPause<HD> : 0;
+  const int pause = (total * nkv + (int)gridDim.x - 1) / (int)gridDim.x >= 4 * kPause ? kPause : 0;
   total = (total + pause * total_rows) * nkv;
   front = (front + pause * front_rows) * nkv;
   mine = (mine + pause * mine_rows) * nkv;
@@ -176,7 +180,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         const int n = x.nb > 0 ? (x.nb + pause) * nkv : 0;
         if (at < row_at + n) break;
         row_at += n;
-        x = row_of(a, ++r);
+        x = row_of<HD>(a, ++r);
       }
       const int from = (at - row_at) % (x.nb + pause), blk = max(0, from - pause), left = x.nb - blk;
       cut_s[i] = from == 0 ? at : left <= slack ? at - from + x.nb + pause : blk <= slack ? at - from : at;
@@ -208,24 +212,26 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
       const int n = at_row.nb > 0 ? (at_row.nb + pause) * nkv : 0;
       if (pos < row_at + n) break;
       row_at += n;
-      at_row = row_of(a, ++row);
+      at_row = row_of<HD>(a, ++row);
     }
     const int nb = at_row.nb, t = at_row.t, kv = at_row.kv;
     const int h = (pos - row_at) / (nb + pause), pair_at = row_at + h * (nb + pause), keys_at = pair_at + pause;
     const int blk0 = max(0, pos - keys_at), blk1 = min(nb, end - keys_at);
-    const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0, base_key = at_row.first * kBlock;
-    const int tile0 = (base_key + blk0 * kBlock) / kTile + warp, tile_end = min((base_key + blk1 * kBlock) / kTile, (kv + kTile - 1) / kTile);
+    const int lo = kv > 0 ? first_visible_key(kv - 1, a.window, 0) : 0, base_key = at_row.first * kBlock<HD>;
+    const int tile0 = (base_key + blk0 * kBlock<HD>) / kKeys<HD> + warp;
+    const int tile_end = min((base_key + blk1 * kBlock<HD>) / kKeys<HD>, (kv + kKeys<HD> - 1) / kKeys<HD>);
     const int* bt = a.block_table + (size_t)at_row.table * a.bt_stride;
 
-    // Page of the tile (P16) or of its key lane & 15; -1: nothing of it is seen.
-    auto page_of = [&](int tile) -> int {
-      const int key = tile * kTile + (P16 ? 0 : lane & 15);
-      if (tile >= tile_end || (!P16 && (key < lo || key >= kv))) return -1;
+    // Page of product u of the tile (P16) or of its key lane & 15; -1: nothing of it is seen.
+    auto page_of = [&](int tile, int u) -> int {
+      const int key = (tile * SUB + u) * kTile + (P16 ? 0 : lane & 15);
+      if (tile >= tile_end || ((SUB > 1 || !P16) && key >= kv) || (!P16 && key < lo)) return -1;
       return bt[a.ps_shift >= 0 ? key >> a.ps_shift : key / a.page_size];
     };
-    auto load_tile = [&](int tile, int stage, int page) {
-      const uint32_t dst = ring_u32 + stage * S::kStageBytes;
-      const int first = tile * kTile;
+    auto load_product = [&](int tile, int stage, int u, int page) {
+      const uint32_t dst = ring_u32 + stage * S::kStageBytes + u * (2 * kTile * HD);
+      const uint32_t scale_to = scales_u32 + ((stage * SUB + u) * 32 + lane) * 4;
+      const int first = (tile * SUB + u) * kTile;
       if constexpr (P16) {
         const int slot = a.ps_shift >= 0 ? first & (a.page_size - 1) : first % a.page_size;
         const long unit = (long)page * nkv + h;
@@ -247,7 +253,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
             cp_async16(dst + kTile * HD + i * 512 + turned_at[i & 1], bytes ? vp + i * 512 : a.v_cache, bytes);
           }
         }
-        if (lane < 2) cp_async4(scales_u32 + (stage * 32 + lane) * 4, (lane ? a.v_scale : a.k_scale) + (page >= 0 ? unit : 0), page >= 0 ? 4 : 0);
+        if (lane < 2) cp_async4(scale_to, (lane ? a.v_scale : a.k_scale) + (page >= 0 ? unit : 0), page >= 0 ? 4 : 0);
       } else {
 #pragma unroll
         for (int i = 0; i < CH / 2; ++i) {
@@ -259,21 +265,29 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           cp_async16(dst + kTile * HD + i * 512 + turned_at[i & 1], a.v_cache + off, pg >= 0 ? 16 : 0);
         }
         const float* from = lane < 16 ? a.k_scale : a.v_scale;
-        cp_async4(scales_u32 + (stage * 32 + lane) * 4, from + (page >= 0 ? (size_t)page * nkv + h : 0), page >= 0 ? 4 : 0);
+        cp_async4(scale_to, from + (page >= 0 ? (size_t)page * nkv + h : 0), page >= 0 ? 4 : 0);
       }
     };
 
-    int page_next;
-    {
-      int pg[NS];
+    auto load_tile = [&](int tile, int stage, const int (&page)[SUB]) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) pg[i] = page_of(tile0 + i * kWarps);
+      for (int u = 0; u < SUB; ++u) load_product(tile, stage, u, page[u]);
+    };
+
+    int page_next[SUB];
+    {
+      int pg[NS][SUB];
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) pg[i][u] = page_of(tile0 + i * kWarps, u);
 #pragma unroll
       for (int i = 0; i < NS - 1; ++i) {
         if (tile0 + i * kWarps < tile_end) load_tile(tile0 + i * kWarps, i, pg[i]);
         cp_commit();
       }
-      page_next = pg[NS - 1];
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) page_next[u] = pg[NS - 1][u];
     }
 
     // q: lane (g, c) holds numbers c * HD / 4 ... of query g
@@ -323,59 +337,74 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
       const int ahead = tile + (NS - 1) * kWarps;
       if (ahead < tile_end) load_tile(ahead, stage == 0 ? NS - 1 : stage - 1, page_next);
       cp_commit();
-      page_next = page_of(ahead + kWarps);
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) page_next[u] = page_of(ahead + kWarps, u);
       cp_wait<NS - 1>();
       __syncwarp();
-      const unsigned char* kt = ring + stage * S::kStageBytes;
-      const unsigned char* vt = kt + kTile * HD;
-      float ks0, ks1, vs0, vs1;
-      if constexpr (P16) {
-        const float2 sc = *reinterpret_cast<const float2*>(scales + stage * 32);
-        ks0 = ks1 = sc.x;
-        vs0 = vs1 = sc.y;
-      } else {
-        ks0 = scales[stage * 32 + g], ks1 = scales[stage * 32 + g + 8], vs0 = scales[stage * 32 + 16 + g], vs1 = scales[stage * 32 + 24 + g];
-      }
-
-      float s[NT][4];
+      const unsigned char* products = ring + stage * S::kStageBytes;
+      // of keys g and g + 8 of each product: scores, scales of the values and their logarithms, whether they are seen
+      float s[SUB][NT][4], vs[SUB][2], lv[SUB][2];
+      bool in[SUB][2], grew = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+      for (int u = 0; u < SUB; ++u) {
+        const unsigned char* kt = products + u * (2 * kTile * HD);
+        const float* sc = scales + (stage * SUB + u) * 32;
+        float ks[2];
+        if constexpr (P16) {
+          const float2 x = *reinterpret_cast<const float2*>(sc);
+          ks[0] = ks[1] = x.x;
+          vs[u][0] = vs[u][1] = x.y;
+          lv[u][0] = lv[u][1] = log2_fast(x.y);
+        } else {
 #pragma unroll
-      for (int i = 0; i < HD / 64; ++i) {
-        const int part = HD == 128 ? ((2 * c + i) ^ g) : (c ^ ((g >> 1) & 3));
-        const uint4 w0 = *reinterpret_cast<const uint4*>(kt + g * HD + part * 16);
-        const uint4 w1 = *reinterpret_cast<const uint4*>(kt + (g + 8) * HD + part * 16);
-        const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t a0, a1, a2, a3;
-          q8_half4(x0[e], a0, a2);
-          q8_half4(x1[e], a1, a3);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][4 * i + e][0], qb[nt][4 * i + e][1]);
+          for (int y = 0; y < 2; ++y) {
+            ks[y] = sc[g + 8 * y];
+            vs[u][y] = sc[16 + g + 8 * y];
+            lv[u][y] = log2_fast(vs[u][y]);
+          }
         }
-      }
-
-      const int key0 = tile * kTile + g;
-      const bool in0 = key0 >= lo && key0 < kv, in1 = key0 + 8 >= lo && key0 + 8 < kv;
-      const float lv0 = log2_fast(vs0), lv1 = P16 ? lv0 : log2_fast(vs1);
-      bool grew = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) s[u][nt][0] = s[u][nt][1] = s[u][nt][2] = s[u][nt][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[nt][e] = in0 ? s[nt][e] * (qf[nt][e] * ks0) : -INFINITY;
-          s[nt][2 + e] = in1 ? s[nt][2 + e] * (qf[nt][e] * ks1) : -INFINITY;
-          const float x = fmaxf(s[nt][e], s[nt][2 + e]), w = P16 ? x + lv0 : fmaxf(s[nt][e] + lv0, s[nt][2 + e] + lv1);
-          grew |= x > m[nt][e] + kSlack || w > mw[nt][e] + kSlack;
+        for (int i = 0; i < HD / 64; ++i) {
+          const int part = HD == 128 ? ((2 * c + i) ^ g) : (c ^ ((g >> 1) & 3));
+          const uint4 w0 = *reinterpret_cast<const uint4*>(kt + g * HD + part * 16);
+          const uint4 w1 = *reinterpret_cast<const uint4*>(kt + (g + 8) * HD + part * 16);
+          const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a0, a1, a2, a3;
+            q8_half4(x0[e], a0, a2);
+            q8_half4(x1[e], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[u][nt], a0, a1, a2, a3, qb[nt][4 * i + e][0], qb[nt][4 * i + e][1]);
+          }
         }
+        const int key0 = (tile * SUB + u) * kTile + g;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) in[u][y] = key0 + 8 * y >= lo && key0 + 8 * y < kv;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) s[u][nt][2 * y + e] = in[u][y] ? s[u][nt][2 * y + e] * (qf[nt][e] * ks[y]) : -INFINITY;
+            const float x = fmaxf(s[u][nt][e], s[u][nt][2 + e]), w = P16 ? x + lv[u][0] : fmaxf(s[u][nt][e] + lv[u][0], s[u][nt][2 + e] + lv[u][1]);
+            grew |= x > m[nt][e] + kSlack || w > mw[nt][e] + kSlack;
+          }
+      }
       if (__any_sync(0xffffffffu, grew)) {      // the sums so far follow the maxima
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float x = fmaxf(s[nt][e], s[nt][2 + e]), w = fmaxf(s[nt][e] + lv0, s[nt][2 + e] + lv1);
+            float x = -INFINITY, w = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+              x = fmaxf(x, fmaxf(s[u][nt][e], s[u][nt][2 + e]));
+              w = fmaxf(w, fmaxf(s[u][nt][e] + lv[u][0], s[u][nt][2 + e] + lv[u][1]));
+            }
 #pragma unroll
             for (int d = 4; d <= 16; d *= 2) {
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
@@ -397,46 +426,49 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           }
         }
       }
-      const float w0 = in0 ? vs0 : 0.f, w1 = in1 ? vs1 : 0.f;
-      uint32_t pb[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float p[4];
+      for (int u = 0; u < SUB; ++u) {
+        uint32_t pb[NT][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float top_s = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-          p[e] = exp2_fast(s[nt][e] - top_s);
-          p[2 + e] = exp2_fast(s[nt][2 + e] - top_s);
-          l[nt][e] += p[e] + p[2 + e];
+        for (int nt = 0; nt < NT; ++nt) {
+          const float w0 = in[u][0] ? vs[u][0] : 0.f, w1 = in[u][1] ? vs[u][1] : 0.f;
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float top = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+            p[e] = exp2_fast(s[u][nt][e] - top);
+            p[2 + e] = exp2_fast(s[u][nt][2 + e] - top);
+            l[nt][e] += p[e] + p[2 + e];
+          }
+          pb[nt][0] = turned(pack_f16(p[0] * (w0 * up[nt][0]), p[1] * (w0 * up[nt][1])));
+          pb[nt][1] = turned(pack_f16(p[2] * (w1 * up[nt][0]), p[3] * (w1 * up[nt][1])));
         }
-        pb[nt][0] = turned(pack_f16(p[0] * (w0 * up[nt][0]), p[1] * (w0 * up[nt][1])));
-        pb[nt][1] = turned(pack_f16(p[2] * (w1 * up[nt][0]), p[3] * (w1 * up[nt][1])));
-      }
-
-      // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
-      constexpr int VW = HD / 32;      // words of 4 codes
-      uint32_t v[4][VW];
+        // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
+        const unsigned char* vt = products + u * (2 * kTile * HD) + kTile * HD;
+        constexpr int VW = HD / 32;      // words of 4 codes
+        uint32_t v[4][VW];
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int key = 2 * c + (y & 1) + (y >> 1) * 8;
-        if constexpr (HD == 128) {
-          const uint4 w = *reinterpret_cast<const uint4*>(vt + key * HD + ((g ^ (key & 7)) * 16));
-          v[y][0] = w.x, v[y][1] = w.y, v[y][2] = w.z, v[y][3] = w.w;
-        } else {
-          const uint2 w = *reinterpret_cast<const uint2*>(vt + key * HD + (((g >> 1) ^ ((key >> 1) & 3)) * 16) + (g & 1) * 8);
-          v[y][0] = w.x, v[y][1] = w.y;
+        for (int y = 0; y < 4; ++y) {
+          const int key = 2 * c + (y & 1) + (y >> 1) * 8;
+          if constexpr (HD == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vt + key * HD + ((g ^ (key & 7)) * 16));
+            v[y][0] = w.x, v[y][1] = w.y, v[y][2] = w.z, v[y][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(vt + key * HD + (((g >> 1) ^ ((key >> 1) & 3)) * 16) + (g & 1) * 8);
+            v[y][0] = w.x, v[y][1] = w.y;
+          }
         }
-      }
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
+        for (int w = 0; w < VW; ++w) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t x = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
-          uint32_t a0, a1, a2, a3;
-          q8_half4(x, a0, a1);
-          q8_half4(y, a2, a3);
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140), y = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+            uint32_t a0, a1, a2, a3;
+            q8_half4(x, a0, a1);
+            q8_half4(y, a2, a3);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
         }
       }
       __syncwarp();
