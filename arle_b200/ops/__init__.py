@@ -2363,8 +2363,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     ``batch``, rows of q and out behind its last token are left alone.
 
     ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
-    bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens read the codes as they are; the keys and values that
-    portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels.  A captured call of decoded tokens goes by the
+    bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens, and those of short portions, read the codes as they are; the keys and values
+    that longer portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels.  A captured call of decoded tokens goes by the
     lengths on the device when it is replayed; one with portions keeps room for the lengths that the host's copies had, and those have to stay."""
     (T, width), (q_stride, q_unit), vd = q.shape, q.stride(), hd if vd is None else int(vd)
     if q_unit != 1 or width != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
@@ -2387,21 +2387,21 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
             and not (qp | kp | vp | op) % 16):
         if batch.q_indptr.dtype is not i32 or batch.kv_lens.dtype is not i32:
             raise KernelError("paged_attention_q8: the batch's q_indptr and kv_lens must be int32")
-        rows, beside, join, pos_p, row_p = batch.num_rows, False, None, None, None
+        rows, beside, join, pos_p, row_p, sms = batch.num_rows, False, None, None, None, _SM_COUNT.get(q.device.index) or sm_count(q.device)
         if batch.max_q_len > 1:
-            if _by_tokens_q8(batch, nkv, hd, w):
+            if _by_tokens_q8(batch, nq, nkv, hd, w, sms):
                 rows, pos_p, row_p = min(T, sum(batch.q_lens)), pp, rp
             else:
                 beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
         if batch.num_single > 0 or pos_p is not None:
             # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
-            ctas = (4 if nq <= 8 * nkv else 3) * (_SM_COUNT.get(q.device.index) or sm_count(q.device))
+            ctas = (4 if nq <= 8 * nkv else 3) * sms
             parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
             counters = batch.ws.get_zeroed("attn_q8_counters", (rows * nkv,), torch.int32)
             at = parts.data_ptr()
             _check(lib.arle_attention_q8_decode(
-                qp, q_stride, op, kp, vp, ksp, vsp, batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), tp, bt_stride, at, at + ctas * 128 * hd, counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks),
-                rows, ctas, int(beside), pos_p, row_p, _stream()), "attention_q8_decode")
+                qp, q_stride, op, kp, vp, ksp, vsp, batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), tp, bt_stride, at, at + ctas * 128 * hd,
+                counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks), rows, ctas, int(beside), pos_p, row_p, _stream()), "attention_q8_decode")
         if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
             join()
         return
@@ -2411,17 +2411,27 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         qp, q_stride, op, _dt(q), kp, vp, ksp, vsp, pp, rp, tp, bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
-# Bytes of codes up to which a step's short portions are read token by token.
-Q8_TOKENS_BYTES = 64 << 20
-
-
-def _by_tokens_q8(batch, nkv: int, hd: int, window: int) -> bool:
-    """Whether a step with portions runs token by token, each token a row of the keys up to its own."""
-    keys = 0
+def _by_tokens_q8(batch, nq: int, nkv: int, hd: int, window: int, sms: int) -> bool:
+    """Whether a step with portions runs token by token, each token a row of the keys up to its own: where that is the shorter of two estimates, in us.
+    By tokens: 9, the codes that the portions' tokens read at 7.5 MB a us (heads of 64: 6), a pair of token and kv head as much as 32 kB.  Expanded: 13, the
+    codes at 2 MB a us, 2.3 for each tile of 128 keys of a block's part (heads of 64: 10 and 21.5 for 1,000 keys), 6 if there are decoded tokens beside
+    them, which by tokens are in the same launch.  Measured by tokens and expanded, 8 kv heads of 128
+    with 32 heads: 9 tokens behind 600 10.4 and 17.5, 16 behind 2,000 19.5 and 23.5, 33 behind 1,200 23.6 and 21.5, 4 behind 8,000 19.9 and 54, 128 behind 1,000
+    46 and 23; heads of 64: 64 behind 1,000 23 and 30, 64 behind 4,000 58 and 100, 256 alone 27 and 13."""
+    read = wide = longest = blocks = 0
     for n, kv in zip(batch.q_lens, batch.kv_lens_host):
         if n > 1:
-            keys += n * (min(kv, window) if window else kv)
-    return keys * nkv * hd * 2 <= Q8_TOKENS_BYTES
+            keys = min(kv, window) if window else kv
+            read += n * (keys * hd * 2 + 32768)
+            seen = min(kv, window + n) if window else kv
+            wide += seen
+            longest = max(longest, min(kv, window + 256) if window else kv)
+            blocks += (n + 255) // 256
+    more = 6 if batch.num_single else 0
+    if hd == 64:
+        return 9 + read * nkv / 6e6 <= 10 + 0.0215 * longest + more
+    parts = max(1, min(sms // (nq * max(1, blocks)), longest // 256))
+    return 9 + read * nkv / 7.5e6 <= 13 + wide * nkv * hd / 1e6 + 2.3 * (-(-longest // 128) / parts) + more
 
 
 def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, window: int, batch, sinks):

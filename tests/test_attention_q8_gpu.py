@@ -179,7 +179,7 @@ PORTIONS = [[(70, 70)], [(300, 700)], [(5, 90), (1, 400), (129, 129), (1, 1), (2
 @pytest.mark.parametrize("window,sink", [(None, False), (40, False), (256, True)])
 @pytest.mark.parametrize("by_tokens", [True, False], ids=["by tokens", "expanded"])
 def test_portions(rows, hd, ps, window, sink, by_tokens, monkeypatch):
-    monkeypatch.setattr(ops, "Q8_TOKENS_BYTES", 1 << 40 if by_tokens else 0)
+    monkeypatch.setattr(ops, "_by_tokens_q8", lambda *a: by_tokens)
     s = _case(rows, 8, 2, hd, ps, seed=7)
     if window:
         for r, (n, kv) in enumerate(rows):
@@ -202,7 +202,7 @@ def test_portions_in_parts(splits, rows, window, monkeypatch):
     """The prompt kernel's key tiles in any number of parts, more than there are tiles among them."""
     s = _case(rows, 8, 2, 128, 16, seed=9)
     monkeypatch.setattr(ops, "prompt_splits_q8", lambda *a: splits)
-    monkeypatch.setattr(ops, "Q8_TOKENS_BYTES", 0)
+    monkeypatch.setattr(ops, "_by_tokens_q8", lambda *a: False)
     for sinks in (None, torch.randn(8, generator=torch.Generator().manual_seed(5)).to(DEV)):
         out = _run(s, window, sinks)
         _near(out, _want(s, window, sinks), 128, 2.0 ** -8, max(s.kvs))
@@ -240,7 +240,7 @@ def test_no_window(rows):
             assert torch.equal(_run(s, window, batch=batch), all_keys)
 
 
-@pytest.mark.parametrize("rows", [[(1, 70), (1, 300)], [(3, 70), (1, 300)], [(200, 1500), (1, 300)]], ids=["decoded", "by tokens", "portions"])
+@pytest.mark.parametrize("rows", [[(1, 70), (1, 300)], [(3, 70), (1, 300)], [(200, 1500), (1, 300)]], ids=["decoded", "few", "many"])
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
 def test_rows_behind_the_last_token_are_left_alone(rows, dtype):
     """A padded batch: queries without a request, whose positions and rows are not numbers that anything may be read by."""
@@ -253,18 +253,15 @@ def test_rows_behind_the_last_token_are_left_alone(rows, dtype):
     _near(out[:real], want, 128, 2.0 ** -8, 1500)
 
 
-def test_an_empty_step():
+def test_an_empty_step(monkeypatch):
     """What step_tables leaves of a step that is not in order: no row has queries or keys, no page is there; nothing is read, in whatever form."""
-    for dtype, bytes_ in ((BF, 1 << 40), (BF, 0), (torch.float32, 0)):
+    for dtype, by_tokens in ((BF, True), (BF, False), (torch.float32, False)):
+        monkeypatch.setattr(ops, "_by_tokens_q8", lambda *a, x=by_tokens: x)
         s = _case([(30, 300), (1, 70)], 8, 2, 128, 16, dtype=dtype)
         for x in (s.batch.q_indptr, s.batch.kv_lens, s.positions, s.row_of):
             x.zero_()
         s.bt.fill_(-1)
-        before, ops.Q8_TOKENS_BYTES = ops.Q8_TOKENS_BYTES, bytes_
-        try:
-            _run(s)
-        finally:
-            ops.Q8_TOKENS_BYTES = before
+        _run(s)
         torch.cuda.synchronize()
 
 
