@@ -2388,16 +2388,20 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         if batch.q_indptr.dtype is not i32 or batch.kv_lens.dtype is not i32:
             raise KernelError("paged_attention_q8: the batch's q_indptr and kv_lens must be int32")
         rows, beside, join, pos_p, row_p, sms = batch.num_rows, False, None, None, None, _SM_COUNT.get(q.device.index) or sm_count(q.device)
-        if batch.max_q_len > 1:
-            if _by_tokens_q8(batch, nq, nkv, hd, w, sms):
-                rows, pos_p, row_p = min(T, sum(batch.q_lens)), pp, rp
-            else:
-                beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
-        if batch.num_single > 0 or pos_p is not None:
-            # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals
+        portions = batch.max_q_len > 1
+        if portions and _by_tokens_q8(batch, nq, nkv, hd, w, sms):
+            portions, rows, pos_p, row_p = False, min(T, sum(batch.q_lens)), pp, rp
+        codes = batch.num_single > 0 or pos_p is not None
+        if codes:
+            # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals.  Asked for
+            # before the prompt kernel, since counters that have to grow are zeroed by a launch: nothing may come between that kernel and the decoded
+            # tokens' beside it, which waits for its end alone, and last.
             ctas = (4 if nq <= 8 * nkv else 3) * sms
             parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
             counters = batch.ws.get_zeroed("attn_q8_counters", (rows * nkv,), torch.int32)
+        if portions:
+            beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
+        if codes:
             at = parts.data_ptr()
             _check(lib.arle_attention_q8_decode(
                 qp, q_stride, op, kp, vp, ksp, vsp, batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), tp, bt_stride, at, at + ctas * 128 * hd,

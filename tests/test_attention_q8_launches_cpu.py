@@ -1,0 +1,76 @@
+"""What attention over the 8-bit cache asks of its workspace and launches, in which order, with the library's place taken by a list."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from arle_b200 import ops
+from arle_b200.engine.batch import Workspace
+
+BF, F8, I32 = torch.bfloat16, torch.float8_e4m3fn, torch.int32
+
+
+class Recorded(Workspace):
+    """A workspace that notes which buffers were made (a zeroed one is a launch) beside the launches."""
+
+    def __init__(self, log):
+        super().__init__("cpu")
+        self.log = log
+
+    def _noted(self, made, name, shape, dtype):
+        before = self.generation
+        out = made(name, shape, dtype)
+        if self.generation != before:
+            self.log.append("made " + name)
+        return out
+
+    def get(self, name, shape, dtype):
+        return self._noted(super().get, name, shape, dtype)
+
+    def get_zeroed(self, name, shape, dtype):
+        return self._noted(super().get_zeroed, name, shape, dtype)
+
+
+@pytest.fixture
+def log(monkeypatch):
+    events = []
+
+    class Library:
+        def __getattr__(self, name):
+            def launch(*args):
+                events.append(name)
+                return 0
+            return launch
+
+    monkeypatch.setattr(ops, "library", lambda: Library())
+    monkeypatch.setattr(ops, "_pointers", lambda what, tensors: map(torch.Tensor.data_ptr, tensors))
+    monkeypatch.setattr(ops, "_ptr", lambda t, name="tensor": None if t is None else t.data_ptr())
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_SM_COUNT", {None: 148})
+    monkeypatch.setattr(ops, "error_flag", lambda device: torch.zeros(1, dtype=I32))
+    return events
+
+
+def attend(ws, rows, nq=8, nkv=2, hd=128, ps=16):
+    """One call; rows: (queries, keys)."""
+    z = lambda *n: torch.zeros(*n, dtype=I32)      # noqa: E731
+    lens, kvs = [n for n, _ in rows], [kv for _, kv in rows]
+    T, R, width = sum(lens), len(rows), -(-max(kvs) // ps)
+    batch = SimpleNamespace(q_indptr=z(R + 1), kv_lens=z(R), q_lens=lens, kv_lens_host=kvs, num_rows=R, max_q_len=max(lens), max_kv_len=max(kvs),
+                            num_single=sum(n == 1 for n in lens), ws=ws, memo={})
+    cache = [torch.zeros(4, nkv, ps, hd, dtype=F8) for _ in range(2)] + [torch.zeros(4, nkv) for _ in range(2)]
+    q = torch.zeros(T, nq * hd, dtype=BF)
+    ops.paged_attention_q8(q, torch.empty_like(q), *cache, z(T), z(T), z(R, width), nq, nkv, hd, ps, 0.1, None, batch=batch)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_nothing_comes_between_the_prompt_kernel_and_the_decoded_tokens_beside_it(log, hd):
+    """The decoded tokens' kernel starts beside the prompt kernel and waits for its end only when it is done itself, so counters that are made for it are
+    zeroed in front of the prompt kernel: at the first mixed step, and where a later one needs more of them."""
+    ws = Recorded(log)
+    for decoded, grows in ((2, True), (5, True), (5, False), (40, True)):
+        del log[:]
+        attend(ws, [(1, 700)] * decoded + [(600, 3000)], hd=hd)
+        prompt = max(i for i, e in enumerate(log) if e.startswith("arle_paged_attention_prefill"))
+        assert log[prompt + 1] == "arle_attention_q8_decode", log
+        assert ("made attn_q8_counters" in log[:prompt]) == grows
