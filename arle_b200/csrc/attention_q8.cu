@@ -15,6 +15,9 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kQuads = 2;      // four numbers of a value each: widths up to 256
+// The values' sums are taken in units of 2^24: values end at 2^128 (448 * 2^119), and what up to 2^24 keys add before the largest score is met, or before the
+// division, stays in float32's range.  Exact, but for products below 2^-102.
+constexpr float kUnit = 16777216.f;
 
 // WIDE: keys of a multiple of 16 numbers, values of a multiple of 4, caches on 16-byte boundaries.
 template <typename T, bool WIDE>
@@ -51,7 +54,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
       const long unit = (long)page * nkv + kvh;
       row = unit * page_size + j % page_size;
       const float ks = k_scale[unit];
-      vs = v_scale[unit];
+      vs = v_scale[unit] * (1.f / kUnit);
       const uint8_t* kp = k_cache + row * hd;
       float d = 0.f;
       if constexpr (WIDE) {
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
     float o = 0.f;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) o += acc_s[i][d] * f[i];
-    op[d] = from_f32<T>(nvis > 0 ? o / ll : 0.f);
+    op[d] = from_f32<T>(nvis > 0 ? o / ll * kUnit : 0.f);
   }
 }
 
