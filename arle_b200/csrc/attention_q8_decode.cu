@@ -15,7 +15,9 @@
 // That maximum is followed only where a score passes it by more than kSlack (in log2): the weights stay below 2^kSlack, most tiles need no reduction across
 // lanes and no correction of the sums.  A weight times its key's v_scale is rounded to float16, 11 bits (bfloat16 would keep 8), relative to a second
 // maximum, of weight times scale, that is followed in the same way: at most 2^(kSlack + kUp) = 2^15, in whole down to 2^(-14 - kUp) of the largest.  So
-// keys that carry a query's result keep their bits however much larger the values of other pages are.
+// keys that carry a query's result keep their bits however much larger the values of other pages are.  The product is one exponential of the score plus
+// the scale's logarithm: scales reach from 2^-100 (a page of zeros) to 2^119, and a weight that is zero in float32 times a factor that passes its range would
+// be NaN.  The values' sums stay relative to the second maximum up to the last rounding, for the same reason.
 // The order of the elements of a head among the k indices of S^T, and among the rows of O^T, is free as long as both operands agree: lane (g, c) owns
 // numbers c * HD / 4 ... of a key and g * HD / 8 ... of the values, so a lane's codes are whole 16-byte reads (8 bytes for the values of heads of 64).
 // Rows lie in shared memory with their 16-byte parts in an order turned by the key, which keeps those reads free of bank conflicts.
@@ -114,7 +116,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   __shared__ int4 sum_s[kWarps];
   __shared__ int start_s[2], cut_s[2], last_s;
   __shared__ Row start_row;
-  __shared__ float ml_s[kWarps][NT * 8][2];
+  __shared__ float ml_s[kWarps][NT * 8][3];         // largest score, sum of weights, second maximum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = a.nq / a.nkv, nkv = a.nkv;
   unsigned char* ring = smem + warp * NS * S::kStageBytes;
@@ -198,10 +200,15 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
   Row at_row = start_row;
 
   // Sums lie in the order in which lanes have them, which keeps their way through shared memory free of bank conflicts: place p = 16 j + 2 g + b is
-  // number g * HD / 8 + 2 j + b.  Four places' results (p a multiple of 4) of a head; none: the row has no keys.
-  auto finish = [&](int t, int head, int p, float M, float L, const float4& O, bool none) {
-    if (a.sinks) L += exp2f(a.sinks[head] * 1.4426950408889634f - (M == -INFINITY ? 0.f : M));
-    const float inv = none ? 0.f : 1.0f / L;
+  // number g * HD / 8 + 2 j + b.  Four places' results (p a multiple of 4) of a head: sums of weights relative to 2^M, of values relative to 2^(MW - kUp);
+  // none: the row has no keys.
+  auto finish = [&](int t, int head, int p, float M, float L, float MW, const float4& O, bool none) {
+    if (a.sinks) {
+      const float sink = a.sinks[head] * 1.4426950408889634f, top = fmaxf(M, sink), base = fabsf(top) == INFINITY ? 0.f : top;
+      L = L * exp2f(M - base) + exp2f(sink - base);
+      M = top;
+    }
+    const float inv = none ? 0.f : exp2f(MW - (fabsf(M) == INFINITY ? 0.f : M) - kUp) / L;
     __nv_bfloat16* to = a.out + ((size_t)t * a.nq + head) * HD + (p % 16 / 2) * (HD / 8) + p / 16 * 2;
     *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(O.x * inv, O.y * inv);
     *reinterpret_cast<__nv_bfloat162*>(to + HD / 8) = __floats2bfloat162_rn(O.z * inv, O.w * inv);
@@ -322,11 +329,11 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     }
 
     float o[NT][MT][4], m[NT][2], l[NT][2];
-    float mw[NT][2], up[NT][2];            // the second maximum, in log2; 2^(m - mw + kUp), which o is multiplied by
+    float mw[NT][2];                       // the second maximum, in log2; o is relative to 2^(mw - kUp)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = up[nt][0] = up[nt][1] = 0.f;
+      l[nt][0] = l[nt][1] = 0.f;
       mw[nt][0] = mw[nt][1] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
@@ -342,8 +349,8 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
       cp_wait<NS - 1>();
       __syncwarp();
       const unsigned char* products = ring + stage * S::kStageBytes;
-      // of keys g and g + 8 of each product: scores, scales of the values and their logarithms, whether they are seen
-      float s[SUB][NT][4], vs[SUB][2], lv[SUB][2];
+      // of keys g and g + 8 of each product: scores, logarithms of the values' scales, whether they are seen
+      float s[SUB][NT][4], lv[SUB][2];
       bool in[SUB][2], grew = false;
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
@@ -353,14 +360,12 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         if constexpr (P16) {
           const float2 x = *reinterpret_cast<const float2*>(sc);
           ks[0] = ks[1] = x.x;
-          vs[u][0] = vs[u][1] = x.y;
           lv[u][0] = lv[u][1] = log2_fast(x.y);
         } else {
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             ks[y] = sc[g + 8 * y];
-            vs[u][y] = sc[16 + g + 8 * y];
-            lv[u][y] = log2_fast(vs[u][y]);
+            lv[u][y] = log2_fast(sc[16 + g + 8 * y]);
           }
         }
 #pragma unroll
@@ -415,7 +420,6 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
             f[e] = wn == -INFINITY ? 1.f : exp2_fast(mw[nt][e] - wn);
             m[nt][e] = mn;
             mw[nt][e] = wn;
-            up[nt][e] = wn == -INFINITY ? 0.f : exp2_fast(mn - wn + kUp);
           }
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
@@ -431,17 +435,16 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          const float w0 = in[u][0] ? vs[u][0] : 0.f, w1 = in[u][1] ? vs[u][1] : 0.f;
-          float p[4];
+          float w[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float top = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
-            p[e] = exp2_fast(s[u][nt][e] - top);
-            p[2 + e] = exp2_fast(s[u][nt][2 + e] - top);
-            l[nt][e] += p[e] + p[2 + e];
+            const float top = m[nt][e] == -INFINITY ? 0.f : m[nt][e], up = mw[nt][e] == -INFINITY ? kUp : kUp - mw[nt][e];
+            l[nt][e] += exp2_fast(s[u][nt][e] - top) + exp2_fast(s[u][nt][2 + e] - top);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) w[2 * y + e] = exp2_fast(s[u][nt][2 * y + e] + (in[u][y] ? lv[u][y] + up : -INFINITY));      // unseen: a scale may be anything
           }
-          pb[nt][0] = turned(pack_f16(p[0] * (w0 * up[nt][0]), p[1] * (w0 * up[nt][1])));
-          pb[nt][1] = turned(pack_f16(p[2] * (w1 * up[nt][0]), p[3] * (w1 * up[nt][1])));
+          pb[nt][0] = turned(pack_f16(w[0], w[1]));
+          pb[nt][1] = turned(pack_f16(w[2], w[3]));
         }
         // values: numbers g * HD / 8 ... of keys 2c, 2c + 1, 2c + 8, 2c + 9; two keys' codes are laced so that a pair of codes is one register of V^T
         const unsigned char* vt = products + u * (2 * kTile * HD) + kTile * HD;
@@ -488,15 +491,15 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         const int query = nt * 8 + 2 * c + e;
-        const float out_by = up[nt][e] > 0.f ? 1.0f / up[nt][e] : 0.f;
         if (g == 0) {
           ml_s[warp][query][0] = m[nt][e];
           ml_s[warp][query][1] = x;
+          ml_s[warp][query][2] = mw[nt][e];
         }
         if (query < G) {
           float* dst = mo + (warp * NT * 8 + query) * S::kPitch + 2 * g;
 #pragma unroll
-          for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(dst + 16 * j) = make_float2(o[nt][j][e] * out_by, o[nt][j][2 + e] * out_by);
+          for (int j = 0; j < MT; ++j) *reinterpret_cast<float2*>(dst + 16 * j) = make_float2(o[nt][j][e], o[nt][j][2 + e]);
         }
       }
     }
@@ -505,24 +508,27 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     const size_t slot = (size_t)blockIdx.x * 2 + (blk0 == 0);      // a CTA has one cut pair's start and one cut pair's further part at most
     for (int i = tid; i < G * (HD / 4); i += kThreads) {
       const int query = i / (HD / 4), p = i % (HD / 4) * 4;
-      float M = -INFINITY;
+      float M = -INFINITY, MW = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml_s[w][query][0]);
-      const float top_s = M == -INFINITY ? 0.f : M;
+      for (int w = 0; w < kWarps; ++w) {
+        M = fmaxf(M, ml_s[w][query][0]);
+        MW = fmaxf(MW, ml_s[w][query][2]);
+      }
+      const float top_s = M == -INFINITY ? 0.f : M, top_w = MW == -INFINITY ? 0.f : MW;
       float L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_fast(ml_s[w][query][0] - top_s);
+        const float f = exp2_fast(ml_s[w][query][2] - top_w);
         const float4 x = *reinterpret_cast<const float4*>(mo + (w * NT * 8 + query) * S::kPitch + p);
-        L += ml_s[w][query][1] * f;
+        L += ml_s[w][query][1] * exp2_fast(ml_s[w][query][0] - top_s);
         O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
       }
       if (whole) {
-        finish(t, h * G + query, p, M, L, O, kv <= 0);
+        finish(t, h * G + query, p, M, L, MW, O, kv <= 0);
       } else {
         *reinterpret_cast<float4*>(a.part_o + (slot * 16 + query) * HD + p) = O;
-        if (p == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * 16 + query) * 2) = make_float2(M, L);
+        if (p == 0) *reinterpret_cast<float4*>(a.part_ml + (slot * 16 + query) * 4) = make_float4(M, L, MW, 0.f);
       }
     }
     if (!whole) {
@@ -543,55 +549,61 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         // four numbers a thread; where there are fewer such quads than threads, `sets` of threads take every sets-th piece of a quad and add up their sums
         const int quads = G * (HD / 4), sets = max(1, min(8, kThreads / quads)), set = tid / quads;
         float4* so = reinterpret_cast<float4*>(smem);
-        float2* sml = reinterpret_cast<float2*>(smem + kThreads * 16);
+        float4* sml = reinterpret_cast<float4*>(smem + kThreads * 16);
         for (int i = sets > 1 ? tid - set * quads : tid; i < quads; i += kThreads) {
           const int query = i / (HD / 4), d = i % (HD / 4) * 4;
-          float M = -INFINITY, L = 0.f;
+          float M = -INFINITY, L = 0.f, MW = -INFINITY;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int k0 = sets > 1 ? set : 0; k0 < (set < sets || sets == 1 ? pieces : 0); k0 += 8 * sets) {      // eight pieces' numbers under way at once
-            float2 ml[8];
-            float4 po[8];
+            float4 ml[8], po[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const int piece = k0 + k * sets;
               const size_t at = ((size_t)(first_cta + piece) * 2 + (piece == 0)) * 16 + query;
-              ml[k] = piece < pieces ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + at) : make_float2(-INFINITY, 0.f);
+              ml[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_ml) + at) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
               po[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
-            float top = M;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
-            const float top_s = top == -INFINITY ? 0.f : top, was = exp2_fast(M - top_s);
-            L *= was;
-            O = make_float4(O.x * was, O.y * was, O.z * was, O.w * was);
-            M = top;
+            float top = M, top_mw = MW;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float f = exp2_fast(ml[k].x - top_s);
-              L += ml[k].y * f;
+              top = fmaxf(top, ml[k].x);
+              top_mw = fmaxf(top_mw, ml[k].z);
+            }
+            const float top_s = top == -INFINITY ? 0.f : top, top_w = top_mw == -INFINITY ? 0.f : top_mw, was = exp2_fast(MW - top_w);
+            L *= exp2_fast(M - top_s);
+            O = make_float4(O.x * was, O.y * was, O.z * was, O.w * was);
+            M = top;
+            MW = top_mw;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float f = exp2_fast(ml[k].z - top_w);
+              L += ml[k].y * exp2_fast(ml[k].x - top_s);
               O = make_float4(O.x + po[k].x * f, O.y + po[k].y * f, O.z + po[k].z * f, O.w + po[k].w * f);
             }
           }
           if (sets > 1) {
             so[tid] = O;
-            sml[tid] = make_float2(M, L);
+            sml[tid] = make_float4(M, L, MW, 0.f);
             continue;
           }
-          finish(t, h * G + query, d, M, L, O, false);
+          finish(t, h * G + query, d, M, L, MW, O, false);
         }
         if (sets > 1) {
           __syncthreads();
           for (int i = tid; i < quads; i += kThreads) {
-            float M = -INFINITY, L = 0.f;
+            float M = -INFINITY, L = 0.f, MW = -INFINITY;
             float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < sets; ++k) M = fmaxf(M, sml[k * quads + i].x);
             for (int k = 0; k < sets; ++k) {
-              const float f = exp2_fast(sml[k * quads + i].x - (M == -INFINITY ? 0.f : M));
+              M = fmaxf(M, sml[k * quads + i].x);
+              MW = fmaxf(MW, sml[k * quads + i].z);
+            }
+            for (int k = 0; k < sets; ++k) {
+              const float f = exp2_fast(sml[k * quads + i].z - (MW == -INFINITY ? 0.f : MW));
               const float4 x = so[k * quads + i];
-              L += sml[k * quads + i].y * f;
+              L += sml[k * quads + i].y * exp2_fast(sml[k * quads + i].x - (M == -INFINITY ? 0.f : M));
               O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
             }
-            finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, O, false);
+            finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, MW, O, false);
           }
         }
       }
@@ -631,7 +643,7 @@ int launch_by(const DecodeArgs& a, int ctas, cudaStream_t s) {
 
 }  // namespace
 
-// Rows with one query; others are left alone.  With positions and row_of_token (int32 [rows]) the rows are the step's tokens, all of them.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 2], counters int32
+// Rows with one query; others are left alone.  With positions and row_of_token (int32 [rows]) the rows are the step's tokens, all of them.  Scratch: part_o float32 [ctas * 2 * 16 * hd], part_ml float32 [ctas * 2 * 16 * 4], counters int32
 // [rows * nkv], zero before the first launch (the kernel leaves them zero).
 // beside: the kernel in front of it on the stream is a prompt kernel launched in stream order that writes none of what this one reads; then this one starts
 // as soon as that one's last block has started, on the SMs that it leaves free.  (It starts when all in front of that kernel is done.)

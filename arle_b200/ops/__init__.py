@@ -2393,11 +2393,11 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
             portions, rows, pos_p, row_p = False, min(T, sum(batch.q_lens)), pp, rp
         codes = batch.num_single > 0 or pos_p is not None
         if codes:
-            # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their maxima and totals.  Asked for
+            # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their two maxima and totals.  Asked for
             # before the prompt kernel, since counters that have to grow are zeroed by a launch: nothing may come between that kernel and the decoded
             # tokens' beside it, which waits for its end alone, and last.
             ctas = (4 if nq <= 8 * nkv else 3) * sms
-            parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 2),), torch.float32)
+            parts = batch.ws.get("attn_q8_parts", (ctas * 32 * (hd + 4),), torch.float32)
             counters = batch.ws.get_zeroed("attn_q8_counters", (rows * nkv,), torch.int32)
         if portions:
             beside, join = _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nkv, hd, page_size, scale, w, batch, sinks)
