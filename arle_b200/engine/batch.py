@@ -103,6 +103,31 @@ class GroupTables:
     slot_mapping: torch.Tensor      # int32 [T]
 
 
+class TablesStatus:
+    """What ``ops.step_tables`` says of a step (a word for each cache group), on its way to the host.  ``check()`` waits for the words alone, which are
+    copied in front of the step's layers, and raises if a group's tables were not in order: that step ran as an empty one, its logits mean nothing."""
+
+    def __init__(self, words: torch.Tensor, host: torch.Tensor, free: List[torch.Tensor]):
+        self._n, self._free, self._codes, self._event = words.numel(), free, None, None
+        self._host = host
+        host[: self._n].copy_(words, non_blocking=True)
+        if words.is_cuda:
+            self._event = torch.cuda.Event()
+            self._event.record()
+
+    def check(self) -> None:
+        if self._codes is None:
+            if self._event is not None:
+                self._event.synchronize()
+            self._codes = self._host[: self._n].tolist()
+            self._free.append(self._host)
+            self._host = None
+        for gi, code in enumerate(self._codes):
+            if code != 0:
+                raise RuntimeError(f"the device's tables of cache group {gi} were not in order (status {code}, see ops.step_tables): the step ran without tokens and "
+                                   "its results are invalid")
+
+
 class StepContext:
     """Device-side description of one step, handed to every part.
 
@@ -139,6 +164,8 @@ class StepContext:
         self._pinned: Optional[torch.Tensor] = None
         self._dev: Optional[torch.Tensor] = None
         self._made: Optional[torch.Tensor] = None            # tables made on the device
+        self.tables_status: Optional[TablesStatus] = None    # of this step, if they were
+        self._status_hosts: List[torch.Tensor] = []          # pinned words not held by a status
         self._copied = torch.cuda.Event() if self.device.type == "cuda" else None
 
     # ------------------------------------------------------------------ build
@@ -170,6 +197,8 @@ class StepContext:
             widths.append(table_width if table_width is not None else need)
         self.table_width = max(widths) if widths else 0
         if cm.device_tables and n_groups:
+            if self.tables_status is not None:
+                self.tables_status.check()      # of the step before this one
             return self._build_on_device(entries, starts, widths)
         # layout of the packed int32 array
         sizes = [T, T, T, R + 1, R, R, max(W, 1), T, max(W, 1)]
@@ -300,18 +329,20 @@ class StepContext:
         self.h2d_bytes = total * 4
         cut = lambda k, n: dev[offs[k]:offs[k] + n]      # noqa: E731
         self.token_ids, self.want_rows, self.want_slots, self.state_slots = cut(0, T), cut(1, W), cut(2, W), cut(3, R)
-        made = [T, T, T, R + 1, R, 1] + [x for w in widths for x in (R * w, T)]
+        made = [T, T, T, R + 1, R, len(cm.groups)] + [x for w in widths for x in (R * w, T)]
         at = np.concatenate([[0], np.cumsum([(s + 3) // 4 * 4 for s in made])])
         if self._made is None or self._made.numel() < at[-1]:
             self._made = torch.zeros(max(int(at[-1]), 4096), dtype=torch.int32, device=self.device)
         piece = lambda k: self._made[at[k]:at[k] + made[k]]      # noqa: E731
         self.positions, self.row_of_token, self.slot_of_token, self.q_indptr, self.kv_lens = (piece(k) for k in range(5))
-        self.groups = []
+        self.groups, status = [], piece(5)
         for gi, g in enumerate(cm.groups):
             bt, sm = piece(6 + 2 * gi).view(R, widths[gi]), piece(7 + 2 * gi)
             ops.step_tables(self.state_slots, cut(4, R), cut(5, R), cut(6 + gi, gained[gi]), g.device_table, g.pool.num_pages, g.page_size, self.q_indptr, self.kv_lens,
-                            self.positions, self.row_of_token, self.slot_of_token, sm, bt, piece(5))
+                            self.positions, self.row_of_token, self.slot_of_token, sm, bt, status[gi: gi + 1])
             self.groups.append(GroupTables(bt, sm))
+        words = self._status_hosts.pop() if self._status_hosts else torch.empty(len(cm.groups), dtype=torch.int32, pin_memory=self._copied is not None)
+        self.tables_status = TablesStatus(status, words, self._status_hosts)
         return self
 
     def _host_buffer(self, n: int) -> torch.Tensor:

@@ -81,7 +81,7 @@ class Engine:
             o.scheduler_mixed_policy), model.spec.stop_token_ids, o.max_tokens)
         self.sampler = Sampler(model.spec.vocab_size, o.device)
         self._rngs: Dict[object, object] = {}
-        self._inflight: list = []           # (plan, sample handle) of the steps launched in the last tick
+        self._inflight: list = []           # (plan, sample handle, status of the device's tables) of the steps launched in the last tick
         self._next_id = 0
 
     @staticmethod
@@ -167,7 +167,7 @@ class Engine:
                                                    [self._rngs[r.rid] for r in sampling],
                                                    self.runner.last_ctx.want_slots, self.runner.last_token)
             self.scheduler.on_launch(plan)
-            launched.append((plan, handle))
+            launched.append((plan, handle, self.runner.last_ctx.tables_status))
         if finished is None:
             finished = self._drain()
         self._inflight = launched
@@ -176,7 +176,9 @@ class Engine:
     def _drain(self) -> list:
         """Reads the tokens of the steps in flight and books them."""
         finished = []
-        for plan, handle in self._inflight:
+        for plan, handle, status in self._inflight:
+            if status is not None:
+                status.check()
             done = self.scheduler.on_step_done(plan, handle.result() if handle is not None else [])
             for r in done:
                 self._rngs.pop(r.rid, None)
