@@ -50,9 +50,8 @@ class Workspace:
         if buf is None or buf.numel() < n:
             if self.frozen:
                 raise RuntimeError(f"workspace buffer '{name}' would have to grow inside a captured graph")
-            buf = torch.empty(max(n, 1), dtype=dtype, device=self.device)
-            self._bufs[key] = buf
-            self.generation += 1
+            last = buf = None                       # or they would keep the smaller one
+            buf = self._grown(torch.empty, key, n)
         view = buf[:n].view(shape)
         self._views[key] = (tuple(shape), view)
         self._cuts.pop(key, None)
@@ -72,13 +71,20 @@ class Workspace:
         if buf is None or buf.numel() < n:
             if self.frozen:
                 raise RuntimeError(f"workspace buffer '{name}' would have to grow inside a captured graph")
-            buf = torch.zeros(max(n, 1), dtype=dtype, device=self.device)
-            self._bufs[key] = buf
-            self.generation += 1
+            last = buf = None                       # or they would keep the smaller one
+            buf = self._grown(torch.zeros, key, n)
         view = buf[:n].view(shape)
         self._views[key] = (tuple(shape), view)
         self._cuts.pop(key, None)
         return view
+
+    def _grown(self, make, key, n: int) -> torch.Tensor:
+        """A larger buffer in the place of the one there was, which goes first: the device never has to hold both."""
+        for kept in (self._bufs, self._views, self._cuts):
+            kept.pop(key, None)
+        self.generation += 1
+        buf = self._bufs[key] = make(max(n, 1), dtype=key[1], device=self.device)
+        return buf
 
     def cut(self, name: str, view: torch.Tensor, first: int, last: int) -> torch.Tensor:
         """``view[:, first: last]`` of a view that ``get`` handed out under this name.  Kept as long as the view is: making one costs the host as

@@ -95,11 +95,10 @@ class Engine:
 
     @staticmethod
     def _bytes_expanded(model, max_seq: int) -> int:
-        """The bfloat16 pages that a step's prompt portions are read from when the cache has 8 bits (one layer's at a time)."""
+        """What attention keeps beside a cache of 8 bits: the bfloat16 pages that a step's prompt portions are read from (one layer's at a time), and sums."""
         from .. import ops
 
-        longest = -(-max_seq // 64) * 64 * 2 * max((n.elements_per_token() for n in model.cache_needs), default=0)
-        return max(ops.Q8_EXPAND_BYTES, longest)
+        return ops.q8_scratch_bytes(-(-max_seq // 64) * 64 * 2 * max((n.elements_per_token() for n in model.cache_needs), default=0))
 
     @staticmethod
     def _bytes_beside_the_cache(model, o: EngineOptions) -> int:

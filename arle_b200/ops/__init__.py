@@ -2415,6 +2415,13 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         qp, q_stride, op, _dt(q), kp, vp, ksp, vsp, pp, rp, tp, bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
 
 
+def q8_scratch_bytes(row_bytes: int, sms: int = 148) -> int:
+    """At most what ``paged_attention_q8`` keeps in a workspace for models whose longest row's keys and values of a layer take ``row_bytes`` in bfloat16:
+    the expanded pages, the sums of the prompt kernel's parts, and those of the decoded tokens, eager and captured (heads of 128).  Tables are not counted."""
+    expanded = Q8_EXPAND_BYTES if row_bytes <= Q8_EXPAND_BYTES else row_bytes // Q8_EXPAND_BYTES * Q8_EXPAND_BYTES + 2 * Q8_EXPAND_BYTES
+    return expanded + 4 * sms * (256 * 130 + 2 * 32 * 132) * 4
+
+
 def _by_tokens_q8(batch, nq: int, nkv: int, hd: int, window: int, sms: int) -> bool:
     """Whether a step with portions runs token by token, each token a row of the keys up to its own: where that is the shorter of two estimates, in us.
     By tokens: 9, the codes that the portions' tokens read at 7.5 MB a us (heads of 64: 6), a pair of token and kv head as much as 32 kB.  Expanded: 13, the
@@ -2463,9 +2470,11 @@ def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nk
                 end = r1                   # rows behind the last one with a portion are left out
         rows, mine = end - r0, q_lens[r0: end]
         longest, single = max(mine), int(min(mine) < 2)
-        kx = ws.get("attn_q8_keys", (total * nkv * page * hd,), torch.bfloat16).data_ptr()
-        vx = ws.get("attn_q8_values", (total * nkv * page * hd,), torch.bfloat16).data_ptr()
-        table = ws.get("attn_q8_table", (rows * width,), torch.int32).data_ptr()
+        # room in powers of two up to what goes at a time, in multiples of that behind it: a prompt's portions see more keys one after the other
+        room = min(1 << (total - 1).bit_length(), most) if total <= most else -(-total // most) * most
+        kx = ws.get("attn_q8_keys", (room * nkv * page * hd,), torch.bfloat16).data_ptr()
+        vx = ws.get("attn_q8_values", (room * nkv * page * hd,), torch.bfloat16).data_ptr()
+        table = ws.get("attn_q8_table", (1 << (rows * width - 1).bit_length(),), torch.int32).data_ptr()
         indptr, lens = indptr0 + 4 * r0, lens0 + 4 * r0
         _check(lib.arle_expand_q8(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), indptr, lens, bt0 + 4 * r0 * bt_stride, bt_stride,
                                   page_size, nkv, hd, window, rows, 2, kx, vx, total, table, width, stream), "expand_q8")
@@ -2480,7 +2489,7 @@ def _portions_q8(q, out, k_cache, v_cache, k_scale, v_scale, block_table, nq, nk
                                                            None, 0, window, rows, longest, single, err, 0, 0.0, 0, None, stream), "paged_attention_prefill_tc")
             else:
                 blocks = nq * -(-longest // 256) * rows * splits
-                part_o = ws.get("attn_q8_prompt_parts", (blocks * 256 * 130,), torch.float32).data_ptr()
+                part_o = ws.get("attn_q8_prompt_parts", (max(blocks, 4 * (_SM_COUNT.get(q.device.index) or sm_count(q.device))) * 256 * 130,), torch.float32).data_ptr()
                 part_ml = part_o + blocks * 256 * 128 * 4
                 _check(lib.arle_paged_attention_prefill_tc_parts(qp, q_stride, T, op, kx, vx, total, indptr, lens, table, width, width, nq, nkv, hd, page, float(scale),
                                                                  window, rows, longest, single, err, splits, part_o, part_ml, stream), "paged_attention_prefill_tc_parts")

@@ -1,4 +1,5 @@
 """What attention over the 8-bit cache asks of its workspace and launches, in which order, with the library's place taken by a list."""
+import weakref
 from types import SimpleNamespace
 
 import pytest
@@ -74,3 +75,35 @@ def test_nothing_comes_between_the_prompt_kernel_and_the_decoded_tokens_beside_i
         prompt = max(i for i, e in enumerate(log) if e.startswith("arle_paged_attention_prefill"))
         assert log[prompt + 1] == "arle_attention_q8_decode", log
         assert ("made attn_q8_counters" in log[:prompt]) == grows
+
+
+def test_a_long_prompt_in_portions_makes_few_buffers(log):
+    """Every portion sees more keys than the one in front of it; its buffers grow by powers of two."""
+    ws = Recorded(log)
+    for portion in range(1, 65):
+        attend(ws, [(512, 512 * portion)])
+    assert max(log.count(e) for e in log if e.startswith("made")) <= 8        # 8 to 512 pages of 64 tokens, with or without their tables
+
+
+@pytest.mark.parametrize("limit", [1 << 20, 3 << 20, 1 << 30])
+@pytest.mark.parametrize("nkv", [2, 3])
+def test_what_the_engine_leaves_room_for_is_enough(log, monkeypatch, limit, nkv):
+    """Steps of all forms, rows that see more than goes at a time among them, against the bytes that are set aside."""
+    monkeypatch.setattr(ops, "Q8_EXPAND_BYTES", limit)
+    ws = Recorded(log)
+    for rows in ([(300, 700)], [(300, 2100), (1, 900), (200, 200)], [(1, 900)] * 30 + [(700, 1200)] * 2, [(64, 9000), (4000, 4000)], [(2, 8000), (1, 1)], [(600, 9000)] * 3):
+        attend(ws, rows, nq=4 * nkv, nkv=nkv)
+        big = sum(b.numel() * b.element_size() for (name, _), b in ws._bufs.items() if name not in ("attn_q8_table", "attn_q8_counters"))
+        assert big <= ops.q8_scratch_bytes(-(-9000 // 64) * 64 * 2 * 2 * nkv * 128)
+
+
+@pytest.mark.parametrize("zeroed", [False, True])
+def test_a_workspace_lets_go_of_a_buffer_before_it_makes_a_larger_one(monkeypatch, zeroed):
+    ws, name = Workspace("cpu"), "zeros" if zeroed else "empty"
+    get, make = ws.get_zeroed if zeroed else ws.get, getattr(torch, name)
+    first = weakref.ref(get("a", (3, 8), torch.float32))
+    ws.cut("a", first(), 0, 4)
+    alive = []
+    monkeypatch.setattr(torch, name, lambda *a, **k: (alive.append(first() is not None), make(*a, **k))[1])
+    assert get("a", (9, 8), torch.float32).shape == (9, 8)
+    assert alive == [False]
