@@ -2314,14 +2314,19 @@ _DTYPE, _NUMEL, _DEVICE, _POINTER, _CONTIGUOUS = (operator.attrgetter("dtype"), 
                                                   torch.Tensor.is_contiguous)
 
 
-def _pointers(what: str, tensors):
-    """The tensors' addresses; all of them are on the current device, whose stream the launch goes to."""
+def _placed(what: str, tensors):
+    """The current device, whose stream the launch goes to, and the tensors' addresses; all of them are there."""
     on = set(map(_DEVICE, tensors))
-    if len(on) != 1 or -1 in on:
+    device = on.pop()
+    if on or device < 0:
         raise KernelError(f"{what}: tensors on {sorted({str(t.device) for t in tensors})}: arle_b200 kernels run on one CUDA device (there is no CPU path)")
-    if torch._C._cuda_getDevice() not in on:
+    if torch._C._cuda_getDevice() != device:
         raise KernelError(f"{what}: the tensors are on {tensors[0].device}, which is not the current device")
-    return map(_POINTER, tensors)
+    return device, map(_POINTER, tensors)
+
+
+def _pointers(what: str, tensors):
+    return _placed(what, tensors)[1]
 
 
 def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
@@ -2366,31 +2371,48 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
     bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens, and those of short portions, read the codes as they are; the keys and values
     that longer portions of prompts see are first written out as bfloat16 pages, which is exact, for the prompt kernels.  A captured call of decoded tokens goes by the
     lengths on the device when it is replayed; one with portions keeps room for the lengths that the host's copies had, and those have to stay."""
-    (T, width), (q_stride, q_unit), vd = q.shape, q.stride(), hd if vd is None else int(vd)
+    (T, width), (q_stride, q_unit), vd, qd = q.shape, q.stride(), hd if vd is None else int(vd), q.dtype
     if q_unit != 1 or width != nq * hd or out.shape != (T, nq * vd) or not out.is_contiguous():
         raise KernelError("paged_attention_q8: q must be [T, nq*hd] with unit inner stride and out contiguous [T, nq*vd]")
-    if out.dtype is not q.dtype:
+    if out.dtype is not qd:
         raise KernelError("paged_attention_q8: q and out must share a type")
-    if hd > 256 or vd > 256 or nq % nkv:
+    if hd > 256 or vd > 256 or nkv <= 0 or nq % nkv:
         raise KernelError(f"paged_attention_q8: head_dim {hd} / value width {vd} / heads {nq}:{nkv} not supported")
     _q8_cache("paged_attention_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
     i32, (bt_stride, bt_unit) = torch.int32, block_table.stride()
     if positions.dtype is not i32 or row_of_token.dtype is not i32 or block_table.dtype is not i32 or bt_unit != 1:
         raise KernelError("paged_attention_q8: positions, row_of_token and block_table must be int32, rows of the block table contiguous")
-    sinks, w = _sinks(sink, nq, q.device) if sink is not None else None, max(0, int(window)) if window else 0
-    qp, op, kp, vp, ksp, vsp, pp, rp, tp = _pointers("paged_attention_q8", (q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table))
+    w = max(0, int(window)) if window else 0
+    sinks = _sinks(sink, nq, q.device) if sink is not None else None
+    # the rows of the fast kernels as fast_attention_supported has them, and (below) 16-byte copies of codes
+    fast = (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and qd is torch.bfloat16 and nq <= 16 * nkv
+            and q_stride % 8 == 0)
+    if fast:
+        indptr, lens, R = batch.q_indptr, batch.kv_lens, batch.num_rows
+        if not (indptr.dtype is lens.dtype is i32 and indptr.is_contiguous() and lens.is_contiguous()):
+            raise KernelError("paged_attention_q8: the batch's q_indptr and kv_lens must be contiguous int32")
+        if indptr.numel() <= R or lens.numel() < R or block_table.shape[0] < R:
+            raise KernelError(f"paged_attention_q8: a batch of {R} rows needs a q_indptr of {R + 1}, their kv_lens and their rows of the block table, got "
+                              f"{indptr.numel()}, {lens.numel()} and {block_table.shape[0]}")
+        given = (q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table, indptr, lens)
+    else:
+        given = (q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table, positions, positions)
+    if sinks is None:
+        device, (qp, op, kp, vp, ksp, vsp, pp, rp, tp, ip, lp) = _placed("paged_attention_q8", given)
+        sink_p = None
+    else:
+        device, (qp, op, kp, vp, ksp, vsp, pp, rp, tp, ip, lp, sink_p) = _placed("paged_attention_q8", given + (sinks,))
     if T == 0:
         return
     lib = library()
-    # the rows of the fast kernels as fast_attention_supported has them, and 16-byte copies of codes
-    if (batch is not None and _KERNEL_SET == "fast" and vd == hd and (hd == 128 or hd == 64) and q.dtype is torch.bfloat16 and nq <= 16 * nkv and q_stride % 8 == 0
-            and not (qp | kp | vp | op) % 16):
-        if batch.q_indptr.dtype is not i32 or batch.kv_lens.dtype is not i32:
-            raise KernelError("paged_attention_q8: the batch's q_indptr and kv_lens must be int32")
-        rows, beside, join, pos_p, row_p, sms = batch.num_rows, False, None, None, None, _SM_COUNT.get(q.device.index) or sm_count(q.device)
+    if fast and not (qp | kp | vp | op) % 16:
+        rows, beside, join, pos_p, row_p, sms = R, False, None, None, None, _SM_COUNT.get(device) or sm_count(q.device)
         portions = batch.max_q_len > 1
+        if portions and not (len(batch.q_lens) == len(batch.kv_lens_host) == R):
+            raise KernelError(f"paged_attention_q8: a batch of {R} rows with {len(batch.q_lens)} q_lens and {len(batch.kv_lens_host)} kv_lens_host")
         if portions and _by_tokens_q8(batch, nq, nkv, hd, w, sms):
             portions, rows, pos_p, row_p = False, min(T, sum(batch.q_lens)), pp, rp
+            _tokens_q8(rows, positions, row_of_token)
         codes = batch.num_single > 0 or pos_p is not None
         if codes:
             # as many CTAs as are resident; scratch: two pieces of a (row, kv head) for each, their sums and then their two maxima and totals.  Asked for
@@ -2404,15 +2426,21 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
         if codes:
             at = parts.data_ptr()
             _check(lib.arle_attention_q8_decode(
-                qp, q_stride, op, kp, vp, ksp, vsp, batch.q_indptr.data_ptr(), batch.kv_lens.data_ptr(), tp, bt_stride, at, at + ctas * 128 * hd,
-                counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, _ptr(sinks), rows, ctas, int(beside), pos_p, row_p, _stream()), "attention_q8_decode")
+                qp, q_stride, op, kp, vp, ksp, vsp, ip, lp, tp, bt_stride, at, at + ctas * 128 * hd,
+                counters.data_ptr(), nq, nkv, hd, page_size, float(scale), w, sink_p, rows, ctas, int(beside), pos_p, row_p, torch._C._cuda_getCurrentRawStream(device)), "attention_q8_decode")
         if join is not None:      # behind the decoded tokens: those run beside the prompt kernel
             join()
         return
     if batch is not None:
         T = min(T, sum(batch.q_lens))
+    _tokens_q8(T, positions, row_of_token)
     _check(lib.arle_attention_q8(
-        qp, q_stride, op, _dt(q), kp, vp, ksp, vsp, pp, rp, tp, bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, _ptr(sinks), T, _stream()), "attention_q8")
+        qp, q_stride, op, _dt(q), kp, vp, ksp, vsp, pp, rp, tp, bt_stride, nq, nkv, hd, vd, page_size, float(scale), w, sink_p, T, torch._C._cuda_getCurrentRawStream(device)), "attention_q8")
+
+
+def _tokens_q8(T: int, positions, row_of_token) -> None:
+    if positions.numel() < T or row_of_token.numel() < T or not positions.is_contiguous() or not row_of_token.is_contiguous():
+        raise KernelError(f"paged_attention_q8: positions and row_of_token must be contiguous and hold {T} numbers, got {tuple(positions.shape)}, {tuple(row_of_token.shape)}")
 
 
 def q8_scratch_bytes(row_bytes: int, sms: int = 148) -> int:

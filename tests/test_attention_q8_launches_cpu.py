@@ -44,24 +44,28 @@ def log(monkeypatch):
             return launch
 
     monkeypatch.setattr(ops, "library", lambda: Library())
-    monkeypatch.setattr(ops, "_pointers", lambda what, tensors: map(torch.Tensor.data_ptr, tensors))
+    monkeypatch.setattr(ops, "_placed", lambda what, tensors: (-1, map(torch.Tensor.data_ptr, tensors)))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0, raising=False)
     monkeypatch.setattr(ops, "_ptr", lambda t, name="tensor": None if t is None else t.data_ptr())
     monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(ops, "_SM_COUNT", {None: 148})
+    monkeypatch.setattr(ops, "_SM_COUNT", {None: 148, -1: 148})
     monkeypatch.setattr(ops, "error_flag", lambda device: torch.zeros(1, dtype=I32))
     return events
 
 
-def attend(ws, rows, nq=8, nkv=2, hd=128, ps=16):
-    """One call; rows: (queries, keys)."""
+def attend(ws, rows, nq=8, nkv=2, hd=128, ps=16, dtype=BF, change=None):
+    """One call; rows: (queries, keys).  ``change``: of the batch and the call's tables."""
     z = lambda *n: torch.zeros(*n, dtype=I32)      # noqa: E731
     lens, kvs = [n for n, _ in rows], [kv for _, kv in rows]
     T, R, width = sum(lens), len(rows), -(-max(kvs) // ps)
     batch = SimpleNamespace(q_indptr=z(R + 1), kv_lens=z(R), q_lens=lens, kv_lens_host=kvs, num_rows=R, max_q_len=max(lens), max_kv_len=max(kvs),
                             num_single=sum(n == 1 for n in lens), ws=ws, memo={})
     cache = [torch.zeros(4, nkv, ps, hd, dtype=F8) for _ in range(2)] + [torch.zeros(4, nkv) for _ in range(2)]
-    q = torch.zeros(T, nq * hd, dtype=BF)
-    ops.paged_attention_q8(q, torch.empty_like(q), *cache, z(T), z(T), z(R, width), nq, nkv, hd, ps, 0.1, None, batch=batch)
+    q = torch.zeros(T, nq * hd, dtype=dtype)
+    tables = dict(positions=z(T), row_of_token=z(T), block_table=z(R, width))
+    if change is not None:
+        change(batch, tables)
+    ops.paged_attention_q8(q, torch.empty_like(q), *cache, *tables.values(), nq, nkv, hd, ps, 0.1, None, batch=batch)
 
 
 @pytest.mark.parametrize("hd", [64, 128])
@@ -75,6 +79,44 @@ def test_nothing_comes_between_the_prompt_kernel_and_the_decoded_tokens_beside_i
         prompt = max(i for i, e in enumerate(log) if e.startswith("arle_paged_attention_prefill"))
         assert log[prompt + 1] == "arle_attention_q8_decode", log
         assert ("made attn_q8_counters" in log[:prompt]) == grows
+
+
+DECODED, SHORT, LONG = [(1, 70), (1, 300)], [(3, 70), (1, 300)], [(200, 3000), (1, 300)]
+I = lambda n, step=1: torch.zeros(n * step, dtype=I32)[::step]      # noqa: E731
+
+
+def _set(what, value):
+    def change(batch, tables):
+        if what in tables:
+            tables[what] = value
+        else:
+            setattr(batch, what, value)
+    return change
+
+
+@pytest.mark.parametrize("rows,dtype,what,value", [
+    (DECODED, BF, "q_indptr", I(2)), (DECODED, BF, "q_indptr", I(3, 2)), (DECODED, BF, "kv_lens", I(1)), (DECODED, BF, "kv_lens", I(2, 2)),
+    (DECODED, BF, "block_table", torch.zeros(1, 19, dtype=I32)), (SHORT, BF, "positions", I(3)), (SHORT, BF, "positions", I(4, 2)), (SHORT, BF, "row_of_token", I(3)),
+    (SHORT, BF, "row_of_token", I(4, 3)), (LONG, BF, "q_lens", [200]), (LONG, BF, "kv_lens_host", [3000]), (LONG, BF, "block_table", torch.zeros(1, 188, dtype=I32)),
+    (DECODED, torch.float32, "positions", I(1)), (DECODED, torch.float32, "row_of_token", I(2, 2))])
+def test_tables_that_are_too_short_or_not_contiguous_are_refused(log, rows, dtype, what, value):
+    """Whatever a kernel would read behind the end of, or past the strides of: nothing is launched."""
+    ws = Recorded(log)
+    attend(ws, rows, dtype=dtype)
+    del log[:]
+    with pytest.raises(ops.KernelError, match="paged_attention_q8"):
+        attend(ws, rows, dtype=dtype, change=_set(what, value))
+    assert not log
+
+
+def test_longer_tables_are_taken(log):
+    for what, value in (("q_indptr", I(9)), ("kv_lens", I(5)), ("positions", I(9)), ("row_of_token", I(9)), ("block_table", torch.zeros(5, 19, dtype=I32))):
+        attend(Recorded(log), SHORT, change=_set(what, value))
+
+
+def test_no_kv_heads(log):
+    with pytest.raises(ops.KernelError, match="heads"):
+        attend(Recorded(log), DECODED, nkv=0)
 
 
 def test_a_long_prompt_in_portions_makes_few_buffers(log):
