@@ -1,7 +1,8 @@
 // Paged causal attention over the 8-bit cache (q8.cuh), the general form: any head size up to 256, values of their own width, any page size, any number
 // of heads and groups, float32 or bfloat16 queries, float32 arithmetic throughout.
 //     s_j = scale * k_scale[page of j] * (q . k_code_j);   out = sum_j exp(s_j - m) v_scale[page of j] v_code_j / (sum_j exp(s_j - m) + exp(sink - m))
-// over the keys j that the query at position p sees (p - window < j <= p), m the largest score; a query that sees no key gets zeros.
+// over the keys j that the query at position p sees (p - window < j <= p), m the largest score; a query that sees no key gets zeros.  A page that is not
+// there (-1) counts as keys and values of zeros, as in the other kernels: nothing is read for it, and an empty step's queries get zeros.
 // One block per (token, query head); warp w takes tiles w, w + 8, ... of 32 keys counted from the first visible one and the partial results are merged at
 // the end, so a token's order of sums depends on its first key and position alone.  In a tile a lane first has a key (whole rows of codes, 16 bytes a load),
 // then four numbers of every value (one load a key, eight keys under way).  Two rows of 817
@@ -46,11 +47,11 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
   for (int i = 0; i < kQuads; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   for (int i0 = w * 32; i0 < nvis; i0 += kWarps * 32) {
     const int j = lo + i0 + lane;
-    const int page = i0 + lane < nvis ? bt[j / page_size] : -1;
-    const bool seen = page >= 0;                     // an empty step's tables have no pages
-    float sc = -INFINITY, vs = 0.f;
-    long row = 0;
-    if (seen) {
+    const bool seen = i0 + lane < nvis;
+    const int page = seen ? bt[j / page_size] : -1;
+    float sc = seen ? 0.f : -INFINITY, vs = 0.f;
+    long row = -1;
+    if (page >= 0) {
       const long unit = (long)page * nkv + kvh;
       row = unit * page_size + j % page_size;
       const float ks = k_scale[unit];
@@ -86,8 +87,8 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
       for (int x = 0; x < 4; ++x) acc[i][x] *= corr;
     m = m_new;
     __syncwarp();
-    p_s[w][lane] = seen ? p * vs : 0.f;
-    row_s[w][lane] = row * vd;
+    p_s[w][lane] = page >= 0 ? p * vs : 0.f;
+    row_s[w][lane] = row * vd;                       // negative: none
     __syncwarp();
     const int nvalid = min(32, nvis - i0);
     if constexpr (WIDE) {
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
           for (int j0 = 0; j0 < nvalid; j0 += 8) {
             uint32_t c[8];
 #pragma unroll
-            for (int x = 0; x < 8; ++x) c[x] = j0 + x < nvalid ? *reinterpret_cast<const uint32_t*>(v_cache + row_s[w][j0 + x] + d) : 0u;
+            for (int x = 0; x < 8; ++x) c[x] = j0 + x < nvalid && row_s[w][min(j0 + x, 31)] >= 0 ? *reinterpret_cast<const uint32_t*>(v_cache + row_s[w][j0 + x] + d) : 0u;
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
               const float pj = p_s[w][min(j0 + x, 31)];
@@ -113,6 +114,7 @@ __global__ void __launch_bounds__(kWarps * 32) attention_q8_kernel(const T* __re
       }
     } else {
       for (int jj = 0; jj < nvalid; ++jj) {
+        if (row_s[w][jj] < 0) continue;
         const float pj = p_s[w][jj];
         const uint8_t* vp = v_cache + row_s[w][jj];
 #pragma unroll

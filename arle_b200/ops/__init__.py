@@ -2365,7 +2365,8 @@ def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, ro
                        window, batch=None, vd: int = None, sink=None) -> None:
     """Causal attention of this step's queries over a paged cache of 8 bits (``store_q8``): ``paged_attention`` with e4m3 codes and their scales
     in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros; with a
-    ``batch``, rows of q and out behind its last token are left alone.
+    ``batch``, rows of q and out behind its last token are left alone.  The block table's entries are pages of the cache or -1
+    (behind a row's pages, in front of a window); a page of -1 among the keys that a query sees counts as keys and values of zeros, whichever kernel runs.
 
     ``batch`` (a StepContext, or whatever has its q_indptr, kv_lens, q_lens, kv_lens_host, num_rows, max_q_len, num_single and ws) lets faster kernels run:
     bfloat16, heads of 64 and 128, up to 16 query heads to a kv head.  Decoded tokens, and those of short portions, read the codes as they are; the keys and values
