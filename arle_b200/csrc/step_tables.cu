@@ -2,7 +2,7 @@
 // more; page_table[slot] lists its pages.  With held_r = ceil(starts[r] / page_size) and pages_r = ceil((starts[r] + q_lens[r]) / page_size), the row takes
 // the next pages_r - held_r of new_pages in the order of rows, and
 //     q_indptr = the sums of q_lens in front of each row;   kv_lens[r] = starts[r] + q_lens[r];   page_table[slot][held_r ..] = its new pages
-//     block_table[r] = page_table[slot] up to pages_r, -1 behind;   for token i of row r: position p = starts[r] + i, slot_mapping = page of p * page_size + p % page_size
+//     block_table[r] = page_table[slot] up to pages_r, -1 behind and for what is no page of the cache;   for token i of row r: position p = starts[r] + i, slot_mapping = page of p * page_size + p % page_size
 // Every block sums the lengths of all rows for itself (a few microseconds of latency once, whatever the grid is, where a second launch or a wait for
 // another block would cost as much again), then writes its share of the tokens and of the tables' entries.  What is in page_table is read only in front of
 // held_r and written only from there on, so blocks do not disturb one another.  Bound by latency, three dependent accesses (lengths, pages, stores): 4.6 us for 8
@@ -121,8 +121,10 @@ __global__ void __launch_bounds__(kThreads) step_tables_kernel(StepTables a) {
     int page = -1;
     if (!bad) {
       const int held = (begin[r] + ps - 1) / ps, before = r ? taken[r - 1] : 0, pages = held + taken[r] - before;
-      if (j < held) page = a.page_table[(long)slot[r] * a.table_width + j];
-      else if (j < pages) {
+      if (j < held) {
+        page = a.page_table[(long)slot[r] * a.table_width + j];
+        if (page < 0 || page >= a.num_pages) page = -1;      // what reads the table reads the cache there
+      } else if (j < pages) {
         page = a.new_pages[before + j - held];
         a.page_table[(long)slot[r] * a.table_width + j] = page;
       }

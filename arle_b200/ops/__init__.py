@@ -2550,13 +2550,14 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     """A step's tables from the lengths of its requests, on the device (everything int32).
 
     In: slots [R], the requests' slots, each once; starts [R], the tokens that they hold; q_lens [R], the tokens that they bring (0 is fine);
-    new_pages [N], pages for what does not fit the pages that they have, taken in the order of the rows (more than needed is fine);
+    new_pages [N], pages for what does not fit the pages that they have, each once, taken in the order of the rows (more than needed is fine);
     page_table [slots, pages a request may have], contiguous: the pages of every request, to which the new ones are added; num_pages: pages of the cache.
 
     Out: q_indptr [R + 1], kv_lens [R], positions, row_of_token, slot_of_token and slot_mapping [T] (what lies behind the step's last token is left as it
     was), block_table [R, width], contiguous: a row's pages, -1 behind them, and status [1]: 0, or the sum of what is wrong with the step: 1 more tokens
     than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
-    cache.  Such a step leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
+    cache.  Numbers that a row's part of page_table already holds and that are no pages of the cache become -1 in block_table and slot_mapping.  A step that is not
+    in order leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
     every = (slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table, status)
     if set(map(_DTYPE, every)) != {torch.int32} or not all(map(_CONTIGUOUS, every)):
         raise KernelError(f"step_tables: every tensor must be contiguous int32, got {[(str(t.dtype), tuple(t.shape), t.stride()) for t in every]}")
