@@ -109,6 +109,8 @@ class CacheManager:
             raise ValueError("tables on the device are for caches that keep all keys: a layer of this model has a window or chunks")
         if device_tables and max_slots > 4096:
             raise ValueError(f"tables on the device are for up to 4,096 requests at a time, not {max_slots}")
+        if (device_tables or dtype == torch.float8_e4m3fn) and num_pages * page_size > 2 ** 31 - 1:
+            raise ValueError(f"a cache of 8 bits and tables on the device number their places in 32 bits: {num_pages} pages of {page_size} tokens are too many")
         self.page_size = page_size
         self.max_slots = max_slots
         self.max_tokens_per_request = max_tokens_per_request
