@@ -111,23 +111,17 @@ class GroupTables:
 
 class TablesStatus:
     """What ``ops.step_tables`` says of a step (a word for each cache group), on its way to the host.  ``check()`` waits for the words alone, which are
-    copied in front of the step's layers, and raises if a group's tables were not in order: that step ran as an empty one, its logits mean nothing."""
+    copied in front of the step's layers, and raises if a group's tables were not in order: that step ran as an empty one, its logits mean nothing.  The pinned
+    words and the event are its context's, which reads them before it hands them to the next step."""
 
-    def __init__(self, words: torch.Tensor, host: torch.Tensor, free: List[torch.Tensor]):
-        self._n, self._free, self._codes, self._event = words.numel(), free, None, None
-        self._host = host
-        host[: self._n].copy_(words, non_blocking=True)
-        if words.is_cuda:
-            self._event = torch.cuda.Event()
-            self._event.record()
+    def __init__(self, host: torch.Tensor, copied):
+        self._host, self._copied, self._codes = host, copied, None
 
     def check(self) -> None:
         if self._codes is None:
-            if self._event is not None:
-                self._event.synchronize()
-            self._codes = self._host[: self._n].tolist()
-            self._free.append(self._host)
-            self._host = None
+            if self._copied is not None:
+                self._copied.synchronize()
+            self._codes = self._host.tolist()
         for gi, code in enumerate(self._codes):
             if code != 0:
                 raise RuntimeError(f"the device's tables of cache group {gi} were not in order (status {code}, see ops.step_tables): the step ran without tokens and "
@@ -171,7 +165,7 @@ class StepContext:
         self._dev: Optional[torch.Tensor] = None
         self._made: Optional[torch.Tensor] = None            # tables made on the device
         self.tables_status: Optional[TablesStatus] = None    # of this step, if they were
-        self._status_hosts: List[torch.Tensor] = []          # pinned words not held by a status
+        self._status_host: Optional[torch.Tensor] = None     # pinned
         self._copied = torch.cuda.Event() if self.device.type == "cuda" else None
 
     # ------------------------------------------------------------------ build
@@ -330,8 +324,6 @@ class StepContext:
         total = int(offs[6 + last]) + gained[last]
         dev = self._device_buffer(int(offs[-1]))
         dev[:total].copy_(host[:total], non_blocking=True)
-        if self._copied is not None:
-            self._copied.record()
         self.h2d_bytes = total * 4
         cut = lambda k, n: dev[offs[k]:offs[k] + n]      # noqa: E731
         self.token_ids, self.want_rows, self.want_slots, self.state_slots = cut(0, T), cut(1, W), cut(2, W), cut(3, R)
@@ -342,13 +334,19 @@ class StepContext:
         piece = lambda k: self._made[at[k]:at[k] + made[k]]      # noqa: E731
         self.positions, self.row_of_token, self.slot_of_token, self.q_indptr, self.kv_lens = (piece(k) for k in range(5))
         self.groups, status = [], piece(5)
-        for gi, g in enumerate(cm.groups):
-            bt, sm = piece(6 + 2 * gi).view(R, widths[gi]), piece(7 + 2 * gi)
-            ops.step_tables(self.state_slots, cut(4, R), cut(5, R), cut(6 + gi, gained[gi]), g.device_table, g.pool.num_pages, g.page_size, self.q_indptr, self.kv_lens,
-                            self.positions, self.row_of_token, self.slot_of_token, sm, bt, status[gi: gi + 1])
-            self.groups.append(GroupTables(bt, sm))
-        words = self._status_hosts.pop() if self._status_hosts else torch.empty(len(cm.groups), dtype=torch.int32, pin_memory=self._copied is not None)
-        self.tables_status = TablesStatus(status, words, self._status_hosts)
+        if self._status_host is None:
+            self._status_host = torch.empty(len(cm.groups), dtype=torch.int32, pin_memory=self._copied is not None)
+        try:
+            for gi, g in enumerate(cm.groups):
+                bt, sm = piece(6 + 2 * gi).view(R, widths[gi]), piece(7 + 2 * gi)
+                ops.step_tables(self.state_slots, cut(4, R), cut(5, R), cut(6 + gi, gained[gi]), g.device_table, g.pool.num_pages, g.page_size, self.q_indptr, self.kv_lens,
+                                self.positions, self.row_of_token, self.slot_of_token, sm, bt, status[gi: gi + 1])
+                self.groups.append(GroupTables(bt, sm))
+            self._status_host.copy_(status, non_blocking=True)
+        finally:
+            if self._copied is not None:
+                self._copied.record()           # one event for the copy to the device and the one from it
+        self.tables_status = TablesStatus(self._status_host, self._copied)
         return self
 
     def _host_buffer(self, n: int) -> torch.Tensor:
