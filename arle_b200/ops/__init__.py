@@ -2325,10 +2325,6 @@ def _placed(what: str, tensors):
     return device, map(_POINTER, tensors)
 
 
-def _pointers(what: str, tensors):
-    return _placed(what, tensors)[1]
-
-
 def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, hd: int, page_size: int, vd: int = None) -> None:
     """The store of a step's keys and values into a cache of 8 bits: e4m3 codes with one float32 scale for each page and head.
 
@@ -2351,10 +2347,11 @@ def store_q8(k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale, nkv: int, h
     pages = _q8_cache("store_q8", k_cache, v_cache, k_scale, v_scale, nkv, hd, vd, page_size)
     if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
         raise KernelError("store_q8: slot_mapping must be contiguous int32")
-    kp, vp, sp, kcp, vcp, ksp, vsp = _pointers("store_q8", (k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale))
+    device, (kp, vp, sp, kcp, vcp, ksp, vsp) = _placed("store_q8", (k, v, slot_mapping, k_cache, v_cache, k_scale, v_scale))
     if T == 0:
         return
-    _check(library().arle_store_q8(kp, k_stride, vp, v_stride, _dt(k), sp, T, kcp, vcp, ksp, vsp, pages, nkv, hd, vd, page_size, _stream()), "store_q8")
+    _check(library().arle_store_q8(kp, k_stride, vp, v_stride, _dt(k), sp, T, kcp, vcp, ksp, vsp, pages, nkv, hd, vd, page_size,
+                                    torch._C._cuda_getCurrentRawStream(device)), "store_q8")
 
 
 # Bytes of bfloat16 keys and values that prompt portions are expanded into at a time; rows that see more go by themselves.
@@ -2565,8 +2562,9 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     if not (rs == rq == rk == R and r1 == R + 1 and tr == ts == tm == T and one == 1 and page_table.dim() == 2 and block_table.dim() == 2 and block_table.shape[0] == R):
         raise KernelError("step_tables: slots, starts, q_lens and kv_lens are [R], q_indptr [R + 1], the tokens' tables [T], block_table [R, width], "
                           "page_table [slots, pages], status [1]")
-    slots, starts, q_lens, new_pages, table, *outs = _pointers("step_tables", every)
+    device, (slots, starts, q_lens, new_pages, table, *outs) = _placed("step_tables", every)
     max_slots, table_width = page_table.shape
     q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, blocks, status = outs
     _check(library().arle_step_tables(slots, starts, q_lens, R, new_pages, news, table, max_slots, table_width, int(num_pages), int(page_size), q_indptr, kv_lens, positions,
-                                      row_of_token, slot_of_token, slot_mapping, T, blocks, block_table.shape[1], status, _stream()), "step_tables")
+                                      row_of_token, slot_of_token, slot_mapping, T, blocks, block_table.shape[1], status,
+                                      torch._C._cuda_getCurrentRawStream(device)), "step_tables")
