@@ -35,6 +35,7 @@ template <int HD> constexpr int kKeys = kTile * kSub<HD>;           // keys of a
 template <int HD> constexpr int kBlock = kWarps * kKeys<HD>;        // keys of a block of work: 16 KB of codes
 constexpr int kUp = 9;
 constexpr float kSlack = 6.0f;
+constexpr float kNone = -3.4028234663852886e38f;      // a maximum of nothing: finite, so that no difference of two is NaN
 
 struct DecodeArgs {
   const __nv_bfloat16* q;
@@ -232,7 +233,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     // Page of product u of the tile (P16) or of its key lane & 15; -1: nothing of it is seen.
     auto page_of = [&](int tile, int u) -> int {
       const int key = (tile * SUB + u) * kTile + (P16 ? 0 : lane & 15);
-      if (tile >= tile_end || ((SUB > 1 || !P16) && key >= kv) || (!P16 && key < lo)) return -1;
+      if (tile >= tile_end || ((SUB > 1 || !P16) && key >= kv) || key + (P16 ? kTile - 1 : 0) < lo) return -1;
       return bt[a.ps_shift >= 0 ? key >> a.ps_shift : key / a.page_size];
     };
     auto load_product = [&](int tile, int stage, int u, int page) {
@@ -332,9 +333,8 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     float mw[NT][2];                       // the second maximum, in log2; o is relative to 2^(mw - kUp)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = mw[nt][0] = mw[nt][1] = kNone;
       l[nt][0] = l[nt][1] = 0.f;
-      mw[nt][0] = mw[nt][1] = -INFINITY;
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
@@ -416,8 +416,8 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
               w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, d));
             }
             const float mn = fmaxf(m[nt][e], x), wn = fmaxf(mw[nt][e], w);
-            l[nt][e] *= mn == -INFINITY ? 1.f : exp2_fast(m[nt][e] - mn);
-            f[e] = wn == -INFINITY ? 1.f : exp2_fast(mw[nt][e] - wn);
+            l[nt][e] *= exp2_fast(m[nt][e] - mn);
+            f[e] = exp2_fast(mw[nt][e] - wn);
             m[nt][e] = mn;
             mw[nt][e] = wn;
           }
@@ -438,10 +438,9 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
           float w[4];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float top = m[nt][e] == -INFINITY ? 0.f : m[nt][e], up = mw[nt][e] == -INFINITY ? kUp : kUp - mw[nt][e];
-            l[nt][e] += exp2_fast(s[u][nt][e] - top) + exp2_fast(s[u][nt][2 + e] - top);
+            l[nt][e] += exp2_fast(s[u][nt][e] - m[nt][e]) + exp2_fast(s[u][nt][2 + e] - m[nt][e]);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) w[2 * y + e] = exp2_fast(s[u][nt][2 * y + e] + (in[u][y] ? lv[u][y] + up : -INFINITY));      // unseen: a scale may be anything
+            for (int y = 0; y < 2; ++y) w[2 * y + e] = exp2_fast(s[u][nt][2 * y + e] + ((lv[u][y] + kUp) - mw[nt][e]));
           }
           pb[nt][0] = turned(pack_f16(w[0], w[1]));
           pb[nt][1] = turned(pack_f16(w[2], w[3]));
@@ -508,20 +507,19 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
     const size_t slot = (size_t)blockIdx.x * 2 + (blk0 == 0);      // a CTA has one cut pair's start and one cut pair's further part at most
     for (int i = tid; i < G * (HD / 4); i += kThreads) {
       const int query = i / (HD / 4), p = i % (HD / 4) * 4;
-      float M = -INFINITY, MW = -INFINITY;
+      float M = kNone, MW = kNone;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         M = fmaxf(M, ml_s[w][query][0]);
         MW = fmaxf(MW, ml_s[w][query][2]);
       }
-      const float top_s = M == -INFINITY ? 0.f : M, top_w = MW == -INFINITY ? 0.f : MW;
       float L = 0.f;
       float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_fast(ml_s[w][query][2] - top_w);
+        const float f = exp2_fast(ml_s[w][query][2] - MW);
         const float4 x = *reinterpret_cast<const float4*>(mo + (w * NT * 8 + query) * S::kPitch + p);
-        L += ml_s[w][query][1] * exp2_fast(ml_s[w][query][0] - top_s);
+        L += ml_s[w][query][1] * exp2_fast(ml_s[w][query][0] - M);
         O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
       }
       if (whole) {
@@ -552,7 +550,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         float4* sml = reinterpret_cast<float4*>(smem + kThreads * 16);
         for (int i = sets > 1 ? tid - set * quads : tid; i < quads; i += kThreads) {
           const int query = i / (HD / 4), d = i % (HD / 4) * 4;
-          float M = -INFINITY, L = 0.f, MW = -INFINITY;
+          float M = kNone, L = 0.f, MW = kNone;
           float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
           for (int k0 = sets > 1 ? set : 0; k0 < (set < sets || sets == 1 ? pieces : 0); k0 += 8 * sets) {      // eight pieces' numbers under way at once
             float4 ml[8], po[8];
@@ -560,7 +558,7 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
             for (int k = 0; k < 8; ++k) {
               const int piece = k0 + k * sets;
               const size_t at = ((size_t)(first_cta + piece) * 2 + (piece == 0)) * 16 + query;
-              ml[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_ml) + at) : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+              ml[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_ml) + at) : make_float4(kNone, 0.f, kNone, 0.f);
               po[k] = piece < pieces ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float top = M, top_mw = MW;
@@ -569,15 +567,15 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
               top = fmaxf(top, ml[k].x);
               top_mw = fmaxf(top_mw, ml[k].z);
             }
-            const float top_s = top == -INFINITY ? 0.f : top, top_w = top_mw == -INFINITY ? 0.f : top_mw, was = exp2_fast(MW - top_w);
-            L *= exp2_fast(M - top_s);
+            const float was = exp2_fast(MW - top_mw);
+            L *= exp2_fast(M - top);
             O = make_float4(O.x * was, O.y * was, O.z * was, O.w * was);
             M = top;
             MW = top_mw;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float f = exp2_fast(ml[k].z - top_w);
-              L += ml[k].y * exp2_fast(ml[k].x - top_s);
+              const float f = exp2_fast(ml[k].z - top_mw);
+              L += ml[k].y * exp2_fast(ml[k].x - top);
               O = make_float4(O.x + po[k].x * f, O.y + po[k].y * f, O.z + po[k].z * f, O.w + po[k].w * f);
             }
           }
@@ -591,16 +589,16 @@ __device__ __forceinline__ void q8_decode(const DecodeArgs& a) {
         if (sets > 1) {
           __syncthreads();
           for (int i = tid; i < quads; i += kThreads) {
-            float M = -INFINITY, L = 0.f, MW = -INFINITY;
+            float M = kNone, L = 0.f, MW = kNone;
             float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int k = 0; k < sets; ++k) {
               M = fmaxf(M, sml[k * quads + i].x);
               MW = fmaxf(MW, sml[k * quads + i].z);
             }
             for (int k = 0; k < sets; ++k) {
-              const float f = exp2_fast(sml[k * quads + i].z - (MW == -INFINITY ? 0.f : MW));
+              const float f = exp2_fast(sml[k * quads + i].z - MW);
               const float4 x = so[k * quads + i];
-              L += sml[k * quads + i].y * exp2_fast(sml[k * quads + i].x - (M == -INFINITY ? 0.f : M));
+              L += sml[k * quads + i].y * exp2_fast(sml[k * quads + i].x - M);
               O = make_float4(O.x + x.x * f, O.y + x.y * f, O.z + x.z * f, O.w + x.w * f);
             }
             finish(t, h * G + i / (HD / 4), i % (HD / 4) * 4, M, L, MW, O, false);
