@@ -6,7 +6,8 @@
 //     s' = s(a) for a run from offset 0, else max(s, s(a));   codes in front of the run: rne(code * s / s');   new codes: rne(x / s')
 // One group of `warps` warps owns a run of one head of the keys or the values, so the page's scale and older codes are read and written by one owner.
 // A page of up to 2,048 numbers a warp stays in registers between the maximum and the rounding (one read of x); what is larger is read again (from L2).
-// Decoded tokens are bound by the latency of three dependent accesses (place, numbers, codes): 2.0 us for one token, 2.2 us for 64.  Prompts come near
+// Decoded tokens are bound by the latency of three dependent accesses (place, numbers, codes): 2.0 us for one token, 2.1 us for 64, where
+// their pages' scales hold them; with all scales growing the rounding of older codes takes 15 us at the end of 64 pages of 16, 55 with pages of 64.  Prompts come near
 // DRAM's rate: 15,000 tokens of 8 heads of 128 in 20.7 us, 4.7 TB/s; what is left is instructions (five for two numbers in the rounding alone).
 #include "q8.cuh"
 using namespace arle;

@@ -5,8 +5,8 @@
 //     block_table[r] = page_table[slot] up to pages_r, -1 behind and for what is no page of the cache;   for token i of row r: position p = starts[r] + i, slot_mapping = page of p * page_size + p % page_size
 // Every block sums the lengths of all rows for itself (a few microseconds of latency once, whatever the grid is, where a second launch or a wait for
 // another block would cost as much again), then writes its share of the tokens and of the tables' entries.  What is in page_table is read only in front of
-// held_r and written only from there on, so blocks do not disturb one another.  Bound by latency, three dependent accesses (lengths, pages, stores): 4.6 us for 8
-// rows, 6.1 for 256 with 15,000 tokens and tables of 1,000 pages.
+// held_r and written only from there on, so blocks do not disturb one another.  Bound by latency, three dependent accesses (lengths, pages, stores): 5.0 us for 8
+// rows, 6.5 for 256 with 15,000 tokens and tables of 1,000 pages.
 // A step that is not in order (bits of *status below) leaves page_table as it is and an empty step in the outputs: lengths of 0, places and pages of -1.
 #include "common.cuh"
 using namespace arle;
