@@ -83,6 +83,7 @@ class CacheGroup:
         # host block tables, one row per slot; logical page -> physical page, -1 = not held
         self.table = np.full((max_slots, max_pages_per_request), -1, dtype=np.int32)
         self.first_held = np.zeros(max_slots, dtype=np.int64)     # first logical page still held (past the kept first pages)
+        self.num_listed = np.zeros(max_slots, dtype=np.int64)     # logical pages that ``device_table`` lists as ``table`` does
         self.num_logical = np.zeros(max_slots, dtype=np.int64)    # logical pages ever given to the slot
         # pages that hold a request's first ``keep_first`` tokens stay for its life: logical pages [0, kept_pages)
         self.kept_pages = -(-int(need.keep_first) // page_size) if need.window is not None and need.keep_first > 0 else 0
@@ -172,6 +173,7 @@ class CacheManager:
             g.table[slot, :hi] = -1
             g.first_held[slot] = 0
             g.num_logical[slot] = 0
+            g.num_listed[slot] = 0
         self._free_slots.append(slot)
 
     # ----------------------------------------------------------------- growth
@@ -259,6 +261,7 @@ class CacheManager:
                 g.pool.free(int(p) for p in g.table[slot, keep:hi])
                 g.table[slot, keep:hi] = -1
                 g.num_logical[slot] = keep
+            g.num_listed[slot] = min(int(g.num_listed[slot]), keep)
         self._tokens[rid] = n_tokens
 
     # ------------------------------------------------------------ step tables

@@ -310,10 +310,15 @@ class StepContext:
         h[offs[3]:offs[3] + R] = slots
         h[offs[4]:offs[4] + R] = starts_np
         h[offs[5]:offs[5] + R] = lens
-        gained = []
+        gained, listed = [], []
         for gi, g in enumerate(cm.groups):
             ps = g.page_size
             held, pages = -(-starts_np // ps), -(-(starts_np + lens) // ps)
+            # room that was made without a step: the kernel reads the device's table up to the tokens in front of this one
+            for r in np.nonzero(g.num_listed[slots] < held)[0]:
+                first, late = int(g.num_listed[slots[r]]), g.table[slots[r], :held[r]]
+                g.device_table[int(slots[r]), first:int(held[r])].copy_(torch.from_numpy(late[first:].copy()))
+            listed.append(pages)
             more = np.nonzero(pages > held)[0]
             new = np.concatenate([g.table[slots[r], held[r]:pages[r]] for r in more]) if more.size else np.zeros(0, dtype=np.int32)
             if (new < 0).any():
@@ -341,6 +346,7 @@ class StepContext:
                 bt, sm = piece(6 + 2 * gi).view(R, widths[gi]), piece(7 + 2 * gi)
                 ops.step_tables(self.state_slots, cut(4, R), cut(5, R), cut(6 + gi, gained[gi]), g.device_table, g.pool.num_pages, g.page_size, self.q_indptr, self.kv_lens,
                                 self.positions, self.row_of_token, self.slot_of_token, sm, bt, status[gi: gi + 1])
+                g.num_listed[slots] = listed[gi]
                 self.groups.append(GroupTables(bt, sm))
             self._status_host.copy_(status, non_blocking=True)
         finally:
