@@ -2360,8 +2360,8 @@ Q8_EXPAND_BYTES = 1 << 30
 
 def paged_attention_q8(q, out, k_cache, v_cache, k_scale, v_scale, positions, row_of_token, block_table, nq: int, nkv: int, hd: int, page_size: int, scale: float,
                        window, batch=None, vd: int = None, sink=None) -> None:
-    """Causal attention of this step's queries over a paged cache of 8 bits (``store_q8``): ``paged_attention`` with e4m3 codes and their scales
-    in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros; with a
+    """Causal attention of this step's queries over a paged cache of 8 bits (``store_q8``): ``paged_attention`` with e4m3 codes and their scales (positive
+    numbers, as the store leaves them) in place of keys and values.  q and out float32 or bfloat16; ``window``, ``vd`` and ``sink`` as there.  A query that sees no key gets zeros; with a
     ``batch``, rows of q and out behind its last token are left alone.  The block table's entries are pages of the cache or -1
     (behind a row's pages, in front of a window); a page of -1 among the keys that a query sees counts as keys and values of zeros, whichever kernel runs.
 
