@@ -2554,7 +2554,8 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     was), block_table [R, width], contiguous: a row's pages, -1 behind them, and status [1]: 0, or the sum of what is wrong with the step: 1 more tokens
     than T; 2 a slot outside the table or named twice; 4 a request longer than the tables are wide; 8 too few new pages; 16 a negative length; 32 a new page outside the
     cache.  Numbers that a row's part of page_table already holds and that are no pages of the cache become -1 in block_table and slot_mapping.  A step that is not
-    in order leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1."""
+    in order leaves page_table as it was and an empty step in the outputs: lengths and sums of 0, places and pages of -1.  That is nothing to read for kernels that go by
+    q_indptr and kv_lens, and for ``paged_attention_q8``; others that go by positions would read the cache at page -1, so look at status before them."""
     every = (slots, starts, q_lens, new_pages, page_table, q_indptr, kv_lens, positions, row_of_token, slot_of_token, slot_mapping, block_table, status)
     if set(map(_DTYPE, every)) != {torch.int32} or not all(map(_CONTIGUOUS, every)):
         raise KernelError(f"step_tables: every tensor must be contiguous int32, got {[(str(t.dtype), tuple(t.shape), t.stride()) for t in every]}")
