@@ -1,0 +1,347 @@
+// Activations and weights as e4m3 codes (q8.cuh), for the products of gemm_q8.cu.
+//
+// Rows: numbers of k are taken in groups of 128 (kb = ceil(K / 128) of them; the last is filled up with codes of zero).  A group's scale is the least
+// power of two s with max |x| <= 448 s (2^-100 to 2^119), stored as its exponent (e8m0: exponent + 127); codes are rne(x / s).  Numbers that are not
+// finite do not count for the scale and become NaN: e4m3 has no infinities, and what was not finite must not come out of a product as if it were.
+// Weights: the same for blocks of 128 x 128, one float32 scale a block.
+// All four kernels read every number once, keep it in registers between the maximum and the rounding, and are bound by DRAM (few rows: by latency).
+#include "q8.cuh"
+using namespace arle;
+
+namespace {
+
+constexpr int kGroup = 128;
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The bits of |v|, 0 where v is not finite.
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = abs_bits(v);
+  return b < kInfBits ? b : 0u;
+}
+__device__ __forceinline__ float finite_or_nan(float v) { return abs_bits(v) < kInfBits ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ float inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two in 2^-100 .. 2^119
+__device__ __forceinline__ uint8_t exponent_byte(float s) { return (uint8_t)(__float_as_uint(s) >> 23); }
+
+// The maximum of `bits` over the 2^k lanes that share lane / LANES.  (Bits of numbers without their sign are ordered as the numbers are.)
+template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t bits) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+  return bits;
+}
+
+// The codes of a group that LANES lanes hold, V consecutive numbers each: returns the scale, words of four codes in `w`.
+template <int LANES, int V> __device__ __forceinline__ float group_codes(float (&v)[V], uint32_t (&w)[V / 4]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) most = max(most, abs_bits(v[j]));
+  most = lanes_max<LANES>(most);
+  if (__any_sync(0xffffffffu, most >= kInfBits)) {
+    most = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) most = max(most, finite_bits(v[j])), v[j] = finite_or_nan(v[j]);
+    most = lanes_max<LANES>(most);
+  }
+  const float s = q8_scale(__uint_as_float(most)), inv = inverse(s);
+#pragma unroll
+  for (int j = 0; j < V / 4; ++j) w[j] = q8_codes4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+  return s;
+}
+
+// V numbers from p on, of which `left` are there (the others are zero).
+template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void load_numbers(const T* p, int left, float (&v)[V]) {
+  if constexpr (ALIGNED) {
+    if (left >= V) {
+      load_vec<T, V>(p, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < left ? to_f32(p[j]) : 0.f;
+  }
+}
+
+// ------------------------------------------------------------------ rows
+// A lane takes 16 bytes: a group is 16 lanes of bfloat16 or 32 of float32.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row_stride, uint8_t* codes, uint8_t* scales, long groups, int K, int kb) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int V = 16 / sizeof(T), LANES = kGroup / V;
+  const long g = ((long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+  const int sub = threadIdx.x % LANES;
+  const bool mine = g < groups;
+  const long row = mine ? g / kb : 0;
+  const int b = (int)(g - row * kb), at = b * kGroup + sub * V;
+  float v[V];
+  load_numbers<T, V, ALIGNED>(x + row * row_stride + at, mine ? K - at : 0, v);
+  uint32_t w[V / 4];
+  const float s = group_codes<LANES, V>(v, w);
+  if (!mine) return;
+  uint8_t* dst = codes + (size_t)g * kGroup + sub * V;
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(dst) = w[0];
+  if (sub == 0) scales[g] = exponent_byte(s);
+}
+
+// ------------------------------------------------------------------ weights
+// A block of 256 threads owns 128 x 128 numbers: 64 a thread, kept as they lie in memory where rows are aligned, read again (from L1) where not.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) quantize_weight_kernel(const T* w, long row_stride, uint8_t* codes, float* scales, int N, int K, int kb) {
+  pdl_launch_dependents();
+  pdl_wait();
+  constexpr int V = 16 / sizeof(T), LANES = kGroup / V, ROWS = 256 / LANES, STEPS = kGroup / ROWS;
+  __shared__ uint32_t most_s[8];
+  const int b = blockIdx.x, n0 = blockIdx.y * kGroup + threadIdx.x / LANES, at = b * kGroup + (threadIdx.x % LANES) * V;
+  Pack<T, V> kept[ALIGNED ? STEPS : 1];
+  auto numbers = [&](int i, float (&v)[V]) {
+    const int n = n0 + i * ROWS;
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = to_f32(kept[i].e[j]);
+    } else {
+      load_numbers<T, V, false>(w + (long)(n < N ? n : 0) * row_stride + at, n < N ? K - at : 0, v);
+    }
+  };
+  if constexpr (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int n = n0 + i * ROWS;
+      if (n < N && at < K) {
+        kept[i] = *reinterpret_cast<const Pack<T, V>*>(w + (long)n * row_stride + at);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) kept[i].e[j] = from_f32<T>(0.f);
+      }
+    }
+  }
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    float v[V];
+    numbers(i, v);
+#pragma unroll
+    for (int j = 0; j < V; ++j) most = max(most, finite_bits(v[j]));
+  }
+  most = lanes_max<32>(most);
+  if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
+  __syncthreads();
+  most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = max(most, most_s[i]);
+  const float s = q8_scale(__uint_as_float(most)), inv = inverse(s);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int n = n0 + i * ROWS;
+    if (n >= N) break;
+    float v[V];
+    numbers(i, v);
+    uint32_t c[V / 4];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = finite_or_nan(v[j]) * inv;
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) c[j] = q8_codes4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    uint8_t* dst = codes + (size_t)n * kb * kGroup + at;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = c[0];
+  }
+  if (threadIdx.x == 0) scales[(size_t)blockIdx.y * kb + b] = s;
+}
+
+// The block's sum, the same in every thread; blocks of whole warps, up to 32 of them.
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (blockDim.x == 32) return v;
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// ------------------------------------------------------------------ residual sum, norm, codes
+// The sum of squares is kept in 64 bits and the factor of a row in two float32 numbers, so that a number in front of its rounding is off by little more than
+// half a float32 step: a code is off where that error carries a number over the border between two codes, in steps of an eighth of the number, and
+// with float32 sums 5,003 rows of 5,120 were 1.2e-4 off 64 bits, four times what a careful float32 form is.  The additions are hidden behind DRAM.
+// One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
+// read twice, number by number.
+template <typename TA, int PER>
+__global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
+                                                          uint8_t* scales, int H, int kb, float eps, float delta_scale) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ double red[32];
+  constexpr int KEEP = PER > 0 ? PER : 1;
+  const long row = blockIdx.x;
+  const float* xr = resid + row * H;
+  const TA* dr = delta ? delta + row * H : nullptr;
+  float* so = sum_out ? sum_out + row * H : nullptr;
+  const int slots = kb * 32;                                // of four numbers
+  double ss = 0.0;
+  float x[KEEP][4], gw[KEEP][4];
+  auto load = [&](int slot, float (&v)[4]) {
+    load_numbers<float, 4, (PER > 0)>(xr + 4 * slot, H - 4 * slot, v);
+    if (dr) {
+      float d[4];
+      load_numbers<TA, 4, (PER > 0)>(dr + 4 * slot, H - 4 * slot, d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = fmaf(delta_scale, d[j], v[j]);
+    }
+  };
+  auto finish = [&](int slot, float (&v)[4], const float (&g)[4], float hi, float lo) {
+    uint32_t w[1];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {                           // v (hi + lo) g, rounded once and a little
+      const float f = hi * g[j], fl = fmaf(lo, g[j], fmaf(hi, g[j], -f)), y = v[j] * f, yl = fmaf(v[j], fl, fmaf(v[j], f, -y));
+      v[j] = abs_bits(yl) < kInfBits ? y + yl : y;
+    }
+    const float s = group_codes<32, 4>(v, w);
+    const size_t group = (size_t)row * kb + (slot >> 5);
+    *reinterpret_cast<uint32_t*>(codes + group * kGroup + 4 * (slot & 31)) = w[0];
+    if ((slot & 31) == 0) scales[group] = exponent_byte(s);
+  };
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int slot = threadIdx.x + i * blockDim.x;
+      if (slot < slots) load(slot, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int slot = threadIdx.x + i * blockDim.x;
+      if (slot >= slots) continue;
+      load_numbers<float, 4, true>(gain + 4 * slot, H - 4 * slot, gw[i]);
+      if (so && 4 * slot < H) store_vec<float, 4>(so + 4 * slot, x[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss = fma((double)x[i][j], (double)x[i][j], ss);
+    }
+  } else {
+    for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
+      load(slot, x[0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss = fma((double)x[0][j], (double)x[0][j], ss);
+    }
+  }
+  const double inv = 1.0 / sqrt(block_sum(ss, red) / H + (double)eps);
+  const float hi = (float)inv, lo = (float)(inv - (double)hi);
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int slot = threadIdx.x + i * blockDim.x;        // whole warps: slots and threads are multiples of 32
+      if (slot < slots) finish(slot, x[i], gw[i], hi, lo);
+    }
+  } else {
+    for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
+      load(slot, x[0]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (so && 4 * slot + j < H) so[4 * slot + j] = x[0][j];
+      load_numbers<float, 4, false>(gain + 4 * slot, H - 4 * slot, gw[0]);
+      finish(slot, x[0], gw[0], hi, lo);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gate
+// y = act(gate) * up from float32 sums [rows, 256 nb] whose columns are 128 of the gate, 128 of the other, and so on: a warp has a group.
+__global__ void __launch_bounds__(256) act_mul_q8_kernel(const float* sums, uint8_t* codes, uint8_t* scales, long groups, int act) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long g = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (g >= groups) return;
+  float gate[4], v[4];
+  load_vec<float, 4>(sums + g * 2 * kGroup + 4 * lane, gate);
+  load_vec<float, 4>(sums + g * 2 * kGroup + kGroup + 4 * lane, v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] *= q8_act(gate[j], act);
+  uint32_t w[1];
+  const float s = group_codes<32, 4>(v, w);
+  *reinterpret_cast<uint32_t*>(codes + (size_t)g * kGroup + 4 * lane) = w[0];
+  if (lane == 0) scales[g] = exponent_byte(s);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+int blocks_of(int n) { return (int)(((long)n + kGroup - 1) / kGroup); }
+
+template <typename T>
+int quantize_rows(const void* x, long row_stride, void* codes, void* scales, int M, int K, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T), per_block = 256 / (kGroup / V);
+  const int kb = blocks_of(K);
+  const long groups = (long)M * kb, blocks = (groups + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
+  const bool fast = K % V == 0 && aligned16(x) && (M == 1 || row_stride % V == 0);
+  launch_kernel(fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
+                (uint8_t*)codes, (uint8_t*)scales, groups, K, kb);
+  return launch_status();
+}
+
+template <typename T>
+int quantize_weight(const void* w, long row_stride, void* codes, void* scales, int N, int K, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const int kb = blocks_of(K), nb = blocks_of(N);
+  if (nb > 65535) return ARLE_E_UNSUPPORTED;
+  const bool fast = K % V == 0 && aligned16(w) && (N == 1 || row_stride % V == 0);
+  launch_kernel(fast ? quantize_weight_kernel<T, true> : quantize_weight_kernel<T, false>, dim3(kb, nb), dim3(256), 0, s, 1, (const T*)w, row_stride,
+                (uint8_t*)codes, (float*)scales, N, K, kb);
+  return launch_status();
+}
+
+template <typename TA>
+int rmsnorm(const float* resid, const void* delta, const float* gain, float* sum_out, void* codes, void* scales, int M, int H, float eps, float delta_scale,
+            cudaStream_t s) {
+  const int kb = blocks_of(H);
+  const bool vec = H % 4 == 0 && aligned16(resid) && aligned16(gain) && ((uintptr_t)delta % (4 * sizeof(TA))) == 0 && aligned16(sum_out);
+  auto kern = rmsnorm_q8_kernel<TA, 0>;
+  int threads = kb >= 32 ? 1024 : 32 * kb;
+  if (vec && kb <= 128) {
+    kern = rmsnorm_q8_kernel<TA, 4>;
+    threads = 32 * ((kb + 3) / 4);
+  }
+  launch_kernel(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, eps, delta_scale);
+  return launch_status();
+}
+
+}  // namespace
+
+// x [M, K] (dtype 0 float32, 1 bfloat16; rows row_stride apart) -> codes [M, 128 ceil(K / 128)] on a 16-byte boundary, scales [M, ceil(K / 128)].
+ARLE_API int arle_quantize_q8(const void* x, int dtype, long row_stride, void* codes, void* scales, int M, int K, cudaStream_t s) {
+  if (M <= 0) return 0;
+  if (K <= 0 || !aligned16(codes)) return ARLE_E_BADARG;
+  if (dtype == 0) return quantize_rows<float>(x, row_stride, codes, scales, M, K, s);
+  if (dtype == 1) return quantize_rows<__nv_bfloat16>(x, row_stride, codes, scales, M, K, s);
+  return ARLE_E_BADARG;
+}
+
+// w [N, K] -> codes [N, 128 ceil(K / 128)], float32 scales [ceil(N / 128), ceil(K / 128)].
+ARLE_API int arle_quantize_weight_q8(const void* w, int dtype, long row_stride, void* codes, void* scales, int N, int K, cudaStream_t s) {
+  if (N <= 0) return 0;
+  if (K <= 0 || !aligned16(codes)) return ARLE_E_BADARG;
+  if (dtype == 0) return quantize_weight<float>(w, row_stride, codes, scales, N, K, s);
+  if (dtype == 1) return quantize_weight<__nv_bfloat16>(w, row_stride, codes, scales, N, K, s);
+  return ARLE_E_BADARG;
+}
+
+// x = resid + delta_scale * delta (delta may be null); sum_out = x (null: not written; may be resid); codes and scales of x * rsqrt(mean(x^2) + eps) * gain.
+ARLE_API int arle_rmsnorm_q8(const float* resid, const void* delta, int dtype, const float* gain, float* sum_out, void* codes, void* scales, int M, int H,
+                             float eps, float delta_scale, cudaStream_t s) {
+  if (M <= 0) return 0;
+  if (H <= 0 || !aligned16(codes)) return ARLE_E_BADARG;
+  if (dtype == 0) return rmsnorm<float>(resid, delta, gain, sum_out, codes, scales, M, H, eps, delta_scale, s);
+  if (dtype == 1) return rmsnorm<__nv_bfloat16>(resid, delta, gain, sum_out, codes, scales, M, H, eps, delta_scale, s);
+  return ARLE_E_BADARG;
+}
+
+// sums [M, 256 nb] float32 -> codes [M, 128 nb], scales [M, nb]; act 0 silu, 1 the tanh form of gelu.
+ARLE_API int arle_act_mul_q8(const float* sums, void* codes, void* scales, int M, int nb, int act, cudaStream_t s) {
+  if (M <= 0 || nb <= 0) return 0;
+  if (act < 0 || act > 1 || !aligned16(sums) || !aligned16(codes)) return ARLE_E_BADARG;
+  const long groups = (long)M * nb, blocks = (groups + 7) / 8;
+  if (blocks > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
+  launch_kernel(act_mul_q8_kernel, dim3((unsigned)blocks), dim3(256), 0, s, 1, sums, (uint8_t*)codes, (uint8_t*)scales, groups, act);
+  return launch_status();
+}

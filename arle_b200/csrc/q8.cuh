@@ -40,6 +40,11 @@ __device__ __forceinline__ float2 q8_float2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// The gates of a feed-forward: silu (0) or the tanh form of gelu (1), in float32.
+__device__ __forceinline__ float q8_act(float g, int act) {
+  return act == 0 ? g / (1.0f + expf(-g)) : 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
+}
+
 __device__ __forceinline__ float q8_float(uint8_t code) { return q8_float2(code).x; }
 
 }  // namespace arle

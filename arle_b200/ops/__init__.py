@@ -135,6 +135,11 @@ _SIGNATURES = {
     "arle_expand_q8": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _I, _P],
     "arle_attention_q8": [_P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _I, _P],
     "arle_attention_q8_decode": [_P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _P, _P, _P],
+    "arle_quantize_q8": [_P, _I, ctypes.c_long, _P, _P, _I, _I, _P],
+    "arle_quantize_weight_q8": [_P, _I, ctypes.c_long, _P, _P, _I, _I, _P],
+    "arle_rmsnorm_q8": [_P, _P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P],
+    "arle_act_mul_q8": [_P, _P, _P, _I, _I, _I, _P],
+    "arle_gemm_q8": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
@@ -2569,3 +2574,178 @@ def step_tables(slots, starts, q_lens, new_pages, page_table, num_pages: int, pa
     _check(library().arle_step_tables(slots, starts, q_lens, R, new_pages, news, table, max_slots, table_width, int(num_pages), int(page_size), q_indptr, kv_lens, positions,
                                       row_of_token, slot_of_token, slot_mapping, T, blocks, block_table.shape[1], status,
                                       torch._C._cuda_getCurrentRawStream(device)), "step_tables")
+
+
+# ------------------------------------------------------------------ linear layers in 8 bits
+Q8_BLOCK = 128                      # numbers of k (and rows of a weight) that share a scale
+_E8M0 = torch.float8_e8m0fnu
+
+
+def q8_width(k: int) -> int:
+    """Codes of a row of ``k`` numbers: filled up to whole blocks, with codes of zero."""
+    return -(-int(k) // Q8_BLOCK) * Q8_BLOCK
+
+
+class Q8Weight:
+    """A weight [out_features, in_features] in 8 bits: ``codes`` contiguous float8_e4m3fn [N, q8_width(K)], zero from column K on, and ``scales`` contiguous
+    float32 [ceil(N / 128), ceil(K / 128)], positive, one for each block of 128 x 128; a number is code * scale.  ``quantize_weight_q8`` makes both from a
+    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two)."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        if codes.dtype is not _E4M3 or codes.dim() != 2 or not codes.is_contiguous() or codes.shape[1] == 0 or codes.shape[1] % Q8_BLOCK:
+            raise KernelError(f"Q8Weight: codes must be contiguous float8_e4m3fn [N, a multiple of {Q8_BLOCK}], got {codes.dtype} {tuple(codes.shape)}")
+        want = (-(-codes.shape[0] // Q8_BLOCK), codes.shape[1] // Q8_BLOCK)
+        if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous() or scales.device != codes.device:
+            raise KernelError(f"Q8Weight: scales must be contiguous float32 {want} beside the codes, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+        if codes.data_ptr() % 16:
+            raise KernelError("Q8Weight: codes must start on a 16-byte boundary")
+        self.codes, self.scales, self.shape = codes, scales, codes.shape
+
+    def bytes(self) -> int:
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def pack_gate_up_q8(gate: Q8Weight, up: Q8Weight) -> Q8Weight:
+    """The weight of ``gemm_act_mul_q8``: 128 rows of the gate, 128 of the up projection, and so on, the last blocks filled up with zeros.  Once, at load."""
+    if gate.shape != up.shape:
+        raise KernelError(f"pack_gate_up_q8: gate {tuple(gate.shape)} and up {tuple(up.shape)} differ")
+    (N, K), nb = gate.shape, gate.scales.shape[0]
+    codes = torch.zeros((nb, 2, Q8_BLOCK, K), dtype=torch.uint8, device=gate.codes.device)
+    whole, left = N // Q8_BLOCK, N % Q8_BLOCK
+    for i, part in enumerate((gate, up)):
+        bits = part.codes.view(torch.uint8)
+        codes[:whole, i] = bits[: whole * Q8_BLOCK].view(whole, Q8_BLOCK, K)
+        if left:
+            codes[whole, i, :left] = bits[whole * Q8_BLOCK:]
+    scales = torch.stack([gate.scales, up.scales], dim=1).reshape(2 * nb, -1).contiguous()
+    return Q8Weight(codes.view(2 * nb * Q8_BLOCK, K).view(_E4M3), scales)
+
+
+def _rows_q8(what: str, codes, scales):
+    """(rows, width) of activations in 8 bits."""
+    shape = codes.shape
+    if (codes.dtype is _E4M3 and scales.dtype is _E8M0 and len(shape) == 2 and shape[1] and shape[1] % Q8_BLOCK == 0
+            and scales.shape == (shape[0], shape[1] // Q8_BLOCK) and codes.is_contiguous() and scales.is_contiguous()):
+        return shape
+    raise KernelError(f"{what}: rows in 8 bits are contiguous float8_e4m3fn [M, a multiple of {Q8_BLOCK}] and contiguous float8_e8m0fnu [M, blocks]; got "
+                      f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+
+
+def _code_pointer(what: str, p: int) -> int:
+    if p % 16:
+        raise KernelError(f"{what}: codes must start on a 16-byte boundary")
+    return p
+
+
+def quantize_q8(x, codes, scales) -> None:
+    """Activations in 8 bits: x [M, K] (float32 or bfloat16, unit inner stride, any row stride) as codes [M, q8_width(K)] (float8_e4m3fn) and scales
+    [M, ceil(K / 128)] (float8_e8m0fnu); a number is code * scale.
+
+    The scale of a row's 128 numbers is the least power of two s with max |x| <= 448 * s (at least 2^-100; at most 2^119, beyond which numbers end at
+    448 * 2^119), a code is x / s rounded to nearest even.  Infinities and NaN become NaN and do not count for the scale.  Columns from K on are zero."""
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise KernelError(f"quantize_q8: x must be [M, K], got {tuple(x.shape)}")
+    M, K = x.shape
+    if _rows_q8("quantize_q8", codes, scales) != (M, q8_width(K)):
+        raise KernelError(f"quantize_q8: x {tuple(x.shape)} needs codes {(M, q8_width(K))}, got {tuple(codes.shape)}")
+    if M and K > 1 and x.stride(1) != 1:
+        raise KernelError("quantize_q8: rows of x must have unit inner stride")
+    dt = _dt(x)
+    device, (xp, cp, sp) = _placed("quantize_q8", (x, codes, scales))
+    if M == 0:
+        return
+    _check(library().arle_quantize_q8(xp, dt, x.stride(0), _code_pointer("quantize_q8", cp), sp, M, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_q8")
+
+
+def quantize_weight_q8(w, codes, scales) -> Q8Weight:
+    """A weight in 8 bits: w [N, K] (float32 or bfloat16, unit inner stride) as codes [N, q8_width(K)] and float32 scales [ceil(N / 128), ceil(K / 128)], and the
+    ``Q8Weight`` of both.  The scale of a block of 128 x 128 is found as a row's in ``quantize_q8``; numbers that are not finite become NaN."""
+    if w.dim() != 2 or w.shape[1] == 0:
+        raise KernelError(f"quantize_weight_q8: w must be [N, K], got {tuple(w.shape)}")
+    N, K = w.shape
+    if tuple(codes.shape) != (N, q8_width(K)):
+        raise KernelError(f"quantize_weight_q8: w {tuple(w.shape)} needs codes {(N, q8_width(K))}, got {tuple(codes.shape)}")
+    weight = Q8Weight(codes, scales)
+    if N and K > 1 and w.stride(1) != 1:
+        raise KernelError("quantize_weight_q8: rows of w must have unit inner stride")
+    dt = _dt(w)
+    device, (wp, cp, sp) = _placed("quantize_weight_q8", (w, codes, scales))
+    if N:
+        _check(library().arle_quantize_weight_q8(wp, dt, w.stride(0), cp, sp, N, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_weight_q8")
+    return weight
+
+
+def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, delta_scale: float = 1.0) -> None:
+    """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's float32 numbers as
+    ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.  ``sum_out`` (float32 [M, H]: ``resid`` itself or a
+    buffer that does not overlap it) gets x; None: x is kept nowhere."""
+    if resid.dim() != 2 or resid.shape[1] == 0 or resid.dtype != torch.float32 or not resid.is_contiguous():
+        raise KernelError("rmsnorm_q8: the residual must be contiguous float32 [M, H]")
+    M, H = resid.shape
+    if weight.dtype != torch.float32 or weight.shape != (H,) or not weight.is_contiguous():
+        raise KernelError("rmsnorm_q8: the weight must be contiguous float32 [H]")
+    if delta is not None and (delta.shape != resid.shape or not delta.is_contiguous()):
+        raise KernelError("rmsnorm_q8: delta must be contiguous and of the residual's shape")
+    if sum_out is not None and (sum_out.shape != resid.shape or sum_out.dtype != torch.float32 or not sum_out.is_contiguous()):
+        raise KernelError("rmsnorm_q8: sum_out must be contiguous float32 like the residual")
+    if _rows_q8("rmsnorm_q8", codes, scales) != (M, q8_width(H)):
+        raise KernelError(f"rmsnorm_q8: rows of {H} need codes {(M, q8_width(H))}, got {tuple(codes.shape)}")
+    dt = _dt(delta) if delta is not None else 0
+    given = [resid, weight, codes, scales] + [t for t in (delta, sum_out) if t is not None]
+    device, (rp, wp, cp, sp, *_) = _placed("rmsnorm_q8", given)
+    so = sum_out.data_ptr() if sum_out is not None else None
+    if so is not None and so != rp and abs(so - rp) < 4 * M * H:
+        raise KernelError("rmsnorm_q8: sum_out overlaps the residual without being it")
+    if M == 0:
+        return
+    _check(library().arle_rmsnorm_q8(rp, delta.data_ptr() if delta is not None else None, dt, wp, so, _code_pointer("rmsnorm_q8", cp), sp, M, H, float(eps),
+                                     float(delta_scale), torch._C._cuda_getCurrentRawStream(device)), "rmsnorm_q8")
+
+
+def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
+    """out[M, N] = x . w^T for rows in 8 bits (``quantize_q8``, ``rmsnorm_q8``, ``gemm_act_mul_q8``) and a weight in 8 bits; out float32 or bfloat16, unit inner
+    stride, any row stride.  Every block of 128 numbers of k is summed on the tensor cores, scaled by the row's and the weight block's scale and added up in
+    float32; the product of the two scales should be a normal float32 number.  The result of a row does not depend on the other rows' numbers."""
+    M, K = _rows_q8("gemm_q8", codes, scales)
+    N = w.shape[0]
+    if w.shape[1] != K or out.shape != (M, N):
+        raise KernelError(f"gemm_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
+    if M and N > 1 and out.stride(1) != 1:
+        raise KernelError("gemm_q8: rows of out must have unit inner stride")
+    dt = _dt(out)
+    device, (xp, sp, wp, wsp, op) = _placed("gemm_q8", (codes, scales, w.codes, w.scales, out))
+    if M == 0 or N == 0:
+        return
+    _check(library().arle_gemm_q8(_code_pointer("gemm_q8", xp), sp, wp, wsp, op, dt, out.stride(0), M, N, K // Q8_BLOCK, torch._C._cuda_getCurrentRawStream(device)),
+           "gemm_q8")
+
+
+def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
+    """The gate behind a packed product: from float32 sums ``gate_up`` [M, 256 * nb], whose columns are 128 of the gate, 128 of the up projection and so on,
+    act(gate) * up as ``quantize_q8`` makes codes [M, 128 * nb] and scales [M, nb]; ``activation`` any of ``ACTIVATIONS``."""
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"act_mul_q8: activation {activation!r} (known: {', '.join(ACTIVATIONS)})")
+    M, I = _rows_q8("act_mul_q8", codes, scales)
+    if gate_up.shape != (M, 2 * I) or gate_up.dtype != torch.float32 or not gate_up.is_contiguous():
+        raise KernelError(f"act_mul_q8: gate_up must be contiguous float32 {(M, 2 * I)}, got {gate_up.dtype} {tuple(gate_up.shape)}")
+    device, (gp, cp, sp) = _placed("act_mul_q8", (gate_up, codes, scales))
+    if M == 0:
+        return
+    if gp % 16:
+        raise KernelError("act_mul_q8: gate_up must start on a 16-byte boundary")
+    _check(library().arle_act_mul_q8(gp, _code_pointer("act_mul_q8", cp), sp, M, I // Q8_BLOCK, ACTIVATIONS[activation],
+                                     torch._C._cuda_getCurrentRawStream(device)), "act_mul_q8")
+
+
+def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, activation: str = "silu") -> None:
+    """The first half of a gated feed-forward in 8 bits: act(x . gate^T) * (x . up^T) for a weight of ``pack_gate_up_q8``, its float32 numbers as ``quantize_q8``
+    makes codes [M, w.shape[0] / 2] and scales.  ``gate_up``: float32 scratch [M, w.shape[0]], contiguous, for few rows, whose sums and gate are two launches."""
+    M, K = _rows_q8("gemm_act_mul_q8", codes, scales)
+    if w.shape[0] % (2 * Q8_BLOCK):
+        raise KernelError(f"gemm_act_mul_q8: a packed weight has a multiple of {2 * Q8_BLOCK} rows, got {w.shape[0]} (see pack_gate_up_q8)")
+    if _rows_q8("gemm_act_mul_q8", out_codes, out_scales) != (M, w.shape[0] // 2):
+        raise KernelError(f"gemm_act_mul_q8: codes of the result must be {(M, w.shape[0] // 2)}, got {tuple(out_codes.shape)}")
+    gemm_q8(codes, scales, w, gate_up)
+    act_mul_q8(gate_up, out_codes, out_scales, activation)
