@@ -11,19 +11,8 @@ using namespace arle;
 namespace {
 
 constexpr int kGroup = 128;
-constexpr uint32_t kInfBits = 0x7f800000u;
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// The bits of |v|, 0 where v is not finite.
-__device__ __forceinline__ uint32_t finite_bits(float v) {
-  const uint32_t b = abs_bits(v);
-  return b < kInfBits ? b : 0u;
-}
-__device__ __forceinline__ float finite_or_nan(float v) { return abs_bits(v) < kInfBits ? v : __uint_as_float(0x7fc00000u); }
-__device__ __forceinline__ float inverse(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two in 2^-100 .. 2^119
-__device__ __forceinline__ uint8_t exponent_byte(float s) { return (uint8_t)(__float_as_uint(s) >> 23); }
-
-// The maximum of `bits` over the 2^k lanes that share lane / LANES.  (Bits of numbers without their sign are ordered as the numbers are.)
+// The maximum of `bits` over the 2^k lanes that share lane / LANES.
 template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t bits) {
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
@@ -42,7 +31,7 @@ template <int LANES, int V> __device__ __forceinline__ float group_codes(float (
     for (int j = 0; j < V; ++j) most = max(most, finite_bits(v[j])), v[j] = finite_or_nan(v[j]);
     most = lanes_max<LANES>(most);
   }
-  const float s = q8_scale(__uint_as_float(most)), inv = inverse(s);
+  const float s = q8_scale(__uint_as_float(most)), inv = inverse_scale(s);
 #pragma unroll
   for (int j = 0; j < V / 4; ++j) w[j] = q8_codes4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
   return s;
@@ -131,7 +120,7 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T* w, long r
   most = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) most = max(most, most_s[i]);
-  const float s = q8_scale(__uint_as_float(most)), inv = inverse(s);
+  const float s = q8_scale(__uint_as_float(most)), inv = inverse_scale(s);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int n = n0 + i * ROWS;
@@ -258,7 +247,7 @@ __global__ void __launch_bounds__(256) act_mul_q8_kernel(const float* sums, uint
   load_vec<float, 4>(sums + g * 2 * kGroup + 4 * lane, gate);
   load_vec<float, 4>(sums + g * 2 * kGroup + kGroup + 4 * lane, v);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] *= q8_act(gate[j], act);
+  for (int j = 0; j < 4; ++j) v[j] *= act == 0 ? q8_silu(gate[j]) : q8_gelu_tanh(gate[j]);
   uint32_t w[1];
   const float s = group_codes<32, 4>(v, w);
   *reinterpret_cast<uint32_t*>(codes + (size_t)g * kGroup + 4 * lane) = w[0];

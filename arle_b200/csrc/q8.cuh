@@ -40,10 +40,21 @@ __device__ __forceinline__ float2 q8_float2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The gates of a feed-forward: silu (0) or the tanh form of gelu (1), in float32.
-__device__ __forceinline__ float q8_act(float g, int act) {
-  return act == 0 ? g / (1.0f + expf(-g)) : 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g)));
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// The bits of |v|, 0 where v is not finite.  (Bits of numbers without their sign are ordered as the numbers are.)
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = abs_bits(v);
+  return b < kInfBits ? b : 0u;
 }
+__device__ __forceinline__ float finite_or_nan(float v) { return abs_bits(v) < kInfBits ? v : __uint_as_float(0x7fc00000u); }
+__device__ __forceinline__ float inverse_scale(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two in 2^-100 .. 2^119
+__device__ __forceinline__ uint8_t exponent_byte(float s) { return (uint8_t)(__float_as_uint(s) >> 23); }                   // the same as e8m0
+
+// The gates of a feed-forward in float32.  The quotient is good to two steps (fdividef gives 0 beyond 2^126, which is what silu is there).
+__device__ __forceinline__ float q8_silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
+__device__ __forceinline__ float q8_gelu_tanh(float g) { return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))); }
 
 __device__ __forceinline__ float q8_float(uint8_t code) { return q8_float2(code).x; }
 

@@ -140,6 +140,8 @@ _SIGNATURES = {
     "arle_rmsnorm_q8": [_P, _P, _I, _P, _P, _P, _P, _I, _I, _F, _F, _P],
     "arle_act_mul_q8": [_P, _P, _P, _I, _I, _I, _P],
     "arle_gemm_q8": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P],
+    "arle_gemm_q8_pair": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P, _P],
+    "arle_gemm_q8_pair_gated": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
 }
@@ -2718,8 +2720,14 @@ def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     device, (xp, sp, wp, wsp, op) = _placed("gemm_q8", (codes, scales, w.codes, w.scales, out))
     if M == 0 or N == 0:
         return
-    _check(library().arle_gemm_q8(_code_pointer("gemm_q8", xp), sp, wp, wsp, op, dt, out.stride(0), M, N, K // Q8_BLOCK, torch._C._cuda_getCurrentRawStream(device)),
-           "gemm_q8")
+    xp, kb, stream = _code_pointer("gemm_q8", xp), K // Q8_BLOCK, torch._C._cuda_getCurrentRawStream(device)
+    if M >= _Q8_PAIR_MIN_ROWS and _KERNEL_SET == "fast":
+        _check(library().arle_gemm_q8_pair(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, _ptr(error_flag(out.device)), stream), "gemm_q8")
+        return
+    _check(library().arle_gemm_q8(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, stream), "gemm_q8")
+
+
+_Q8_PAIR_MIN_ROWS = 33            # 32 rows of 4,096 x 12,288 43 us on the kernel of few rows, 53 on pairs of SMs; 64 rows 73 and 46
 
 
 def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
@@ -2747,5 +2755,17 @@ def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, 
         raise KernelError(f"gemm_act_mul_q8: a packed weight has a multiple of {2 * Q8_BLOCK} rows, got {w.shape[0]} (see pack_gate_up_q8)")
     if _rows_q8("gemm_act_mul_q8", out_codes, out_scales) != (M, w.shape[0] // 2):
         raise KernelError(f"gemm_act_mul_q8: codes of the result must be {(M, w.shape[0] // 2)}, got {tuple(out_codes.shape)}")
+    if activation not in ACTIVATIONS:
+        raise KernelError(f"gemm_act_mul_q8: activation {activation!r} (known: {', '.join(ACTIVATIONS)})")
+    if gate_up.shape != (M, w.shape[0]) or gate_up.dtype != torch.float32 or not gate_up.is_contiguous():
+        raise KernelError(f"gemm_act_mul_q8: gate_up must be contiguous float32 {(M, w.shape[0])}, got {gate_up.dtype} {tuple(gate_up.shape)}")
+    if w.shape[1] != K:
+        raise KernelError(f"gemm_act_mul_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)}")
+    if M >= _Q8_PAIR_MIN_ROWS and _KERNEL_SET == "fast":
+        device, (xp, sp, wp, wsp, ocp, osp, _) = _placed("gemm_act_mul_q8", (codes, scales, w.codes, w.scales, out_codes, out_scales, gate_up))
+        _check(library().arle_gemm_q8_pair_gated(_code_pointer("gemm_act_mul_q8", xp), sp, wp, wsp, _code_pointer("gemm_act_mul_q8", ocp), osp, M,
+                                                 w.shape[0] // (2 * Q8_BLOCK), K // Q8_BLOCK, ACTIVATIONS[activation], _ptr(error_flag(codes.device)),
+                                                 torch._C._cuda_getCurrentRawStream(device)), "gemm_act_mul_q8")
+        return
     gemm_q8(codes, scales, w, gate_up)
     act_mul_q8(gate_up, out_codes, out_scales, activation)
