@@ -192,13 +192,15 @@ inline cudaError_t launch_early(void (*kernel)(KArgs...), dim3 grid, dim3 block,
 // keeps one of these per kernel and raises the limit once on each device.
 class SharedLimit {
  public:
-  cudaError_t raise(const void* kernel, size_t bytes) {
+  // `all`: the SM's memory goes to its blocks as far as it can (else the driver gives what one block needs, and two do not fit).
+  cudaError_t raise(const void* kernel, size_t bytes, bool all = false) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;       // further devices are set every time
     if (done_.load(std::memory_order_acquire) & bit) return cudaSuccess;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && all) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e == cudaSuccess) done_.fetch_or(bit, std::memory_order_release);
     return e;
   }

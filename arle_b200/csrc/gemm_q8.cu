@@ -16,71 +16,81 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A block of eight warps owns 16 rows of w and up to 8 MT rows of x; warp i takes the blocks i, i + 8, ... of k.  The order of k inside a block of 128 is
-// free as long as both operands have the same: lane (g, t) takes bytes 32t .. 32t + 31 of its row's block, so a warp's loads cover whole 128-byte lines,
-// and words 2i and 2i + 1 of those are the operands of the i-th of four mma.
-template <int MT, typename OutT>
-__global__ void __launch_bounds__(256) gemm_q8_rows_kernel(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const float* sw, OutT* out, long ldo, int M,
-                                                           int N, int kb) {
+__device__ __forceinline__ uint4 load_once(const uint8_t* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }      // a plain load of what is read once
+
+// Few rows: bound by the bytes of w, read straight from memory into the operands of mma.sync.  A block owns 16 rows of w and up to eight rows of x; its warp i
+// takes the blocks i, i + WARPS, ... of k.  The order of k inside a block of 128 is free as long as both operands have the same: lane (g, t) takes bytes
+// 32t .. 32t + 31 of its row's block, so a warp's loads cover whole 128-byte lines, and words 2i and 2i + 1 of those are the operands of the i-th of
+// four mma.  What hides the memory is many warps, a block of k each on its way, not several blocks in a warp: with two, and with rings of four that go on
+// across rows, all sizes took longer (4,096 x 12,288 for one row 15 to 26 us instead of 10.3), and so did x fetched a block ahead.
+// The first block of w is asked for before the kernel in front has ended (what makes weights lets nothing start before its end).
+// One row, us and TB/s: 4,096 x 4,096 4.2 (4.0), 4,096 x 12,288 10.3 (4.9), 6,144 x 4,096 6.1 (4.1), 24,576 x 4,096 18.6 (5.4), 5,120 x 25,600 27.3 (4.8); eight
+// rows some 3 % more.
+template <int WARPS, int BLOCKS, typename OutT>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const float* sw, OutT* out, long ldo,
+                                                                         int M, int N, int kb) {
   pdl_launch_dependents();
-  pdl_wait();
-  constexpr int TOKENS = 8 * MT;
-  __shared__ float part[8][16][TOKENS + 1];
+  __shared__ float part[WARPS][16][9];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * TOKENS;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8;
   const size_t K = (size_t)kb * kBlock;
-  const uint8_t* wr[2] = {w + min(n0 + g, N - 1) * K + 32 * t, w + min(n0 + g + 8, N - 1) * K + 32 * t};
+  const uint8_t* w0 = w + (size_t)min(n0 + g, N - 1) * K + 32 * t;
+  const uint8_t* w1 = w + (size_t)min(n0 + g + 8, N - 1) * K + 32 * t;
   const float* swr = sw + (size_t)(n0 / kBlock) * kb;
-  float acc[MT][4] = {};
-  for (int b = warp; b < kb; b += 8) {
-    uint4 a[2][2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) a[r][h] = *reinterpret_cast<const uint4*>(wr[r] + (size_t)b * kBlock + 16 * h);
-    const float s = swr[b];
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const uint8_t* xr = x + min(m0 + 8 * j + g, M - 1) * K + (size_t)b * kBlock + 32 * t;
-      const uint4 x0 = *reinterpret_cast<const uint4*>(xr), x1 = *reinterpret_cast<const uint4*>(xr + 16);
-      float d[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_e4m3(d, a[0][0].x, a[1][0].x, a[0][0].y, a[1][0].y, x0.x, x0.y);
-      mma_e4m3(d, a[0][0].z, a[1][0].z, a[0][0].w, a[1][0].w, x0.z, x0.w);
-      mma_e4m3(d, a[0][1].x, a[1][1].x, a[0][1].y, a[1][1].y, x1.x, x1.y);
-      mma_e4m3(d, a[0][1].z, a[1][1].z, a[0][1].w, a[1][1].w, x1.z, x1.w);
-      const int ma = min(m0 + 8 * j + 2 * t, M - 1), mb = min(m0 + 8 * j + 2 * t + 1, M - 1);
-      const float fa = s * __uint_as_float((uint32_t)sx[(size_t)ma * kb + b] << 23), fb = s * __uint_as_float((uint32_t)sx[(size_t)mb * kb + b] << 23);
-      acc[j][0] = fmaf(d[0], fa, acc[j][0]), acc[j][1] = fmaf(d[1], fb, acc[j][1]);
-      acc[j][2] = fmaf(d[2], fa, acc[j][2]), acc[j][3] = fmaf(d[3], fb, acc[j][3]);
+  uint4 a[4];
+  auto ask = [&](int b) {
+    if (b < kb) {
+      const size_t at = (size_t)b * kBlock;
+      a[0] = load_once(w0 + at), a[1] = load_once(w0 + at + 16), a[2] = load_once(w1 + at), a[3] = load_once(w1 + at + 16);
     }
+  };
+  ask(warp);
+  pdl_wait();
+  const uint8_t* xr = x + (size_t)min(m0 + g, M - 1) * K + 32 * t;
+  const uint8_t* sxa = sx + (size_t)min(m0 + 2 * t, M - 1) * kb;
+  const uint8_t* sxb = sx + (size_t)min(m0 + 2 * t + 1, M - 1) * kb;
+  float acc[4] = {};
+  for (int b = warp; b < kb; b += WARPS) {
+    const uint4 x0 = *reinterpret_cast<const uint4*>(xr + (size_t)b * kBlock), x1 = *reinterpret_cast<const uint4*>(xr + (size_t)b * kBlock + 16);
+    const float s = swr[b], fa = s * __uint_as_float((uint32_t)sxa[b] << 23), fb = s * __uint_as_float((uint32_t)sxb[b] << 23);
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+    mma_e4m3(d, a[0].x, a[2].x, a[0].y, a[2].y, x0.x, x0.y);
+    mma_e4m3(d, a[0].z, a[2].z, a[0].w, a[2].w, x0.z, x0.w);
+    mma_e4m3(d, a[1].x, a[3].x, a[1].y, a[3].y, x1.x, x1.y);
+    mma_e4m3(d, a[1].z, a[3].z, a[1].w, a[3].w, x1.z, x1.w);
+    acc[0] = fmaf(d[0], fa, acc[0]), acc[1] = fmaf(d[1], fb, acc[1]);
+    acc[2] = fmaf(d[2], fa, acc[2]), acc[3] = fmaf(d[3], fb, acc[3]);
+    ask(b + WARPS);
   }
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[j][e];
+  for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][2 * t + (e & 1)] = acc[e];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * TOKENS; i += 256) {
-    const int n = i & 15, m = i >> 4;
+  if (threadIdx.x < 128) {                                 // added up in the order of the warps
+    const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += part[k][n][m];
+    for (int k = 0; k < WARPS; ++k) v += part[k][n][m];
     if (n0 + n < N && m0 + m < M) out[(size_t)(m0 + m) * ldo + n0 + n] = from_f32<OutT>(v);
   }
 }
 
-template <int MT, typename OutT>
-int launch_rows(const void* x, const void* sx, const void* w, const float* sw, void* out, long ldo, int M, int N, int kb, cudaStream_t s) {
-  const int tiles_m = (M + 8 * MT - 1) / (8 * MT);
-  if (tiles_m > 65535) return ARLE_E_UNSUPPORTED;
-  launch_kernel(gemm_q8_rows_kernel<MT, OutT>, dim3((N + 15) / 16, tiles_m), dim3(256), 0, s, 1, (const uint8_t*)x, (const uint8_t*)sx, (const uint8_t*)w, sw,
-                (OutT*)out, ldo, M, N, kb);
-  return launch_status();
-}
-
 template <typename OutT>
 int product(const void* x, const void* sx, const void* w, const float* sw, void* out, long ldo, int M, int N, int kb, cudaStream_t s) {
-  if (M <= 8) return launch_rows<1, OutT>(x, sx, w, sw, out, ldo, M, N, kb, s);
-  return launch_rows<4, OutT>(x, sx, w, sw, out, ldo, M, N, kb, s);
+  const int tiles = (N + 15) / 16, tiles_m = (M + 7) / 8;
+  if (tiles_m > 65535) return ARLE_E_UNSUPPORTED;
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // 16 warps to a tile where all tiles are under way at once, else eight: us for one row with 16 warps, eight in three blocks an SM and eight in four, 4,096 x 12,288 (256
+  // tiles) 10.3, 13.4 and 15.0; 6,144 x 4,096 (384) 7.1, 6.1 and 6.7; 24,576 x 4,096 (1,536) 19.8, 20.1 and 18.6
+  auto go = [&](auto kern, int warps) {
+    launch_early(kern, dim3(tiles, tiles_m), dim3(32 * warps), 0, s, 1, (const uint8_t*)x, (const uint8_t*)sx, (const uint8_t*)w, sw, (OutT*)out, ldo, M, N, kb);
+    return launch_status();
+  };
+  const long blocks = (long)tiles * tiles_m;
+  if (blocks <= 2l * sms) return go(gemm_q8_rows_kernel<16, 2, OutT>, 16);
+  if (blocks <= 3l * sms) return go(gemm_q8_rows_kernel<8, 3, OutT>, 8);
+  return go(gemm_q8_rows_kernel<8, 4, OutT>, 8);
 }
 
 }  // namespace

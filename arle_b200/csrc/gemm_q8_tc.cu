@@ -83,7 +83,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_
                                                                    const uint8_t* __restrict__ sx, const float* __restrict__ sw, OutT* __restrict__ out,
                                                                    long ldo, uint8_t* __restrict__ out_scales, int M, int N, int kb, int act,
                                                                    int* __restrict__ err) {
-  pdl_launch_dependents();
   pdl_wait();
   constexpr uint32_t STAGE = 2 * kTile;
   extern __shared__ unsigned char smem_dyn[];
@@ -132,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();                                      // the partner's barriers exist before anything arrives on them
+  pdl_launch_dependents();                                 // with its tensor memory in hand: who starts beside it may want some too
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
   const volatile int* aborted = &abort_flag;

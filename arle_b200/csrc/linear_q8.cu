@@ -79,8 +79,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row
 // A block of 256 threads owns 128 x 128 numbers: 64 a thread, kept as they lie in memory where rows are aligned, read again (from L1) where not.
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) quantize_weight_kernel(const T* w, long row_stride, uint8_t* codes, float* scales, int N, int K, int kb) {
-  pdl_launch_dependents();
-  pdl_wait();
+  pdl_wait();      // and lets nothing start early: the products ask for weights before they wait for the kernel in front of them
   constexpr int V = 16 / sizeof(T), LANES = kGroup / V, ROWS = 256 / LANES, STEPS = kGroup / ROWS;
   __shared__ uint32_t most_s[8];
   const int b = blockIdx.x, n0 = blockIdx.y * kGroup + threadIdx.x / LANES, at = b * kGroup + (threadIdx.x % LANES) * V;

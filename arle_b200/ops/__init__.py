@@ -18,6 +18,7 @@ cuBLAS through ``torch.mm``, as cklxx/arle calls cuBLASLt for all its projection
 from __future__ import annotations
 
 import ctypes
+import functools
 import operator
 import threading
 from ctypes import c_float, c_int, c_void_p
@@ -141,6 +142,9 @@ _SIGNATURES = {
     "arle_act_mul_q8": [_P, _P, _P, _I, _I, _I, _P],
     "arle_gemm_q8": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P],
     "arle_gemm_q8_pair": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P, _P],
+    "arle_gemm_q8_split": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _P, _P],
+    "arle_gemm_q8_split_clusters": [_I],
+    "arle_gemm_q8_few": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _P, _P],
     "arle_gemm_q8_pair_gated": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
     "arle_moe_combine": [_P, _I, _P, _P, _I, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P],
@@ -2721,13 +2725,67 @@ def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     if M == 0 or N == 0:
         return
     xp, kb, stream = _code_pointer("gemm_q8", xp), K // Q8_BLOCK, torch._C._cuda_getCurrentRawStream(device)
-    if M >= _Q8_PAIR_MIN_ROWS and _KERNEL_SET == "fast":
+    _launch_gemm_q8(_q8_route(M, N, kb, device) if _KERNEL_SET == "fast" else ("rows", 1, 0.0), xp, sp, wp, wsp, op, dt, out, M, N, kb, stream)
+
+
+def _launch_gemm_q8(route, xp, sp, wp, wsp, op, dt: int, out, M: int, N: int, kb: int, stream) -> None:
+    kind, parts, _ = route
+    if kind == "rows":
+        _check(library().arle_gemm_q8(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, stream), "gemm_q8")
+    elif kind == "few":
+        _check(library().arle_gemm_q8_few(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, parts, _ptr(error_flag(out.device)), stream), "gemm_q8")
+    elif kind == "split":
+        _check(library().arle_gemm_q8_split(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, parts, _ptr(error_flag(out.device)), stream), "gemm_q8")
+    else:
         _check(library().arle_gemm_q8_pair(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, _ptr(error_flag(out.device)), stream), "gemm_q8")
-        return
-    _check(library().arle_gemm_q8(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, stream), "gemm_q8")
 
 
-_Q8_PAIR_MIN_ROWS = 33            # 32 rows of 4,096 x 12,288 43 us on the kernel of few rows, 53 on pairs of SMs; 64 rows 73 and 46
+@functools.lru_cache(maxsize=None)
+def _q8_clusters(parts: int, device: int) -> int:
+    """How many clusters of ``parts`` SMs run at a time, one block an SM: an SM's neighbours in a cluster are of its own part of the device, so 148 SMs hold 15
+    clusters of eight."""
+    n = library().arle_gemm_q8_split_clusters(parts)
+    if n <= 0:
+        raise KernelError(f"gemm_q8: CUDA error while asking for the number of clusters of {parts}")
+    return n
+
+
+@functools.lru_cache(maxsize=4096)
+def _q8_route(M: int, N: int, kb: int, device: int):
+    """(kernel, parts that a tile's k is cut into, estimated us) of a product, by its sizes alone.  Figures in us, alone in a graph:
+
+    * "rows", one launch without shared memory, up to 8 rows: one row of 4,096 x 4,096 4.2 and 6.3 with "few", 4,096 x 12,288 10.3 and 10.8; longer sums are
+      shorter there (5,120 x 25,600 27.3 and 23.2);
+    * "few", up to 64 rows, bound by w's bytes.  Parts: the cheapest of what runs at once, 0.3 a block of k (0.45 for more than 32 rows), 0.1 (0.25) a part, 1.5 a
+      wave, 0.9 where two blocks share an SM.  32 tiles of 32 blocks of k, one row: 2, 4, 6 and 8 parts 7.9, 6.3, 6.6 and 7.2; 48 tiles 8.9, 8.0, 10.2 (more than
+      run at once) and 9.9, five 7.5; 32 tiles of 96 blocks 17.4, 12.4, 11.9 and 10.9;
+    * "split" and "pair" for more rows: one SM to a tile of 128 x 128, 0.32 a block of k, and two to one of 256 x 256, 0.42.  4,096 x 4,096: 128 rows 9.6 with four
+      parts and 18.2, 512 rows 15.0 and 18.7, 1,024 rows 29.7 and 19.8; 333 rows of 5,120 x 25,600 76 and 81."""
+    sms = sm_count(device)
+    if M <= 8 and kb <= 128:
+        return "rows", 1, 0.0
+    tiles = -(-N // Q8_BLOCK)
+    if M <= 64:
+        rows = 16 if M <= 16 else 32 if M <= 32 else 64
+        block, part = (0.3, 0.1) if rows < 64 else (0.45, 0.25)
+        best = None
+        for parts in (1, 2, 3, 4, 5, 6, 7, 8):
+            if parts > kb or (rows == 64 and parts in (5, 7)):
+                continue
+            waves = -(-tiles // (2 * _q8_clusters(parts, device)))        # two blocks share an SM
+            cost = waves * (-(-kb // parts) * block + 1.5) + part * parts + (0.9 if tiles * parts > sms else 0.0) + 1.5
+            if best is None or cost < best[2]:
+                best = ("few", parts, cost)
+        return best
+    tiles *= -(-M // 128)
+    best = ("pair", 1, -(-(-(-N // 256) * -(-M // 256)) // (sms // 2)) * kb * 0.42 + 6.0)
+    for parts in (1, 2, 3, 4, 5, 6, 7, 8):
+        if parts > kb:
+            break
+        cost = -(-tiles // _q8_clusters(parts, device)) * (-(-kb // parts) * 0.32 + 4.0) + 0.7 + (1.2 + 0.65 * parts if parts > 1 else 0.0)
+        if cost < best[2]:
+            best = ("split", parts, cost)
+    return best
 
 
 def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
@@ -2747,6 +2805,16 @@ def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
                                      torch._C._cuda_getCurrentRawStream(device)), "act_mul_q8")
 
 
+@functools.lru_cache(maxsize=4096)
+def _q8_gate_in_pair(M: int, N: int, kb: int, device: int) -> bool:
+    """Whether a packed product's gate goes into the epilogue of the kernel for pairs of SMs, which writes codes: where the other kernels, another launch and
+    the sums' way through memory (float32, written and read) take longer by estimate.  24,576 x 4,096, us: 64 rows 33.9 in one and 28.6 in two, 128 rows 40 and 41."""
+    if M <= 64 or device < 0:
+        return False
+    pair = -(-(-(-N // 256) * -(-M // 256)) // (sm_count(device) // 2)) * kb * 0.42 + 6.0
+    return pair <= _q8_route(M, N, kb, device)[2] + 2.0 + 8.0 * M * N / 5.0e6
+
+
 def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, activation: str = "silu") -> None:
     """The first half of a gated feed-forward in 8 bits: act(x . gate^T) * (x . up^T) for a weight of ``pack_gate_up_q8``, its float32 numbers as ``quantize_q8``
     makes codes [M, w.shape[0] / 2] and scales.  ``gate_up``: float32 scratch [M, w.shape[0]], contiguous, for few rows, whose sums and gate are two launches."""
@@ -2761,7 +2829,7 @@ def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, 
         raise KernelError(f"gemm_act_mul_q8: gate_up must be contiguous float32 {(M, w.shape[0])}, got {gate_up.dtype} {tuple(gate_up.shape)}")
     if w.shape[1] != K:
         raise KernelError(f"gemm_act_mul_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)}")
-    if M >= _Q8_PAIR_MIN_ROWS and _KERNEL_SET == "fast":
+    if _KERNEL_SET == "fast" and _q8_gate_in_pair(M, w.shape[0], K // Q8_BLOCK, codes.get_device()):
         device, (xp, sp, wp, wsp, ocp, osp, _) = _placed("gemm_act_mul_q8", (codes, scales, w.codes, w.scales, out_codes, out_scales, gate_up))
         _check(library().arle_gemm_q8_pair_gated(_code_pointer("gemm_act_mul_q8", xp), sp, wp, wsp, _code_pointer("gemm_act_mul_q8", ocp), osp, M,
                                                  w.shape[0] // (2 * Q8_BLOCK), K // Q8_BLOCK, ACTIVATIONS[activation], _ptr(error_flag(codes.device)),
