@@ -14,9 +14,13 @@ constexpr int kGroup = 128;
 
 // The maximum of `bits` over the 2^k lanes that share lane / LANES.
 template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t bits) {
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(0xffffffffu, bits);
+  } else {
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
-  return bits;
+    for (int o = LANES / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    return bits;
+  }
 }
 
 // The codes of a group that LANES lanes hold, V consecutive numbers each: returns the scale, words of four codes in `w`.
@@ -53,123 +57,164 @@ template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void load_
 }
 
 // ------------------------------------------------------------------ rows
-// A lane takes 16 bytes: a group is 16 lanes of bfloat16 or 32 of float32.
+// A lane takes 16 bytes of a group: a group is 16 lanes of bfloat16 or 32 of float32; it takes them of kAtOnce groups, which are under way together.
+constexpr int kAtOnce = 4;
+
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row_stride, uint8_t* codes, uint8_t* scales, long groups, int K, int kb) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row_stride, uint8_t* codes, uint8_t* scales, uint32_t groups, int K, uint32_t kb) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int V = 16 / sizeof(T), LANES = kGroup / V;
-  const long g = ((long)blockIdx.x * blockDim.x + threadIdx.x) / LANES;
+  constexpr int V = 16 / sizeof(T), LANES = kGroup / V, GROUPS = 256 / LANES;
   const int sub = threadIdx.x % LANES;
-  const bool mine = g < groups;
-  const long row = mine ? g / kb : 0;
-  const int b = (int)(g - row * kb), at = b * kGroup + sub * V;
-  float v[V];
-  load_numbers<T, V, ALIGNED>(x + row * row_stride + at, mine ? K - at : 0, v);
-  uint32_t w[V / 4];
-  const float s = group_codes<LANES, V>(v, w);
-  if (!mine) return;
-  uint8_t* dst = codes + (size_t)g * kGroup + sub * V;
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(dst) = w[0];
-  if (sub == 0) scales[g] = exponent_byte(s);
+  const uint32_t g0 = blockIdx.x * (GROUPS * kAtOnce) + threadIdx.x / LANES;
+  float v[kAtOnce][V];
+#pragma unroll
+  for (int u = 0; u < kAtOnce; ++u) {
+    const uint32_t g = g0 + u * GROUPS, row = g / kb;
+    const int at = (int)(g - row * kb) * kGroup + sub * V;
+    load_numbers<T, V, ALIGNED>(x + (long)(g < groups ? row : 0) * row_stride + at, g < groups ? K - at : 0, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kAtOnce; ++u) {
+    const uint32_t g = g0 + u * GROUPS;
+    uint32_t w[V / 4];
+    const float s = group_codes<LANES, V>(v[u], w);
+    if (g >= groups) continue;
+    uint8_t* dst = codes + (size_t)g * kGroup + sub * V;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(dst) = w[0];
+    if (sub == 0) scales[g] = exponent_byte(s);
+  }
 }
 
 // ------------------------------------------------------------------ weights
-// A block of 256 threads owns 128 x 128 numbers: 64 a thread, kept as they lie in memory where rows are aligned, read again (from L1) where not.
+// A block of 256 threads owns 128 x 128 numbers, which are all under way at once and stay as they lie in memory between the maximum and the rounding.  Where rows
+// are not aligned, or a number is not finite, they are read again (from L1 or L2).
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) quantize_weight_kernel(const T* w, long row_stride, uint8_t* codes, float* scales, int N, int K, int kb) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) quantize_weight_kernel(const T* w, long row_stride, uint8_t* codes, float* scales, int N, int K, int kb) {
   pdl_wait();      // and lets nothing start early: the products ask for weights before they wait for the kernel in front of them
   constexpr int V = 16 / sizeof(T), LANES = kGroup / V, ROWS = 256 / LANES, STEPS = kGroup / ROWS;
   __shared__ uint32_t most_s[8];
-  const int b = blockIdx.x, n0 = blockIdx.y * kGroup + threadIdx.x / LANES, at = b * kGroup + (threadIdx.x % LANES) * V;
-  Pack<T, V> kept[ALIGNED ? STEPS : 1];
-  auto numbers = [&](int i, float (&v)[V]) {
-    const int n = n0 + i * ROWS;
-    if constexpr (ALIGNED) {
+  const int b = blockIdx.x, sub = threadIdx.x % LANES, n0 = blockIdx.y * kGroup + threadIdx.x / LANES, at = b * kGroup + sub * V;
+  uint8_t* dst = codes + (size_t)n0 * kb * kGroup + at;
+  const size_t step = (size_t)ROWS * kb * kGroup;
+  auto block_max = [&](uint32_t most) {
+    most = lanes_max<32>(most);
+    if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
+    __syncthreads();
+    most = most_s[0];
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = to_f32(kept[i].e[j]);
-    } else {
-      load_numbers<T, V, false>(w + (long)(n < N ? n : 0) * row_stride + at, n < N ? K - at : 0, v);
-    }
+    for (int i = 1; i < 8; ++i) most = max(most, most_s[i]);
+    return most;
+  };
+  auto put = [&](int i, const float (&v)[V], float inv) {
+    uint32_t c[V / 4];
+#pragma unroll
+    for (int j = 0; j < V / 4; ++j) c[j] = q8_codes4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst + i * step) = make_uint2(c[0], c[1]);
+    else *reinterpret_cast<uint32_t*>(dst + i * step) = c[0];
   };
   if constexpr (ALIGNED) {
+    uint4 kept[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int n = n0 + i * ROWS;
-      if (n < N && at < K) {
-        kept[i] = *reinterpret_cast<const Pack<T, V>*>(w + (long)n * row_stride + at);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) kept[i].e[j] = from_f32<T>(0.f);
-      }
+      kept[i] = n < N && at < K ? *reinterpret_cast<const uint4*>(w + (long)n * row_stride + at) : make_uint4(0u, 0u, 0u, 0u);
     }
-  }
-  uint32_t most = 0;
+    uint32_t most = 0;                                     // over whole words, two bfloat16 at a time
 #pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const uint4 q = kept[i];
+      if constexpr (sizeof(T) == 2) most = __vmaxu2(__vmaxu2(most, __vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu)), __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
+      else most = max(max(most, max(q.x & 0x7fffffffu, q.y & 0x7fffffffu)), max(q.z & 0x7fffffffu, q.w & 0x7fffffffu));
+    }
+    most = block_max(sizeof(T) == 2 ? max(most << 16, most & 0xffff0000u) : most);
+    if (most < kInfBits) {
+      const float s = q8_scale(__uint_as_float(most)), inv = inverse_scale(s);
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        if (n0 + i * ROWS >= N) break;
+        const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(&kept[i]);
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = to_f32(p.e[j]);
+        put(i, v, inv);
+      }
+      if (threadIdx.x == 0) scales[(size_t)blockIdx.y * kb + b] = s;
+      return;
+    }
+    __syncthreads();                                       // the maxima have been read
+  }
+  auto numbers = [&](int i, float (&v)[V]) {
+    const int n = n0 + i * ROWS;
+    load_numbers<T, V, false>(w + (long)(n < N ? n : 0) * row_stride + at, n < N ? K - at : 0, v);
+  };
+  uint32_t most = 0;
+#pragma unroll 2
   for (int i = 0; i < STEPS; ++i) {
     float v[V];
     numbers(i, v);
 #pragma unroll
     for (int j = 0; j < V; ++j) most = max(most, finite_bits(v[j]));
   }
-  most = lanes_max<32>(most);
-  if ((threadIdx.x & 31) == 0) most_s[threadIdx.x >> 5] = most;
-  __syncthreads();
-  most = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) most = max(most, most_s[i]);
-  const float s = q8_scale(__uint_as_float(most)), inv = inverse_scale(s);
-#pragma unroll
+  const float s = q8_scale(__uint_as_float(block_max(most))), inv = inverse_scale(s);
+#pragma unroll 2
   for (int i = 0; i < STEPS; ++i) {
-    const int n = n0 + i * ROWS;
-    if (n >= N) break;
+    if (n0 + i * ROWS >= N) break;
     float v[V];
     numbers(i, v);
-    uint32_t c[V / 4];
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = finite_or_nan(v[j]) * inv;
-#pragma unroll
-    for (int j = 0; j < V / 4; ++j) c[j] = q8_codes4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    uint8_t* dst = codes + (size_t)n * kb * kGroup + at;
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
-    else *reinterpret_cast<uint32_t*>(dst) = c[0];
+    for (int j = 0; j < V; ++j) v[j] = finite_or_nan(v[j]);
+    put(i, v, inv);
   }
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * kb + b] = s;
 }
 
-// The block's sum, the same in every thread; blocks of whole warps, up to 32 of them.
-__device__ __forceinline__ double block_sum(double v, double* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (blockDim.x == 32) return v;
+// The block's sum as two numbers, the same in every thread; blocks of whole warps, up to 32 of them.  Inside a warp the additions are plain (their errors are
+// independent from warp to warp and average out), across warps what an addition rounds off is kept.
+__device__ __forceinline__ float2 block_sum2(float v, float* scratch) {
+  v = warp_sum(v);
+  if (blockDim.x == 32) return make_float2(v, 0.f);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : 0.0;
+  float s = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : 0.f, e = 0.f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int o = 16; o > 0; o >>= 1) {
+    const float s2 = __shfl_xor_sync(0xffffffffu, s, o), e2 = __shfl_xor_sync(0xffffffffu, e, o);
+    const float t = s + s2, back = t - s;
+    e += e2 + ((s - (t - back)) + (s2 - back));
+    s = t;
+  }
+  return make_float2(s, e);
+}
+
+// 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).
+__device__ __forceinline__ float2 inverse_root(double m) {
+  const float mh = (float)m, ml = (float)(m - (double)mh), y = rsqrtf(mh);
+  const float q = y * y, ql = fmaf(y, y, -q);
+  const float r = fmaf(-mh, q, 1.0f) - fmaf(mh, ql, ml * q);
+  return make_float2(y, 0.5f * y * r);
 }
 
 // ------------------------------------------------------------------ residual sum, norm, codes
-// The sum of squares is kept in 64 bits and the factor of a row in two float32 numbers, so that a number in front of its rounding is off by little more than
+// The sum of squares and the factor of a row are pairs of float32 numbers, so that a number in front of its rounding is off by little more than
 // half a float32 step: a code is off where that error carries a number over the border between two codes, in steps of an eighth of the number, and
 // with float32 sums 5,003 rows of 5,120 were 1.2e-4 off 64 bits, four times what a careful float32 form is.  The additions are hidden behind DRAM.
 // One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
 // read twice, number by number.
-template <typename TA, int PER>
-__global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
-                                                          uint8_t* scales, int H, int kb, float eps, float delta_scale) {
+template <typename TA, int PER, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 320 ? 4 : 1) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
+                                                          uint8_t* scales, int H, int kb, double inv_h, float eps, float delta_scale) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ double red[32];
+  __shared__ float red[32];
   constexpr int KEEP = PER > 0 ? PER : 1;
   const long row = blockIdx.x;
   const float* xr = resid + row * H;
   const TA* dr = delta ? delta + row * H : nullptr;
   float* so = sum_out ? sum_out + row * H : nullptr;
   const int slots = kb * 32;                                // of four numbers
-  double ss = 0.0;
+  float ss = 0.f;
   float x[KEEP][4], gw[KEEP][4];
   auto load = [&](int slot, float (&v)[4]) {
     load_numbers<float, 4, (PER > 0)>(xr + 4 * slot, H - 4 * slot, v);
@@ -183,9 +228,9 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const float* resid, co
   auto finish = [&](int slot, float (&v)[4], const float (&g)[4], float hi, float lo) {
     uint32_t w[1];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {                           // v (hi + lo) g, rounded once and a little
-      const float f = hi * g[j], fl = fmaf(lo, g[j], fmaf(hi, g[j], -f)), y = v[j] * f, yl = fmaf(v[j], fl, fmaf(v[j], f, -y));
-      v[j] = abs_bits(yl) < kInfBits ? y + yl : y;
+    for (int j = 0; j < 4; ++j) {                           // v (hi + lo) g, rounded once and a little (not finite: NaN)
+      const float f = hi * g[j], fl = fmaf(lo, g[j], fmaf(hi, g[j], -f)), y = v[j] * f;
+      v[j] = y + fmaf(v[j], fl, fmaf(v[j], f, -y));
     }
     const float s = group_codes<32, 4>(v, w);
     const size_t group = (size_t)row * kb + (slot >> 5);
@@ -199,28 +244,32 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const float* resid, co
       if (slot < slots) load(slot, x[i]);
     }
 #pragma unroll
+    for (int i = 0; i < PER; ++i) {                         // the gains too in front of the first store, which they could not pass
+      const int slot = threadIdx.x + i * blockDim.x;
+      if (slot < slots) load_numbers<float, 4, true>(gain + 4 * slot, H - 4 * slot, gw[i]);
+    }
+#pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int slot = threadIdx.x + i * blockDim.x;
       if (slot >= slots) continue;
-      load_numbers<float, 4, true>(gain + 4 * slot, H - 4 * slot, gw[i]);
       if (so && 4 * slot < H) store_vec<float, 4>(so + 4 * slot, x[i]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss = fma((double)x[i][j], (double)x[i][j], ss);
+      for (int j = 0; j < 4; ++j) ss = fmaf(x[i][j], x[i][j], ss);
     }
   } else {
     for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
       load(slot, x[0]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss = fma((double)x[0][j], (double)x[0][j], ss);
+      for (int j = 0; j < 4; ++j) ss = fmaf(x[0][j], x[0][j], ss);
     }
   }
-  const double inv = 1.0 / sqrt(block_sum(ss, red) / H + (double)eps);
-  const float hi = (float)inv, lo = (float)(inv - (double)hi);
+  const float2 total = block_sum2(ss, red);
+  const float2 inv = inverse_root(((double)total.x + (double)total.y) * inv_h + (double)eps);
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int slot = threadIdx.x + i * blockDim.x;        // whole warps: slots and threads are multiples of 32
-      if (slot < slots) finish(slot, x[i], gw[i], hi, lo);
+      if (slot < slots) finish(slot, x[i], gw[i], inv.x, inv.y);
     }
   } else {
     for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
@@ -229,7 +278,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_q8_kernel(const float* resid, co
       for (int j = 0; j < 4; ++j)
         if (so && 4 * slot + j < H) so[4 * slot + j] = x[0][j];
       load_numbers<float, 4, false>(gain + 4 * slot, H - 4 * slot, gw[0]);
-      finish(slot, x[0], gw[0], hi, lo);
+      finish(slot, x[0], gw[0], inv.x, inv.y);
     }
   }
 }
@@ -258,13 +307,13 @@ int blocks_of(int n) { return (int)(((long)n + kGroup - 1) / kGroup); }
 
 template <typename T>
 int quantize_rows(const void* x, long row_stride, void* codes, void* scales, int M, int K, cudaStream_t s) {
-  constexpr int V = 16 / sizeof(T), per_block = 256 / (kGroup / V);
+  constexpr int V = 16 / sizeof(T), per_block = 256 / (kGroup / V) * kAtOnce;
   const int kb = blocks_of(K);
   const long groups = (long)M * kb, blocks = (groups + per_block - 1) / per_block;
-  if (blocks > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
+  if (groups + per_block > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
   const bool fast = K % V == 0 && aligned16(x) && (M == 1 || row_stride % V == 0);
   launch_kernel(fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
-                (uint8_t*)codes, (uint8_t*)scales, groups, K, kb);
+                (uint8_t*)codes, (uint8_t*)scales, (uint32_t)groups, K, (uint32_t)kb);
   return launch_status();
 }
 
@@ -284,13 +333,16 @@ int rmsnorm(const float* resid, const void* delta, const float* gain, float* sum
             cudaStream_t s) {
   const int kb = blocks_of(H);
   const bool vec = H % 4 == 0 && aligned16(resid) && aligned16(gain) && ((uintptr_t)delta % (4 * sizeof(TA))) == 0 && aligned16(sum_out);
-  auto kern = rmsnorm_q8_kernel<TA, 0>;
+  auto kern = rmsnorm_q8_kernel<TA, 0, 1024>;
   int threads = kb >= 32 ? 1024 : 32 * kb;
   if (vec && kb <= 128) {
-    kern = rmsnorm_q8_kernel<TA, 4>;
-    threads = 32 * ((kb + 3) / 4);
+    // few rows: as many threads as the row has pieces, the shortest way through it; many: four pieces a thread
+    const int per = M <= 256 ? (kb + 31) / 32 : 4;
+    threads = 32 * ((kb + per - 1) / per);
+    kern = per == 1 ? rmsnorm_q8_kernel<TA, 1, 1024> : per == 2 ? rmsnorm_q8_kernel<TA, 2, 1024> : threads <= 320 ? rmsnorm_q8_kernel<TA, 4, 320> : rmsnorm_q8_kernel<TA, 4, 1024>;
   }
-  launch_kernel(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, eps, delta_scale);
+  launch_kernel(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
+                delta_scale);
   return launch_status();
 }
 

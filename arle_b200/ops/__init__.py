@@ -2629,20 +2629,55 @@ def pack_gate_up_q8(gate: Q8Weight, up: Q8Weight) -> Q8Weight:
     return Q8Weight(codes.view(2 * nb * Q8_BLOCK, K).view(_E4M3), scales)
 
 
+# These run between the products of every layer, and a step of few rows is as long as their checks: what is in order costs one expression, the reason is looked
+# for only where something is not.
+def _bad_rows_q8(what: str, codes, scales, want=None):
+    raise KernelError(f"{what}: rows in 8 bits are contiguous float8_e4m3fn [M, a multiple of {Q8_BLOCK}] and contiguous float8_e8m0fnu [M, blocks]; got "
+                      f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}" + (f", wanted {want[0]} rows of {want[1]}" if want else ""))
+
+
 def _rows_q8(what: str, codes, scales):
     """(rows, width) of activations in 8 bits."""
     shape = codes.shape
-    if (codes.dtype is _E4M3 and scales.dtype is _E8M0 and len(shape) == 2 and shape[1] and shape[1] % Q8_BLOCK == 0
-            and scales.shape == (shape[0], shape[1] // Q8_BLOCK) and codes.is_contiguous() and scales.is_contiguous()):
+    if (codes.dtype is _E4M3 and scales.dtype is _E8M0 and len(shape) == 2 and shape[1] and not shape[1] & 127 and scales.shape == (shape[0], shape[1] >> 7)
+            and codes.is_contiguous() and scales.is_contiguous()):
         return shape
-    raise KernelError(f"{what}: rows in 8 bits are contiguous float8_e4m3fn [M, a multiple of {Q8_BLOCK}] and contiguous float8_e8m0fnu [M, blocks]; got "
-                      f"{codes.dtype} {tuple(codes.shape)} and {scales.dtype} {tuple(scales.shape)}")
+    _bad_rows_q8(what, codes, scales)
 
 
-def _code_pointer(what: str, p: int) -> int:
-    if p % 16:
-        raise KernelError(f"{what}: codes must start on a 16-byte boundary")
-    return p
+def _rows_q8_for(what: str, codes, scales, M: int, K: int) -> None:
+    """Checks that ``codes`` and ``scales`` are room for M rows of K numbers."""
+    kb = (K + 127) >> 7
+    if not (codes.dtype is _E4M3 and scales.dtype is _E8M0 and codes.shape == (M, kb << 7) and scales.shape == (M, kb) and codes.is_contiguous()
+            and scales.is_contiguous()):
+        _bad_rows_q8(what, codes, scales, (M, kb << 7))
+
+
+def _on_device(what: str, device: int, *tensors) -> None:
+    """Checks that all tensors are on the device of this number and that it is the current one."""
+    if device >= 0 and torch._C._cuda_getDevice() == device:
+        for t in tensors:
+            if t.get_device() != device:
+                break
+        else:
+            return
+    _placed(what, tensors)                # says what is wrong
+    raise KernelError(f"{what}: tensors on different devices")
+
+
+def _misaligned(what: str):
+    raise KernelError(f"{what}: codes and float32 sums must start on a 16-byte boundary")
+
+
+_ERR_BY_INDEX = {}
+
+
+def _error_word(device: int) -> int:
+    """The address of a device's error word (see ``error_flag``), by the device's number."""
+    flag = _ERR_BY_INDEX.get(device)
+    if flag is None:
+        flag = _ERR_BY_INDEX[device] = error_flag(torch.device("cuda", device))
+    return flag.data_ptr()
 
 
 def quantize_q8(x, codes, scales) -> None:
@@ -2651,18 +2686,23 @@ def quantize_q8(x, codes, scales) -> None:
 
     The scale of a row's 128 numbers is the least power of two s with max |x| <= 448 * s (at least 2^-100; at most 2^119, beyond which numbers end at
     448 * 2^119), a code is x / s rounded to nearest even.  Infinities and NaN become NaN and do not count for the scale.  Columns from K on are zero."""
-    if x.dim() != 2 or x.shape[1] == 0:
+    if x.dim() != 2:
         raise KernelError(f"quantize_q8: x must be [M, K], got {tuple(x.shape)}")
     M, K = x.shape
-    if _rows_q8("quantize_q8", codes, scales) != (M, q8_width(K)):
-        raise KernelError(f"quantize_q8: x {tuple(x.shape)} needs codes {(M, q8_width(K))}, got {tuple(codes.shape)}")
-    if M and K > 1 and x.stride(1) != 1:
+    if K == 0:
+        raise KernelError(f"quantize_q8: x must be [M, K], got {tuple(x.shape)}")
+    _rows_q8_for("quantize_q8", codes, scales, M, K)
+    stride, unit = x.stride()
+    if unit != 1 and K > 1 and M:
         raise KernelError("quantize_q8: rows of x must have unit inner stride")
     dt = _dt(x)
-    device, (xp, cp, sp) = _placed("quantize_q8", (x, codes, scales))
-    if M == 0:
-        return
-    _check(library().arle_quantize_q8(xp, dt, x.stride(0), _code_pointer("quantize_q8", cp), sp, M, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_q8")
+    device = x.get_device()
+    _on_device("quantize_q8", device, x, codes, scales)
+    cp = codes.data_ptr()
+    if cp & 15:
+        _misaligned("quantize_q8")
+    if M:
+        _check((_LIB or library()).arle_quantize_q8(x.data_ptr(), dt, stride, cp, scales.data_ptr(), M, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_q8")
 
 
 def quantize_weight_q8(w, codes, scales) -> Q8Weight:
@@ -2671,15 +2711,18 @@ def quantize_weight_q8(w, codes, scales) -> Q8Weight:
     if w.dim() != 2 or w.shape[1] == 0:
         raise KernelError(f"quantize_weight_q8: w must be [N, K], got {tuple(w.shape)}")
     N, K = w.shape
-    if tuple(codes.shape) != (N, q8_width(K)):
+    if codes.shape != (N, q8_width(K)):
         raise KernelError(f"quantize_weight_q8: w {tuple(w.shape)} needs codes {(N, q8_width(K))}, got {tuple(codes.shape)}")
     weight = Q8Weight(codes, scales)
-    if N and K > 1 and w.stride(1) != 1:
+    stride, unit = w.stride()
+    if unit != 1 and K > 1 and N:
         raise KernelError("quantize_weight_q8: rows of w must have unit inner stride")
     dt = _dt(w)
-    device, (wp, cp, sp) = _placed("quantize_weight_q8", (w, codes, scales))
+    device = w.get_device()
+    _on_device("quantize_weight_q8", device, w, codes, scales)
     if N:
-        _check(library().arle_quantize_weight_q8(wp, dt, w.stride(0), cp, sp, N, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_weight_q8")
+        _check((_LIB or library()).arle_quantize_weight_q8(w.data_ptr(), dt, stride, codes.data_ptr(), scales.data_ptr(), N, K,
+                                                           torch._C._cuda_getCurrentRawStream(device)), "quantize_weight_q8")
     return weight
 
 
@@ -2687,57 +2730,74 @@ def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, de
     """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's float32 numbers as
     ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.  ``sum_out`` (float32 [M, H]: ``resid`` itself or a
     buffer that does not overlap it) gets x; None: x is kept nowhere."""
-    if resid.dim() != 2 or resid.shape[1] == 0 or resid.dtype != torch.float32 or not resid.is_contiguous():
+    f32 = torch.float32
+    if resid.dim() != 2 or resid.dtype is not f32 or not resid.is_contiguous():
         raise KernelError("rmsnorm_q8: the residual must be contiguous float32 [M, H]")
-    M, H = resid.shape
-    if weight.dtype != torch.float32 or weight.shape != (H,) or not weight.is_contiguous():
-        raise KernelError("rmsnorm_q8: the weight must be contiguous float32 [H]")
-    if delta is not None and (delta.shape != resid.shape or not delta.is_contiguous()):
-        raise KernelError("rmsnorm_q8: delta must be contiguous and of the residual's shape")
-    if sum_out is not None and (sum_out.shape != resid.shape or sum_out.dtype != torch.float32 or not sum_out.is_contiguous()):
+    M, H = shape = resid.shape
+    if H == 0 or weight.dtype is not f32 or weight.shape != (H,) or not weight.is_contiguous():
+        raise KernelError("rmsnorm_q8: the weight must be contiguous float32 [H], H at least 1")
+    _rows_q8_for("rmsnorm_q8", codes, scales, M, H)
+    device = resid.get_device()
+    dp = so = None
+    dt = 0
+    if delta is not None:
+        if delta.shape != shape or not delta.is_contiguous():
+            raise KernelError("rmsnorm_q8: delta must be contiguous and of the residual's shape")
+        dt, dp = _dt(delta), delta.data_ptr()
+    if sum_out is not None and (sum_out.shape != shape or sum_out.dtype is not f32 or not sum_out.is_contiguous()):
         raise KernelError("rmsnorm_q8: sum_out must be contiguous float32 like the residual")
-    if _rows_q8("rmsnorm_q8", codes, scales) != (M, q8_width(H)):
-        raise KernelError(f"rmsnorm_q8: rows of {H} need codes {(M, q8_width(H))}, got {tuple(codes.shape)}")
-    dt = _dt(delta) if delta is not None else 0
-    given = [resid, weight, codes, scales] + [t for t in (delta, sum_out) if t is not None]
-    device, (rp, wp, cp, sp, *_) = _placed("rmsnorm_q8", given)
-    so = sum_out.data_ptr() if sum_out is not None else None
-    if so is not None and so != rp and abs(so - rp) < 4 * M * H:
-        raise KernelError("rmsnorm_q8: sum_out overlaps the residual without being it")
-    if M == 0:
-        return
-    _check(library().arle_rmsnorm_q8(rp, delta.data_ptr() if delta is not None else None, dt, wp, so, _code_pointer("rmsnorm_q8", cp), sp, M, H, float(eps),
-                                     float(delta_scale), torch._C._cuda_getCurrentRawStream(device)), "rmsnorm_q8")
+    given = (resid, weight, codes, scales)
+    if delta is not None:
+        given += (delta,)
+    if sum_out is not None:
+        given += (sum_out,)
+    _on_device("rmsnorm_q8", device, *given)
+    rp, cp = resid.data_ptr(), codes.data_ptr()
+    if sum_out is not None:
+        so = sum_out.data_ptr()
+        if so != rp and abs(so - rp) < 4 * M * H:
+            raise KernelError("rmsnorm_q8: sum_out overlaps the residual without being it")
+    if cp & 15:
+        _misaligned("rmsnorm_q8")
+    if M:
+        _check((_LIB or library()).arle_rmsnorm_q8(rp, dp, dt, weight.data_ptr(), so, cp, scales.data_ptr(), M, H, eps, delta_scale,
+                                                   torch._C._cuda_getCurrentRawStream(device)), "rmsnorm_q8")
 
 
 def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     """out[M, N] = x . w^T for rows in 8 bits (``quantize_q8``, ``rmsnorm_q8``, ``gemm_act_mul_q8``) and a weight in 8 bits; out float32 or bfloat16, unit inner
     stride, any row stride.  Every block of 128 numbers of k is summed on the tensor cores, scaled by the row's and the weight block's scale and added up in
-    float32; the product of the two scales should be a normal float32 number.  The result of a row does not depend on the other rows' numbers."""
+    float32; the product of the two scales should be a normal float32 number.  The result of a row does not depend on the other rows' numbers (on how many there
+    are, in its last bits)."""
     M, K = _rows_q8("gemm_q8", codes, scales)
+    wc, ws = w.codes, w.scales
     N = w.shape[0]
     if w.shape[1] != K or out.shape != (M, N):
         raise KernelError(f"gemm_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
-    if M and N > 1 and out.stride(1) != 1:
+    stride, unit = out.stride()
+    if unit != 1 and N > 1 and M:
         raise KernelError("gemm_q8: rows of out must have unit inner stride")
     dt = _dt(out)
-    device, (xp, sp, wp, wsp, op) = _placed("gemm_q8", (codes, scales, w.codes, w.scales, out))
+    device = out.get_device()
+    _on_device("gemm_q8", device, codes, scales, wc, ws, out)
+    xp = codes.data_ptr()
+    if xp & 15:
+        _misaligned("gemm_q8")
     if M == 0 or N == 0:
         return
-    xp, kb, stream = _code_pointer("gemm_q8", xp), K // Q8_BLOCK, torch._C._cuda_getCurrentRawStream(device)
-    _launch_gemm_q8(_q8_route(M, N, kb, device) if _KERNEL_SET == "fast" else ("rows", 1, 0.0), xp, sp, wp, wsp, op, dt, out, M, N, kb, stream)
-
-
-def _launch_gemm_q8(route, xp, sp, wp, wsp, op, dt: int, out, M: int, N: int, kb: int, stream) -> None:
-    kind, parts, _ = route
+    kb = K >> 7
+    kind, parts, _ = _q8_route(M, N, kb, device) if _KERNEL_SET == "fast" else ("rows", 1, 0.0)
+    args = (xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), out.data_ptr(), dt, stride, M, N, kb)
+    lib, stream = _LIB or library(), torch._C._cuda_getCurrentRawStream(device)
     if kind == "rows":
-        _check(library().arle_gemm_q8(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, stream), "gemm_q8")
+        code = lib.arle_gemm_q8(*args, stream)
     elif kind == "few":
-        _check(library().arle_gemm_q8_few(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, parts, _ptr(error_flag(out.device)), stream), "gemm_q8")
+        code = lib.arle_gemm_q8_few(*args, parts, _error_word(device), stream)
     elif kind == "split":
-        _check(library().arle_gemm_q8_split(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, parts, _ptr(error_flag(out.device)), stream), "gemm_q8")
+        code = lib.arle_gemm_q8_split(*args, parts, _error_word(device), stream)
     else:
-        _check(library().arle_gemm_q8_pair(xp, sp, wp, wsp, op, dt, out.stride(0), M, N, kb, _ptr(error_flag(out.device)), stream), "gemm_q8")
+        code = lib.arle_gemm_q8_pair(*args, _error_word(device), stream)
+    _check(code, "gemm_q8")
 
 
 @functools.lru_cache(maxsize=None)
@@ -2791,18 +2851,19 @@ def _q8_route(M: int, N: int, kb: int, device: int):
 def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
     """The gate behind a packed product: from float32 sums ``gate_up`` [M, 256 * nb], whose columns are 128 of the gate, 128 of the up projection and so on,
     act(gate) * up as ``quantize_q8`` makes codes [M, 128 * nb] and scales [M, nb]; ``activation`` any of ``ACTIVATIONS``."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise KernelError(f"act_mul_q8: activation {activation!r} (known: {', '.join(ACTIVATIONS)})")
     M, I = _rows_q8("act_mul_q8", codes, scales)
-    if gate_up.shape != (M, 2 * I) or gate_up.dtype != torch.float32 or not gate_up.is_contiguous():
+    if gate_up.shape != (M, 2 * I) or gate_up.dtype is not torch.float32 or not gate_up.is_contiguous():
         raise KernelError(f"act_mul_q8: gate_up must be contiguous float32 {(M, 2 * I)}, got {gate_up.dtype} {tuple(gate_up.shape)}")
-    device, (gp, cp, sp) = _placed("act_mul_q8", (gate_up, codes, scales))
-    if M == 0:
-        return
-    if gp % 16:
-        raise KernelError("act_mul_q8: gate_up must start on a 16-byte boundary")
-    _check(library().arle_act_mul_q8(gp, _code_pointer("act_mul_q8", cp), sp, M, I // Q8_BLOCK, ACTIVATIONS[activation],
-                                     torch._C._cuda_getCurrentRawStream(device)), "act_mul_q8")
+    device = codes.get_device()
+    _on_device("act_mul_q8", device, gate_up, codes, scales)
+    gp, cp = gate_up.data_ptr(), codes.data_ptr()
+    if (gp | cp) & 15:
+        _misaligned("act_mul_q8")
+    if M:
+        _check((_LIB or library()).arle_act_mul_q8(gp, cp, scales.data_ptr(), M, I >> 7, act, torch._C._cuda_getCurrentRawStream(device)), "act_mul_q8")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2817,23 +2878,31 @@ def _q8_gate_in_pair(M: int, N: int, kb: int, device: int) -> bool:
 
 def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, activation: str = "silu") -> None:
     """The first half of a gated feed-forward in 8 bits: act(x . gate^T) * (x . up^T) for a weight of ``pack_gate_up_q8``, its float32 numbers as ``quantize_q8``
-    makes codes [M, w.shape[0] / 2] and scales.  ``gate_up``: float32 scratch [M, w.shape[0]], contiguous, for few rows, whose sums and gate are two launches."""
+    makes codes [M, w.shape[0] / 2] and scales.  ``gate_up``: float32 scratch [M, w.shape[0]], contiguous, for the sums where they and the gate are two launches
+    (few rows; what is in it afterwards is left open)."""
     M, K = _rows_q8("gemm_act_mul_q8", codes, scales)
-    if w.shape[0] % (2 * Q8_BLOCK):
-        raise KernelError(f"gemm_act_mul_q8: a packed weight has a multiple of {2 * Q8_BLOCK} rows, got {w.shape[0]} (see pack_gate_up_q8)")
-    if _rows_q8("gemm_act_mul_q8", out_codes, out_scales) != (M, w.shape[0] // 2):
-        raise KernelError(f"gemm_act_mul_q8: codes of the result must be {(M, w.shape[0] // 2)}, got {tuple(out_codes.shape)}")
-    if activation not in ACTIVATIONS:
+    N = w.shape[0]
+    if N % (2 * Q8_BLOCK) or w.shape[1] != K:
+        raise KernelError(f"gemm_act_mul_q8: a packed weight for rows of {K} is [a multiple of {2 * Q8_BLOCK}, {K}], got {tuple(w.shape)} (see pack_gate_up_q8)")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise KernelError(f"gemm_act_mul_q8: activation {activation!r} (known: {', '.join(ACTIVATIONS)})")
-    if gate_up.shape != (M, w.shape[0]) or gate_up.dtype != torch.float32 or not gate_up.is_contiguous():
-        raise KernelError(f"gemm_act_mul_q8: gate_up must be contiguous float32 {(M, w.shape[0])}, got {gate_up.dtype} {tuple(gate_up.shape)}")
-    if w.shape[1] != K:
-        raise KernelError(f"gemm_act_mul_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)}")
-    if _KERNEL_SET == "fast" and _q8_gate_in_pair(M, w.shape[0], K // Q8_BLOCK, codes.get_device()):
-        device, (xp, sp, wp, wsp, ocp, osp, _) = _placed("gemm_act_mul_q8", (codes, scales, w.codes, w.scales, out_codes, out_scales, gate_up))
-        _check(library().arle_gemm_q8_pair_gated(_code_pointer("gemm_act_mul_q8", xp), sp, wp, wsp, _code_pointer("gemm_act_mul_q8", ocp), osp, M,
-                                                 w.shape[0] // (2 * Q8_BLOCK), K // Q8_BLOCK, ACTIVATIONS[activation], _ptr(error_flag(codes.device)),
-                                                 torch._C._cuda_getCurrentRawStream(device)), "gemm_act_mul_q8")
+    if gate_up.shape != (M, N) or gate_up.dtype is not torch.float32 or not gate_up.is_contiguous():
+        raise KernelError(f"gemm_act_mul_q8: gate_up must be contiguous float32 {(M, N)}, got {gate_up.dtype} {tuple(gate_up.shape)}")
+    _rows_q8_for("gemm_act_mul_q8", out_codes, out_scales, M, N >> 1)
+    wc, ws = w.codes, w.scales
+    device = codes.get_device()
+    _on_device("gemm_act_mul_q8", device, codes, scales, wc, ws, gate_up, out_codes, out_scales)
+    xp, gp, op = codes.data_ptr(), gate_up.data_ptr(), out_codes.data_ptr()
+    if (xp | gp | op) & 15:
+        _misaligned("gemm_act_mul_q8")
+    if M == 0 or N == 0:
+        return
+    kb, nb = K >> 7, N >> 8
+    lib, stream = _LIB or library(), torch._C._cuda_getCurrentRawStream(device)
+    if _KERNEL_SET == "fast" and _q8_gate_in_pair(M, N, kb, device):
+        _check(lib.arle_gemm_q8_pair_gated(xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), op, out_scales.data_ptr(), M, nb, kb, act, _error_word(device), stream),
+               "gemm_act_mul_q8")
         return
     gemm_q8(codes, scales, w, gate_up)
-    act_mul_q8(gate_up, out_codes, out_scales, activation)
+    _check(lib.arle_act_mul_q8(gp, op, out_scales.data_ptr(), M, nb, act, stream), "act_mul_q8")
