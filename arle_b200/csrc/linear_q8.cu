@@ -4,6 +4,7 @@
 // power of two s with max |x| <= 448 s (2^-100 to 2^119), stored as its exponent (e8m0: exponent + 127); codes are rne(x / s).  Numbers that are not
 // finite do not count for the scale and become NaN: e4m3 has no infinities, and what was not finite must not come out of a product as if it were.
 // Weights: the same for blocks of 128 x 128, one float32 scale a block.
+// Up to kEarlyRows rows are launched early: plain loads, and all of a row's ahead of the first store.
 // All four kernels read every number once, keep it in registers between the maximum and the rounding, and are bound by DRAM (few rows: by latency).
 #include "q8.cuh"
 using namespace arle;
@@ -312,7 +313,7 @@ int quantize_rows(const void* x, long row_stride, void* codes, void* scales, int
   const long groups = (long)M * kb, blocks = (groups + per_block - 1) / per_block;
   if (groups + per_block > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
   const bool fast = K % V == 0 && aligned16(x) && (M == 1 || row_stride % V == 0);
-  launch_kernel(fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
+  launch_kernel_as(M <= kEarlyRows || (pdl_enabled() & 1) != 0, fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
                 (uint8_t*)codes, (uint8_t*)scales, (uint32_t)groups, K, (uint32_t)kb);
   return launch_status();
 }
@@ -341,7 +342,7 @@ int rmsnorm(const float* resid, const void* delta, const float* gain, float* sum
     threads = 32 * ((kb + per - 1) / per);
     kern = per == 1 ? rmsnorm_q8_kernel<TA, 1, 1024> : per == 2 ? rmsnorm_q8_kernel<TA, 2, 1024> : threads <= 320 ? rmsnorm_q8_kernel<TA, 4, 320> : rmsnorm_q8_kernel<TA, 4, 1024>;
   }
-  launch_kernel(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
+  launch_kernel_as(M <= kEarlyRows || (pdl_enabled() & 1) != 0, kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
                 delta_scale);
   return launch_status();
 }
@@ -382,6 +383,6 @@ ARLE_API int arle_act_mul_q8(const float* sums, void* codes, void* scales, int M
   if (act < 0 || act > 1 || !aligned16(sums) || !aligned16(codes)) return ARLE_E_BADARG;
   const long groups = (long)M * nb, blocks = (groups + 7) / 8;
   if (blocks > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
-  launch_kernel(act_mul_q8_kernel, dim3((unsigned)blocks), dim3(256), 0, s, 1, sums, (uint8_t*)codes, (uint8_t*)scales, groups, act);
+  launch_kernel_as(M <= kEarlyRows || (pdl_enabled() & 1) != 0, act_mul_q8_kernel, dim3((unsigned)blocks), dim3(256), 0, s, 1, sums, (uint8_t*)codes, (uint8_t*)scales, groups, act);
   return launch_status();
 }

@@ -41,6 +41,7 @@ class EngineOptions:
     cuda_graph: bool = True
     kernel_set: str = "fast"                   # "plain": the general kernels only, whatever the shapes
     cache_dtype: str = "auto"                  # "auto": keys and values as the model computes them; "float8_e4m3": 8-bit codes, a scale per page and head
+    weight_dtype: str = "auto"                 # "auto": as the model computes; "float8_e4m3": the blocks' matrices as 8-bit codes, a scale per 128 x 128
     device_tables: bool = False                # a step's tables are made on the device from its requests' lengths, instead of copied there
 
 
@@ -61,9 +62,11 @@ class Engine:
         if model is None:
             if model_path is None:
                 raise ValueError("Engine needs a model folder (model_path) or a loaded model")
-            model = load_model(model_path, dtype, o.device)
+            model = load_model(model_path, dtype, o.device, o.weight_dtype)
         elif model.dtype != dtype:
             raise ValueError(f"the given model was loaded as {model.dtype}, the options ask for {dtype}")
+        elif o.weight_dtype not in ("auto", getattr(model, "weight_dtype", "auto")):
+            raise ValueError(f"the given model was loaded with weights {getattr(model, 'weight_dtype', 'auto')!r}, the options ask for {o.weight_dtype!r}")
         self.model = model
         max_seq = o.max_seq_len or model.spec.max_position
         if o.cache_dtype not in ("auto", "float8_e4m3"):

@@ -21,21 +21,22 @@ def parse_dtype(dtype) -> torch.dtype:
     raise ValueError(f"dtype must be bfloat16 or float32, got {dtype!r}")
 
 
-def load_model(model_dir: str, dtype="bfloat16", device="cuda") -> DecoderModel:
+def load_model(model_dir: str, dtype="bfloat16", device="cuda", weight_dtype: str = "auto") -> DecoderModel:
     """The model class is chosen by ``architectures`` in config.json; weights are
-    bound by tensor name from model.safetensors (or its sharded index)."""
+    bound by tensor name from model.safetensors (or its sharded index).  ``weight_dtype``
+    "float8_e4m3": the blocks' matrices in 8 bits, with the checkpoint's own codes and scales where it has them."""
     dtype = parse_dtype(dtype)
     config = load_config(model_dir)
     spec = config.to_model_spec()
     model = build_model(spec)
     tensors = load_weights(model_dir, model.weight_decls(), spec.ignored_tensors)
-    model.load(tensors, dtype, device)
+    model.load(tensors, dtype, device, **({} if weight_dtype == "auto" else {"weight_dtype": weight_dtype}))
     model.config = config
     return model
 
 
 def random_model(config: dict, seed: int, dtype="bfloat16", device="cuda", sigma: float = 0.02,
-                 gain_jitter: float = 0.1, num_layers: int = None) -> DecoderModel:
+                 gain_jitter: float = 0.1, num_layers: int = None, weight_dtype: str = "auto") -> DecoderModel:
     """A model with seeded random weights made directly on the device (no files).
     ``num_layers`` keeps only the first blocks of the configuration (the
     benchmark's way of fitting time or memory; layer sizes stay)."""
@@ -48,6 +49,6 @@ def random_model(config: dict, seed: int, dtype="bfloat16", device="cuda", sigma
     spec = cfg.to_model_spec()
     model = build_model(spec)
     tensors = random_tensors(model.weight_decls(), seed, sigma, gain_jitter, torch.bfloat16, device)
-    model.load(tensors, dtype, device)
+    model.load(tensors, dtype, device, **({} if weight_dtype == "auto" else {"weight_dtype": weight_dtype}))
     model.config = cfg
     return model

@@ -2612,6 +2612,19 @@ class Q8Weight:
     def bytes(self) -> int:
         return self.codes.numel() + 4 * self.scales.numel()
 
+    def first_rows(self, n: int) -> "Q8Weight":
+        """The weight of the first ``n`` output features (a view)."""
+        return Q8Weight(self.codes[:n], self.scales[: -(-n // Q8_BLOCK)])
+
+
+class Q8Rows:
+    """Activations in 8 bits on their way to a product: ``codes`` and ``scales`` (see ``quantize_q8``) of rows [M, K] that ``dtype`` would hold otherwise."""
+
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes, scales, shape, dtype):
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, tuple(shape), dtype
+
 
 def pack_gate_up_q8(gate: Q8Weight, up: Q8Weight) -> Q8Weight:
     """The weight of ``gemm_act_mul_q8``: 128 rows of the gate, 128 of the up projection, and so on, the last blocks filled up with zeros.  Once, at load."""
@@ -2876,10 +2889,15 @@ def _q8_gate_in_pair(M: int, N: int, kb: int, device: int) -> bool:
     return pair <= _q8_route(M, N, kb, device)[2] + 2.0 + 8.0 * M * N / 5.0e6
 
 
+def gate_needs_sums_q8(M: int, w: Q8Weight) -> bool:
+    """Whether ``gemm_act_mul_q8`` of M rows wants its scratch: by the sizes and the kernel set alone."""
+    return _KERNEL_SET != "fast" or not _q8_gate_in_pair(M, w.shape[0], w.shape[1] >> 7, w.codes.get_device())
+
+
 def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, activation: str = "silu") -> None:
     """The first half of a gated feed-forward in 8 bits: act(x . gate^T) * (x . up^T) for a weight of ``pack_gate_up_q8``, its float32 numbers as ``quantize_q8``
     makes codes [M, w.shape[0] / 2] and scales.  ``gate_up``: float32 scratch [M, w.shape[0]], contiguous, for the sums where they and the gate are two launches
-    (few rows; what is in it afterwards is left open)."""
+    (few rows; what is in it afterwards is left open); None will do where ``gate_needs_sums_q8`` says so."""
     M, K = _rows_q8("gemm_act_mul_q8", codes, scales)
     N = w.shape[0]
     if N % (2 * Q8_BLOCK) or w.shape[1] != K:
@@ -2887,13 +2905,15 @@ def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, 
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise KernelError(f"gemm_act_mul_q8: activation {activation!r} (known: {', '.join(ACTIVATIONS)})")
-    if gate_up.shape != (M, N) or gate_up.dtype is not torch.float32 or not gate_up.is_contiguous():
+    if gate_up is not None and (gate_up.shape != (M, N) or gate_up.dtype is not torch.float32 or not gate_up.is_contiguous()):
         raise KernelError(f"gemm_act_mul_q8: gate_up must be contiguous float32 {(M, N)}, got {gate_up.dtype} {tuple(gate_up.shape)}")
     _rows_q8_for("gemm_act_mul_q8", out_codes, out_scales, M, N >> 1)
     wc, ws = w.codes, w.scales
     device = codes.get_device()
-    _on_device("gemm_act_mul_q8", device, codes, scales, wc, ws, gate_up, out_codes, out_scales)
-    xp, gp, op = codes.data_ptr(), gate_up.data_ptr(), out_codes.data_ptr()
+    given = (codes, scales, wc, ws, out_codes, out_scales)
+    _on_device("gemm_act_mul_q8", device, *(given if gate_up is None else given + (gate_up,)))
+    xp, op = codes.data_ptr(), out_codes.data_ptr()
+    gp = gate_up.data_ptr() if gate_up is not None else 0
     if (xp | gp | op) & 15:
         _misaligned("gemm_act_mul_q8")
     if M == 0 or N == 0:
@@ -2904,5 +2924,7 @@ def gemm_act_mul_q8(codes, scales, w: Q8Weight, gate_up, out_codes, out_scales, 
         _check(lib.arle_gemm_q8_pair_gated(xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), op, out_scales.data_ptr(), M, nb, kb, act, _error_word(device), stream),
                "gemm_act_mul_q8")
         return
+    if gate_up is None:
+        raise KernelError(f"gemm_act_mul_q8: {M} rows need gate_up for their sums (see gate_needs_sums_q8)")
     gemm_q8(codes, scales, w, gate_up)
     _check(lib.arle_act_mul_q8(gp, op, out_scales.data_ptr(), M, nb, act, stream), "act_mul_q8")

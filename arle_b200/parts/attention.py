@@ -46,7 +46,8 @@ from typing import ClassVar, Optional, Tuple
 import torch
 
 from .. import ops
-from .base import CacheNeed, Mixer, StateNeed, WeightDecl
+from ..weights.q8 import as_q8_weight
+from .base import CacheNeed, Mixer, StateNeed, WeightDecl, product, q8_weight
 from .registry import build_part, register_part
 
 
@@ -236,7 +237,23 @@ class Attention(Mixer):
             self.w_conv = torch.cat([tensors[self._name(r) + s.conv_suffix].to(device=device, dtype=torch.float32) for r in ("q", "k", "v")],
                                     dim=0).contiguous()
 
+    # weights in 8 bits: the plain form, whose products all go through ``product``
+    def takes_q8_weights(self):
+        return self.plain_form and not self.general_form and not self.post_form
+
+    def quantize_weights(self, tensors):
+        if not self.takes_q8_weights():
+            super().quantize_weights(tensors)
+        device = self.w_o.device
+        self.w_qkv = as_q8_weight([tensors[self._name(r)] for r in ("q", "k", "v")], device) or q8_weight(self.w_qkv)
+        self.w_o = as_q8_weight([tensors[self._name("o")]], device) or q8_weight(self.w_o)
+
+    def takes_q8_rows(self):
+        return isinstance(self.w_qkv, ops.Q8Weight)
+
     def weight_bytes(self):
+        if self.takes_q8_rows():
+            return self.w_qkv.bytes() + self.w_o.bytes()
         return sum(t.numel() * t.element_size() for t in (self.w_qkv, self.w_o))
 
     def scratch_elements_per_token(self):
@@ -260,10 +277,10 @@ class Attention(Mixer):
         return None
 
     def takes_scaled_rows(self, num_rows):
-        return not self.post_form and ops.fused_gemm_shape_ok(num_rows, self.w_qkv)
+        return not self.post_form and not self.takes_q8_rows() and ops.fused_gemm_shape_ok(num_rows, self.w_qkv)
 
     def can_sink(self, num_rows):
-        return not self.post_form and self.b_o is None and ops.fused_gemm_shape_ok(num_rows, self.w_o)
+        return not self.post_form and not self.takes_q8_rows() and self.b_o is None and ops.fused_gemm_shape_ok(num_rows, self.w_o)
 
     def _angles(self, qkv, ctx, inv_freq, rdim, general=False):
         """Cosines and sines of the step's positions, evaluated once for all layers that rotate by the same
@@ -303,7 +320,7 @@ class Attention(Mixer):
 
     def _next_product(self, rows, sink):
         """What the attention is told of the output projection behind it: where that may be one of the small products that start early."""
-        return {"product": (self.w_o, sink)} if ops.fused_gemm_shape_ok(rows, self.w_o) else {}
+        return {"product": (self.w_o, sink)} if not self.takes_q8_rows() and ops.fused_gemm_shape_ok(rows, self.w_o) else {}
 
     # ------------------------------------------------- biases, convolution, kept first tokens, capped scores, sinks
     def _forward_general(self, x, ctx, cache, state, sink=None):
@@ -364,7 +381,7 @@ class Attention(Mixer):
         eps = s.qk_norm_eps if s.qk_norm_eps is not None else 0.0
         name, columns = ("qkv", (nq + 2 * nkv) * hd) if cache.writable else ("q_only", nq * hd)
         proj = ctx.ws.get(name, (T, columns), x.dtype)
-        ops.gemm(x, self.w_qkv if cache.writable else self.w_qkv[:columns], proj)
+        product(ctx.ws, x, self._input_weight(cache), proj)
         q = ctx.ws.cut(name, proj, 0, nq * hd)
         angles = self._angles(proj, ctx, inv_freq, rdim)
         ops.attention_prep(q, ctx.positions, None, self.q_norm, None, eps, inv_freq, rdim, None, None, nq, 0, hd, cache.page_size, angles=angles)
@@ -377,7 +394,7 @@ class Attention(Mixer):
         ops.paged_attention_q8(q, attn, cache.k, cache.v, *cache.scales, ctx.positions, ctx.row_of_token, cache.block_table, nq, nkv, hd, cache.page_size,
                                s.scale, s.window, batch=ctx)
         out = ctx.ws.get("mixer_out", (T, s.hidden_size), x.dtype)
-        return None if ops.gemm(attn, self.w_o, out, sink=sink) else out
+        return None if product(ctx.ws, attn, self.w_o, out, sink) else out
 
     # ------------------------------------------------- the general form, up to the output projection
     def pre_output_width(self):
@@ -420,6 +437,13 @@ class Attention(Mixer):
         ops.head_gate(attn, gate, scale, into, s.num_heads, s.head_dim)
 
     # ---------------------------------------------------------------- forward
+    def _input_weight(self, cache):
+        """The packed input projection, or its query rows where the run reads another run's keys."""
+        columns = self.spec.num_heads * self.spec.head_dim
+        if cache.writable:
+            return self.w_qkv
+        return self.w_qkv.first_rows(columns) if self.takes_q8_rows() else self.w_qkv[:columns]
+
     def forward(self, x, ctx, cache, state, sink=None):
         s = self.spec
         T = x.shape[0]
@@ -446,26 +470,26 @@ class Attention(Mixer):
         attn = ctx.ws.get("attn_out", (T, nq * hd), x.dtype)
         if cache.writable:
             qkv = ctx.ws.get("qkv", (T, (nq + 2 * nkv) * hd), x.dtype)
-            ops.gemm(x, self.w_qkv, qkv)
+            product(ctx.ws, x, self.w_qkv, qkv)
             if ops.fused_decode_supported(qkv, ctx, cache.k.dtype, nq, nkv, hd, cache.page_size, rdim):
                 # a step of decoded tokens only: norm, rotation, cache store and attention in one launch
                 ops.decode_attention_with_prep(qkv, attn, cache.k, cache.v, cache.slot_mapping, self.q_norm, self.k_norm, eps,
                                                inv_freq if rdim else None, cache.block_table, nq, nkv, hd, cache.page_size,
                                                s.scale, s.window, ctx, **self._next_product(T, sink))
                 out = ctx.ws.get("mixer_out", (T, s.hidden_size), x.dtype)
-                return None if ops.gemm(attn, self.w_o, out, sink=sink) else out
+                return None if product(ctx.ws, attn, self.w_o, out, sink) else out
             ops.attention_prep(qkv, ctx.positions, cache.slot_mapping, self.q_norm, self.k_norm, eps, inv_freq, rdim,
                                cache.k, cache.v, nq, nkv, hd, cache.page_size, angles=self._angles(qkv, ctx, inv_freq, rdim))
         else:
             qkv = ctx.ws.get("q_only", (T, nq * hd), x.dtype)
-            ops.gemm(x, self.w_qkv[: nq * hd], qkv)
+            product(ctx.ws, x, self._input_weight(cache), qkv)
             ops.attention_prep(qkv, ctx.positions, None, self.q_norm, None, eps, inv_freq, rdim, None, None, nq, 0, hd,
                                cache.page_size, angles=self._angles(qkv, ctx, inv_freq, rdim))
         q = ctx.ws.cut("qkv" if cache.writable else "q_only", qkv, 0, nq * hd)
         ops.paged_attention(q, attn, cache.k, cache.v, ctx.positions, ctx.row_of_token,
                             cache.block_table, nq, nkv, hd, cache.page_size, s.scale, s.window, batch=ctx, **self._next_product(T, sink))
         out = ctx.ws.get("mixer_out", (T, s.hidden_size), x.dtype)
-        if ops.gemm(attn, self.w_o, out, sink=sink):
+        if product(ctx.ws, attn, self.w_o, out, sink):
             return None                       # summed into the residual by the product itself
         return out
 

@@ -31,6 +31,8 @@ from typing import Optional, Sequence, Tuple
 
 import torch
 
+from .. import ops
+
 
 @dataclass(frozen=True)
 class WeightDecl:
@@ -134,6 +136,45 @@ class Part:
         return False
 
 
+    # Weights in 8 bits: a part that says yes to ``takes_q8_weights`` turns its matrices into ``ops.Q8Weight`` when ``quantize_weights`` is called (once,
+    # behind ``load``, with the same tensors), and its input then comes as ``ops.Q8Rows``, which the norm in front of it writes.
+    def takes_q8_weights(self) -> bool:
+        return False
+
+    def quantize_weights(self, tensors: dict) -> None:
+        raise ValueError(f"{type(self).__name__} does not keep its weights in 8 bits")
+
+    def takes_q8_rows(self) -> bool:
+        """Whether this part's input is wanted as ``ops.Q8Rows`` (its weights are in 8 bits now)."""
+        return False
+
+
+def q8_weight(matrix) -> "ops.Q8Weight":
+    """A matrix on the device as codes and scales."""
+    n, k = matrix.shape
+    codes = torch.empty((n, ops.q8_width(k)), dtype=torch.float8_e4m3fn, device=matrix.device)
+    return ops.quantize_weight_q8(matrix, codes, torch.empty((-(-n // ops.Q8_BLOCK), codes.shape[1] // ops.Q8_BLOCK), dtype=torch.float32, device=matrix.device))
+
+
+def q8_rows(ws, name: str, rows: int, width: int, dtype) -> "ops.Q8Rows":
+    """Room for rows in 8 bits among the step's buffers."""
+    k = ops.q8_width(width)
+    return ops.Q8Rows(ws.get(name + "_codes", (rows, k), torch.float8_e4m3fn), ws.get(name + "_scales", (rows, k // ops.Q8_BLOCK), torch.float8_e8m0fnu),
+                      (rows, width), dtype)
+
+
+def product(ws, x, w, out, sink=None) -> bool:
+    """``ops.gemm``, or its counterpart in 8 bits where ``w`` is a ``Q8Weight``; rows that are not codes yet become codes on the way."""
+    if not isinstance(w, ops.Q8Weight):
+        return ops.gemm(x, w, out, sink=sink)
+    if not isinstance(x, ops.Q8Rows):
+        rows = q8_rows(ws, "product", x.shape[0], x.shape[1], x.dtype)
+        ops.quantize_q8(x, rows.codes, rows.scales)
+        x = rows
+    ops.gemm_q8(x.codes, x.scales, w, out)
+    return False
+
+
 class Norm(Part):
     """y = norm(x) over the last axis.  ``forward(stream, ...)`` is driven by the
     ``ResidualStream`` so that the sum of the pending branch output into the
@@ -141,6 +182,7 @@ class Norm(Part):
 
     eps: float
     weight: torch.Tensor
+    deferred_form = False           # whether ``deferred`` says a gain and eps (known before the weights are)
     takes_scaled_delta = False      # whether ``apply`` takes a factor on the pending branch and rows that join the residual with it
 
     def deferred(self):

@@ -55,12 +55,22 @@ class PreNormBlock(Block):
         return (self.mixer_norm.scratch_elements_per_token() + self.ffn_norm.scratch_elements_per_token()
                 + max(self.mixer.scratch_elements_per_token(), self.ffn.scratch_elements_per_token()))
 
+    def takes_q8_weights(self):
+        return all(n is None or n.deferred_form for n in (self.mixer_norm, self.ffn_norm)) and all(p is None or p.takes_q8_weights() for p in (self.mixer, self.ffn))
+
+    def quantize_weights(self, tensors):
+        if not self.takes_q8_weights():
+            super().quantize_weights(tensors)
+        for p in (self.mixer, self.ffn):
+            if p is not None:
+                p.quantize_weights(tensors)
+
     def entry(self):
         return self.mixer_norm, self.mixer
 
     def forward(self, stream, ctx, cache, state):
         T = ctx.num_tokens
-        h = stream.normed(self.mixer_norm, "normed_a")
+        h = stream.normed_for(self.mixer, self.mixer_norm, "normed_a")
         if self.ffn is None:
             nxt = stream.next_entry
             sink = stream.sink_for(nxt[0], nxt[1], "normed_a", last=True) if nxt is not None and self.mixer.can_sink(T) else None
@@ -73,7 +83,7 @@ class PreNormBlock(Block):
             stream.add(self.mixer.forward(h, ctx, cache, state, sink=sink))
         else:
             stream.add(self.mixer.forward(h, ctx, cache, state))
-        h = stream.normed(self.ffn_norm, "normed_b")
+        h = stream.normed_for(self.ffn, self.ffn_norm, "normed_b")
         nxt = stream.next_entry
         sink = stream.sink_for(nxt[0], nxt[1], "normed_a", last=True) if nxt is not None and self.ffn.can_sink(T) else None
         if sink is not None:

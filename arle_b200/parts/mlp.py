@@ -11,7 +11,8 @@ from typing import ClassVar, Tuple
 import torch
 
 from .. import ops
-from .base import FeedForward, WeightDecl
+from ..weights.q8 import as_q8_weight
+from .base import FeedForward, WeightDecl, q8_rows, q8_weight
 from .registry import register_part
 
 
@@ -53,17 +54,44 @@ class GatedMlp(FeedForward):
         self.w_gate_up = torch.stack([g, u], dim=1).reshape(2 * g.shape[0], g.shape[1]).contiguous()
         self.w_down = d.to(device=device, dtype=dtype if dtype == torch.bfloat16 else d.dtype).contiguous()
 
+    # weights in 8 bits: 128 rows of the gate, 128 of the up projection and so on, so that a tile of the product holds both numbers of a group of results
+    def takes_q8_weights(self):
+        return not self.clamped
+
+    def quantize_weights(self, tensors):
+        if not self.takes_q8_weights():
+            super().quantize_weights(tensors)
+        g, u, d = (tensors[self.spec.prefix + n] for n in self.spec.names)
+        device = self.w_down.device
+        self.w_gate_up = ops.pack_gate_up_q8(as_q8_weight([g], device) or q8_weight(self.w_gate_up[0::2]), as_q8_weight([u], device) or q8_weight(self.w_gate_up[1::2]))
+        self.w_down = as_q8_weight([d], device) or q8_weight(self.w_down)
+
+    def takes_q8_rows(self):
+        return isinstance(self.w_down, ops.Q8Weight)
+
+    def _forward_q8(self, x, ctx):
+        s, T = self.spec, x.shape[0]
+        sums = ctx.ws.get("gate_up_sums", (T, self.w_gate_up.shape[0]), torch.float32) if ops.gate_needs_sums_q8(T, self.w_gate_up) else None
+        act = q8_rows(ctx.ws, "ffn_act", T, s.intermediate_size, x.dtype)
+        ops.gemm_act_mul_q8(x.codes, x.scales, self.w_gate_up, sums, act.codes, act.scales, activation=s.activation)
+        out = ctx.ws.get("ffn_out", (T, s.hidden_size), x.dtype)
+        ops.gemm_q8(act.codes, act.scales, self.w_down, out)
+        return out
+
     def weight_bytes(self):
+        if self.takes_q8_rows():
+            return self.w_gate_up.bytes() + self.w_down.bytes()
         return sum(t.numel() * t.element_size() for t in (self.w_gate_up, self.w_down))
 
     def scratch_elements_per_token(self):
-        return 3 * self.spec.intermediate_size + self.spec.hidden_size
+        # (in 8 bits the sums may be kept in float32: 4 intermediate sizes of 16 bits, and the codes)
+        return (5 if self.takes_q8_rows() else 3) * self.spec.intermediate_size + self.spec.hidden_size
 
     def takes_scaled_rows(self, num_rows):
-        return not self.clamped and ops.fused_gemm_shape_ok(num_rows, self.w_gate_up, gated=True)
+        return not self.clamped and not self.takes_q8_rows() and ops.fused_gemm_shape_ok(num_rows, self.w_gate_up, gated=True)
 
     def can_sink(self, num_rows):
-        return ops.fused_gemm_shape_ok(num_rows, self.w_down)
+        return not self.takes_q8_rows() and ops.fused_gemm_shape_ok(num_rows, self.w_down)
 
     # the feed-forward up to its last product
     def pre_output_width(self):
@@ -78,6 +106,8 @@ class GatedMlp(FeedForward):
         ops.gemm_act_mul(x, self.w_gate_up, gu, into, s.activation)
 
     def forward(self, x, ctx, sink=None):
+        if self.takes_q8_rows():
+            return self._forward_q8(x, ctx)
         s = self.spec
         T = x.shape[0]
         gu = ctx.ws.get("gate_up", (T, 2 * s.intermediate_size), x.dtype)

@@ -14,7 +14,7 @@ import torch
 
 from .. import ops
 from ..config.model_spec import ModelSpec
-from .base import WeightDecl
+from .base import WeightDecl, q8_rows
 from .registry import build_part, register_model
 
 
@@ -206,6 +206,20 @@ class ResidualStream:
         self.pending = None
         return out
 
+    def normed_for(self, reader, norm, buffer_name: str):
+        """``normed`` for the part that reads it: rows in 8 bits where that is what its weights are in."""
+        if not reader.takes_q8_rows():
+            return self.normed(norm, buffer_name)
+        self._settle()
+        gain, eps = norm.deferred()
+        rows = q8_rows(self.ws, buffer_name, *self.resid.shape, self.act_dtype)
+        ops.rmsnorm_q8(self.resid, self.pending, gain, eps, rows.codes, rows.scales, sum_out=self.resid if self.pending is not None else None,
+                       delta_scale=self.scale)
+        if self.pending is not None:
+            self._copy = None
+        self.pending = None
+        return rows
+
     def normed_rows(self, norm, rows: torch.Tensor, buffer_name: str) -> torch.Tensor:
         """Norm of the rows listed only (the residual itself is left as it is)."""
         self._settle()
@@ -252,6 +266,7 @@ class DecoderModel:
             raise ValueError("a factor on the branches goes with blocks that add a branch's output as it is")
         self.readds_embedding = any(e.add_embedding for e in spec.schedule)
         self.dtype = None
+        self.weight_dtype = "auto"
         # cache layers: one per schedule entry that keeps keys of its own
         self.cache_needs = []
         self.entry_cache_layer: List[Optional[int]] = []
@@ -282,7 +297,16 @@ class DecoderModel:
     def weight_decls(self):
         return declared_weights(self.spec)
 
-    def load(self, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device) -> "DecoderModel":
+    def load(self, tensors: Dict[str, torch.Tensor], dtype: torch.dtype, device, weight_dtype: str = "auto") -> "DecoderModel":
+        """``weight_dtype`` "float8_e4m3": the blocks' matrices as 8-bit codes with a scale for each block of 128 x 128 (a checkpoint's own where it has
+        them), embedding and output projection as they are."""
+        if weight_dtype not in ("auto", "float8_e4m3"):
+            raise ValueError(f"weight_dtype must be 'auto' or 'float8_e4m3', got {weight_dtype!r}")
+        if weight_dtype != "auto":
+            odd = [type(b).__name__ for b in self.blocks if not b.takes_q8_weights()]
+            if odd:
+                raise ValueError(f"weights in 8 bits need pre-norm blocks of plain attention and a gated feed-forward behind RMS norms; this model has {odd[0]}")
+        self.weight_dtype = weight_dtype
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"engine dtype must be bfloat16 or float32, got {dtype}")
         device = torch.device(device)
@@ -303,6 +327,8 @@ class DecoderModel:
                     raise ValueError("a float32 position table needs a float32 embedding table")
         for b in self.blocks:
             b.load(tensors, dtype, device)
+            if weight_dtype != "auto":
+                b.quantize_weights(tensors)
         self.final_norm.load(tensors, dtype, device)
         if self.embed_norm is not None:
             self.embed_norm.load(tensors, dtype, device)

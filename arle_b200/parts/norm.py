@@ -50,6 +50,8 @@ class RmsNorm(Norm):
     def scratch_elements_per_token(self):
         return self.spec.size
 
+    deferred_form = True
+
     def deferred(self):
         return self.weight, self.eps
 

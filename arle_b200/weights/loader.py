@@ -9,7 +9,8 @@ tensor are read and checked, and all problems are reported in ONE error: the
 missing names, the unexpected names and the wrong shapes together.
 
 Precision kept in memory: floating tensors stored in 16 bits become bfloat16,
-tensors stored in 32 bits stay float32, integer tables become int32.
+tensors stored in 32 bits stay float32, integer tables become int32.  A matrix stored as
+8-bit codes comes with its scales, "<name>_scale_inv", as a ``StoredQ8``.
 """
 from __future__ import annotations
 
@@ -20,6 +21,7 @@ from typing import Dict, Iterable, Sequence
 import torch
 
 from ..parts.base import WeightDecl
+from .q8 import SCALE_SUFFIX, StoredQ8
 from .safetensors_io import SafetensorsError, SafetensorsFile
 
 
@@ -80,7 +82,8 @@ def load_weights(model_dir: str, decls: Sequence[WeightDecl], ignored: Iterable[
                 twice.append(f"tensor {n} is stored in two files: {os.path.basename(where[n].path)} and {os.path.basename(f.path)}")
             where[n] = f
     wanted = {d.name: d for d in decls}
-    ignored = set(ignored)
+    codes = [n for n in wanted if n in where and where[n].info(n)[0] == torch.float8_e4m3fn]
+    ignored = set(ignored) | {n + SCALE_SUFFIX for n in codes}
     missing = [n for n in wanted if n not in where]
     unexpected = sorted(n for n in where if n not in wanted and n not in ignored)
     wrong = []
@@ -89,10 +92,20 @@ def load_weights(model_dir: str, decls: Sequence[WeightDecl], ignored: Iterable[
             _, shape = where[n].info(n)
             if tuple(shape) != tuple(d.shape):
                 wrong.append((n, d.shape, shape))
+    for n in codes:
+        s = n + SCALE_SUFFIX
+        want = tuple(-(-int(v) // 128) for v in wanted[n].shape)
+        if s not in where:
+            missing.append(s)
+        elif tuple(where[s].info(s)[1]) != want or len(want) != 2:
+            wrong.append((s, want, where[s].info(s)[1]))
     if missing or unexpected or wrong or twice:
         raise WeightError(model_dir, missing, unexpected, wrong, twice)
     out = {}
     for n, d in wanted.items():
         t = where[n].tensor(n)
+        if t.dtype == torch.float8_e4m3fn:
+            out[n] = StoredQ8(t, where[n + SCALE_SUFFIX].tensor(n + SCALE_SUFFIX))
+            continue
         out[n] = t.to(device=device, dtype=kept_dtype(t.dtype, d.integer))
     return out

@@ -1,0 +1,50 @@
+"""Weights that a checkpoint stores in 8 bits: e4m3 codes "<name>" beside float32 (or 16-bit) scales "<name>_scale_inv", one for each block of 128 x 128; a
+weight is code * scale.  cklxx/arle reads such pairs for its quantised weights (infer/src/weight_loader.rs); here they are kept as they are by the parts that run on
+them and turned into 16 bits by all others.
+"""
+from __future__ import annotations
+
+from typing import Optional, Sequence
+
+import torch
+
+BLOCK = 128
+SCALE_SUFFIX = "_scale_inv"
+
+
+class StoredQ8:
+    """A stored matrix [N, K]: ``codes`` float8_e4m3fn [N, K] and ``scales`` float32 [ceil(N / 128), ceil(K / 128)], on the host.  ``to`` gives its numbers,
+    so a part that knows nothing of codes loads it like any other tensor (rounded to bfloat16 where it asks for that)."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        n, k = codes.shape
+        if tuple(scales.shape) != (-(-n // BLOCK), -(-k // BLOCK)):
+            raise ValueError(f"scales {tuple(scales.shape)} do not fit codes {tuple(codes.shape)} in blocks of {BLOCK}")
+        self.codes, self.scales, self.shape = codes, scales.to(torch.float32), codes.shape
+        self.dtype = torch.bfloat16
+
+    def to(self, device=None, dtype=None) -> torch.Tensor:
+        codes, scales = self.codes.to(device=device), self.scales.to(device=device)
+        n, k = self.shape
+        out = torch.empty((n, k), dtype=dtype or self.dtype, device=codes.device)
+        for i in range(0, n, 32 * BLOCK):                  # a few blocks of rows at a time: in float32 a matrix is four times its codes
+            j = min(n, i + 32 * BLOCK)
+            s = scales[i // BLOCK: -(-j // BLOCK)].repeat_interleave(BLOCK, dim=0)[: j - i].repeat_interleave(BLOCK, dim=1)[:, :k]
+            out[i:j] = (codes[i:j].to(torch.float32) * s).to(out.dtype)
+        return out
+
+
+def as_q8_weight(parts: Sequence, device) -> Optional["ops.Q8Weight"]:
+    """Stored matrices one under the other as one weight with their own codes and scales; None where that cannot be (one of them is not stored in 8 bits, or ends
+    inside a block that the next one would share)."""
+    from .. import ops
+
+    if not all(isinstance(p, StoredQ8) for p in parts) or any(p.shape[0] % BLOCK for p in parts[:-1]):
+        return None
+    n, k = sum(p.shape[0] for p in parts), parts[0].shape[1]
+    codes = torch.zeros((n, ops.q8_width(k)), dtype=torch.uint8, device=device)
+    at = 0
+    for p in parts:
+        codes[at: at + p.shape[0], :k] = p.codes.view(torch.uint8).to(device)
+        at += p.shape[0]
+    return ops.Q8Weight(codes.view(torch.float8_e4m3fn), torch.cat([p.scales for p in parts]).to(device).contiguous())

@@ -18,7 +18,7 @@ import torch
 _DTYPES = {
     "F64": (torch.float64, 8), "F32": (torch.float32, 4), "F16": (torch.float16, 2), "BF16": (torch.bfloat16, 2),
     "I64": (torch.int64, 8), "I32": (torch.int32, 4), "I16": (torch.int16, 2), "I8": (torch.int8, 1),
-    "U8": (torch.uint8, 1), "BOOL": (torch.bool, 1),
+    "U8": (torch.uint8, 1), "BOOL": (torch.bool, 1), "F8_E4M3": (torch.float8_e4m3fn, 1),
 }
 _NAMES = {v[0]: k for k, v in _DTYPES.items()}
 
