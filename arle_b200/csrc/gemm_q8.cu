@@ -83,14 +83,11 @@ int product(const void* x, const void* sx, const void* w, const float* sw, void*
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   // 16 warps to a tile where all tiles are under way at once, else eight: us for one row with 16 warps, eight in three blocks an SM and eight in four, 4,096 x 12,288 (256
   // tiles) 10.3, 13.4 and 15.0; 6,144 x 4,096 (384) 7.1, 6.1 and 6.7; 24,576 x 4,096 (1,536) 19.8, 20.1 and 18.6
-  auto go = [&](auto kern, int warps) {
-    launch_early(kern, dim3(tiles, tiles_m), dim3(32 * warps), 0, s, 1, (const uint8_t*)x, (const uint8_t*)sx, (const uint8_t*)w, sw, (OutT*)out, ldo, M, N, kb);
-    return launch_status();
-  };
   const long blocks = (long)tiles * tiles_m;
-  if (blocks <= 2l * sms) return go(gemm_q8_rows_kernel<16, 2, OutT>, 16);
-  if (blocks <= 3l * sms) return go(gemm_q8_rows_kernel<8, 3, OutT>, 8);
-  return go(gemm_q8_rows_kernel<8, 4, OutT>, 8);
+  const int warps = blocks <= 2l * sms ? 16 : 8;
+  auto kern = blocks <= 2l * sms ? gemm_q8_rows_kernel<16, 2, OutT> : blocks <= 3l * sms ? gemm_q8_rows_kernel<8, 3, OutT> : gemm_q8_rows_kernel<8, 4, OutT>;
+  launch_early(kern, dim3(tiles, tiles_m), dim3(32 * warps), 0, s, 1, (const uint8_t*)x, (const uint8_t*)sx, (const uint8_t*)w, sw, (OutT*)out, ldo, M, N, kb);
+  return launch_status();
 }
 
 }  // namespace

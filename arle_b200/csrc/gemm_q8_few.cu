@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
   // copies may still be under way where a wait ran out: every one is counted on a barrier of this block
   __syncthreads();
   if (*aborted && warp == kProducer && lane == 0)
-    for (int s = 0; s < STAGES; ++s) mbar_wait_plain(full0 + 8 * s, 0), mbar_wait_plain(full0 + 8 * s, 1);
+    for (int s = 0; s < STAGES; ++s) mbar_wait_plain(smem_addr(&full_bar[s]), 0), mbar_wait_plain(smem_addr(&full_bar[s]), 1);
   if (*aborted) __syncthreads();
 
   // the group of rows 4q .. 4q + 3 is added up by block q % parts of the cluster, as its group q / parts

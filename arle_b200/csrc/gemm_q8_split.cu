@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_split_kernel(const __grid
   // copies may still be under way where a wait ran out: every one is counted on a barrier of this SM
   __syncthreads();
   if (*aborted && warp == kProducer && lane == 0)
-    for (int s = 0; s < kStages; ++s) mbar_wait_plain(full0 + 8 * s, 0), mbar_wait_plain(full0 + 8 * s, 1);
+    for (int s = 0; s < kStages; ++s) mbar_wait_plain(smem_addr(&full_bar[s]), 0), mbar_wait_plain(smem_addr(&full_bar[s]), 1);
   if (*aborted) __syncthreads();
 
   if (parts > 1) {
