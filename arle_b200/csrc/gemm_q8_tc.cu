@@ -208,17 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_
       for (int i = 0; i < 32; ++i) acc[0][i] = acc[1][i] = 0;
       uint32_t sx_next = sxr[0];
       float w0_next = sw0[0], w1_next = sw1[0];
-#pragma unroll 1
-      for (int b = 0; b < kb; ++b, ++done) {
-        const uint32_t buf = done & 1, src = lanes + buf * BN;
-        const float fx = __uint_as_float(sx_next << 23);
-        const uint64_t f[2] = {both(fx * w0_next), both(fx * w1_next)};
-        if (b + 1 < kb) sx_next = sxr[b + 1], w0_next = sw0[b + 1], w1_next = sw1[b + 1];
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(acc_full0 + 8 * buf, (done >> 1) & 1, aborted))) {
-          abort_flag = 1;
-          lost = true;
-          break;
-        }
+      auto block = [&](uint32_t src, uint32_t full, uint32_t phase, uint32_t empty, uint64_t f0, uint64_t f1) {
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(full, phase, aborted))) return false;
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -226,14 +217,27 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_
           tmem_ld32(src + h * 128, r[0]);
           tmem_ld32(src + h * 128 + 32, r[1]);
           tmem_ld_wait(r[0]);
-          tmem_ld_wait(r[1]);
+          asm volatile("" : "+r"(r[1][0]), "+r"(r[1][1]), "+r"(r[1][2]), "+r"(r[1][3]), "+r"(r[1][4]), "+r"(r[1][5]), "+r"(r[1][6]), "+r"(r[1][7]), "+r"(r[1][8]), "+r"(r[1][9]), "+r"(r[1][10]), "+r"(r[1][11]), "+r"(r[1][12]), "+r"(r[1][13]), "+r"(r[1][14]), "+r"(r[1][15]), "+r"(r[1][16]), "+r"(r[1][17]), "+r"(r[1][18]), "+r"(r[1][19]), "+r"(r[1][20]), "+r"(r[1][21]), "+r"(r[1][22]), "+r"(r[1][23]), "+r"(r[1][24]), "+r"(r[1][25]), "+r"(r[1][26]), "+r"(r[1][27]), "+r"(r[1][28]), "+r"(r[1][29]), "+r"(r[1][30]), "+r"(r[1][31]) :: "memory");
           if (h == 1) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_relaxed(acc_empty_leader + 8 * buf);
+            if (lane == 0) mbar_arrive_relaxed(empty);
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) fma2(acc[h][i], r[i >> 4][2 * (i & 15)], r[i >> 4][2 * (i & 15) + 1], f[h]);
+          for (int i = 0; i < 32; ++i) fma2(acc[h][i], r[i >> 4][2 * (i & 15)], r[i >> 4][2 * (i & 15) + 1], h ? f1 : f0);
+        }
+        return true;
+      };
+#pragma unroll 1
+      for (int b = 0; b < kb; ++b, ++done) {
+        const uint32_t buf = done & 1;
+        const float fx = __uint_as_float(sx_next << 23);
+        const uint64_t f0 = both(fx * w0_next), f1 = both(fx * w1_next);
+        if (b + 1 < kb) sx_next = sxr[b + 1], w0_next = sw0[b + 1], w1_next = sw1[b + 1];
+        if (!block(lanes + buf * BN, acc_full0 + 8 * buf, (done >> 1) & 1, acc_empty_leader + 8 * buf, f0, f1)) {
+          abort_flag = 1;
+          lost = true;
+          break;
         }
       }
       if (lost) break;

@@ -142,7 +142,7 @@ _SIGNATURES = {
     "arle_act_mul_q8": [_P, _P, _P, _I, _I, _I, _P],
     "arle_gemm_q8": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P],
     "arle_gemm_q8_pair": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P, _P],
-    "arle_gemm_q8_split": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _P, _P],
+    "arle_gemm_q8_split": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _I, _P, _P],
     "arle_gemm_q8_split_clusters": [_I],
     "arle_gemm_q8_few": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _P, _P],
     "arle_gemm_q8_pair_gated": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
@@ -2806,8 +2806,8 @@ def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
         code = lib.arle_gemm_q8(*args, stream)
     elif kind == "few":
         code = lib.arle_gemm_q8_few(*args, parts, _error_word(device), stream)
-    elif kind == "split":
-        code = lib.arle_gemm_q8_split(*args, parts, _error_word(device), stream)
+    elif kind != "pair":
+        code = lib.arle_gemm_q8_split(*args, parts, 2 if kind == "split2" else 1, _error_word(device), stream)
     else:
         code = lib.arle_gemm_q8_pair(*args, _error_word(device), stream)
     _check(code, "gemm_q8")
@@ -2823,6 +2823,10 @@ def _q8_clusters(parts: int, device: int) -> int:
     return n
 
 
+def _q8_pair_cost(M: int, N: int, kb: int, sms: int) -> float:
+    return -(-(-(-N // 256) * -(-M // 256)) // (sms // 2)) * (kb * 0.42 + 3.5) + 3.0
+
+
 @functools.lru_cache(maxsize=4096)
 def _q8_route(M: int, N: int, kb: int, device: int):
     """(kernel, parts that a tile's k is cut into, estimated us) of a product, by its sizes alone.  Figures in us, alone in a graph:
@@ -2832,8 +2836,9 @@ def _q8_route(M: int, N: int, kb: int, device: int):
     * "few", up to 64 rows, bound by w's bytes.  Parts: the cheapest of what runs at once, 0.3 a block of k (0.45 for more than 32 rows), 0.1 (0.25) a part, 1.5 a
       wave, 0.9 where two blocks share an SM.  32 tiles of 32 blocks of k, one row: 2, 4, 6 and 8 parts 7.9, 6.3, 6.6 and 7.2; 48 tiles 8.9, 8.0, 10.2 (more than
       run at once) and 9.9, five 7.5; 32 tiles of 96 blocks 17.4, 12.4, 11.9 and 10.9;
-    * "split" and "pair" for more rows: one SM to a tile of 128 x 128, 0.32 a block of k, and two to one of 256 x 256, 0.42.  4,096 x 4,096: 128 rows 9.6 with four
-      parts and 18.2, 512 rows 15.0 and 18.7, 1,024 rows 29.7 and 19.8; 333 rows of 5,120 x 25,600 76 and 81."""
+    * "split", "split2" and "pair" for more rows: one SM to a tile of 128 x 128, 0.32 a block of k, or of 128 x 256, 0.45, and two to one of 256 x 256, 0.42; some 4
+      a wave, and what the parts cost to be put together.  4,096 x 4,096: 128 rows 10.4 with four parts, 14.3 as "split2" and 18.1 as "pair", 512 rows 15.8, 17.6 and
+      18.7, 1,024 rows 30.2, 20.8 and 19.8; 333 rows of 5,120 x 25,600 74.5, 60.8 with two parts and 80.5; 128 rows of 24,576 x 4,096 33.7, 25.4 and 38.5."""
     sms = sm_count(device)
     if M <= 8 and kb <= 128:
         return "rows", 1, 0.0
@@ -2850,14 +2855,15 @@ def _q8_route(M: int, N: int, kb: int, device: int):
             if best is None or cost < best[2]:
                 best = ("few", parts, cost)
         return best
-    tiles *= -(-M // 128)
-    best = ("pair", 1, -(-(-(-N // 256) * -(-M // 256)) // (sms // 2)) * kb * 0.42 + 6.0)
-    for parts in (1, 2, 3, 4, 5, 6, 7, 8):
-        if parts > kb:
-            break
-        cost = -(-tiles // _q8_clusters(parts, device)) * (-(-kb // parts) * 0.32 + 4.0) + 0.7 + (1.2 + 0.65 * parts if parts > 1 else 0.0)
-        if cost < best[2]:
-            best = ("split", parts, cost)
+    best = ("pair", 1, _q8_pair_cost(M, N, kb, sms))
+    for kind, width, block, join, part in (("split", 1, 0.32, 1.2, 0.65), ("split2", 2, 0.45, 4.5, 0.7)):
+        count = -(-tiles // width) * -(-M // 128)
+        for parts in (1, 2, 3, 4, 5, 6, 7, 8):
+            if parts > kb:
+                break
+            cost = -(-count // _q8_clusters(parts, device)) * (-(-kb // parts) * block + 4.0 + (join + part * parts if parts > 1 else 0.0)) + 0.7
+            if cost < best[2]:
+                best = (kind, parts, cost)
     return best
 
 
@@ -2882,11 +2888,10 @@ def act_mul_q8(gate_up, codes, scales, activation: str = "silu") -> None:
 @functools.lru_cache(maxsize=4096)
 def _q8_gate_in_pair(M: int, N: int, kb: int, device: int) -> bool:
     """Whether a packed product's gate goes into the epilogue of the kernel for pairs of SMs, which writes codes: where the other kernels, another launch and
-    the sums' way through memory (float32, written and read) take longer by estimate.  24,576 x 4,096, us: 64 rows 33.9 in one and 28.6 in two, 128 rows 40 and 41."""
+    the sums' way through memory (float32, written and read) take longer by estimate.  24,576 x 4,096, us: 64 rows 33.7 in one and 25.2 in two, 128 rows 34.8 and 34.2, 200 rows 34.8 and 47.7."""
     if M <= 64 or device < 0:
         return False
-    pair = -(-(-(-N // 256) * -(-M // 256)) // (sm_count(device) // 2)) * kb * 0.42 + 6.0
-    return pair <= _q8_route(M, N, kb, device)[2] + 2.0 + 8.0 * M * N / 5.0e6
+    return _q8_pair_cost(M, N, kb, sm_count(device)) <= _q8_route(M, N, kb, device)[2] + 2.0 + 8.0 * M * N / 5.0e6
 
 
 def gate_needs_sums_q8(M: int, w: Q8Weight) -> bool:
