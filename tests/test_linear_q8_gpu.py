@@ -120,7 +120,7 @@ def _near_codes(codes, scales, y, rel):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32, None])
-@pytest.mark.parametrize("m,h", [(1, 1), (1, 128), (3, 127), (5, 1000), (8, 4096), (2, 5120), (3, 1030), (300, 256), (2, 16384), (2, 16500), (1, 20000)])
+@pytest.mark.parametrize("m,h", [(1, 1), (1, 128), (3, 127), (5, 1000), (8, 4096), (2, 5120), (3, 1030), (300, 256), (2, 16384), (2, 16500), (1, 20000), (2050, 128), (2048, 1000), (2600, 516), (2100, 1280)])
 def test_rmsnorm(m, h, dtype):
     g = torch.Generator().manual_seed(m + h)
     resid, gain = _x(m, h, h, 1.0), 1 + 0.3 * torch.randn(h, generator=g)
