@@ -52,8 +52,14 @@ __device__ __forceinline__ float finite_or_nan(float v) { return abs_bits(v) < k
 __device__ __forceinline__ float inverse_scale(float s) { return __uint_as_float((254u << 23) - __float_as_uint(s)); }      // of a power of two in 2^-100 .. 2^119
 __device__ __forceinline__ uint8_t exponent_byte(float s) { return (uint8_t)(__float_as_uint(s) >> 23); }                   // the same as e8m0
 
-// The gates of a feed-forward in float32.  The quotient is good to two steps (fdividef gives 0 beyond 2^126, which is what silu is there).
-__device__ __forceinline__ float q8_silu(float g) { return __fdividef(g, 1.0f + expf(-g)); }
+// The gates of a feed-forward in float32.  Silu's exponential is 2^(-g log2 e) by the special function unit: off by |g| 2^-24 of itself beside its two steps, as much
+// as sums of some thousand products are (expf, which keeps that, cost the gated product of 4,096 rows 2 % of its time); the quotient is good to two steps and 0
+// beyond 2^126, which is what silu is there.
+__device__ __forceinline__ float q8_silu(float g) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  return __fdividef(g, 1.0f + e);
+}
 __device__ __forceinline__ float q8_gelu_tanh(float g) { return 0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))); }
 
 __device__ __forceinline__ float q8_float(uint8_t code) { return q8_float2(code).x; }
