@@ -325,7 +325,7 @@ int quantize_rows(const void* x, long row_stride, void* codes, void* scales, int
   const long groups = (long)M * kb, blocks = (groups + per_block - 1) / per_block;
   if (groups + per_block > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
   const bool fast = K % V == 0 && aligned16(x) && (M == 1 || row_stride % V == 0);
-  launch_kernel_as(M <= kEarlyRows || (pdl_enabled() & 1) != 0, fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
+  launch_early(fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
                 (uint8_t*)codes, (uint8_t*)scales, (uint32_t)groups, K, (uint32_t)kb);
   return launch_status();
 }
@@ -336,7 +336,7 @@ int quantize_weight(const void* w, long row_stride, void* codes, void* scales, i
   const int kb = blocks_of(K), nb = blocks_of(N);
   if (nb > 65535) return ARLE_E_UNSUPPORTED;
   const bool fast = K % V == 0 && aligned16(w) && (N == 1 || row_stride % V == 0);
-  launch_kernel(fast ? quantize_weight_kernel<T, true> : quantize_weight_kernel<T, false>, dim3(kb, nb), dim3(256), 0, s, 1, (const T*)w, row_stride,
+  launch_early(fast ? quantize_weight_kernel<T, true> : quantize_weight_kernel<T, false>, dim3(kb, nb), dim3(256), 0, s, 1, (const T*)w, row_stride,
                 (uint8_t*)codes, (float*)scales, N, K, kb);
   return launch_status();
 }
@@ -354,7 +354,7 @@ int rmsnorm(const float* resid, const void* delta, const float* gain, float* sum
     threads = 32 * ((kb + per - 1) / per);
     kern = per == 1 ? rmsnorm_q8_kernel<TA, 1, 1024> : per == 2 ? rmsnorm_q8_kernel<TA, 2, 1024> : threads <= 320 ? rmsnorm_q8_kernel<TA, 4, 320> : rmsnorm_q8_kernel<TA, 4, 1024>;
   }
-  launch_kernel_as(M <= kEarlyRows || (pdl_enabled() & 1) != 0, kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
+  launch_early(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
                 delta_scale);
   return launch_status();
 }

@@ -2595,7 +2595,8 @@ def q8_width(k: int) -> int:
 class Q8Weight:
     """A weight [out_features, in_features] in 8 bits: ``codes`` contiguous float8_e4m3fn [N, q8_width(K)], zero from column K on, and ``scales`` contiguous
     float32 [ceil(N / 128), ceil(K / 128)], positive, one for each block of 128 x 128; a number is code * scale.  ``quantize_weight_q8`` makes both from a
-    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two)."""
+    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two).  Products may ask for a weight before the kernel in front of
+    them in the stream has ended, so it is written by ``quantize_weight_q8``, by torch or by a copy, not by another of this package's kernels."""
 
     __slots__ = ("codes", "scales", "shape")
 
@@ -2607,6 +2608,8 @@ class Q8Weight:
             raise KernelError(f"Q8Weight: scales must be contiguous float32 {want} beside the codes, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
         if codes.data_ptr() % 16:
             raise KernelError("Q8Weight: codes must start on a 16-byte boundary")
+        if codes.is_cuda:
+            _error_word(codes.get_device())          # made here and not by a first product, which may be one that a graph captures
         self.codes, self.scales, self.shape = codes, scales, codes.shape
 
     def bytes(self) -> int:
@@ -2666,16 +2669,23 @@ def _rows_q8_for(what: str, codes, scales, M: int, K: int) -> None:
         _bad_rows_q8(what, codes, scales, (M, kb << 7))
 
 
+_current_device, _raw_stream = (getattr(torch._C, n, None) for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
+_TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _misplaced(what: str, *tensors):
+    """Says what is wrong with the devices of these tensors."""
+    _placed(what, tensors)
+    raise KernelError(f"{what}: tensors on different devices")
+
+
 def _on_device(what: str, device: int, *tensors) -> None:
     """Checks that all tensors are on the device of this number and that it is the current one."""
-    if device >= 0 and torch._C._cuda_getDevice() == device:
-        for t in tensors:
-            if t.get_device() != device:
-                break
-        else:
-            return
-    _placed(what, tensors)                # says what is wrong
-    raise KernelError(f"{what}: tensors on different devices")
+    for t in tensors:
+        if t.get_device() != device:
+            _misplaced(what, *tensors)
+    if device < 0 or _current_device() != device:
+        _misplaced(what, *tensors)
 
 
 def _misaligned(what: str):
@@ -2699,23 +2709,32 @@ def quantize_q8(x, codes, scales) -> None:
 
     The scale of a row's 128 numbers is the least power of two s with max |x| <= 448 * s (at least 2^-100; at most 2^119, beyond which numbers end at
     448 * 2^119), a code is x / s rounded to nearest even.  Infinities and NaN become NaN and do not count for the scale.  Columns from K on are zero."""
-    if x.dim() != 2:
+    global _LAUNCHES
+    shape = x.shape
+    if len(shape) != 2 or shape[1] == 0:
         raise KernelError(f"quantize_q8: x must be [M, K], got {tuple(x.shape)}")
-    M, K = x.shape
-    if K == 0:
-        raise KernelError(f"quantize_q8: x must be [M, K], got {tuple(x.shape)}")
-    _rows_q8_for("quantize_q8", codes, scales, M, K)
+    M, K = shape
+    kb = (K + 127) >> 7
+    if not (codes.dtype is _E4M3 and scales.dtype is _E8M0 and codes.shape == (M, kb << 7) and scales.shape == (M, kb) and codes.is_contiguous()
+            and scales.is_contiguous()):
+        _bad_rows_q8("quantize_q8", codes, scales, (M, kb << 7))
     stride, unit = x.stride()
     if unit != 1 and K > 1 and M:
         raise KernelError("quantize_q8: rows of x must have unit inner stride")
-    dt = _dt(x)
+    dt = _TYPE_CODES.get(x.dtype)
+    if dt is None:
+        _dt(x)
     device = x.get_device()
-    _on_device("quantize_q8", device, x, codes, scales)
+    if device < 0 or codes.get_device() != device or scales.get_device() != device or _current_device() != device:
+        _misplaced("quantize_q8", x, codes, scales)
     cp = codes.data_ptr()
     if cp & 15:
         _misaligned("quantize_q8")
     if M:
-        _check((_LIB or library()).arle_quantize_q8(x.data_ptr(), dt, stride, cp, scales.data_ptr(), M, K, torch._C._cuda_getCurrentRawStream(device)), "quantize_q8")
+        code = (_LIB or library()).arle_quantize_q8(x.data_ptr(), dt, stride, cp, scales.data_ptr(), M, K, _raw_stream(device))
+        if code:
+            _check(code, "quantize_q8")
+        _LAUNCHES += 1
 
 
 def quantize_weight_q8(w, codes, scales) -> Q8Weight:
@@ -2743,56 +2762,73 @@ def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, de
     """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's float32 numbers as
     ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.  ``sum_out`` (float32 [M, H]: ``resid`` itself or a
     buffer that does not overlap it) gets x; None: x is kept nowhere."""
-    f32 = torch.float32
-    if resid.dim() != 2 or resid.dtype is not f32 or not resid.is_contiguous():
+    global _LAUNCHES
+    f32, shape = torch.float32, resid.shape
+    if len(shape) != 2 or resid.dtype is not f32 or not resid.is_contiguous():
         raise KernelError("rmsnorm_q8: the residual must be contiguous float32 [M, H]")
-    M, H = shape = resid.shape
+    M, H = shape
     if H == 0 or weight.dtype is not f32 or weight.shape != (H,) or not weight.is_contiguous():
         raise KernelError("rmsnorm_q8: the weight must be contiguous float32 [H], H at least 1")
-    _rows_q8_for("rmsnorm_q8", codes, scales, M, H)
+    kb = (H + 127) >> 7
+    if not (codes.dtype is _E4M3 and scales.dtype is _E8M0 and codes.shape == (M, kb << 7) and scales.shape == (M, kb) and codes.is_contiguous()
+            and scales.is_contiguous()):
+        _bad_rows_q8("rmsnorm_q8", codes, scales, (M, kb << 7))
     device = resid.get_device()
+    here = device >= 0 and weight.get_device() == device and codes.get_device() == device and scales.get_device() == device and _current_device() == device
+    given = [resid, weight, codes, scales]
     dp = so = None
     dt = 0
     if delta is not None:
         if delta.shape != shape or not delta.is_contiguous():
             raise KernelError("rmsnorm_q8: delta must be contiguous and of the residual's shape")
-        dt, dp = _dt(delta), delta.data_ptr()
-    if sum_out is not None and (sum_out.shape != shape or sum_out.dtype is not f32 or not sum_out.is_contiguous()):
-        raise KernelError("rmsnorm_q8: sum_out must be contiguous float32 like the residual")
-    given = (resid, weight, codes, scales)
-    if delta is not None:
-        given += (delta,)
-    if sum_out is not None:
-        given += (sum_out,)
-    _on_device("rmsnorm_q8", device, *given)
+        dt = _TYPE_CODES.get(delta.dtype)
+        if dt is None:
+            _dt(delta)
+        here = here and delta.get_device() == device
+        given.append(delta)
+        dp = delta.data_ptr()
     rp, cp = resid.data_ptr(), codes.data_ptr()
     if sum_out is not None:
+        if sum_out is not resid:
+            if sum_out.shape != shape or sum_out.dtype is not f32 or not sum_out.is_contiguous():
+                raise KernelError("rmsnorm_q8: sum_out must be contiguous float32 like the residual")
+            here = here and sum_out.get_device() == device
+            given.append(sum_out)
         so = sum_out.data_ptr()
-        if so != rp and abs(so - rp) < 4 * M * H:
-            raise KernelError("rmsnorm_q8: sum_out overlaps the residual without being it")
+    if not here:
+        _misplaced("rmsnorm_q8", *given)
+    if so is not None and so != rp and abs(so - rp) < 4 * M * H:
+        raise KernelError("rmsnorm_q8: sum_out overlaps the residual without being it")
     if cp & 15:
         _misaligned("rmsnorm_q8")
     if M:
-        _check((_LIB or library()).arle_rmsnorm_q8(rp, dp, dt, weight.data_ptr(), so, cp, scales.data_ptr(), M, H, eps, delta_scale,
-                                                   torch._C._cuda_getCurrentRawStream(device)), "rmsnorm_q8")
+        code = (_LIB or library()).arle_rmsnorm_q8(rp, dp, dt, weight.data_ptr(), so, cp, scales.data_ptr(), M, H, eps, delta_scale, _raw_stream(device))
+        if code:
+            _check(code, "rmsnorm_q8")
+        _LAUNCHES += 1
 
 
 def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     """out[M, N] = x . w^T for rows in 8 bits (``quantize_q8``, ``rmsnorm_q8``, ``gemm_act_mul_q8``) and a weight in 8 bits; out float32 or bfloat16, unit inner
     stride, any row stride.  Every block of 128 numbers of k is summed on the tensor cores, scaled by the row's and the weight block's scale and added up in
-    float32; the product of the two scales should be a normal float32 number.  The result of a row does not depend on the other rows' numbers (on how many there
+    float32; the product of the two scales should be a normal float32 number (rows' scales are 2^-100 to 2^119 where an operator made them).  The result of a row does not depend on the other rows' numbers (on how many there
     are, in its last bits)."""
+    global _LAUNCHES
     M, K = _rows_q8("gemm_q8", codes, scales)
     wc, ws = w.codes, w.scales
-    N = w.shape[0]
-    if w.shape[1] != K or out.shape != (M, N):
+    N, wk = w.shape
+    if wk != K or out.shape != (M, N):
         raise KernelError(f"gemm_q8: shapes x {tuple(codes.shape)} w {tuple(w.shape)} out {tuple(out.shape)}")
     stride, unit = out.stride()
-    if unit != 1 and N > 1 and M:
-        raise KernelError("gemm_q8: rows of out must have unit inner stride")
-    dt = _dt(out)
+    if M and ((unit != 1 and N > 1) or (stride < N and M > 1)):
+        raise KernelError("gemm_q8: rows of out must have unit inner stride and not overlap")
+    dt = _TYPE_CODES.get(out.dtype)
+    if dt is None:
+        _dt(out)
     device = out.get_device()
-    _on_device("gemm_q8", device, codes, scales, wc, ws, out)
+    if (device < 0 or codes.get_device() != device or scales.get_device() != device or wc.get_device() != device or ws.get_device() != device
+            or _current_device() != device):
+        _misplaced("gemm_q8", codes, scales, wc, ws, out)
     xp = codes.data_ptr()
     if xp & 15:
         _misaligned("gemm_q8")
@@ -2800,17 +2836,20 @@ def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
         return
     kb = K >> 7
     kind, parts, _ = _q8_route(M, N, kb, device) if _KERNEL_SET == "fast" else ("rows", 1, 0.0)
-    args = (xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), out.data_ptr(), dt, stride, M, N, kb)
-    lib, stream = _LIB or library(), torch._C._cuda_getCurrentRawStream(device)
+    lib, stream = _LIB or library(), _raw_stream(device)
     if kind == "rows":
-        code = lib.arle_gemm_q8(*args, stream)
-    elif kind == "few":
-        code = lib.arle_gemm_q8_few(*args, parts, _error_word(device), stream)
-    elif kind != "pair":
-        code = lib.arle_gemm_q8_split(*args, parts, 2 if kind == "split2" else 1, _error_word(device), stream)
+        code = lib.arle_gemm_q8(xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), out.data_ptr(), dt, stride, M, N, kb, stream)
     else:
-        code = lib.arle_gemm_q8_pair(*args, _error_word(device), stream)
-    _check(code, "gemm_q8")
+        args = (xp, scales.data_ptr(), wc.data_ptr(), ws.data_ptr(), out.data_ptr(), dt, stride, M, N, kb)
+        if kind == "few":
+            code = lib.arle_gemm_q8_few(*args, parts, _error_word(device), stream)
+        elif kind != "pair":
+            code = lib.arle_gemm_q8_split(*args, parts, 2 if kind == "split2" else 1, _error_word(device), stream)
+        else:
+            code = lib.arle_gemm_q8_pair(*args, _error_word(device), stream)
+    if code:
+        _check(code, "gemm_q8")
+    _LAUNCHES += 1
 
 
 @functools.lru_cache(maxsize=None)

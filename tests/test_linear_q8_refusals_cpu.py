@@ -80,7 +80,7 @@ def test_norm(changed):
         _norm(**changed)
 
 
-@pytest.mark.parametrize("changed", ROWS + [dict(out=z(4, 299)), dict(out=z(3, 300)), dict(out=z(300, 4).t()), dict(out=z(4, 300, dtype=torch.float16)), dict(w=_weight(300, 384))])
+@pytest.mark.parametrize("changed", ROWS + [dict(out=z(4, 299)), dict(out=z(3, 300)), dict(out=z(300, 4).t()), dict(out=z(1, 300).expand(4, 300)), dict(out=z(4, 300, dtype=torch.float16)), dict(w=_weight(300, 384))])
 def test_product(changed):
     with pytest.raises(ops.KernelError):
         _product(**changed)
@@ -128,3 +128,15 @@ def test_pack(i, k):
         assert torch.equal(rows[:i], refs.weight_values(refs.host(q.codes), refs.host(q.scales))) and (rows[i:] == 0).all()
     with pytest.raises(ops.KernelError):
         ops.pack_gate_up_q8(gate, ops.Q8Weight(z(i + 1, k, dtype=F8), z(-(-(i + 1) // 128), k // 128)))
+
+
+def test_first_rows():
+    c, s = refs.quantize_weight(torch.randn(300, 256, generator=torch.Generator().manual_seed(0)).double())
+    q = ops.Q8Weight(c.to(F8), s.float())
+    for n in (1, 128, 129, 300):
+        part = q.first_rows(n)
+        assert torch.equal(refs.weight_values(refs.host(part.codes), refs.host(part.scales)), refs.weight_values(c, s)[:n])
+
+
+def test_widths():
+    assert [ops.q8_width(k) for k in (1, 127, 128, 129, 4096)] == [128, 128, 128, 256, 4096]
