@@ -5,8 +5,8 @@
 // lanes x 256 columns is one block of k (four tcgen05.mma of 32), two of them take turns in the 512 columns of tensor memory, and the epilogue warps add
 // block after block into registers, acc += (sx[row] sw[block of columns]) * sum.  A lane is a row of x and 128 columns are one block of w, so that
 // factor is one number a thread and 128 columns.  A block's products take the tensor cores 512 clocks, reading and adding its sums takes the warps some 270
-// beside one another, handing accumulators back and forth between the two SMs the rest: 760 clocks a block (4,096 rows of 4,096 x 12,288).
-// 4,096 rows of 4,096 x 12,288 184 us alone (2.2 PFLOP/s), some 220 back to back, where 1,000 W hold the clock at 1.3 GHz.
+// beside one another, handing accumulators back and forth between the two SMs the rest: 670 to 790 clocks a block (4,096 rows of 4,096 x 12,288).
+// 4,096 rows of 4,096 x 12,288 181 us alone (2.3 PFLOP/s), 214 back to back, where 1,000 W hold the clock at 1.4 GHz; gated, 24,576 x 4,096, 351 and 408.
 //
 // Per CTA, by warp:
 //   warps 0-7        : epilogue of the CTA's 128 rows; warp i reads lanes 32 (i % 4) .. + 31, of columns 64 h .. 64 h + 63 and 128 + 64 h .. (h = i / 4).  Gated,
@@ -41,7 +41,7 @@ __device__ __forceinline__ float2 halves(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-// Registers move from the third group of four warps to the first two, which keep 128 sums a thread: 2 x 240 + 72 = 3 x 168, what the block is launched with.
+// Registers move from the third group of four warps to the first two, which keep 128 sums a thread: 2 x 216 + 72 = 3 x 168, what the block is launched with.
 __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n"); }
 __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n"); }
 

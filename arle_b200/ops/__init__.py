@@ -2595,8 +2595,8 @@ def q8_width(k: int) -> int:
 class Q8Weight:
     """A weight [out_features, in_features] in 8 bits: ``codes`` contiguous float8_e4m3fn [N, q8_width(K)], zero from column K on, and ``scales`` contiguous
     float32 [ceil(N / 128), ceil(K / 128)], positive, one for each block of 128 x 128; a number is code * scale.  ``quantize_weight_q8`` makes both from a
-    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two).  Products may ask for a weight before the kernel in front of
-    them in the stream has ended, so it is written by ``quantize_weight_q8``, by torch or by a copy, not by another of this package's kernels."""
+    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two).  Products may ask for a weight before the kernel in
+    front of them in the stream has ended, so it is written by ``quantize_weight_q8``, by torch or by a copy, not by another of this package's kernels."""
 
     __slots__ = ("codes", "scales", "shape")
 
@@ -2760,8 +2760,8 @@ def quantize_weight_q8(w, codes, scales) -> Q8Weight:
 
 def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, delta_scale: float = 1.0) -> None:
     """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's float32 numbers as
-    ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.  ``sum_out`` (float32 [M, H]: ``resid`` itself or a
-    buffer that does not overlap it) gets x; None: x is kept nowhere."""
+    ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.
+    ``sum_out`` (float32 [M, H]: ``resid`` itself or a buffer that overlaps no other argument) gets x; None: x is kept nowhere."""
     global _LAUNCHES
     f32, shape = torch.float32, resid.shape
     if len(shape) != 2 or resid.dtype is not f32 or not resid.is_contiguous():
@@ -2811,8 +2811,8 @@ def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, de
 def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     """out[M, N] = x . w^T for rows in 8 bits (``quantize_q8``, ``rmsnorm_q8``, ``gemm_act_mul_q8``) and a weight in 8 bits; out float32 or bfloat16, unit inner
     stride, any row stride.  Every block of 128 numbers of k is summed on the tensor cores, scaled by the row's and the weight block's scale and added up in
-    float32; the product of the two scales should be a normal float32 number (rows' scales are 2^-100 to 2^119 where an operator made them).  The result of a row does not depend on the other rows' numbers (on how many there
-    are, in its last bits)."""
+    float32; the product of the two scales should be a normal float32 number (rows' scales that an operator made are 2^-100 to 2^119).  The result of a row
+    does not depend on the other rows' numbers (on how many there are, in its last bits)."""
     global _LAUNCHES
     M, K = _rows_q8("gemm_q8", codes, scales)
     wc, ws = w.codes, w.scales

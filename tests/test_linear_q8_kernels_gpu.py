@@ -1,4 +1,8 @@
 """Every kernel of the 8-bit products with every number of parts, whatever the sizes would choose, and what they share: shared workspaces of captured graphs, streams."""
+import subprocess
+import sys
+import threading
+
 import pytest
 import torch
 
@@ -199,3 +203,73 @@ def test_offsets_beyond_32_bits():
     ops.gemm_q8(xs[:64], ss[:64], q, first)
     # both are roundings of sums in other orders of the same 128 products
     assert torch.equal(out[-8:], out[m - 8 - 64 * 10: m - 64 * 10]) and ((out[:64].float() - first.float()).abs() <= 2.0 ** -7 * first.float().abs() + 1e-3).all()
+
+
+def test_two_threads_at_once():
+    """Calls from two threads, a stream each."""
+    sizes = ((4, 1000, 2048), (150, 640, 1024))
+    made = [_operands(*size, 3) for size in sizes]
+    want = []
+    for (m, n, _), (x, sx, q) in zip(sizes, made):
+        want.append(torch.empty((m, n), device=DEV))
+        ops.gemm_q8(x, sx, q, want[-1])
+    torch.cuda.synchronize()
+    same = [None, None]
+
+    def work(j):
+        (m, n, _), (x, sx, q) = sizes[j], made[j]
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [torch.empty((m, n), device=DEV) for _ in range(40)]
+            for out in outs:
+                ops.gemm_q8(x, sx, q, out)
+            torch.cuda.current_stream().synchronize()
+            same[j] = all(torch.equal(out, want[j]) for out in outs)
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True, True]
+
+
+FIRST_CALLS = """
+import torch
+from arle_b200 import ops
+g = torch.Generator().manual_seed(0)
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+q = ops.Q8Weight(torch.randint(0, 100, (512, 1024), dtype=torch.uint8, generator=g).cuda().view(E4M3), torch.ones((4, 8), device="cuda"))
+x = torch.randn((300, 1024), generator=g).cuda()
+codes, scales = torch.empty((300, 1024), dtype=E4M3, device="cuda"), torch.empty((300, 8), dtype=torch.uint8, device="cuda").view(E8M0)
+gc, gs = torch.empty((300, 256), dtype=E4M3, device="cuda"), torch.empty((300, 2), dtype=torch.uint8, device="cuda").view(E8M0)
+sums = torch.empty((300, 512), device="cuda")
+outs = {m: torch.zeros((m, 512), device="cuda") for m in (1, 20, 130, 300)}
+torch.cuda.synchronize()
+
+def calls():
+    ops.quantize_q8(x, codes, scales)
+    for m, out in outs.items():
+        ops.gemm_q8(codes[:m], scales[:m], q, out)
+    ops.gemm_act_mul_q8(codes, scales, q, sums, gc, gs)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+graph.replay()
+torch.cuda.synchronize()
+kept = {m: out.clone() for m, out in outs.items()}
+gated = gc.view(torch.uint8).clone()
+calls()
+torch.cuda.synchronize()
+assert all(torch.equal(kept[m], out) and out.abs().max() > 0 for m, out in outs.items()) and torch.equal(gated, gc.view(torch.uint8))
+ops.check_errors(x.device)
+print("captured")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured():
+    """What a kernel's first launch needs (shared memory limits, how many clusters run, the error word) is there or may be had while a graph is captured."""
+    from pathlib import Path
+
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=Path(__file__).parent.parent, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
