@@ -4,10 +4,11 @@
 // power of two s with max |x| <= 448 s (2^-100 to 2^119), stored as its exponent (e8m0: exponent + 127); codes are rne(x / s).  Numbers that are not
 // finite do not count for the scale and become NaN: e4m3 has no infinities, and what was not finite must not come out of a product as if it were.
 // Weights: the same for blocks of 128 x 128, one float32 scale a block.
-// All are launched early: plain loads, and what a block loads is small beside what its neighbours have under way.  One token's codes 2.3 -> 1.9 us in a chain, those of
-// 6,001 tokens 30.8 -> 29.9, 24,576 x 4,096 numbers of a weight 47.2 -> 45.0, the norm of 5,003 rows 61.1 -> 59.4 (a weight's kernel lets nothing start before its end).
+// All are launched early: plain loads, and what a block loads is small beside what its neighbours have under way.  It saves one token's codes 0.4 us in a
+// chain, a weight of 24,576 x 4,096 2, the norm of 1,024 rows of 4,096 0.4 and that of 4,096 rows 0.9 (a weight's kernel lets nothing start before its end).
 // All four kernels read every number once, keep it in registers between the maximum and the rounding, and are bound by DRAM (few rows: by latency).
 #include "q8.cuh"
+#include "scan_utils.cuh"
 using namespace arle;
 
 namespace {
@@ -25,12 +26,8 @@ template <int LANES> __device__ __forceinline__ uint32_t lanes_max(uint32_t bits
   }
 }
 
-// The codes of a group that LANES lanes hold, V consecutive numbers each: returns the scale, words of four codes in `w`.
-template <int LANES, int V> __device__ __forceinline__ float group_codes(float (&v)[V], uint32_t (&w)[V / 4]) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int j = 0; j < V; ++j) most = max(most, abs_bits(v[j]));
-  most = lanes_max<LANES>(most);
+// The codes of a group that LANES lanes hold, V consecutive numbers each, from the bits of its largest: returns the scale, words of four codes in `w`.
+template <int LANES, int V> __device__ __forceinline__ float group_codes(float (&v)[V], uint32_t (&w)[V / 4], uint32_t most) {
   if (LANES == 32 ? most >= kInfBits : __any_sync(0xffffffffu, most >= kInfBits) != 0) {
     most = 0;
 #pragma unroll
@@ -42,6 +39,33 @@ template <int LANES, int V> __device__ __forceinline__ float group_codes(float (
   for (int j = 0; j < V / 4; ++j) w[j] = q8_codes4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
   return s;
 }
+
+template <int LANES, int V> __device__ __forceinline__ float group_codes(float (&v)[V], uint32_t (&w)[V / 4]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) most = max(most, abs_bits(v[j]));
+  return group_codes<LANES, V>(v, w, lanes_max<LANES>(most));
+}
+
+// 16 bytes of a row as they lie in memory, of which `left` numbers are there (the others are zero), and their largest without its sign: bfloat16 numbers two at a
+// time, `fold` brings the two together as the bits of a float32 number.
+template <typename T, bool ALIGNED> __device__ __forceinline__ uint4 load_words(const T* p, int left) {
+  if constexpr (ALIGNED) {
+    return left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+  } else {
+    constexpr int V = 16 / sizeof(T);
+    Pack<T, V> e;
+#pragma unroll
+    for (int j = 0; j < V; ++j) e.e[j] = j < left ? p[j] : from_f32<T>(0.f);
+    return *reinterpret_cast<const uint4*>(&e);
+  }
+}
+template <typename T> __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) { return sizeof(T) == 2 ? __vmaxu2(a, b) : max(a, b); }
+template <typename T> __device__ __forceinline__ uint32_t largest(uint4 q) {
+  constexpr uint32_t magnitude = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+  return largest<T>(largest<T>(q.x & magnitude, q.y & magnitude), largest<T>(q.z & magnitude, q.w & magnitude));
+}
+template <typename T> __device__ __forceinline__ uint32_t fold(uint32_t m) { return sizeof(T) == 2 ? max(m << 16, m & 0xffff0000u) : m; }
 
 // V numbers from p on, of which `left` are there (the others are zero).
 template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void load_numbers(const T* p, int left, float (&v)[V]) {
@@ -60,28 +84,40 @@ template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void load_
 
 // ------------------------------------------------------------------ rows
 // A lane takes 16 bytes of a group: a group is 16 lanes of bfloat16 or 32 of float32; it takes them of kAtOnce groups, which are under way together (one at a time
-// 6,001 rows of 8,192 bfloat16 took 37 us, so 28: 5.3 TB/s).  One row of 4,096 1.8 us alone.
+// 6,001 rows of 8,192 bfloat16 took 37 us, four 28), and stay as they lie in memory up to the rounding: maxima of two bfloat16 at a time, and a multiplication for
+// the division by the row's groups, 23.5: 6.4 TB/s.  One row of 4,096 1.5 us alone.
 constexpr int kAtOnce = 4;
 
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row_stride, uint8_t* codes, uint8_t* scales, uint32_t groups, int K, uint32_t kb) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row_stride, uint8_t* codes, uint8_t* scales, uint32_t groups, int K, uint32_t kb, uint32_t magic,
+                                                            int shift) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int V = 16 / sizeof(T), LANES = kGroup / V, GROUPS = 256 / LANES;
   const int sub = threadIdx.x % LANES;
   const uint32_t g0 = blockIdx.x * (GROUPS * kAtOnce) + threadIdx.x / LANES;
-  float v[kAtOnce][V];
+  uint4 kept[kAtOnce];
 #pragma unroll
   for (int u = 0; u < kAtOnce; ++u) {
-    const uint32_t g = g0 + u * GROUPS, row = g / kb;
+    const uint32_t g = g0 + u * GROUPS, row = __umulhi(2u * g, magic) >> shift;      // g / kb
     const int at = (int)(g - row * kb) * kGroup + sub * V;
-    load_numbers<T, V, ALIGNED>(x + (long)(g < groups ? row : 0) * row_stride + at, g < groups ? K - at : 0, v[u]);
+    kept[u] = load_words<T, ALIGNED>(x + (long)(g < groups ? row : 0) * row_stride + at, g < groups ? K - at : 0);
   }
 #pragma unroll
   for (int u = 0; u < kAtOnce; ++u) {
     const uint32_t g = g0 + u * GROUPS;
-    uint32_t w[V / 4];
-    const float s = group_codes<LANES, V>(v[u], w);
+    const Pack<T, V> p = *reinterpret_cast<const Pack<T, V>*>(&kept[u]);
+    uint32_t most = largest<T>(kept[u]), w[V / 4];
+    if constexpr (LANES == 32) {
+      most = __reduce_max_sync(0xffffffffu, most);
+    } else {
+#pragma unroll
+      for (int o = LANES / 2; o > 0; o >>= 1) most = largest<T>(most, __shfl_xor_sync(0xffffffffu, most, o));
+    }
+    float v[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = to_f32(p.e[j]);
+    const float s = group_codes<LANES, V>(v, w, fold<T>(most));
     if (g >= groups) continue;
     uint8_t* dst = codes + (size_t)g * kGroup + sub * V;
     if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
@@ -122,24 +158,12 @@ __global__ void __launch_bounds__(256, ALIGNED && sizeof(T) == 2 ? 4 : 2) quanti
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int n = n0 + i * ROWS;
-      const T* from = w + (long)n * row_stride + at;
-      if constexpr (ALIGNED) {
-        kept[i] = n < N && at < K ? *reinterpret_cast<const uint4*>(from) : make_uint4(0u, 0u, 0u, 0u);
-      } else {
-        Pack<T, V> p;
-#pragma unroll
-        for (int j = 0; j < V; ++j) p.e[j] = n < N && at + j < K ? from[j] : from_f32<T>(0.f);
-        kept[i] = *reinterpret_cast<const uint4*>(&p);
-      }
+      kept[i] = load_words<T, ALIGNED>(w + (long)n * row_stride + at, n < N ? K - at : 0);
     }
-    uint32_t most = 0;                                     // over whole words, two bfloat16 at a time
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const uint4 q = kept[i];
-      if constexpr (sizeof(T) == 2) most = __vmaxu2(__vmaxu2(most, __vmaxu2(q.x & 0x7fff7fffu, q.y & 0x7fff7fffu)), __vmaxu2(q.z & 0x7fff7fffu, q.w & 0x7fff7fffu));
-      else most = max(max(most, max(q.x & 0x7fffffffu, q.y & 0x7fffffffu)), max(q.z & 0x7fffffffu, q.w & 0x7fffffffu));
-    }
-    most = block_max(sizeof(T) == 2 ? max(most << 16, most & 0xffff0000u) : most);
+    for (int i = 0; i < STEPS; ++i) most = largest<T>(most, largest<T>(kept[i]));
+    most = block_max(fold<T>(most));
     if (most < kInfBits) {
       const float s = q8_scale(__uint_as_float(most)), inv = inverse_scale(s);
 #pragma unroll
@@ -181,22 +205,18 @@ __global__ void __launch_bounds__(256, ALIGNED && sizeof(T) == 2 ? 4 : 2) quanti
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * kb + b] = s;
 }
 
-// The block's sum as two numbers, the same in every thread; blocks of whole warps, up to 32 of them.  Inside a warp the additions are plain (their errors are
-// independent from warp to warp and average out), across warps what an addition rounds off is kept.
-__device__ __forceinline__ float2 block_sum2(float v, float* scratch) {
-  v = warp_sum(v);
-  if (blockDim.x == 32) return make_float2(v, 0.f);
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+// The block's sum, the same in every thread; blocks of whole warps, up to 32 of them.  Inside a warp the additions are of 32 bits (their errors are independent from
+// warp to warp and average out), across warps of 64.
+__device__ __forceinline__ double block_sum64(float v, double* scratch) {
+  double s = (double)warp_sum(v);
+  if (blockDim.x == 32) return s;
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = s;
   __syncthreads();
-  float s = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : 0.f, e = 0.f;
+  s = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : 0.0;
+  if (blockDim.x > 512) s += __shfl_xor_sync(0xffffffffu, s, 16);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float s2 = __shfl_xor_sync(0xffffffffu, s, o), e2 = __shfl_xor_sync(0xffffffffu, e, o);
-    const float t = s + s2, back = t - s;
-    e += e2 + ((s - (t - back)) + (s2 - back));
-    s = t;
-  }
-  return make_float2(s, e);
+  for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return __shfl_sync(0xffffffffu, s, 0);                    // (lanes from 16 on have added zeros only)
 }
 
 // 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).
@@ -208,15 +228,20 @@ __device__ __forceinline__ float2 inverse_root(double m) {
 }
 
 // ------------------------------------------------------------------ residual sum, norm, codes
-// The sum of squares and the factor of a row are pairs of float32 numbers, so that a number in front of its rounding is off by little more than
+// The sum of squares is of 64 bits and the factor of a row a pair of float32 numbers, so that a number in front of its rounding is off by little more than
 // half a float32 step: a code is off where that error carries a number over the border between two codes, in steps of an eighth of the number, and
 // with float32 sums 5,003 rows of 5,120 were 1.2e-4 off 64 bits, four times what a careful float32 form is.  The additions are hidden behind DRAM.
-__device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], float hi, float lo, uint8_t* codes, uint8_t* scales, size_t first_group, int slot) {
+struct RowFactor { f32x2 hi, lo, minus_hi, minus_lo; };       // each twice
+
+__device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], const RowFactor& r, uint8_t* codes, uint8_t* scales, size_t first_group, int slot) {
   uint32_t w[1];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {                             // v (hi + lo) g, rounded once and a little (not finite: NaN)
-    const float f = hi * g[j], fl = fmaf(lo, g[j], fmaf(hi, g[j], -f)), y = v[j] * f;
-    v[j] = y + fmaf(v[j], fl, fmaf(v[j], f, -y));
+  for (int j = 0; j < 4; j += 2) {                          // v (hi + lo) g, rounded once and a little (not finite: NaN)
+    const f32x2 v2 = pair2(v[j], v[j + 1]), g2 = pair2(g[j], g[j + 1]);
+    const f32x2 f = mul2(r.hi, g2), minus_f = mul2(r.minus_hi, g2), y = mul2(v2, f);
+    const f32x2 minus_fl = fma2(r.minus_lo, g2, fma2(r.minus_hi, g2, f));           // what f lacks, with its sign turned
+    const f32x2 minus_rest = fma2(v2, minus_fl, fma2(v2, minus_f, y));
+    v[j] = low2(y) - low2(minus_rest), v[j + 1] = high2(y) - high2(minus_rest);
   }
   const float s = group_codes<32, 4>(v, w);
   const size_t group = first_group + (slot >> 5);
@@ -225,21 +250,21 @@ __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], 
 }
 
 // One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
-// read twice, number by number.  5,003 rows of 5,120 59 us, 4.8 TB/s: instructions (some 45 a number) beside DRAM; blocks that stay and copy the next row to shared
-// memory meanwhile took 65.  Eight rows of 4,096 2.5 us alone.
-template <typename TA, int PER, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 320 ? 4 : 1) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
+// read twice, number by number.  5,003 rows of 5,120 54.5 us, 5.0 TB/s (58.5 with half the warps on an SM, 65 with blocks that stay and copy the next row to shared
+// memory meanwhile): reads, a sum over the block and writes of a row follow one another, and what hides that is other rows' warps.  Eight rows of 4,096 2.4 us alone.
+template <typename TA, int PER>
+__global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
                                                           uint8_t* scales, int H, int kb, double inv_h, float eps, float delta_scale) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float red[32];
+  __shared__ double red[32];
   constexpr int KEEP = PER > 0 ? PER : 1;
   const long row = blockIdx.x;
   const float* xr = resid + row * H;
   const TA* dr = delta ? delta + row * H : nullptr;
   float* so = sum_out ? sum_out + row * H : nullptr;
   const int slots = kb * 32;                                // of four numbers
-  float ss = 0.f;
+  f32x2 ss = 0;                                             // two sums, of even and odd places
   float x[KEEP][4], gw[KEEP][4];
   auto load = [&](int slot, float (&v)[4]) {
     load_numbers<float, 4, (PER > 0)>(xr + 4 * slot, H - 4 * slot, v);
@@ -247,10 +272,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 4 : 1) rmsnorm_q8_ke
       float d[4];
       load_numbers<TA, 4, (PER > 0)>(dr + 4 * slot, H - 4 * slot, d);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = fmaf(delta_scale, d[j], v[j]);
+      for (int j = 0; j < 4; j += 2) {
+        const f32x2 sum = fma2(pair2(delta_scale, delta_scale), pair2(d[j], d[j + 1]), pair2(v[j], v[j + 1]));
+        v[j] = low2(sum), v[j + 1] = high2(sum);
+      }
     }
   };
-  auto finish = [&](int slot, float (&v)[4], const float (&g)[4], float hi, float lo) { finish_four(v, g, hi, lo, codes, scales, (size_t)row * kb, slot); };
+  auto add_squares = [&](const float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) ss = fma2(pair2(v[j], v[j + 1]), pair2(v[j], v[j + 1]), ss);
+  };
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -267,23 +298,21 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 4 : 1) rmsnorm_q8_ke
       const int slot = threadIdx.x + i * blockDim.x;
       if (slot >= slots) continue;
       if (so && 4 * slot < H) store_vec<float, 4>(so + 4 * slot, x[i]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ss = fmaf(x[i][j], x[i][j], ss);
+      add_squares(x[i]);
     }
   } else {
     for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
       load(slot, x[0]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) ss = fmaf(x[0][j], x[0][j], ss);
+      add_squares(x[0]);
     }
   }
-  const float2 total = block_sum2(ss, red);
-  const float2 inv = inverse_root(((double)total.x + (double)total.y) * inv_h + (double)eps);
+  const float2 inv = inverse_root(block_sum64(low2(ss) + high2(ss), red) * inv_h + (double)eps);
+  const RowFactor factor = {pair2(inv.x, inv.x), pair2(inv.y, inv.y), pair2(-inv.x, -inv.x), pair2(-inv.y, -inv.y)};
   if constexpr (PER > 0) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int slot = threadIdx.x + i * blockDim.x;        // whole warps: slots and threads are multiples of 32
-      if (slot < slots) finish(slot, x[i], gw[i], inv.x, inv.y);
+      if (slot < slots) finish_four(x[i], gw[i], factor, codes, scales, (size_t)row * kb, slot);
     }
   } else {
     for (int slot = threadIdx.x; slot < slots; slot += blockDim.x) {
@@ -292,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 320 ? 4 : 1) rmsnorm_q8_ke
       for (int j = 0; j < 4; ++j)
         if (so && 4 * slot + j < H) so[4 * slot + j] = x[0][j];
       load_numbers<float, 4, false>(gain + 4 * slot, H - 4 * slot, gw[0]);
-      finish(slot, x[0], gw[0], inv.x, inv.y);
+      finish_four(x[0], gw[0], factor, codes, scales, (size_t)row * kb, slot);
     }
   }
 }
@@ -326,8 +355,12 @@ int quantize_rows(const void* x, long row_stride, void* codes, void* scales, int
   const long groups = (long)M * kb, blocks = (groups + per_block - 1) / per_block;
   if (groups + per_block > 0x7fffffffl) return ARLE_E_UNSUPPORTED;
   const bool fast = K % V == 0 && aligned16(x) && (M == 1 || row_stride % V == 0);
+  // magic = (2^(31 + shift) + e) / kb with e < kb <= 2^shift, so for g below 2^31 g magic / 2^(31 + shift) is g / kb and less than 1 / kb more
+  int shift = 0;
+  while ((1l << shift) < kb) ++shift;
+  const uint32_t magic = (uint32_t)(((1ull << (31 + shift)) + kb - 1) / kb);
   launch_early(fast ? quantize_rows_kernel<T, true> : quantize_rows_kernel<T, false>, dim3((unsigned)blocks), dim3(256), 0, s, 1, (const T*)x, row_stride,
-                (uint8_t*)codes, (uint8_t*)scales, (uint32_t)groups, K, (uint32_t)kb);
+                (uint8_t*)codes, (uint8_t*)scales, (uint32_t)groups, K, (uint32_t)kb, magic, shift);
   return launch_status();
 }
 
@@ -347,13 +380,14 @@ int rmsnorm(const float* resid, const void* delta, const float* gain, float* sum
             cudaStream_t s) {
   const int kb = blocks_of(H);
   const bool vec = H % 4 == 0 && aligned16(resid) && aligned16(gain) && ((uintptr_t)delta % (4 * sizeof(TA))) == 0 && aligned16(sum_out);
-  auto kern = rmsnorm_q8_kernel<TA, 0, 1024>;
+  auto kern = rmsnorm_q8_kernel<TA, 0>;
   int threads = kb >= 32 ? 1024 : 32 * kb;
   if (vec && kb <= 128) {
-    // few rows: as many threads as the row has pieces, the shortest way through it; many: four pieces a thread
-    const int per = M <= 256 ? (kb + 31) / 32 : 4;
+    // few rows: as many threads as the row has pieces, the shortest way through it; many: two pieces a thread, so that three blocks of 5,120 numbers are on an SM
+    // (four pieces, 48 registers and four blocks of half the threads: 58 us for 5,003 rows; one piece for 4,096 rows of 4,096: 42, two 35, four 39)
+    const int per = M <= 256 || kb > 64 ? (kb + 31) / 32 : 2;
     threads = 32 * ((kb + per - 1) / per);
-    kern = per == 1 ? rmsnorm_q8_kernel<TA, 1, 1024> : per == 2 ? rmsnorm_q8_kernel<TA, 2, 1024> : threads <= 320 ? rmsnorm_q8_kernel<TA, 4, 320> : rmsnorm_q8_kernel<TA, 4, 1024>;
+    kern = per == 1 ? rmsnorm_q8_kernel<TA, 1> : per == 2 ? rmsnorm_q8_kernel<TA, 2> : rmsnorm_q8_kernel<TA, 4>;
   }
   launch_early(kern, dim3(M), dim3(threads), 0, s, 1, resid, (const TA*)delta, gain, sum_out, (uint8_t*)codes, (uint8_t*)scales, H, kb, 1.0 / H, eps,
                 delta_scale);
