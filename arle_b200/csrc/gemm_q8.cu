@@ -23,13 +23,14 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) { return __ldcs(rei
 // 32t .. 32t + 31 of its row's block, so a warp's loads cover whole 128-byte lines, and words 2i and 2i + 1 of those are the operands of the i-th of
 // four mma.  What hides the memory is many warps, a block of k each on its way, not several blocks in a warp: with two, and with rings of four that go on
 // across rows, all sizes took longer (4,096 x 12,288 for one row 15 to 26 us instead of 10.3), and so did x fetched a block ahead.
-// The first block of w is asked for before the kernel in front has ended (what makes weights lets nothing start before its end).
+// The first block of w is asked for before the kernel in front has ended (what makes weights lets nothing start before its end).  The next kernel may start when a
+// block's sums are done and not before: long blocks that start early gather on the SMs that have room (the decode attention of eight requests behind a product, and so a layer of
+// 8B sizes, took 20 us more: 81 and 61), and short ones gain nothing (norms, codes and the four products of a layer for one row 46.1 and 44.8 us).
 // One row, us and TB/s: 4,096 x 4,096 4.2 (4.0), 4,096 x 12,288 10.3 (4.9), 6,144 x 4,096 6.1 (4.1), 24,576 x 4,096 18.6 (5.4), 5,120 x 25,600 27.3 (4.8); eight
 // rows some 3 % more.
 template <int WARPS, int BLOCKS, typename OutT>
 __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const float* sw, OutT* out, long ldo,
                                                                          int M, int N, int kb) {
-  pdl_launch_dependents();
   __shared__ float part[WARPS][16][9];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8;
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const 
 #pragma unroll
   for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][2 * t + (e & 1)] = acc[e];
   __syncthreads();
+  pdl_launch_dependents();
   if (threadIdx.x < 128) {                                 // added up in the order of the warps
     const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
     float v = 0.f;

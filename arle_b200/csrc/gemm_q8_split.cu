@@ -70,8 +70,8 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
       tma_load_2d(ring + i * STAGE, &map_w, (b0 + i) * BK, n0, full0 + 8 * i);
     }
   __syncwarp();
-  // Tensor memory is asked for when the kernel in front has ended, and the next kernel may start when it is had: a block that held some while it waited for
-  // one that still has to get it on the same SM would wait for good.
+  // Tensor memory is asked for when the kernel in front has ended, and the next kernel may start when it is had (in fact far later): a block that held some while it
+  // waited for one that still has to get it on the same SM would wait for good.
   pdl_wait();
   if (warp == kIssuer) {
     tmem_alloc(smem_addr(&tmem_base_slot), kTmemCols);
@@ -79,7 +79,6 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
   }
   tc_fence_before();
   __syncthreads();
-  pdl_launch_dependents();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
   const volatile int* aborted = &abort_flag;
@@ -249,6 +248,7 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
     for (int s = 0; s < kStages; ++s) mbar_wait_plain(smem_addr(&full_bar[s]), 0), mbar_wait_plain(smem_addr(&full_bar[s]), 1);
   tc_fence_before();
   __syncthreads();
+  pdl_launch_dependents();
   if (warp == kIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
