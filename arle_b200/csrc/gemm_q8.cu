@@ -23,10 +23,12 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) { return __ldcs(rei
 // 32t .. 32t + 31 of its row's block, so a warp's loads cover whole 128-byte lines, and words 2i and 2i + 1 of those are the operands of the i-th of
 // four mma.  What hides the memory is many warps, a block of k each on its way, not several blocks in a warp: with two, and with rings of four that go on
 // across rows, all sizes took longer (4,096 x 12,288 for one row 15 to 26 us instead of 10.3), and so did x fetched a block ahead.
+// A warp has the block of k behind the next one brought to L2 meanwhile: in decode steps of 14 layers of 8B sizes, 193 MB each, a layer takes 53.6 us for 56.0 (one
+// request; the products by themselves gain 0 to 3 %, as weights in turn of 2 GB; everything a warp has left brought at once, or by bulk copies, takes 3 to 7 us more).
 // The first block of w is asked for before the kernel in front has ended (what makes weights lets nothing start before its end).  The next kernel may start when a
 // block's sums are done and not before: long blocks that start early gather on the SMs that have room (the decode attention of eight requests behind a product, and so a layer of
 // 8B sizes, took 20 us more: 81 and 61), and short ones gain nothing (norms, codes and the four products of a layer for one row 46.1 and 44.8 us).
-// One row, us and TB/s: 4,096 x 4,096 4.2 (4.0), 4,096 x 12,288 10.3 (4.9), 6,144 x 4,096 6.1 (4.1), 24,576 x 4,096 18.6 (5.4), 5,120 x 25,600 27.3 (4.8); eight
+// One row, us and TB/s, weights in turn of 2 GB: 4,096 x 4,096 5.2 (3.2), 4,096 x 12,288 10.4 (4.8), 6,144 x 4,096 6.4 (3.9), 24,576 x 4,096 18.4 (5.5); eight
 // rows some 3 % more.
 template <int WARPS, int BLOCKS, typename OutT>
 __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const float* sw, OutT* out, long ldo,
@@ -45,7 +47,14 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const 
       a[0] = load_once(w0 + at), a[1] = load_once(w0 + at + 16), a[2] = load_once(w1 + at), a[3] = load_once(w1 + at + 16);
     }
   };
+  auto hint = [&](int b) {                                 // a row's block of k is one line
+    if (t == 0 && b < kb) {
+      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(w0 + (size_t)b * kBlock) : "memory");
+      asm volatile("prefetch.global.L2 [%0];\n" ::"l"(w1 + (size_t)b * kBlock) : "memory");
+    }
+  };
   ask(warp);
+  hint(warp + WARPS);
   pdl_wait();
   const uint8_t* xr = x + (size_t)min(m0 + g, M - 1) * K + 32 * t;
   const uint8_t* sxa = sx + (size_t)min(m0 + 2 * t, M - 1) * kb;
@@ -61,6 +70,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const 
     mma_e4m3(d, a[1].z, a[3].z, a[1].w, a[3].w, x1.z, x1.w);
     acc[0] = fmaf(d[0], fa, acc[0]), acc[1] = fmaf(d[1], fb, acc[1]);
     acc[2] = fmaf(d[2], fa, acc[2]), acc[3] = fmaf(d[3], fb, acc[3]);
+    hint(b + 2 * WARPS);
     ask(b + WARPS);
   }
 #pragma unroll
