@@ -93,8 +93,8 @@ int product(const void* x, const void* sx, const void* w, const float* sw, void*
   int dev = 0, sms = 0;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // 16 warps to a tile where all tiles are under way at once, else eight: us for one row with 16 warps, eight in three blocks an SM and eight in four, 4,096 x 12,288 (256
-  // tiles) 10.3, 13.4 and 15.0; 6,144 x 4,096 (384) 7.1, 6.1 and 6.7; 24,576 x 4,096 (1,536) 19.8, 20.1 and 18.6
+  // 16 warps to a tile where all tiles are under way at once, else eight: us for one row behind the launch of its codes with 16 warps, eight in three blocks an SM and
+  // eight in four, 4,096 x 12,288 (256 tiles) 11.4, 12.1 and 13.0; 6,144 x 4,096 (384) 8.6, 7.1 and 7.4; 24,576 x 4,096 (1,536) 21.5, 20.0 and 19.4
   const long blocks = (long)tiles * tiles_m;
   const int warps = blocks <= 2l * sms ? 16 : 8;
   auto kern = blocks <= 2l * sms ? gemm_q8_rows_kernel<16, 2, OutT> : blocks <= 3l * sms ? gemm_q8_rows_kernel<8, 3, OutT> : gemm_q8_rows_kernel<8, 4, OutT>;

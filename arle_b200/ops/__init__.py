@@ -2870,8 +2870,8 @@ def _q8_pair_cost(M: int, N: int, kb: int, sms: int) -> float:
 def _q8_route(M: int, N: int, kb: int, device: int):
     """(kernel, parts that a tile's k is cut into, estimated us) of a product, by its sizes alone.  Figures in us, alone in a graph:
 
-    * "rows", one launch without shared memory, up to 8 rows: one row of 4,096 x 4,096 4.2 and 6.3 with "few", 4,096 x 12,288 10.3 and 10.8; longer sums are
-      shorter there (5,120 x 25,600 27.3 and 23.2);
+    * "rows", operands from memory to registers, up to 8 rows: one row of 4,096 x 4,096 behind the launch of its codes 5.8 and 7.5 with "few", 4,096 x 12,288 11.3
+      and 12.8, 24,576 x 4,096 19.3 and 20.2; longer sums are no shorter there (5,120 x 25,600 24.8 and 24.7, eight rows more);
     * "few", up to 64 rows, bound by w's bytes.  Parts: the cheapest of what runs at once, 0.3 a block of k (0.45 for more than 32 rows), 0.1 (0.25) a part, 1.5 a
       wave, 0.9 where two blocks share an SM.  32 tiles of 32 blocks of k, one row: 2, 4, 6 and 8 parts 7.9, 6.3, 6.6 and 7.2; 48 tiles 8.9, 8.0, 10.2 (more than
       run at once) and 9.9, five 7.5; 32 tiles of 96 blocks 17.4, 12.4, 11.9 and 10.9;
