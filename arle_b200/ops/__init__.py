@@ -2601,16 +2601,17 @@ class Q8Weight:
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        if codes.dtype is not _E4M3 or codes.dim() != 2 or not codes.is_contiguous() or codes.shape[1] == 0 or codes.shape[1] % Q8_BLOCK:
-            raise KernelError(f"Q8Weight: codes must be contiguous float8_e4m3fn [N, a multiple of {Q8_BLOCK}], got {codes.dtype} {tuple(codes.shape)}")
-        want = (-(-codes.shape[0] // Q8_BLOCK), codes.shape[1] // Q8_BLOCK)
-        if scales.dtype != torch.float32 or tuple(scales.shape) != want or not scales.is_contiguous() or scales.device != codes.device:
+        shape = codes.shape
+        if codes.dtype is not _E4M3 or len(shape) != 2 or shape[1] == 0 or shape[1] & 127 or not codes.is_contiguous():
+            raise KernelError(f"Q8Weight: codes must be contiguous float8_e4m3fn [N, a multiple of {Q8_BLOCK}], got {codes.dtype} {tuple(shape)}")
+        want, device = ((shape[0] + 127) >> 7, shape[1] >> 7), codes.get_device()
+        if scales.dtype is not torch.float32 or scales.shape != want or not scales.is_contiguous() or scales.get_device() != device:
             raise KernelError(f"Q8Weight: scales must be contiguous float32 {want} beside the codes, got {scales.dtype} {tuple(scales.shape)} on {scales.device}")
-        if codes.data_ptr() % 16:
+        if codes.data_ptr() & 15:
             raise KernelError("Q8Weight: codes must start on a 16-byte boundary")
-        if codes.is_cuda:
-            _error_word(codes.get_device())          # made here and not by a first product, which may be one that a graph captures
-        self.codes, self.scales, self.shape = codes, scales, codes.shape
+        if device >= 0 and device not in _ERR_BY_INDEX:
+            _error_word(device)                          # made here and not by a first product, which may be one that a graph captures
+        self.codes, self.scales, self.shape = codes, scales, shape
 
     def bytes(self) -> int:
         return self.codes.numel() + 4 * self.scales.numel()
@@ -2740,21 +2741,28 @@ def quantize_q8(x, codes, scales) -> None:
 def quantize_weight_q8(w, codes, scales) -> Q8Weight:
     """A weight in 8 bits: w [N, K] (float32 or bfloat16, unit inner stride) as codes [N, q8_width(K)] and float32 scales [ceil(N / 128), ceil(K / 128)], and the
     ``Q8Weight`` of both.  The scale of a block of 128 x 128 is found as a row's in ``quantize_q8``; numbers that are not finite become NaN."""
-    if w.dim() != 2 or w.shape[1] == 0:
-        raise KernelError(f"quantize_weight_q8: w must be [N, K], got {tuple(w.shape)}")
-    N, K = w.shape
-    if codes.shape != (N, q8_width(K)):
-        raise KernelError(f"quantize_weight_q8: w {tuple(w.shape)} needs codes {(N, q8_width(K))}, got {tuple(codes.shape)}")
+    global _LAUNCHES
+    shape = w.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise KernelError(f"quantize_weight_q8: w must be [N, K], got {tuple(shape)}")
+    N, K = shape
+    if codes.shape != (N, (K + 127) >> 7 << 7):
+        raise KernelError(f"quantize_weight_q8: w {tuple(shape)} needs codes {(N, q8_width(K))}, got {tuple(codes.shape)}")
     weight = Q8Weight(codes, scales)
     stride, unit = w.stride()
     if unit != 1 and K > 1 and N:
         raise KernelError("quantize_weight_q8: rows of w must have unit inner stride")
-    dt = _dt(w)
+    dt = _TYPE_CODES.get(w.dtype)
+    if dt is None:
+        _dt(w)
     device = w.get_device()
-    _on_device("quantize_weight_q8", device, w, codes, scales)
+    if device < 0 or codes.get_device() != device or _current_device() != device:
+        _misplaced("quantize_weight_q8", w, codes, scales)
     if N:
-        _check((_LIB or library()).arle_quantize_weight_q8(w.data_ptr(), dt, stride, codes.data_ptr(), scales.data_ptr(), N, K,
-                                                           torch._C._cuda_getCurrentRawStream(device)), "quantize_weight_q8")
+        code = (_LIB or library()).arle_quantize_weight_q8(w.data_ptr(), dt, stride, codes.data_ptr(), scales.data_ptr(), N, K, _raw_stream(device))
+        if code:
+            _check(code, "quantize_weight_q8")
+        _LAUNCHES += 1
     return weight
 
 
