@@ -219,6 +219,16 @@ __device__ __forceinline__ double block_sum64(float v, double* scratch) {
   return __shfl_sync(0xffffffffu, s, 0);                    // (lanes from 16 on have added zeros only)
 }
 
+// Two differences a - b, rounded towards zero, the last bit set where that left something out: a number that lies beside a border between two codes (or
+// two scales), which have zeros there, stays on its side of it, as if nothing had been rounded.
+__device__ __forceinline__ void subtract_sticky(f32x2 a, f32x2 b, float& lo, float& hi) {
+  f32x2 s, back;
+  asm("sub.rz.f32x2 %0, %1, %2;" : "=l"(s) : "l"(a), "l"(b));
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(back) : "l"(a), "l"(s));            // b where s is a - b, with no rounding of its own (|b| is far below |a|)
+  lo = low2(back) != low2(b) ? __uint_as_float(__float_as_uint(low2(s)) | 1u) : low2(s);
+  hi = high2(back) != high2(b) ? __uint_as_float(__float_as_uint(high2(s)) | 1u) : high2(s);
+}
+
 // 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).
 __device__ __forceinline__ float2 inverse_root(double m) {
   const float mh = (float)m, ml = (float)(m - (double)mh), y = rsqrtf(mh);
@@ -228,20 +238,29 @@ __device__ __forceinline__ float2 inverse_root(double m) {
 }
 
 // ------------------------------------------------------------------ residual sum, norm, codes
-// The sum of squares is of 64 bits and the factor of a row a pair of float32 numbers, so that a number in front of its rounding is off by little more than
-// half a float32 step: a code is off where that error carries a number over the border between two codes, in steps of an eighth of the number, and
-// with float32 sums 5,003 rows of 5,120 were 1.2e-4 off 64 bits, four times what a careful float32 form is.  The additions are hidden behind DRAM.
+// A code is off where an error carries a number over the border between two codes, in steps of an eighth of the number.  So the sum of squares is of 64 bits from a
+// warp's sums on, the factor of a row is a pair of float32 numbers, and where its product with a number would round onto a border it is rounded as subtract_sticky
+// does.  Of the 25.6 million codes of 5,003 rows of 5,120, 17 are off in a careful float32 form, 14 with products rounded to float32 (54.0 us), three so (55.6 us; four
+// and 56.9 with every product rounded so).
 struct RowFactor { f32x2 hi, lo, minus_hi, minus_lo; };       // each twice
 
 __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], const RowFactor& r, uint8_t* codes, uint8_t* scales, size_t first_group, int slot) {
   uint32_t w[1];
+  f32x2 ys[2], rests[2];
 #pragma unroll
-  for (int j = 0; j < 4; j += 2) {                          // v (hi + lo) g, rounded once and a little (not finite: NaN)
+  for (int j = 0; j < 4; j += 2) {                          // v (hi + lo) g, to some 2^-45 (not finite: NaN)
     const f32x2 v2 = pair2(v[j], v[j + 1]), g2 = pair2(g[j], g[j + 1]);
     const f32x2 f = mul2(r.hi, g2), minus_f = mul2(r.minus_hi, g2), y = mul2(v2, f);
     const f32x2 minus_fl = fma2(r.minus_lo, g2, fma2(r.minus_hi, g2, f));           // what f lacks, with its sign turned
     const f32x2 minus_rest = fma2(v2, minus_fl, fma2(v2, minus_f, y));
+    ys[j / 2] = y, rests[j / 2] = minus_rest;
     v[j] = low2(y) - low2(minus_rest), v[j + 1] = high2(y) - high2(minus_rest);
+  }
+  // (the borders' last 19 bits are zeros: four bits say which code, or half a step more)
+  auto low_bits = [](float a) { return __float_as_uint(a) & 0x7ffffu; };
+  if (min(min(low_bits(v[0]), low_bits(v[1])), min(low_bits(v[2]), low_bits(v[3]))) == 0) {
+    subtract_sticky(ys[0], rests[0], v[0], v[1]);
+    subtract_sticky(ys[1], rests[1], v[2], v[3]);
   }
   const float s = group_codes<32, 4>(v, w);
   const size_t group = first_group + (slot >> 5);
@@ -250,8 +269,8 @@ __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], 
 }
 
 // One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
-// read twice, number by number.  5,003 rows of 5,120 54.5 us, 5.0 TB/s (58.5 with half the warps on an SM, 65 with blocks that stay and copy the next row to shared
-// memory meanwhile): reads, a sum over the block and writes of a row follow one another, and what hides that is other rows' warps.  Eight rows of 4,096 2.4 us alone.
+// read twice, number by number.  5,003 rows of 5,120 55.6 us, 5.0 TB/s (4 more with half the warps on an SM, 65 with blocks that stay and copy the next row to shared
+// memory meanwhile): reads, a sum over the block and writes of a row follow one another, and what hides that is other rows' warps.  Eight rows of 4,096 2.5 us alone.
 template <typename TA, int PER>
 __global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,
                                                           uint8_t* scales, int H, int kb, double inv_h, float eps, float delta_scale) {

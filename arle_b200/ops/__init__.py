@@ -2767,8 +2767,8 @@ def quantize_weight_q8(w, codes, scales) -> Q8Weight:
 
 
 def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, delta_scale: float = 1.0) -> None:
-    """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's float32 numbers as
-    ``quantize_q8`` makes codes and scales.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.
+    """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's codes and
+    scales as ``quantize_q8`` has them (y is rounded to its codes, not to float32 before).  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.
     ``sum_out`` (float32 [M, H]: ``resid`` itself or a buffer that overlaps no other argument) gets x; None: x is kept nowhere."""
     global _LAUNCHES
     f32, shape = torch.float32, resid.shape
