@@ -145,6 +145,34 @@ def test_rmsnorm(m, h, dtype):
     assert torch.equal(r, total[:m]) and torch.equal(again.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(sagain.view(torch.uint8), scales.view(torch.uint8))
 
 
+def _beside_borders(h):
+    """A row and gains whose norm lies within 2^-25 of borders between two codes (of itself), on either side: whole numbers, whose squares' sums float32 holds, so that
+    the mean is exact and the numbers in 64 bits are known to 2^-50."""
+    g = torch.Generator().manual_seed(h)
+    v = torch.randint(1, 256, (h,), generator=g).float()
+    border = (torch.randint(8, 16, (h,), generator=g) + 0.5) / 8 * 2.0 ** torch.randint(0, 8, (h,), generator=g)
+    border[::128] = 400.0                                   # every group's largest: its scale is 1
+    root = v.double().square().mean().sqrt()
+    gain = (border.double() * root / v.double()).float()
+    return v, gain, v.double() * gain.double() / root, border.double()
+
+
+@pytest.mark.parametrize("m,h", [(1, 4096), (1, 128), (300, 4096), (300, 1028), (2, 1030), (1, 16384), (3, 16400)])
+def test_rmsnorm_beside_borders_between_codes(m, h):
+    """A number is rounded once, to its code: rounded to float32 before, four in ten of these would go to the wrong side of the border.  The kernels' factor and
+    products are good to 2^-43 (pairs of float32 numbers): numbers that are nearer than 2^-40 to the border do not count."""
+    v, gain, y, border = _beside_borders(h)
+    codes, scales = _rows(m, h)
+    ops.rmsnorm_q8(v.expand(m, h).contiguous().to(DEV), None, gain.to(DEV), 0.0, codes[:m], scales[:m])
+    c, s = refs.host(codes[:m]), refs.host(scales[:m])
+    want, ws = refs.quantize(y[None])
+    sure = ((y - border).abs() > 2.0 ** -40 * border) | (border == 400.0)
+    assert sure.double().mean() > 0.99 and (s == ws).all()
+    assert (c[:, :h] == want[:, :h])[:, sure].all()
+    once, _ = refs.quantize(y[None].float().double())
+    assert h < 1000 or (once[:, :h] != want[:, :h]).sum() > h / 10          # (the row tells the two apart)
+
+
 def test_rmsnorm_rows_at_odd_places():
     """Rows and sums that do not start on 16-byte boundaries take the kernel that reads number by number: the same codes."""
     h = 516
