@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
   }
   __syncthreads();
+  if (parts > 1) cluster_started();
   const uint32_t ring = __shfl_sync(0xffffffffu, smem_addr(tiles), 0), full0 = smem_addr(&full_bar[0]), empty0 = smem_addr(&empty_bar[0]),
                  acc_full0 = smem_addr(&acc_full[0]), acc_empty0 = smem_addr(&acc_empty[0]);
   const int ahead = min(STAGES, b1 - b0);
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
   // the group of rows 4q .. 4q + 3 is added up by block q % parts of the cluster, as its group q / parts
   const int slots = (ROWS / 4 + parts - 1) / parts;
   if (parts > 1) {
+    cluster_all_started();
     if (warp < kAddWarps) {
       uint32_t to = 0, slot = smem_addr(sums) + ((uint32_t)(part * slots) * 128 + threadIdx.x) * 16;
 #pragma unroll

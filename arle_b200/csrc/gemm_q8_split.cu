@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
     asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
   }
   __syncthreads();
+  if (NB == 1 && parts > 1) cluster_started();             // (with two blocks of columns a barrier of its own stands in front of the stores)
   const uint32_t ring = __shfl_sync(0xffffffffu, smem_addr(tiles), 0), full0 = smem_addr(&full_bar[0]), empty0 = smem_addr(&empty_bar[0]),
                  acc_full0 = smem_addr(&acc_full[0]), acc_empty0 = smem_addr(&acc_empty[0]);
   const int ahead = min(kStages, b1 - b0);
@@ -203,6 +204,7 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
       // Row l is added up by SM l % parts of the cluster, as its row j = l / parts: 512 NB bytes from each part as pieces of 16 bytes, piece p at p ^ (j % 8), so
       // that eight rows' pieces lie in different banks.  Behind the ring, or in it when no SM of the cluster has use for it any more.
       if (NB == 2) cluster_sync_all();
+      else cluster_all_started();
       const uint32_t slots = (uint32_t)((rows + parts - 1) / parts);
       if (lrow < rows) {
         const uint32_t j = (uint32_t)(lrow / parts),
@@ -216,7 +218,10 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
     }
   }
   if (parts > 1) {
-    if (NB == 2 && warp >= kEpilogueWarps) cluster_sync_all();
+    if (warp >= kEpilogueWarps) {
+      if (NB == 2) cluster_sync_all();
+      else cluster_all_started();
+    }
     cluster_sync_all();
     const int slots = (rows + parts - 1) / parts;
     const unsigned char* mine = tiles + (NB == 2 ? 0u : kStages * STAGE);

@@ -102,6 +102,10 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// A block's shared memory may be written by the cluster's others once it has started (that they run at the same time does not say that it has): every thread
+// says that it has started and waits for the others' word in front of the first store to another block.
+__device__ __forceinline__ void cluster_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_all_started() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 // The cluster address of the same shared-memory location in the CTA of the given rank.
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
   uint32_t r;
