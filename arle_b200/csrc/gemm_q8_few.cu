@@ -168,6 +168,9 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
       const float4* f4 = reinterpret_cast<const float4*>(fs + (done % SCALED) * ROWS);
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(acc_full0 + 8 * buf, (done / kAccs) & 1, aborted))) {
         abort_flag = 1;
+        // another warp's poll may have succeeded: this one still comes to the barriers that are left, which have no limit
+        for (uint32_t later = done + 1; later < (uint32_t)(b1 - b0); ++later)
+          if (later % SCALED == 0) bar_adders();
         break;
       }
       tc_fence_after();

@@ -240,7 +240,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_
           break;
         }
       }
-      if (lost) break;
+      if (lost) {
+        if constexpr (GATED)                               // the other half's warp may go on: this one still comes to the barriers that the two share
+          for (; t < num_tiles; t += npairs) bar_pair(1 + (warp & 3)), bar_pair(1 + (warp & 3));
+        break;
+      }
       if constexpr (GATED) {
         // the row's largest result is known to both of its threads after one exchange
         uint32_t most = 0;
