@@ -205,10 +205,8 @@ __global__ void __launch_bounds__(256, ALIGNED && sizeof(T) == 2 ? 4 : 2) quanti
   if (threadIdx.x == 0) scales[(size_t)blockIdx.y * kb + b] = s;
 }
 
-// The block's sum, the same in every thread; blocks of whole warps, up to 32 of them.  Inside a warp the additions are of 32 bits (their errors are independent from
-// warp to warp and average out), across warps of 64.
-__device__ __forceinline__ double block_sum64(float v, double* scratch) {
-  double s = (double)warp_sum(v);
+// The block's sum of its warps' sums, the same in every thread; blocks of whole warps, up to 32 of them.
+__device__ __forceinline__ double block_sum64(double s, double* scratch) {
   if (blockDim.x == 32) return s;
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = s;
   __syncthreads();
@@ -229,7 +227,9 @@ __device__ __forceinline__ void subtract_sticky(f32x2 a, f32x2 b, float& lo, flo
   hi = high2(back) != high2(b) ? __uint_as_float(__float_as_uint(high2(s)) | 1u) : high2(s);
 }
 
-// 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).
+// 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).  For m in kLeastMean .. kMostMean,
+// where y^2, its rounding error and what m has beside its float32 number are all normal numbers, and the sums of squares behind m are.
+constexpr double kLeastMean = 0x1p-90, kMostMean = 0x1p100;
 __device__ __forceinline__ float2 inverse_root(double m) {
   const float mh = (float)m, ml = (float)(m - (double)mh), y = rsqrtf(mh);
   const float q = y * y, ql = fmaf(y, y, -q);
@@ -266,6 +266,39 @@ __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], 
   const size_t group = first_group + (slot >> 5);
   *reinterpret_cast<uint32_t*>(codes + group * kGroup + 4 * (slot & 31)) = w[0];
   if ((slot & 31) == 0) scales[group] = exponent_byte(s);
+}
+
+// A row whose mean square float32 does not carry: numbers whose squares leave its range (from some 10^15 on, or below 10^-13 beside no eps), infinities
+// (they come out as NaN and the row's finite numbers as zero, 1 / sqrt(inf) times them), NaN (all of the row).  Everything in 64 bits, from the numbers in memory:
+// `x` and, where it is still to be added, `delta`; sum_out is null where it has been written.  The filled-up columns are zero whatever the row holds.
+template <typename TA>
+__device__ __noinline__ void extreme_row(const float* x, const TA* delta, float delta_scale, const float* gain, float* sum_out, uint8_t* codes, uint8_t* scales, int H,
+                                         int kb, double inv_h, float eps, double* scratch) {
+  auto number = [&](int at) { return at >= H ? 0.f : delta ? fmaf(delta_scale, to_f32(delta[at]), x[at]) : x[at]; };
+  double ss = 0.0;
+  for (int slot = threadIdx.x; slot < 32 * kb; slot += blockDim.x)
+    for (int j = 0; j < 4; ++j) {
+      const double v = number(4 * slot + j);
+      ss += v * v;
+    }
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  __syncthreads();                                          // the scratch has been read
+  const double r = 1.0 / sqrt(block_sum64(ss, scratch) * inv_h + (double)eps);
+  for (int slot = threadIdx.x; slot < 32 * kb; slot += blockDim.x) {
+    float v[4];
+    for (int j = 0; j < 4; ++j) {
+      const int at = 4 * slot + j;
+      const float sum = number(at);
+      if (sum_out && at < H) sum_out[at] = sum;
+      const double y = at < H ? (double)sum * r * (double)gain[at] : 0.0;
+      v[j] = __double2float_rz(y);                          // the last bit set where that left something out (see subtract_sticky)
+      if ((double)v[j] != y) v[j] = __uint_as_float(__float_as_uint(v[j]) | 1u);
+    }
+    uint32_t w[1];
+    const float s = group_codes<32, 4>(v, w);
+    *reinterpret_cast<uint32_t*>(codes + 4 * (size_t)slot) = w[0];
+    if ((slot & 31) == 0) scales[slot >> 5] = exponent_byte(s);
+  }
 }
 
 // One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
@@ -325,7 +358,15 @@ __global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(cons
       add_squares(x[0]);
     }
   }
-  const float2 inv = inverse_root(block_sum64(low2(ss) + high2(ss), red) * inv_h + (double)eps);
+  // (inside a warp additions of 32 bits, whose errors are independent from warp to warp and average out, across warps of 64)
+  const double mean = block_sum64((double)warp_sum(low2(ss) + high2(ss)), red) * inv_h + (double)eps;
+  if (!(mean > kLeastMean && mean < kMostMean)) {
+    const bool written = PER > 0 && so;
+    extreme_row<TA>(written ? so : xr, written ? nullptr : dr, delta_scale, gain, PER > 0 ? nullptr : so, codes + (size_t)row * kb * kGroup, scales + (size_t)row * kb, H,
+                    kb, inv_h, eps, red);
+    return;
+  }
+  const float2 inv = inverse_root(mean);
   const RowFactor factor = {pair2(inv.x, inv.x), pair2(inv.y, inv.y), pair2(-inv.x, -inv.x), pair2(-inv.y, -inv.y)};
   if constexpr (PER > 0) {
 #pragma unroll
