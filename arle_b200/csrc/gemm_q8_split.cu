@@ -300,16 +300,22 @@ ARLE_API int arle_gemm_q8_split(const void* x, const void* sx, const void* w, co
   return ARLE_E_BADARG;
 }
 
-// How many clusters of `parts` SMs the current device runs at a time (an SM holds one block); negative: an error.
-ARLE_API int arle_gemm_q8_split_clusters(int parts) {
+// How many clusters of `parts` SMs a device runs at a time (an SM holds one block); negative: an error.  The current device stays what it is.
+ARLE_API int arle_gemm_q8_split_clusters(int parts, int device) {
   if (parts < 1 || parts > kMostParts) return ARLE_E_BADARG;
+  int was = 0;
+  if (cudaGetDevice(&was) != cudaSuccess || (device != was && cudaSetDevice(device) != cudaSuccess)) return -1;
   auto kern = gemm_q8_split_kernel<1, float>;
-  if (cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedBytes<1>) != cudaSuccess) return -1;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = parts, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kThreadsOf<1>), cfg.gridDim = dim3(parts), cfg.dynamicSmemBytes = kSharedBytes<1>, cfg.attrs = &attr, cfg.numAttrs = 1;
-  int n = 0;
-  return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : -1;
+  int n = -1;
+  if (cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedBytes<1>) == cudaSuccess) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = parts, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreadsOf<1>), cfg.gridDim = dim3(parts), cfg.dynamicSmemBytes = kSharedBytes<1>, cfg.attrs = &attr, cfg.numAttrs = 1;
+    int found = 0;
+    if (cudaOccupancyMaxActiveClusters(&found, kern, &cfg) == cudaSuccess) n = found;
+  }
+  if (device != was && cudaSetDevice(was) != cudaSuccess) return -1;
+  return n;
 }

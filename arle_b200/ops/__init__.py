@@ -143,7 +143,7 @@ _SIGNATURES = {
     "arle_gemm_q8": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P],
     "arle_gemm_q8_pair": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _P, _P],
     "arle_gemm_q8_split": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _I, _P, _P],
-    "arle_gemm_q8_split_clusters": [_I],
+    "arle_gemm_q8_split_clusters": [_I, _I],
     "arle_gemm_q8_few": [_P, _P, _P, _P, _P, _I, ctypes.c_long, _I, _I, _I, _I, _P, _P],
     "arle_gemm_q8_pair_gated": [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P],
     "arle_step_tables": [_P, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _I, _P, _P],
@@ -2862,9 +2862,9 @@ def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
 
 @functools.lru_cache(maxsize=None)
 def _q8_clusters(parts: int, device: int) -> int:
-    """How many clusters of ``parts`` SMs run at a time, one block an SM: an SM's neighbours in a cluster are of its own part of the device, so 148 SMs hold 15
-    clusters of eight."""
-    n = library().arle_gemm_q8_split_clusters(parts)
+    """How many clusters of ``parts`` SMs run at a time on the device of this number, one block an SM: an SM's neighbours in a cluster are of its own part of the
+    device, so 148 SMs hold 15 clusters of eight."""
+    n = library().arle_gemm_q8_split_clusters(parts, device)
     if n <= 0:
         raise KernelError(f"gemm_q8: CUDA error while asking for the number of clusters of {parts}")
     return n
