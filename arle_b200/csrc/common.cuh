@@ -122,12 +122,13 @@ template <typename T> struct HeadTail {
   }
 };
 
-// Programmatic dependent launch.  Every kernel of this library starts with
-// pdl_launch_dependents() (the next kernel of the stream may be scheduled as soon as
-// all CTAs of this one have started) and calls pdl_wait() before it first touches
-// memory that an earlier kernel may have written (until then it may only set up
-// barriers and fetch weights, which no kernel writes).  Both are no-ops for a kernel
-// launched in the ordinary way.
+// Programmatic dependent launch.  A kernel says by pdl_launch_dependents() that the next kernel
+// of the stream may be scheduled (as soon as all its CTAs have said so): most at their start, those
+// with tensor memory once they hold it, those whose followers would take SMs from them at their end,
+// some never.  It calls pdl_wait() before it first reads or writes memory that an earlier kernel may
+// have touched: until then it only sets up barriers and brings lines to L2.  (One exception: the
+// ring product of 16-bit weights, launched so by bit 1 below, fills its ring with weights that no
+// kernel of this library writes.)  Both are no-ops for a kernel launched in the ordinary way.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 

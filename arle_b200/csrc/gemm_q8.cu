@@ -16,7 +16,12 @@ __device__ __forceinline__ void mma_e4m3(float (&c)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint4 load_once(const uint8_t* p) { return __ldcs(reinterpret_cast<const uint4*>(p)); }      // a plain load of what is read once
+// A plain load of what is read once, which stays behind pdl_wait.
+__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 
 // Few rows: bound by the bytes of w, read straight from memory into the operands of mma.sync.  A block owns 16 rows of w and up to eight rows of x; its warp i
 // takes the blocks i, i + WARPS, ... of k.  The order of k inside a block of 128 is free as long as both operands have the same: lane (g, t) takes bytes
@@ -25,10 +30,11 @@ __device__ __forceinline__ uint4 load_once(const uint8_t* p) { return __ldcs(rei
 // across rows, all sizes took longer (4,096 x 12,288 for one row 15 to 26 us instead of 10.3), and so did x fetched a block ahead.
 // A warp has the block of k behind the next one brought to L2 meanwhile: in decode steps of 14 layers of 8B sizes, 193 MB each, a layer takes 53.6 us for 56.0 (one
 // request; the products by themselves gain 0 to 3 %, as weights in turn of 2 GB; everything a warp has left brought at once, or by bulk copies, takes 3 to 7 us more).
-// The first block of w is asked for before the kernel in front has ended (what makes weights lets nothing start before its end).  The next kernel may start when a
-// block's sums are done and not before: long blocks that start early gather on the SMs that have room (the decode attention of eight requests behind a product, and so a layer of
-// 8B sizes, took 20 us more: 81 and 61), and short ones gain nothing (norms, codes and the four products of a layer for one row 46.1 and 44.8 us).
-// One row, us and TB/s, weights in turn of 2 GB: 4,096 x 4,096 5.2 (3.2), 4,096 x 12,288 10.4 (4.8), 6,144 x 4,096 6.4 (3.9), 24,576 x 4,096 18.4 (5.5); eight
+// The first two blocks of w of every warp are brought to L2 while the kernel in front ends and read behind the wait for it, since it may have written them (read in front
+// of it: 5.1 us for 5.3, one row of 4,096 x 4,096; a layer of 8B sizes for one request 54.2 for 55.3).  The next kernel may start when a block's sums are done and not
+// before: long blocks that start early gather on the SMs that have room (the decode attention of eight requests behind a product, and so a layer of 8B sizes, took
+// 20 us more: 81 and 61), and short ones gain nothing (norms, codes and the four products of a layer for one row 46.1 and 44.8 us).
+// One row, us and TB/s, weights in turn of 2 GB: 4,096 x 4,096 5.3 (3.1), 4,096 x 12,288 10.4 (4.8), 6,144 x 4,096 6.4 (3.9), 24,576 x 4,096 18.5 (5.4); eight
 // rows some 3 % more.
 template <int WARPS, int BLOCKS, typename OutT>
 __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const float* sw, OutT* out, long ldo,
@@ -53,9 +59,10 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) gemm_q8_rows_kernel(const 
       asm volatile("prefetch.global.L2 [%0];\n" ::"l"(w1 + (size_t)b * kBlock) : "memory");
     }
   };
-  ask(warp);
+  hint(warp);
   hint(warp + WARPS);
   pdl_wait();
+  ask(warp);
   const uint8_t* xr = x + (size_t)min(m0 + g, M - 1) * K + 32 * t;
   const uint8_t* sxa = sx + (size_t)min(m0 + 2 * t, M - 1) * kb;
   const uint8_t* sxb = sx + (size_t)min(m0 + 2 * t + 1, M - 1) * kb;

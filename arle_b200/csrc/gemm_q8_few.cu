@@ -2,8 +2,8 @@
 // bytes of w: a block owns 128 rows of w, which are the lanes of the tensor cores' accumulators, and all rows of x, which are their columns; a tile's k is cut into
 // parts for a cluster of up to eight blocks.
 //
-// Two blocks share an SM (100 KB and 192 threads each), so one loads while the other starts, hands over or ends, and their first tiles of w are loaded before the kernel
-// in front has ended (what makes weights lets nothing start before its end).  The next kernel may start when a block has joined its parts: norms, codes and the four
+// Two blocks share an SM (100 KB and 192 threads each), so one loads while the other starts, hands over or ends, and their first tiles of w are brought to L2 while the
+// kernel in front ends (and loaded behind the wait for it, since it may have written them: no slower from 16 rows on than loaded in front of it).  The next kernel may start when a block has joined its parts: norms, codes and the four
 // products of a layer of 8B sizes take 55.4 us for 16 rows and 67.6 for 64 when it may start at once, 53.2 and 63.9 so.  The parts of a tile meet in one cluster: each sends a row of x's
 // sums into the shared memory of the block that adds that row up over all parts, in their order, so results do not depend on who was first.
 //   warps 0-3 : lanes 32 i .. + 31: tcgen05.ld, acc[column] += (sx[column] sw) * sum; those factors lie in shared memory, 256 at a time
@@ -75,12 +75,8 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
   if (parts > 1) cluster_started();
   const uint32_t ring = __shfl_sync(0xffffffffu, smem_addr(tiles), 0), full0 = smem_addr(&full_bar[0]), empty0 = smem_addr(&empty_bar[0]),
                  acc_full0 = smem_addr(&acc_full[0]), acc_empty0 = smem_addr(&acc_empty[0]);
-  const int ahead = min(STAGES, b1 - b0);
-  if (warp == kProducer && elect_one())                    // w is not written by the kernel in front
-    for (int i = 0; i < ahead; ++i) {
-      mbar_expect_tx(full0 + 8 * i, STAGE);
-      tma_load_2d(ring + i * STAGE, &map_w, (b0 + i) * BK, n0, full0 + 8 * i);
-    }
+  if (warp == kProducer && elect_one())                    // to L2 and no further: a program may write w in the kernel in front
+    for (int b = b0; b < min(b0 + STAGES, b1); ++b) tma_prefetch_2d(&map_w, b * BK, n0);
   __syncwarp();
   // Tensor memory is asked for when the kernel in front has ended, and the next kernel may start when it is had (in fact far later): a block that held some while it
   // waited for one that still has to get it on the same SM would wait for good.
@@ -100,16 +96,13 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_q8_few_kernel(const __grid_c
     int s = 0;
     uint32_t phase = 1;
     for (int b = b0; b < b1; ++b) {
-      const bool first = b - b0 < ahead;
-      if (!__all_sync(0xffffffffu, first || mbar_wait_bounded(empty0 + 8 * s, phase, aborted))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty0 + 8 * s, phase, aborted))) {
         abort_flag = 1;
         break;
       }
       if (elect_one()) {
-        if (!first) {
-          mbar_expect_tx(full0 + 8 * s, STAGE);
-          tma_load_2d(ring + s * STAGE, &map_w, b * BK, n0, full0 + 8 * s);
-        }
+        mbar_expect_tx(full0 + 8 * s, STAGE);
+        tma_load_2d(ring + s * STAGE, &map_w, b * BK, n0, full0 + 8 * s);
         tma_load_2d(ring + s * STAGE + kTile, &map_x, b * BK, 0, full0 + 8 * s);
       }
       __syncwarp();

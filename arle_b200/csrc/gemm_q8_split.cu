@@ -10,7 +10,7 @@
 // measured).  A tile of 256 columns reads x once for twice the products, 768 and 512 clocks, and is taken where k is long: 333 rows of 5,120 x 25,600 take 75 us in tiles
 // of 128 and 61 in two parts of tiles of 256; its sums go where the ring was, behind one more barrier of the cluster.
 //   warps 0-7        : lanes 32 (i % 4) .. + 31, columns 64 (i / 4) .. + 63 of every 128: tcgen05.ld, acc += (sx sw) * sum
-//   warp 8           : producer, a TMA load of 128 rows of x and one of w a stage; what of w fits the ring is asked for before the kernel in front has ended
+//   warp 8           : producer, a TMA load of 128 rows of x and one of w a stage; what of w fits the ring is brought to L2 while the kernel in front ends
 //   warp 9           : issues the products (128 x 128 or 256 x 32)
 // Edges: TMA fills rows beyond M and N with zeros; stores are guarded.  Every wait is bounded; who gives up raises the error word and still comes to the
 // cluster's barriers.
@@ -64,12 +64,8 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
   if (NB == 1 && parts > 1) cluster_started();             // (with two blocks of columns a barrier of its own stands in front of the stores)
   const uint32_t ring = __shfl_sync(0xffffffffu, smem_addr(tiles), 0), full0 = smem_addr(&full_bar[0]), empty0 = smem_addr(&empty_bar[0]),
                  acc_full0 = smem_addr(&acc_full[0]), acc_empty0 = smem_addr(&acc_empty[0]);
-  const int ahead = min(kStages, b1 - b0);
-  if (warp == kProducer && elect_one())                    // w is not written by the kernel in front
-    for (int i = 0; i < ahead; ++i) {
-      mbar_expect_tx(full0 + 8 * i, STAGE);
-      tma_load_2d(ring + i * STAGE, &map_w, (b0 + i) * BK, n0, full0 + 8 * i);
-    }
+  if (warp == kProducer && elect_one())                    // to L2 and no further: a program may write w in the kernel in front
+    for (int b = b0; b < min(b0 + kStages, b1); ++b) tma_prefetch_2d(&map_w, b * BK, n0);
   __syncwarp();
   // Tensor memory is asked for when the kernel in front has ended, and the next kernel may start when it is had (in fact far later): a block that held some while it
   // waited for one that still has to get it on the same SM would wait for good.
@@ -88,16 +84,13 @@ __global__ void __launch_bounds__(kThreadsOf<NB>, 1) gemm_q8_split_kernel(const 
     int s = 0;
     uint32_t phase = 1;
     for (int b = b0; b < b1; ++b) {
-      const bool first = b - b0 < ahead;
-      if (!__all_sync(0xffffffffu, first || mbar_wait_bounded(empty0 + 8 * s, phase, aborted))) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(empty0 + 8 * s, phase, aborted))) {
         abort_flag = 1;
         break;
       }
       if (elect_one()) {
-        if (!first) {
-          mbar_expect_tx(full0 + 8 * s, STAGE);
-          tma_load_2d(ring + s * STAGE, &map_w, b * BK, n0, full0 + 8 * s);
-        }
+        mbar_expect_tx(full0 + 8 * s, STAGE);
+        tma_load_2d(ring + s * STAGE, &map_w, b * BK, n0, full0 + 8 * s);
         tma_load_2d(ring + s * STAGE + NB * kTile, &map_x, b * BK, m0, full0 + 8 * s);
       }
       __syncwarp();

@@ -5,7 +5,7 @@
 // finite do not count for the scale and become NaN: e4m3 has no infinities, and what was not finite must not come out of a product as if it were.
 // Weights: the same for blocks of 128 x 128, one float32 scale a block.
 // All are launched early: plain loads, and what a block loads is small beside what its neighbours have under way.  It saves one token's codes 0.4 us in a
-// chain, a weight of 24,576 x 4,096 2, the norm of 1,024 rows of 4,096 0.4 and that of 4,096 rows 0.9 (a weight's kernel lets nothing start before its end).
+// chain, a weight of 24,576 x 4,096 2, the norm of 1,024 rows of 4,096 0.4 and that of 4,096 rows 0.9 (a weight's kernel lets nothing start before its end: it runs once, at load).
 // All four kernels read every number once, keep it in registers between the maximum and the rounding, and are bound by DRAM (few rows: by latency).
 #include "q8.cuh"
 #include "scan_utils.cuh"
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* x, long row
 // number is not finite they are read again.  24,576 x 4,096 bfloat16 45 us, 6.7 TB/s; 1,001 x 777 float32, whose rows are not aligned, 3.3 us (6.4 when they were read twice).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256, ALIGNED && sizeof(T) == 2 ? 4 : 2) quantize_weight_kernel(const T* w, long row_stride, uint8_t* codes, float* scales, int N, int K, int kb) {
-  pdl_wait();      // and lets nothing start early: the products ask for weights before they wait for the kernel in front of them
+  pdl_wait();
   constexpr int V = 16 / sizeof(T), LANES = kGroup / V, ROWS = 256 / LANES, STEPS = kGroup / ROWS;
   __shared__ uint32_t most_s[8];
   const int b = blockIdx.x, sub = threadIdx.x % LANES, n0 = blockIdx.y * kGroup + threadIdx.x / LANES, at = b * kGroup + sub * V;

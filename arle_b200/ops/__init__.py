@@ -2595,8 +2595,8 @@ def q8_width(k: int) -> int:
 class Q8Weight:
     """A weight [out_features, in_features] in 8 bits: ``codes`` contiguous float8_e4m3fn [N, q8_width(K)], zero from column K on, and ``scales`` contiguous
     float32 [ceil(N / 128), ceil(K / 128)], positive, one for each block of 128 x 128; a number is code * scale.  ``quantize_weight_q8`` makes both from a
-    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two).  Products may ask for a weight before the kernel in
-    front of them in the stream has ended, so it is written by ``quantize_weight_q8``, by torch or by a copy, not by another of this package's kernels."""
+    matrix; checkpoints of block-wise 8-bit models store them (their scales need not be powers of two).  Products read a weight
+    behind the wait for the kernel in front of them in the stream, whichever that is."""
 
     __slots__ = ("codes", "scales", "shape")
 
