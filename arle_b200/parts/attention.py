@@ -46,8 +46,8 @@ from typing import ClassVar, Optional, Tuple
 import torch
 
 from .. import ops
-from ..weights.q8 import as_q8_weight
-from .base import CacheNeed, Mixer, StateNeed, WeightDecl, product, q8_weight
+from ..weights.q8 import stored_q8_weight
+from .base import CacheNeed, Mixer, StateNeed, WeightDecl, product
 from .registry import build_part, register_part
 
 
@@ -245,8 +245,8 @@ class Attention(Mixer):
         if not self.takes_q8_weights():
             super().quantize_weights(tensors)
         device = self.w_o.device
-        self.w_qkv = as_q8_weight([tensors[self._name(r)] for r in ("q", "k", "v")], device) or q8_weight(self.w_qkv)
-        self.w_o = as_q8_weight([tensors[self._name("o")]], device) or q8_weight(self.w_o)
+        self.w_qkv = stored_q8_weight(tensors, [self._name(r) for r in ("q", "k", "v")], device)
+        self.w_o = stored_q8_weight(tensors, [self._name("o")], device)
 
     def takes_q8_rows(self):
         return isinstance(self.w_qkv, ops.Q8Weight)

@@ -149,13 +149,6 @@ class Part:
         return False
 
 
-def q8_weight(matrix) -> "ops.Q8Weight":
-    """A matrix on the device as codes and scales."""
-    n, k = matrix.shape
-    codes = torch.empty((n, ops.q8_width(k)), dtype=torch.float8_e4m3fn, device=matrix.device)
-    return ops.quantize_weight_q8(matrix, codes, torch.empty((-(-n // ops.Q8_BLOCK), codes.shape[1] // ops.Q8_BLOCK), dtype=torch.float32, device=matrix.device))
-
-
 def q8_rows(ws, name: str, rows: int, width: int, dtype) -> "ops.Q8Rows":
     """Room for rows in 8 bits among the step's buffers."""
     k = ops.q8_width(width)

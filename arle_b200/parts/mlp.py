@@ -11,8 +11,8 @@ from typing import ClassVar, Tuple
 import torch
 
 from .. import ops
-from ..weights.q8 import as_q8_weight
-from .base import FeedForward, WeightDecl, q8_rows, q8_weight
+from ..weights.q8 import stored_q8_weight
+from .base import FeedForward, WeightDecl, q8_rows
 from .registry import register_part
 
 
@@ -61,10 +61,8 @@ class GatedMlp(FeedForward):
     def quantize_weights(self, tensors):
         if not self.takes_q8_weights():
             super().quantize_weights(tensors)
-        g, u, d = (tensors[self.spec.prefix + n] for n in self.spec.names)
-        device = self.w_down.device
-        self.w_gate_up = ops.pack_gate_up_q8(as_q8_weight([g], device) or q8_weight(self.w_gate_up[0::2]), as_q8_weight([u], device) or q8_weight(self.w_gate_up[1::2]))
-        self.w_down = as_q8_weight([d], device) or q8_weight(self.w_down)
+        g, u, d = (stored_q8_weight(tensors, [self.spec.prefix + n], self.w_down.device) for n in self.spec.names)
+        self.w_gate_up, self.w_down = ops.pack_gate_up_q8(g, u), d
 
     def takes_q8_rows(self):
         return isinstance(self.w_down, ops.Q8Weight)

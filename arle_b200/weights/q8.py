@@ -4,6 +4,7 @@ them and turned into 16 bits by all others.
 """
 from __future__ import annotations
 
+import warnings
 from typing import Optional, Sequence
 
 import torch
@@ -48,3 +49,25 @@ def as_q8_weight(parts: Sequence, device) -> Optional["ops.Q8Weight"]:
         codes[at: at + p.shape[0], :k] = p.codes.view(torch.uint8).to(device)
         at += p.shape[0]
     return ops.Q8Weight(codes.view(torch.float8_e4m3fn), torch.cat([p.scales for p in parts]).to(device).contiguous())
+
+
+def q8_weight(matrix) -> "ops.Q8Weight":
+    """A matrix on the device as codes and scales."""
+    from .. import ops
+
+    n, k = matrix.shape
+    codes = torch.empty((n, ops.q8_width(k)), dtype=torch.float8_e4m3fn, device=matrix.device)
+    return ops.quantize_weight_q8(matrix, codes, torch.empty((-(-n // ops.Q8_BLOCK), codes.shape[1] // ops.Q8_BLOCK), dtype=torch.float32, device=matrix.device))
+
+
+def stored_q8_weight(tensors: dict, names: Sequence[str], device) -> "ops.Q8Weight":
+    """The named matrices one under the other as codes and scales: a checkpoint's own where one weight can have them, else found from the numbers as they are stored (in
+    16 or 32 bits; code * scale in 32), so that these are rounded once."""
+    matrices = [tensors[n] for n in names]
+    own = as_q8_weight(matrices, device)
+    if own is not None:
+        return own
+    if any(isinstance(m, StoredQ8) for m in matrices):
+        warnings.warn(f"{', '.join(names)}: stored in 8 bits, but not all of them, or two would share a block of 128 rows: the codes are found anew")
+    wide = torch.bfloat16 if all(m.dtype == torch.bfloat16 and not isinstance(m, StoredQ8) for m in matrices) else torch.float32
+    return q8_weight(torch.cat([m.to(device=device, dtype=wide) for m in matrices]))
