@@ -1,6 +1,6 @@
 """Weights that a checkpoint stores in 8 bits: e4m3 codes "<name>" beside float32 (or 16-bit) scales "<name>_scale_inv", one for each block of 128 x 128; a
 weight is code * scale.  cklxx/arle reads such pairs for its quantised weights (infer/src/weight_loader.rs); here they are kept as they are by the parts that run on
-them and turned into 16 bits by all others.
+them and turned into the engine's type by all others.
 """
 from __future__ import annotations
 
@@ -14,20 +14,21 @@ SCALE_SUFFIX = "_scale_inv"
 
 
 class StoredQ8:
-    """A stored matrix [N, K]: ``codes`` float8_e4m3fn [N, K] and ``scales`` float32 [ceil(N / 128), ceil(K / 128)], on the host.  ``to`` gives its numbers,
-    so a part that knows nothing of codes loads it like any other tensor (rounded to bfloat16 where it asks for that)."""
+    """A stored matrix [N, K]: ``codes`` float8_e4m3fn [N, K] and ``scales`` float32 [ceil(N / 128), ceil(K / 128)], on the host.  ``to`` gives its numbers
+    (bfloat16 where no type is asked for), so a part that knows nothing of codes loads it like any other tensor.  ``dtype`` is what holds them, four bits times a float32
+    scale: an engine of 32 bits keeps them as such."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         n, k = codes.shape
         if tuple(scales.shape) != (-(-n // BLOCK), -(-k // BLOCK)):
             raise ValueError(f"scales {tuple(scales.shape)} do not fit codes {tuple(codes.shape)} in blocks of {BLOCK}")
         self.codes, self.scales, self.shape = codes, scales.to(torch.float32), codes.shape
-        self.dtype = torch.bfloat16
+        self.dtype = torch.float32
 
     def to(self, device=None, dtype=None) -> torch.Tensor:
         codes, scales = self.codes.to(device=device), self.scales.to(device=device)
         n, k = self.shape
-        out = torch.empty((n, k), dtype=dtype or self.dtype, device=codes.device)
+        out = torch.empty((n, k), dtype=dtype or torch.bfloat16, device=codes.device)
         for i in range(0, n, 32 * BLOCK):                  # a few blocks of rows at a time: in float32 a matrix is four times its codes
             j = min(n, i + 32 * BLOCK)
             s = scales[i // BLOCK: -(-j // BLOCK)].repeat_interleave(BLOCK, dim=0)[: j - i].repeat_interleave(BLOCK, dim=1)[:, :k]
@@ -69,5 +70,5 @@ def stored_q8_weight(tensors: dict, names: Sequence[str], device) -> "ops.Q8Weig
         return own
     if any(isinstance(m, StoredQ8) for m in matrices):
         warnings.warn(f"{', '.join(names)}: stored in 8 bits, but not all of them, or two would share a block of 128 rows: the codes are found anew")
-    wide = torch.bfloat16 if all(m.dtype == torch.bfloat16 and not isinstance(m, StoredQ8) for m in matrices) else torch.float32
+    wide = torch.bfloat16 if all(m.dtype == torch.bfloat16 for m in matrices) else torch.float32
     return q8_weight(torch.cat([m.to(device=device, dtype=wide) for m in matrices]))

@@ -71,3 +71,18 @@ def test_nothing_is_said_where_codes_are_kept(q8_kernels):  # noqa: F811
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         model.load(tensors, torch.bfloat16, "cpu", weight_dtype="float8_e4m3")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_stored_codes_in_the_engine_s_type(dtype):
+    """Without ``weight_dtype`` stored codes become numbers of the engine's type, rounded to it once: a float32 engine has code * scale as float32 holds it."""
+    tensors, model = _tensors(dict(CONFIG, num_hidden_layers=1, tie_word_embeddings=False), 3, lambda name, t: _stored(t))
+    tensors["lm_head.weight"] = _stored(tensors["lm_head.weight"])
+    model.load(tensors, dtype, "cpu")
+    mixer, ffn = model.blocks[0].mixer, model.blocks[0].ffn
+    want = {r: _numbers(tensors[LAYER + f"{p}.{r}_proj.weight"]).to(torch.float32).to(dtype)
+            for p, rs in (("self_attn", "qkvo"), ("mlp", ("gate", "up", "down"))) for r in rs}
+    assert torch.equal(mixer.w_qkv, torch.cat([want[r] for r in "qkv"])) and torch.equal(mixer.w_o, want["o"])
+    assert torch.equal(ffn.w_gate_up[0::2], want["gate"]) and torch.equal(ffn.w_gate_up[1::2], want["up"]) and torch.equal(ffn.w_down, want["down"])
+    assert torch.equal(model.head, _numbers(tensors["lm_head.weight"]).to(torch.float32).to(dtype))
+    assert model.head.dtype == mixer.w_o.dtype == ffn.w_down.dtype == dtype
