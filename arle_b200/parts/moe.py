@@ -27,6 +27,7 @@ from typing import ClassVar, Optional, Tuple
 import torch
 
 from .. import ops
+from ..weights.q8 import as_tensor
 from .base import FeedForward, WeightDecl
 from .registry import build_part, register_part
 
@@ -116,9 +117,9 @@ class RoutedExperts(FeedForward):
             self.correction = tensors[self._name("correction")].to(device=device, dtype=torch.float32).contiguous()
         gu, dn = [], []
         for e in range(s.num_experts):
-            u, d = (tensors[self._name(n, e)] for n in ("up", "down"))
+            u, d = (as_tensor(tensors[self._name(n, e)], dtype) for n in ("up", "down"))
             if s.gated:
-                u = torch.stack([tensors[self._name("gate", e)], u], dim=1).reshape(2 * s.expert_ff, s.hidden_size)      # rows 2i, 2i + 1: gate_i, up_i
+                u = torch.stack([as_tensor(tensors[self._name("gate", e)], dtype), u], dim=1).reshape(2 * s.expert_ff, s.hidden_size)      # rows 2i, 2i + 1: gate_i, up_i
             gu.append(u)
             dn.append(d)
         self.w_gate_up = torch.stack(gu).to(device=device, dtype=kept(gu)).contiguous()

@@ -36,6 +36,11 @@ class StoredQ8:
         return out
 
 
+def as_tensor(t, dtype: torch.dtype) -> torch.Tensor:
+    """A stored tensor as one: codes become the numbers of an engine of this type."""
+    return t.to(dtype=dtype) if isinstance(t, StoredQ8) else t
+
+
 def as_q8_weight(parts: Sequence, device) -> Optional["ops.Q8Weight"]:
     """Stored matrices one under the other as one weight with their own codes and scales; None where that cannot be (one of them is not stored in 8 bits, or ends
     inside a block that the next one would share)."""

@@ -6,6 +6,7 @@ import torch
 
 import q8_linear_refs as refs
 from arle_b200.engine.loading import random_model
+from arle_b200.parts.moe import RoutedExperts, RoutedExpertsSpec
 from arle_b200.weights import random_tensors
 from arle_b200.weights.q8 import StoredQ8
 from test_weights_q8_engine_cpu import CONFIG, q8_kernels  # noqa: F401 (a fixture)
@@ -86,3 +87,22 @@ def test_stored_codes_in_the_engine_s_type(dtype):
     assert torch.equal(ffn.w_gate_up[0::2], want["gate"]) and torch.equal(ffn.w_gate_up[1::2], want["up"]) and torch.equal(ffn.w_down, want["down"])
     assert torch.equal(model.head, _numbers(tensors["lm_head.weight"]).to(torch.float32).to(dtype))
     assert model.head.dtype == mixer.w_o.dtype == ffn.w_down.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gated", [True, False])
+def test_stored_codes_of_experts(dtype, gated):
+    """Parts that know nothing of codes load them like any other tensor, experts (which are stacked) among them."""
+    spec = RoutedExpertsSpec(prefix="m.", hidden_size=130, num_experts=3, top=1, expert_ff=40, correction=False, gated=gated, activation="silu" if gated else "square_relu")
+    loaded = []
+    for stored in (True, False):
+        part = RoutedExperts(spec)
+        tensors = {}
+        for i, d in enumerate(part.weight_decls()):
+            q = _stored(torch.randn(d.shape, generator=torch.Generator().manual_seed(i)), i)
+            tensors[d.name] = q if stored else q.to(dtype=dtype)
+        part.load(tensors, dtype, "cpu")
+        loaded.append(part)
+    for name in ("w_router", "w_gate_up", "w_down"):
+        a, b = (getattr(p, name) for p in loaded)
+        assert a.dtype == b.dtype == dtype and torch.equal(a, b)
