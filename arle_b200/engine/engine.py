@@ -41,8 +41,8 @@ class EngineOptions:
     cuda_graph: bool = True
     kernel_set: str = "fast"                   # "plain": the general kernels only, whatever the shapes
     cache_dtype: str = "auto"                  # "auto": keys and values as the model computes them; "float8_e4m3": 8-bit codes, a scale per page and head
-    weight_dtype: str = "auto"                 # "auto": as the model computes; "float8_e4m3": the blocks' matrices as 8-bit codes, a scale per 128 x 128
     device_tables: bool = False                # a step's tables are made on the device from its requests' lengths, instead of copied there
+    weight_dtype: str = "auto"                 # "auto": as the model computes; "float8_e4m3": the blocks' matrices as 8-bit codes, a scale per 128 x 128
 
 
 @dataclass
