@@ -229,7 +229,7 @@ __device__ __forceinline__ void subtract_sticky(f32x2 a, f32x2 b, float& lo, flo
 
 // 1 / sqrt(m) as two float32 numbers: an approximation y and half its residual, y + y (1 - m y^2) / 2 (one step of Newton's method).  For m in kLeastMean .. kMostMean,
 // where y^2, its rounding error and what m has beside its float32 number are all normal numbers, and the sums of squares behind m are.
-constexpr double kLeastMean = 0x1p-90, kMostMean = 0x1p100;
+constexpr float kLeastMean = 0x1p-90f, kMostMean = 0x1p100f;
 __device__ __forceinline__ float2 inverse_root(double m) {
   const float mh = (float)m, ml = (float)(m - (double)mh), y = rsqrtf(mh);
   const float q = y * y, ql = fmaf(y, y, -q);
@@ -270,10 +270,12 @@ __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], 
 
 // A row whose mean square float32 does not carry: numbers whose squares leave its range (from some 10^15 on, or below 10^-13 beside no eps), infinities
 // (they come out as NaN and the row's finite numbers as zero, 1 / sqrt(inf) times them), NaN (all of the row).  Everything in 64 bits, from the numbers in memory:
-// `x` and, where it is still to be added, `delta`; sum_out is null where it has been written.  The filled-up columns are zero whatever the row holds.
+// `x` and, where their sum is kept nowhere, `delta`.  The filled-up columns are zero whatever the row holds.  It comes behind the others' path and writes over what
+// that made, each thread its own places: a branch in the middle, around which the compiler moves nothing, made all rows slower (5,003 rows of 5,120, alone in a graph,
+// 57.5 us; at the end 56.6; with no second path 55.5).
 template <typename TA>
-__device__ __noinline__ void extreme_row(const float* x, const TA* delta, float delta_scale, const float* gain, float* sum_out, uint8_t* codes, uint8_t* scales, int H,
-                                         int kb, double inv_h, float eps, double* scratch) {
+__device__ __noinline__ void extreme_row(const float* x, const TA* delta, float delta_scale, const float* gain, uint8_t* codes, uint8_t* scales, int H, int kb,
+                                         double inv_h, float eps, double* scratch) {
   auto number = [&](int at) { return at >= H ? 0.f : delta ? fmaf(delta_scale, to_f32(delta[at]), x[at]) : x[at]; };
   double ss = 0.0;
   for (int slot = threadIdx.x; slot < 32 * kb; slot += blockDim.x)
@@ -288,9 +290,7 @@ __device__ __noinline__ void extreme_row(const float* x, const TA* delta, float 
     float v[4];
     for (int j = 0; j < 4; ++j) {
       const int at = 4 * slot + j;
-      const float sum = number(at);
-      if (sum_out && at < H) sum_out[at] = sum;
-      const double y = at < H ? (double)sum * r * (double)gain[at] : 0.0;
+      const double y = at < H ? (double)number(at) * r * (double)gain[at] : 0.0;
       v[j] = __double2float_rz(y);                          // the last bit set where that left something out (see subtract_sticky)
       if ((double)v[j] != y) v[j] = __uint_as_float(__float_as_uint(v[j]) | 1u);
     }
@@ -360,12 +360,7 @@ __global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(cons
   }
   // (inside a warp additions of 32 bits, whose errors are independent from warp to warp and average out, across warps of 64)
   const double mean = block_sum64((double)warp_sum(low2(ss) + high2(ss)), red) * inv_h + (double)eps;
-  if (!(mean > kLeastMean && mean < kMostMean)) {
-    const bool written = PER > 0 && so;
-    extreme_row<TA>(written ? so : xr, written ? nullptr : dr, delta_scale, gain, PER > 0 ? nullptr : so, codes + (size_t)row * kb * kGroup, scales + (size_t)row * kb, H,
-                    kb, inv_h, eps, red);
-    return;
-  }
+  const bool extreme = !((float)mean > kLeastMean && (float)mean < kMostMean);
   const float2 inv = inverse_root(mean);
   const RowFactor factor = {pair2(inv.x, inv.x), pair2(inv.y, inv.y), pair2(-inv.x, -inv.x), pair2(-inv.y, -inv.y)};
   if constexpr (PER > 0) {
@@ -384,6 +379,7 @@ __global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(cons
       finish_four(x[0], gw[0], factor, codes, scales, (size_t)row * kb, slot);
     }
   }
+  if (extreme) extreme_row<TA>(so ? so : xr, so ? nullptr : dr, delta_scale, gain, codes + (size_t)row * kb * kGroup, scales + (size_t)row * kb, H, kb, inv_h, eps, red);
 }
 
 // ------------------------------------------------------------------ gate
