@@ -80,9 +80,8 @@ __device__ __forceinline__ void store_row(OutT* dst, const uint64_t (&acc)[C], i
 
 template <int STAGES, bool GATED, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1) gemm_q8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                                                                   const uint8_t* __restrict__ sx, const float* __restrict__ sw, OutT* __restrict__ out,
-                                                                   long ldo, uint8_t* __restrict__ out_scales, int M, int N, int kb, int act,
-                                                                   int* __restrict__ err) {
+                                                                   const uint8_t* sx, const float* sw, OutT* out, long ldo, uint8_t* out_scales, int M,
+                                                                   int N, int kb, int act, int* err) {
   pdl_wait();
   constexpr uint32_t STAGE = 2 * kTile;
   extern __shared__ unsigned char smem_dyn[];

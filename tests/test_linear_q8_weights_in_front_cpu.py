@@ -27,3 +27,11 @@ def test_nothing_is_loaded_in_front_of_the_wait(name):
 
 def test_all_products():
     assert set(FILES) == {"gemm_q8.cu", "gemm_q8_few.cu", "gemm_q8_split.cu", "gemm_q8_tc.cu"}
+
+
+@pytest.mark.parametrize("name", FILES + ["linear_q8.cu"])
+def test_operands_are_read_by_plain_loads(name):
+    """A kernel that may live beside the one in front of it (all of these, when programmatic launches are on) reads what that one writes by plain loads: not by the way for
+    memory that nobody writes meanwhile, which the compiler takes for pointers that are const and restrict."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(build.CSRC, name)).read())
+    assert not re.search(r"const\s+\w+\s*\*\s*__restrict__|__ldg\(|ld\.global\.nc", text)

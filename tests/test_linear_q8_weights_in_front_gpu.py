@@ -42,3 +42,37 @@ def test_codes_that_a_kernel_has_just_written(m, n, k):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(out, want[i % 2]) for i, out in enumerate(outs))
+
+
+@pytest.mark.parametrize("kind,parts,m", [("pair", 1, 300), ("pair", 1, 2100), ("split", 3, 300), ("split2", 2, 300), ("few", 4, 60), ("rows", 1, 8)])
+def test_chains_with_every_kernel_launched_early(kind, parts, m, monkeypatch):
+    """Forty links of codes, product and codes again, all kernels launched programmatically: the same as with a wait behind each."""
+    h = 1024
+    monkeypatch.setattr(ops, "_q8_route", lambda M, N, kb, device: (kind, parts, 0.0))
+    g = torch.Generator().manual_seed(m)
+    ws = [_operands(1, h, h, 70 + i)[2] for i in range(3)]
+    for q in ws:
+        q.scales.mul_(10.0)
+    x, y = torch.randn(m, h, generator=g).to(DEV), torch.empty((m, h), device=DEV)
+    c, s = torch.empty((m, h), dtype=E4M3, device=DEV), torch.empty((m, h // 128), dtype=torch.uint8, device=DEV).view(E8M0)
+
+    def chain(wait):
+        ops.quantize_q8(x, c, s)
+        for i in range(40):
+            ops.gemm_q8(c, s, ws[i % 3], y)
+            if wait:
+                torch.cuda.synchronize()
+            ops.quantize_q8(y, c, s)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return y.clone()
+
+    want = chain(True)
+    ops.set_programmatic_launch(1)
+    try:
+        got = chain(False)
+    finally:
+        ops.set_programmatic_launch(0)
+    assert want.isfinite().all() and torch.equal(got, want)
+    ops.check_errors(DEV)
