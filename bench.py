@@ -444,6 +444,8 @@ def main() -> int:
                     help="with --only gemm: one product only (for a profiler capture)")
     ap.add_argument("--context", type=int, default=CONTEXT, help="with --only decode: tokens each request holds")
     ap.add_argument("--prefill-tokens", type=int, default=PREFILL_TOKENS, help="with --only prefill: tokens of the prompt")
+    ap.add_argument("--weight-dtype", choices=["auto", "float8_e4m3"], default="auto",
+                    help="with --only decode / --only prefill: float8_e4m3, the layers' matrices in 8 bits (a layer's time: two runs' difference, --layers 14 and 2)")
     ap.add_argument("--no-cuda-graph", action="store_true")
     ap.add_argument("--no-kernel-times", action="store_true",
                     help="with --design: leave out the per-kernel times (they come from torch's profiler, which cannot run under another profiler)")
@@ -471,6 +473,9 @@ def main() -> int:
     if args.only == "all" and not args.design and (args.context != CONTEXT or args.prefill_tokens != PREFILL_TOKENS):
         print("bench.py: --context and --prefill-tokens go with --only decode / --only prefill; the full run keeps the contract's sizes")
         return 2
+    if args.weight_dtype != "auto" and (args.only not in ("decode", "prefill") or args.design):
+        print("bench.py: --weight-dtype goes with --only decode / --only prefill; the full run is of 16 bits")
+        return 2
     globals()["CONTEXT"], globals()["PREFILL_TOKENS"] = args.context, args.prefill_tokens
 
     import torch
@@ -495,7 +500,7 @@ def main() -> int:
     if args.only == "gemm":
         return gemm_table(args, sizes, torch, ops)
     layers = args.layers or sizes["num_hidden_layers"]
-    model = random_model(sizes, seed=0, dtype="bfloat16", device=dev, num_layers=layers)
+    model = random_model(sizes, seed=0, dtype="bfloat16", device=dev, num_layers=layers, weight_dtype=args.weight_dtype)
     spec = model.spec
     vocab = spec.vocab_size
     page = 16
@@ -562,7 +567,7 @@ def main() -> int:
 
     if args.only == "decode":
         ms, launches, _ = decode_run(args.batch, args.steps, args.warmup)
-        rec = {"only": "decode", "batch": args.batch, "layers": layers, "ms_per_step": round(ms, 4), "gpu_launches": int(launches)}
+        rec = {"only": "decode", "batch": args.batch, "layers": layers, "weight_dtype": args.weight_dtype, "ms_per_step": round(ms, 4), "gpu_launches": int(launches)}
         if args.timeline:
             from torch.profiler import ProfilerActivity, profile
             with profile(activities=[ProfilerActivity.CUDA]) as prof:
@@ -616,7 +621,7 @@ def main() -> int:
             apart.append(prefill_once(f"a{i}"))
         pf_ms = sorted(apart)[2]
     if args.only == "prefill":
-        rec = {"only": "prefill", "layers": layers, "ms": round(pf_ms, 3)}
+        rec = {"only": "prefill", "layers": layers, "weight_dtype": args.weight_dtype, "ms": round(pf_ms, 3)}
         if args.timeline:
             from torch.profiler import ProfilerActivity, profile
             with profile(activities=[ProfilerActivity.CUDA]) as prof:
