@@ -1,7 +1,8 @@
 // Products of e4m3 codes with a scale for each block of 128 numbers of k:
 //     out[m, n] = sum over blocks b of  sx[m, b] * sw[n / 128, b] * sum over k in b of  x[m, k] * w[n, k]
 // x [M, K] and w [N, K] codes, K = 128 kb (filled up with codes of zero), sx powers of two (one byte: exponent + 127), sw float32.  A block's inner sum is
-// formed by the tensor cores, every block's sum is scaled and added up in float32 registers; the only rounding is the store (bfloat16 or none).
+// formed by the tensor cores in float32 (products of two codes are exact), every block's sum is scaled by sx sw and added up in float32, in the order of k and then of
+// the warps or parts that shared k: (127 + kb + 2) half steps of the terms' magnitudes at most.  The store rounds to bfloat16 or not at all.
 #include "q8.cuh"
 using namespace arle;
 

@@ -8,7 +8,7 @@
 // As in gemm_q8_tc.cu the tensor cores hand over every block's sums and the warps add them into registers; four accumulators of 128 columns, or two of 256, take
 // turns.  A tile of 128 x 128 is bound by shared memory: 32 KB a block of k arrive and are read again, 512 clocks of it beside the 256 of the products (some 600
 // measured).  A tile of 256 columns reads x once for twice the products, 768 and 512 clocks, and is taken where k is long: 333 rows of 5,120 x 25,600 take 75 us in tiles
-// of 128 and 61 in two parts of tiles of 256; its sums go where the ring was, behind one more barrier of the cluster.
+// of 128 and 61 in two parts of tiles of 256, alone in a graph (72 among calls one by one, at the power limit's clocks); its sums go where the ring was, behind one more barrier of the cluster.
 //   warps 0-7        : lanes 32 (i % 4) .. + 31, columns 64 (i / 4) .. + 63 of every 128: tcgen05.ld, acc += (sx sw) * sum
 //   warp 8           : producer, a TMA load of 128 rows of x and one of w a stage; what of w fits the ring is brought to L2 while the kernel in front ends
 //   warp 9           : issues the products (128 x 128 or 256 x 32)

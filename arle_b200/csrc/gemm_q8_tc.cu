@@ -4,9 +4,9 @@
 // A scale that changes every 128 numbers of k cannot be applied behind the whole sum, so the tensor cores hand over every block's sum: an accumulator of 128
 // lanes x 256 columns is one block of k (four tcgen05.mma of 32), two of them take turns in the 512 columns of tensor memory, and the epilogue warps add
 // block after block into registers, acc += (sx[row] sw[block of columns]) * sum.  A lane is a row of x and 128 columns are one block of w, so that
-// factor is one number a thread and 128 columns.  A block's products take the tensor cores 512 clocks, reading and adding its sums takes the warps some 270
-// beside one another, handing accumulators back and forth between the two SMs the rest: 670 to 790 clocks a block (4,096 rows of 4,096 x 12,288).
-// 4,096 rows of 4,096 x 12,288 181 us alone (2.3 PFLOP/s), 214 back to back, where 1,000 W hold the clock at 1.4 GHz; gated, 24,576 x 4,096, 351 and 408.
+// factor is one number a thread and 128 columns.  A block's products take the tensor cores 512 clocks, reading and adding its sums takes the warps some 270,
+// and a block takes 670 to 790 (4,096 rows of 4,096 x 12,288).  With two accumulators in turn the 270 should be hidden; what the rest waits for has not been measured.
+// 4,096 rows of 4,096 x 12,288 179 us alone (2.3 PFLOP/s), 209 to 212 back to back, where 1,000 W hold the clock at 1.4 GHz; gated, 24,576 x 4,096, 350 and 408.
 //
 // Per CTA, by warp:
 //   warps 0-7        : epilogue of the CTA's 128 rows; warp i reads lanes 32 (i % 4) .. + 31, of columns 64 h .. 64 h + 63 and 128 + 64 h .. (h = i / 4).  Gated,

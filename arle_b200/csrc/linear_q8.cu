@@ -6,7 +6,8 @@
 // Weights: the same for blocks of 128 x 128, one float32 scale a block.
 // All are launched early: plain loads, and what a block loads is small beside what its neighbours have under way.  It saves one token's codes 0.4 us in a
 // chain, a weight of 24,576 x 4,096 2, the norm of 1,024 rows of 4,096 0.4 and that of 4,096 rows 0.9 (a weight's kernel lets nothing start before its end: it runs once, at load).
-// All four kernels read every number once, keep it in registers between the maximum and the rounding, and are bound by DRAM (few rows: by latency).
+// The kernels read a number once and keep it in registers between the maximum and the rounding (twice: norms whose rows are not on 16-byte boundaries or too long to keep,
+// weights with numbers that are not finite, rows of extreme_row), and are bound by DRAM (few rows: by latency).  Times are those of a kernel alone in a captured graph.
 #include "q8.cuh"
 #include "scan_utils.cuh"
 using namespace arle;
@@ -85,7 +86,7 @@ template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void load_
 // ------------------------------------------------------------------ rows
 // A lane takes 16 bytes of a group: a group is 16 lanes of bfloat16 or 32 of float32; it takes them of kAtOnce groups, which are under way together (one at a time
 // 6,001 rows of 8,192 bfloat16 took 37 us, four 28), and stay as they lie in memory up to the rounding: maxima of two bfloat16 at a time, and a multiplication for
-// the division by the row's groups, 23.5: 6.4 TB/s.  One row of 4,096 1.5 us alone.
+// the division by the row's groups, 23.6: 6.4 TB/s (26.6 among calls from Python one by one).  One row of 4,096 1.6 us.
 constexpr int kAtOnce = 4;
 
 template <typename T, bool ALIGNED>
@@ -240,8 +241,8 @@ __device__ __forceinline__ float2 inverse_root(double m) {
 // ------------------------------------------------------------------ residual sum, norm, codes
 // A code is off where an error carries a number over the border between two codes, in steps of an eighth of the number.  So the sum of squares is of 64 bits from a
 // warp's sums on, the factor of a row is a pair of float32 numbers, and where its product with a number would round onto a border it is rounded as subtract_sticky
-// does.  Of the 25.6 million codes of 5,003 rows of 5,120, 17 are off in a careful float32 form, 14 with products rounded to float32 (54.0 us), three so (55.6 us; four
-// and 56.9 with every product rounded so).
+// does.  Of the 25.6 million codes of 5,003 rows of 5,120, 17 are off in a careful float32 form, 14 with products rounded to float32, three so (54.0 and 55.6 us when that
+// was chosen; four and 56.9 with every product rounded so).
 struct RowFactor { f32x2 hi, lo, minus_hi, minus_lo; };       // each twice
 
 __device__ __forceinline__ void finish_four(float (&v)[4], const float (&g)[4], const RowFactor& r, uint8_t* codes, uint8_t* scales, size_t first_group, int slot) {
@@ -302,7 +303,7 @@ __device__ __noinline__ void extreme_row(const float* x, const TA* delta, float 
 }
 
 // One block a row; a warp and step hold one group.  PER > 0: a thread keeps PER float4 of the row (rows on 16-byte boundaries); PER = 0: the row is
-// read twice, number by number.  5,003 rows of 5,120 55.6 us, 5.0 TB/s (4 more with half the warps on an SM, 65 with blocks that stay and copy the next row to shared
+// read twice, number by number.  5,003 rows of 5,120 56.6 us, 5.0 TB/s, 60 among calls from Python one by one (4 more with half the warps on an SM, 65 with blocks that stay and copy the next row to shared
 // memory meanwhile): reads, a sum over the block and writes of a row follow one another, and what hides that is other rows' warps.  Eight rows of 4,096 2.5 us alone.
 template <typename TA, int PER>
 __global__ void __launch_bounds__(1024, PER == 4 ? 1 : 2) rmsnorm_q8_kernel(const float* resid, const TA* delta, const float* gain, float* sum_out, uint8_t* codes,

@@ -2768,7 +2768,8 @@ def quantize_weight_q8(w, codes, scales) -> Q8Weight:
 
 def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, delta_scale: float = 1.0) -> None:
     """``rmsnorm`` in front of an 8-bit product: x = resid (+ delta_scale * delta), y = x * rsqrt(mean(x^2) + eps) * weight, and y's codes and
-    scales as ``quantize_q8`` has them (y is rounded to its codes, not to float32 before).  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.
+    scales as ``quantize_q8`` has them (y is rounded to its codes, not to float32 before).  The mean is
+    that of 64 bits where float32 does not carry it: an infinity is NaN in its place and zero beside it, as the formula has it.  resid float32 [M, H], delta float32 or bfloat16 [M, H] or None, weight float32 [H], all contiguous.
     ``sum_out`` (float32 [M, H]: ``resid`` itself or a buffer that overlaps no other argument) gets x; None: x is kept nowhere."""
     global _LAUNCHES
     f32, shape = torch.float32, resid.shape
@@ -2819,7 +2820,8 @@ def rmsnorm_q8(resid, delta, weight, eps: float, codes, scales, sum_out=None, de
 def gemm_q8(codes, scales, w: Q8Weight, out) -> None:
     """out[M, N] = x . w^T for rows in 8 bits (``quantize_q8``, ``rmsnorm_q8``, ``gemm_act_mul_q8``) and a weight in 8 bits; out float32 or bfloat16, unit inner
     stride, any row stride.  Every block of 128 numbers of k is summed on the tensor cores, scaled by the row's and the weight block's scale and added up in
-    float32; the product of the two scales should be a normal float32 number (rows' scales that an operator made are 2^-100 to 2^119).  The result of a row
+    float32; the product of the two scales should be a normal float32 number (rows' scales that an operator made are 2^-100 to 2^119; of other e8m0 codes 0 counts as 0 and
+    255, which stands for NaN, as an infinity).  The result of a row
     does not depend on the other rows' numbers (on how many there are, in its last bits)."""
     global _LAUNCHES
     M, K = _rows_q8("gemm_q8", codes, scales)
@@ -2878,8 +2880,8 @@ def _q8_pair_cost(M: int, N: int, kb: int, sms: int) -> float:
 def _q8_route(M: int, N: int, kb: int, device: int):
     """(kernel, parts that a tile's k is cut into, estimated us) of a product, by its sizes alone.  Figures in us, alone in a graph:
 
-    * "rows", operands from memory to registers, up to 8 rows: one row of 4,096 x 4,096 behind the launch of its codes 5.8 and 7.5 with "few", 4,096 x 12,288 11.3
-      and 12.8, 24,576 x 4,096 19.3 and 20.2; longer sums are no shorter there (5,120 x 25,600 24.8 and 24.7, eight rows more);
+    * "rows", operands from memory to registers, up to 8 rows: one row of 4,096 x 4,096 behind the launch of its codes 6.1 and 7.5 with "few", 4,096 x 12,288 11.6
+      and 12.9, 24,576 x 4,096 19.4 and 19.8; longer sums are no shorter there (5,120 x 25,600 25.2 and 24.6, eight rows 26.4 and 25.3);
     * "few", up to 64 rows, bound by w's bytes.  Parts: the cheapest of what runs at once, 0.3 a block of k (0.45 for more than 32 rows), 0.1 (0.25) a part, 1.5 a
       wave, 0.9 where two blocks share an SM.  32 tiles of 32 blocks of k, one row: 2, 4, 6 and 8 parts 7.9, 6.3, 6.6 and 7.2; 48 tiles 8.9, 8.0, 10.2 (more than
       run at once) and 9.9, five 7.5; 32 tiles of 96 blocks 17.4, 12.4, 11.9 and 10.9;
